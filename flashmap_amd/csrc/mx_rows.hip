@@ -1,0 +1,501 @@
+// Rows to microscaled form (mx_device.h) and back: quantization with an MLP's activation on
+// the way, and the two norms in front of the projections (root mean square with the
+// residual's addition; the DiT's gated residual and modulated LayerNorm), which then write
+// 8 (or 4) bits a value in place of 16.
+//
+// Bound: HBM for prompts and full batches, latency for one user's 16 rows. A thread holds 8
+// consecutive values (one 16-byte load of bf16), so that a block of 32 is four neighbouring
+// lanes and its maximum two DPP steps.
+//
+// Everything between the inputs and the codes is float32, rounded once: the residual stream
+// is stored rounded to bf16, the norm is taken of the unrounded sum.
+#include <limits.h>
+
+#include <type_traits>
+
+#include "fm_host.h"
+#include "mx_device.h"
+
+namespace fm {
+
+constexpr int ROW_THREADS = 256;
+constexpr int64_t MAX_ITEMS = (int64_t)1 << 30;  // threads per launch (a launch counts at most 2^32)
+
+// Quad-wide maximum (lanes 4 i .. 4 i + 3), the same bits in all four.
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+  const uint32_t a = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, true);  // quad_perm [1, 0, 3, 2]
+  v = v > a ? v : a;
+  const uint32_t b = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, true);  // quad_perm [2, 3, 0, 1]
+  return v > b ? v : b;
+}
+
+// 8 values of a row from column c, zeros from `cols` on; `vec`: 16-byte loads are aligned.
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+struct bf16_raw { uint16_t v; };
+template <>
+__device__ __forceinline__ float to_f32<bf16_raw>(bf16_raw v) { return bf16_to_f32(v.v); }
+template <>
+__device__ __forceinline__ float to_f32<_Float16>(_Float16 v) { return (float)v; }
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) { return v; }
+
+template <typename T>
+__device__ __forceinline__ void load8(const T *row, int32_t c, int32_t cols, bool vec, float (&v)[8]) {
+  if (vec && c + 8 <= cols) {
+    if constexpr (sizeof(T) == 4) {
+      const f32x4_t a = *reinterpret_cast<const f32x4_t *>(row + c), b = *reinterpret_cast<const f32x4_t *>(row + c + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+    } else {
+      const u32x4_t a = load16(row + c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, bf16_raw>::value)
+          v[2 * i] = bf16_lo(a[i]), v[2 * i + 1] = bf16_hi(a[i]);
+        else
+          v[2 * i] = f16_lo(a[i]), v[2 * i + 1] = f16_hi(a[i]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? to_f32(row[c + i]) : 0.f;
+  }
+}
+
+__device__ __forceinline__ void store8_bf16(uint16_t *row, int32_t c, int32_t cols, bool vec, const float (&v)[8]) {
+  if (vec && c + 8 <= cols) {
+    u32x4_t w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+    store16(row + c, w);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < cols) row[c + i] = (uint16_t)(pack_bf16x2(v[i], 0.f) & 0xffffu);
+  }
+}
+
+// The codes of 8 values (four neighbouring lanes hold a block) and, from the block's first
+// lane, its scale byte. Every lane of the quad has to call this.
+template <int BITS>
+__device__ __forceinline__ void store_block(const float (&v)[8], int32_t c, uint8_t *codes, uint8_t *scales) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t m = magnitude(v[i]);
+    top = top > m ? top : m;
+  }
+  const uint32_t byte = mx_scale_byte<BITS>(quad_max(top));
+  const float scale = mx_scale_value(byte);
+  if constexpr (BITS == 8)
+    *reinterpret_cast<u32x2_t *>(codes + c) =
+        u32x2_t{mx_pack_e4m3x4(v[0], v[1], v[2], v[3], scale), mx_pack_e4m3x4(v[4], v[5], v[6], v[7], scale)};
+  else
+    *reinterpret_cast<uint32_t *>(codes + (c >> 1)) = mx_pack_e2m1x8(v, scale);
+  if ((c & 31) == 0) scales[c >> 5] = (uint8_t)byte;
+}
+
+// -------------------------------------------------------------------------- quantization
+
+struct QuantArgs {
+  const void *x;
+  uint8_t *codes, *scales;
+  int64_t xs, cs, ss;  // row strides (elements, bytes, bytes)
+  int64_t rows;
+  int32_t cols;
+  uint32_t chunks;  // 8-value chunks of a stored row
+  int32_t vec;
+};
+
+enum { ACT_NONE = 0, ACT_GELU = 1, ACT_SWIGLU = 2 };
+
+// x Phi(x) from erfc, which keeps its relative accuracy for negative x.
+__device__ __forceinline__ float gelu(float x) { return 0.5f * x * erfcf(x * -0.70710678f); }
+__device__ __forceinline__ float swiglu(float gate, float up) { return gate / (1.f + expf(-gate)) * up; }
+
+template <typename T, int BITS, int ACT>
+__global__ __launch_bounds__(ROW_THREADS) void mx_quantize_kernel(const QuantArgs a) {
+  const uint32_t item = blockIdx.x * ROW_THREADS + threadIdx.x;
+  const uint32_t row = item / a.chunks;
+  if (row >= a.rows) return;  // chunks of a row are a multiple of 16: whole quads leave
+  const int32_t c = 8 * (int32_t)(item - row * a.chunks);
+  const T *x = (const T *)a.x + row * a.xs;
+  float v[8];
+  load8(x, c, a.cols, a.vec != 0, v);
+  if constexpr (ACT == ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = gelu(v[i]);
+  } else if constexpr (ACT == ACT_SWIGLU) {
+    float u[8];
+    load8(x + a.cols, c, a.cols, a.vec != 0 && a.cols % 8 == 0, u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = swiglu(v[i], u[i]);
+  }
+  store_block<BITS>(v, c, a.codes + row * a.cs, a.scales + row * a.ss);
+}
+
+// ------------------------------------------------------------------------- reading back
+
+struct DequantArgs {
+  const uint8_t *codes, *scales;
+  void *out;
+  int64_t cs, ss, os;
+  int64_t rows;
+  int32_t cols;
+  uint32_t chunks;
+  int32_t vec;
+};
+
+template <typename T, int BITS>
+__global__ __launch_bounds__(ROW_THREADS) void mx_dequantize_kernel(const DequantArgs a) {
+  const uint32_t item = blockIdx.x * ROW_THREADS + threadIdx.x;
+  const uint32_t row = item / a.chunks;
+  if (row >= a.rows) return;
+  const int32_t c = 8 * (int32_t)(item - row * a.chunks);
+  if (c >= a.cols) return;
+  const uint32_t byte = a.scales[row * a.ss + (c >> 5)];
+  const float scale = byte == 255u ? __uint_as_float(0x7fc00000u) : mx_scale_value(byte);
+  float v[8];
+  typedef __attribute__((ext_vector_type(2))) float f32x2_t;
+  if constexpr (BITS == 8) {
+    const u32x2_t w = *reinterpret_cast<const u32x2_t *>(a.codes + row * a.cs + c);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
+      v[4 * i] = lo[0] * scale, v[4 * i + 1] = lo[1] * scale, v[4 * i + 2] = hi[0] * scale, v[4 * i + 3] = hi[1] * scale;
+    }
+  } else {
+    const uint32_t w = *reinterpret_cast<const uint32_t *>(a.codes + row * a.cs + (c >> 1));
+    const f32x2_t p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 0), p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 1);
+    const f32x2_t p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 2), p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 3);
+    v[0] = p0[0] * scale, v[1] = p0[1] * scale, v[2] = p1[0] * scale, v[3] = p1[1] * scale;
+    v[4] = p2[0] * scale, v[5] = p2[1] * scale, v[6] = p3[0] * scale, v[7] = p3[1] * scale;
+  }
+  if constexpr (std::is_same<T, bf16_raw>::value) {
+    store8_bf16((uint16_t *)a.out + row * a.os, c, a.cols, a.vec != 0, v);
+  } else {
+    T *out = (T *)a.out + row * a.os;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < a.cols) out[c + i] = (T)v[i];
+  }
+}
+
+// --------------------------------------------------------------------------------- norms
+
+struct NormArgs {
+  const uint16_t *x, *y;          // y NULL: nothing is added
+  const uint16_t *gate;           // NULL: y is added as it is
+  const float *weight;            // root mean square: the weights; else NULL
+  const uint16_t *scale, *shift;  // modulated LayerNorm
+  uint16_t *x_out;                // NULL: the stream is not stored
+  uint8_t *codes, *scales;
+  int64_t xs, ys, xos, cs, ss;
+  int64_t rows;
+  int32_t cols, gate_rows;
+  uint32_t chunks;
+  int32_t vec_x, vec_y, vec_p, vec_o;  // which rows may be read or written 16 bytes at a time
+  float eps;
+};
+
+// The sum over a row's TPR threads, the same bits in all of them.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float *lds) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+  if constexpr (TPR > 64) {
+    const int wave = wave_id();
+    __syncthreads();  // the last sum has been read
+    if ((threadIdx.x & 63) == 0) lds[wave] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int w = 0; w < TPR / 64; ++w) v += lds[w];
+  }
+  return v;
+}
+
+template <int TPR, int NCH, bool RMS, int BITS>
+__global__ __launch_bounds__(ROW_THREADS) void mx_norm_kernel(const NormArgs a) {
+  __shared__ float lds[ROW_THREADS / 64];
+  const int t = threadIdx.x % TPR;
+  const int64_t row = (int64_t)blockIdx.x * (ROW_THREADS / TPR) + threadIdx.x / TPR;
+  if (row >= a.rows) return;  // a whole wavefront, and with TPR 256 a whole workgroup
+  float v[NCH][8];
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    const int32_t c = 8 * (t + TPR * i);
+    load8((const bf16_raw *)a.x + row * a.xs, c, a.cols, a.vec_x != 0, v[i]);
+    if (a.y != nullptr) {
+      float y[8], g[8];
+      load8((const bf16_raw *)a.y + row * a.ys, c, a.cols, a.vec_y != 0, y);
+      if (a.gate == nullptr) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] += y[j];
+      } else {
+        if (a.gate_rows) {
+          const float gr = bf16_to_f32(a.gate[row]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) g[j] = gr;
+        } else {
+          load8((const bf16_raw *)a.gate, c, a.cols, a.vec_p != 0, g);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = __builtin_fmaf(g[j], y[j], v[i][j]);
+      }
+      if (a.x_out != nullptr && c < a.cols) store8_bf16(a.x_out + row * a.xos, c, a.cols, a.vec_o != 0, v[i]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum += RMS ? v[i][j] * v[i][j] : v[i][j];
+  }
+  const float n = (float)a.cols;
+  sum = row_sum<TPR>(sum, lds);
+  float mean = 0.f;
+  if constexpr (!RMS) {
+    mean = sum / n;
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float d = 8 * (t + TPR * i) + j < a.cols ? v[i][j] - mean : 0.f;
+        sum += d * d;
+      }
+    sum = row_sum<TPR>(sum, lds);
+  }
+  const float r = rsqrtf(sum / n + a.eps);
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    const int32_t c = 8 * (t + TPR * i);
+    if (c >= 8 * (int32_t)a.chunks) break;  // whole quads: chunks is a multiple of 16
+    float p[8], q[8];
+    if constexpr (RMS) {
+      load8(a.weight, c, a.cols, a.vec_p != 0, p);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] *= r * p[j];
+    } else {
+      load8((const bf16_raw *)a.scale, c, a.cols, a.vec_p != 0, p);
+      load8((const bf16_raw *)a.shift, c, a.cols, a.vec_p != 0, q);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[i][j] = c + j < a.cols ? __builtin_fmaf((v[i][j] - mean) * r, 1.f + p[j], q[j]) : 0.f;
+    }
+    store_block<BITS>(v[i], c, a.codes + row * a.cs, a.scales + row * a.ss);
+  }
+}
+
+static bool aligned(const void *p, int64_t n) { return ((uintptr_t)p % (uintptr_t)n) == 0; }
+static bool vec_rows(const void *p, int64_t stride, int64_t size) { return aligned(p, 16) && stride * size % 16 == 0; }
+
+// What every call checks of its microscaled rows.
+static int check_rows(const void *codes, int64_t codes_stride, const void *scales, int64_t scales_stride, int32_t bits,
+                      int64_t cols) {
+  FM_REQUIRE(bits == 4 || bits == 8, "bits %d: 4 or 8", bits);
+  FM_REQUIRE(codes && scales, "NULL codes or scales");
+  FM_REQUIRE(aligned(codes, 16) && codes_stride % 16 == 0 && codes_stride >= mx_padded(cols) * bits / 8,
+             "codes must be 16-byte aligned rows of %lld bytes", (long long)(mx_padded(cols) * bits / 8));
+  FM_REQUIRE(aligned(scales, 4) && scales_stride % 4 == 0 && scales_stride >= mx_padded(cols) / MX_BLOCK,
+             "scales must be 4-byte aligned rows of %lld bytes", (long long)(mx_padded(cols) / MX_BLOCK));
+  return FM_OK;
+}
+
+// f(first row, rows) for slices of at most MAX_ITEMS threads.
+template <typename F>
+static int by_slices(int64_t rows, int64_t threads_per_row, F f) {
+  const int64_t most = MAX_ITEMS / threads_per_row;
+  for (int64_t first = 0; first < rows; first += most) {
+    f(first, rows - first < most ? rows - first : most);
+    FM_CHECK_HIP(hipGetLastError());
+  }
+  return FM_OK;
+}
+
+template <typename F>
+static void by_dtype(int32_t dtype, F f) {
+  if (dtype == 0)
+    f(bf16_raw{});
+  else if (dtype == 1)
+    f((_Float16)0);
+  else
+    f(0.f);
+}
+
+static int launch_norm(const NormArgs &base, bool rms, int32_t bits, hipStream_t stream) {
+  // A wavefront a row while it holds the row in 4 chunks a lane, else a workgroup.
+  const int tpr = base.chunks <= 256 ? 64 : 256;
+  const int nch = (int)((base.chunks + tpr - 1) / tpr);
+  return by_slices(base.rows, tpr, [&](int64_t first, int64_t rows) {
+    NormArgs a = base;
+    a.rows = rows;
+    a.x += first * a.xs;
+    if (a.y) a.y += first * a.ys;
+    if (a.gate && a.gate_rows) a.gate += first;
+    if (a.x_out) a.x_out += first * a.xos;
+    a.codes += first * a.cs;
+    a.scales += first * a.ss;
+    const int per = ROW_THREADS / tpr;
+    const dim3 grid((unsigned)((rows + per - 1) / per));
+    auto go = [&](auto t, auto c, auto r, auto b) {
+      mx_norm_kernel<decltype(t)::value, decltype(c)::value, decltype(r)::value, decltype(b)::value>
+          <<<grid, dim3(ROW_THREADS), 0, stream>>>(a);
+    };
+    auto with_bits = [&](auto t, auto c, auto r) {
+      if (bits == 8)
+        go(t, c, r, std::integral_constant<int, 8>{});
+      else
+        go(t, c, r, std::integral_constant<int, 4>{});
+    };
+    auto with_kind = [&](auto t, auto c) {
+      if (rms)
+        with_bits(t, c, std::true_type{});
+      else
+        with_bits(t, c, std::false_type{});
+    };
+    if (tpr == 64) {
+      if (nch == 1)
+        with_kind(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
+      else if (nch == 2)
+        with_kind(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+      else
+        with_kind(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
+    } else {
+      if (nch <= 2)
+        with_kind(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
+      else if (nch <= 4)
+        with_kind(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
+      else
+        with_kind(std::integral_constant<int, 256>{}, std::integral_constant<int, 8>{});
+    }
+  });
+}
+
+}  // namespace fm
+
+extern "C" int fm_mx_quantize(const void *x, int32_t dtype, int64_t x_stride, int32_t activation, int32_t bits,
+                              void *codes, int64_t codes_stride, void *scales, int64_t scales_stride, int64_t rows,
+                              int64_t cols, void *stream) {
+  using namespace fm;
+  FM_REQUIRE(rows >= 0 && cols > 0, "bad sizes: rows=%lld cols=%lld", (long long)rows, (long long)cols);
+  if (rows == 0) return FM_OK;
+  FM_REQUIRE(dtype >= 0 && dtype <= 2, "dtype %d: 0 bf16, 1 fp16, 2 fp32", dtype);
+  FM_REQUIRE(activation >= 0 && activation <= 2, "activation %d: 0 none, 1 gelu, 2 swiglu", activation);
+  if (cols > 1 << 26) return fail(FM_ERR_UNSUPPORTED, "rows of %lld values: at most 2^26", (long long)cols);
+  const int64_t width = activation == ACT_SWIGLU ? 2 * cols : cols;
+  const int64_t size = dtype == 2 ? 4 : 2;
+  FM_REQUIRE(x != nullptr, "NULL tensor pointer");
+  FM_REQUIRE(aligned(x, size) && (rows == 1 || x_stride >= width), "rows of x overlap: stride %lld, %lld values",
+             (long long)x_stride, (long long)width);
+  const int rc = check_rows(codes, codes_stride, scales, scales_stride, bits, cols);
+  if (rc != FM_OK) return rc;
+  const int64_t chunks = mx_padded(cols) / 8;
+  return by_slices(rows, chunks, [&](int64_t first, int64_t n) {
+    by_dtype(dtype, [&](auto tag) {
+      typedef decltype(tag) T;
+      QuantArgs a{(const T *)x + first * x_stride, (uint8_t *)codes + first * codes_stride,
+                  (uint8_t *)scales + first * scales_stride, x_stride, codes_stride, scales_stride, n, (int32_t)cols,
+                  (uint32_t)chunks, vec_rows(x, x_stride, size)};
+      const dim3 grid((unsigned)((n * chunks + ROW_THREADS - 1) / ROW_THREADS));
+      auto go = [&](auto b, auto act) {
+        mx_quantize_kernel<T, decltype(b)::value, decltype(act)::value>
+            <<<grid, dim3(ROW_THREADS), 0, (hipStream_t)stream>>>(a);
+      };
+      auto with_act = [&](auto b) {
+        if (activation == ACT_GELU)
+          go(b, std::integral_constant<int, ACT_GELU>{});
+        else if (activation == ACT_SWIGLU)
+          go(b, std::integral_constant<int, ACT_SWIGLU>{});
+        else
+          go(b, std::integral_constant<int, ACT_NONE>{});
+      };
+      if (bits == 8)
+        with_act(std::integral_constant<int, 8>{});
+      else
+        with_act(std::integral_constant<int, 4>{});
+    });
+  });
+}
+
+extern "C" int fm_mx_dequantize(const void *codes, int64_t codes_stride, const void *scales, int64_t scales_stride,
+                                int32_t bits, void *out, int32_t dtype, int64_t out_stride, int64_t rows, int64_t cols,
+                                void *stream) {
+  using namespace fm;
+  FM_REQUIRE(rows >= 0 && cols > 0, "bad sizes: rows=%lld cols=%lld", (long long)rows, (long long)cols);
+  if (rows == 0) return FM_OK;
+  FM_REQUIRE(dtype >= 0 && dtype <= 2, "dtype %d: 0 bf16, 1 fp16, 2 fp32", dtype);
+  if (cols > 1 << 26) return fail(FM_ERR_UNSUPPORTED, "rows of %lld values: at most 2^26", (long long)cols);
+  const int64_t size = dtype == 2 ? 4 : 2;
+  FM_REQUIRE(out != nullptr, "NULL tensor pointer");
+  FM_REQUIRE(aligned(out, size) && (rows == 1 || out_stride >= cols), "rows of out overlap: stride %lld, %lld values",
+             (long long)out_stride, (long long)cols);
+  const int rc = check_rows(codes, codes_stride, scales, scales_stride, bits, cols);
+  if (rc != FM_OK) return rc;
+  const int64_t chunks = mx_padded(cols) / 8;
+  return by_slices(rows, chunks, [&](int64_t first, int64_t n) {
+    by_dtype(dtype, [&](auto tag) {
+      typedef decltype(tag) T;
+      DequantArgs a{(const uint8_t *)codes + first * codes_stride, (const uint8_t *)scales + first * scales_stride,
+                    (T *)out + first * out_stride, codes_stride, scales_stride, out_stride, n, (int32_t)cols,
+                    (uint32_t)chunks, vec_rows(out, out_stride, size)};
+      const dim3 grid((unsigned)((n * chunks + ROW_THREADS - 1) / ROW_THREADS));
+      if (bits == 8)
+        mx_dequantize_kernel<T, 8><<<grid, dim3(ROW_THREADS), 0, (hipStream_t)stream>>>(a);
+      else
+        mx_dequantize_kernel<T, 4><<<grid, dim3(ROW_THREADS), 0, (hipStream_t)stream>>>(a);
+    });
+  });
+}
+
+extern "C" int fm_rms_norm_mx(const void *x, int64_t x_stride, const void *residual, int64_t residual_stride,
+                              const float *weight, float eps, void *x_out, int64_t x_out_stride, int32_t bits,
+                              void *codes, int64_t codes_stride, void *scales, int64_t scales_stride, int64_t rows,
+                              int32_t cols, void *stream) {
+  using namespace fm;
+  FM_REQUIRE(rows >= 0 && cols > 0, "bad sizes: rows=%lld cols=%d", (long long)rows, cols);
+  if (rows == 0) return FM_OK;
+  if (cols > 16384) return fail(FM_ERR_UNSUPPORTED, "rows of %d values: at most 16384", cols);
+  FM_REQUIRE(x && weight && aligned(x, 2) && aligned(weight, 4), "x and weight must be given, aligned to their values");
+  FM_REQUIRE((residual != nullptr) == (x_out != nullptr), "a residual and the stream x_out go together");
+  FM_REQUIRE(rows == 1 || (x_stride >= cols && (!residual || (residual_stride >= cols && x_out_stride >= cols))),
+             "row strides must cover a row");
+  const int rc = check_rows(codes, codes_stride, scales, scales_stride, bits, cols);
+  if (rc != FM_OK) return rc;
+  NormArgs a{};
+  a.x = (const uint16_t *)x, a.y = (const uint16_t *)residual, a.weight = weight, a.x_out = (uint16_t *)x_out;
+  a.codes = (uint8_t *)codes, a.scales = (uint8_t *)scales;
+  a.xs = x_stride, a.ys = residual_stride, a.xos = x_out_stride, a.cs = codes_stride, a.ss = scales_stride;
+  a.rows = rows, a.cols = cols, a.chunks = (uint32_t)(mx_padded(cols) / 8), a.eps = eps;
+  a.vec_x = vec_rows(x, x_stride, 2), a.vec_y = vec_rows(residual, residual_stride, 2);
+  a.vec_p = aligned(weight, 16), a.vec_o = vec_rows(x_out, x_out_stride, 2);
+  return launch_norm(a, true, bits, (hipStream_t)stream);
+}
+
+extern "C" int fm_adaln_residual_mx(const void *x, int64_t x_stride, const void *y, int64_t y_stride, const void *gate,
+                                    int32_t gate_per_row, const void *scale, const void *shift, void *x_out,
+                                    int64_t x_out_stride, float eps, int32_t bits, void *codes, int64_t codes_stride,
+                                    void *scales, int64_t scales_stride, int64_t rows, int32_t cols, void *stream) {
+  using namespace fm;
+  FM_REQUIRE(rows >= 0 && cols > 0, "bad sizes: rows=%lld cols=%d", (long long)rows, cols);
+  if (rows == 0) return FM_OK;
+  if (cols > 16384) return fail(FM_ERR_UNSUPPORTED, "rows of %d values: at most 16384", cols);
+  FM_REQUIRE(x && scale && shift, "NULL tensor pointer");
+  FM_REQUIRE(!y || (gate && x_out), "a residual needs its gate and x_out");
+  FM_REQUIRE(y || !x_out, "x_out without a residual");
+  FM_REQUIRE(aligned(x, 2) && aligned(y, 2) && aligned(gate, 2) && aligned(scale, 2) && aligned(shift, 2) && aligned(x_out, 2),
+             "tensors must be aligned to their values");
+  FM_REQUIRE(x_stride == 0 || rows == 1 || x_stride >= cols, "row strides must cover a row");
+  FM_REQUIRE(rows == 1 || !y || (y_stride >= cols && x_out_stride >= cols), "row strides must cover a row");
+  FM_REQUIRE(x_stride != 0 || x != x_out || rows == 1, "x_out may not alias a shared x row");
+  const int rc = check_rows(codes, codes_stride, scales, scales_stride, bits, cols);
+  if (rc != FM_OK) return rc;
+  NormArgs a{};
+  a.x = (const uint16_t *)x, a.y = (const uint16_t *)y, a.gate = (const uint16_t *)gate;
+  a.scale = (const uint16_t *)scale, a.shift = (const uint16_t *)shift, a.x_out = (uint16_t *)x_out;
+  a.codes = (uint8_t *)codes, a.scales = (uint8_t *)scales;
+  a.xs = x_stride, a.ys = y_stride, a.xos = x_out_stride, a.cs = codes_stride, a.ss = scales_stride;
+  a.rows = rows, a.cols = cols, a.gate_rows = gate_per_row, a.chunks = (uint32_t)(mx_padded(cols) / 8), a.eps = eps;
+  a.vec_x = vec_rows(x, x_stride, 2), a.vec_y = vec_rows(y, y_stride, 2), a.vec_o = vec_rows(x_out, x_out_stride, 2);
+  a.vec_p = aligned(scale, 16) && aligned(shift, 16) && (!y || gate_per_row || aligned(gate, 16));
+  return launch_norm(a, false, bits, (hipStream_t)stream);
+}

@@ -19,8 +19,10 @@ from . import _native
 from ._native import call
 
 __all__ = [
+    "MX",
     "Rope",
     "adaln_residual",
+    "adaln_residual_mx",
     "noise_rows",
     "argmax_rows",
     "attention_plan",
@@ -31,6 +33,10 @@ __all__ = [
     "block_attention_token_paged",
     "block_attention_token_paged_fp8",
     "block_self_attention",
+    "mx_dequantize",
+    "mx_linear",
+    "mx_quantize",
+    "rms_norm_mx",
     "rms_norm_rope",
     "rope_from_cat",
     "rope_from_split",
@@ -1303,6 +1309,305 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     """``F.linear``, by the framework's kernel where :func:`linear_rows` takes the call."""
     out = linear_rows(x, weight, bias)
     return torch.nn.functional.linear(x, weight, bias) if out is None else out
+
+
+# ------------------------------------------------------------------- microscaled rows
+
+MX_BLOCK = 32  # values that share a scale
+MX_PAD = 128  # stored rows hold a multiple of this many values
+MX_MAX = 1 << 26  # rows, columns
+MX_NORM_COLS = 16384
+_ACTIVATIONS = {None: 0, "gelu": 1, "swiglu": 2}
+
+
+@dataclass(frozen=True)
+class MX:
+    """A tensor of ``shape (..., cols)`` in OCP microscaling: per block of 32 values of a row
+    one scale ``2^(byte - 127)`` and 8-bit (e4m3) or 4-bit (e2m1) codes. ``codes`` uint8
+    ``(rows, pad)`` (8 bits) or ``(rows, pad / 2)`` (4 bits, the even column in a byte's low
+    half) and ``scales`` uint8 ``(rows, pad / 32)``, ``pad`` the columns rounded up to 128 and
+    filled with zeros. A scale byte of 255 makes its block NaN. :func:`mx_quantize`,
+    :func:`rms_norm_mx` and :func:`adaln_residual_mx` make them."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    bits: int
+    shape: tuple
+
+    @property
+    def cols(self) -> int:
+        return self.shape[-1]
+
+    @property
+    def rows(self) -> int:
+        return math.prod(self.shape[:-1])
+
+    def view(self, *lead: int) -> "MX":
+        """The same rows under other leading dimensions."""
+        if math.prod(lead) != self.rows:
+            raise ValueError(f"{self.rows} rows cannot be viewed as {lead}")
+        return MX(self.codes, self.scales, self.bits, (*lead, self.cols))
+
+    def to(self, *args, **kwargs) -> "MX":
+        """On another device (``Tensor.to`` of the codes and the scales)."""
+        codes, scales = self.codes.to(*args, **kwargs), self.scales.to(*args, **kwargs)
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError("the codes and scales are bytes: mx_dequantize gives the values in a dtype")
+        return MX(codes, scales, self.bits, self.shape)
+
+
+def _mx_new(shape: tuple, bits: int, device: torch.device) -> MX:
+    if bits not in (4, 8):
+        raise ValueError(f"bits must be 4 or 8, got {bits}")
+    rows, cols = math.prod(shape[:-1]), shape[-1]
+    if not 0 < cols <= MX_MAX or rows > MX_MAX:
+        raise ValueError(f"microscaled rows: 1 to 2^26 columns and at most 2^26 rows, got {rows} x {cols}")
+    pad = -(-cols // MX_PAD) * MX_PAD
+    return MX(torch.empty(rows, pad * bits // 8, dtype=torch.uint8, device=device),
+              torch.empty(rows, pad // MX_BLOCK, dtype=torch.uint8, device=device), bits, tuple(shape))
+
+
+def _mx_args(q: MX, name: str) -> list:
+    """(codes, stride, scales, stride) of rows as the kernels read them."""
+    codes, scales = q.codes, q.scales
+    pad = -(-q.cols // MX_PAD) * MX_PAD
+    rows = q.rows
+    if q.bits not in (4, 8) or codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8:
+        raise TypeError(f"{name} must hold uint8 codes of 4 or 8 bits and uint8 scales")
+    if not 0 < q.cols <= MX_MAX or rows > MX_MAX:
+        raise ValueError(f"{name}: 1 to 2^26 columns and at most 2^26 rows, got {rows} x {q.cols}")
+    if tuple(codes.shape) != (rows, pad * q.bits // 8) or tuple(scales.shape) != (rows, pad // MX_BLOCK):
+        raise ValueError(f"{name} of shape {q.shape} in {q.bits} bits holds codes ({rows}, {pad * q.bits // 8}) and "
+                         f"scales ({rows}, {pad // MX_BLOCK}); got {tuple(codes.shape)} and {tuple(scales.shape)}")
+    return [*_mx_bytes(codes, 16), *_mx_bytes(scales, 4)]
+
+
+def _mx_bytes(t: torch.Tensor, unit: int) -> tuple[torch.Tensor, int]:
+    """``t`` as byte rows aligned to ``unit`` that do not overlap (a copy if needed), and their
+    stride (a lone row's is whatever its tensor was cut from; the kernels never step by it)."""
+    rows, width = t.shape
+    if t.data_ptr() % unit or t.stride(1) != 1 or (rows > 1 and (t.stride(0) % unit or t.stride(0) < width)):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride(0) if rows > 1 else width
+
+
+def _mx_ptrs(args: list) -> list:
+    return [args[0].data_ptr(), args[1], args[2].data_ptr(), args[3]]
+
+
+def _mx_call(name: str, device: torch.device, *args) -> None:
+    """``call`` with ``device`` current (the kernels are launched there)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args)
+
+
+def _no_gradient(name: str, *tensors: torch.Tensor | None) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or on detached tensors")
+
+
+def _plain_rows(t: torch.Tensor, cols: int, name: str) -> tuple[torch.Tensor, int]:
+    """``t (..., cols)`` as ``(rows, cols)`` with unit column stride (a copy where the leading
+    dimensions do not flatten to one stride of at least a row) and that stride."""
+    if t.dim() == 0 or t.shape[-1] != cols:
+        raise ValueError(f"{name} must be (..., {cols}), got {tuple(t.shape)}")
+    r = t.reshape(-1, cols)
+    if (cols > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and r.stride(0) < cols):
+        r = r.contiguous()
+    return r, (r.stride(0) if r.shape[0] > 1 else cols)
+
+
+def _bf16_out(x_out: torch.Tensor | None, shape: tuple, device: torch.device,
+              name: str) -> tuple[torch.Tensor, torch.Tensor, int]:
+    """The bf16 tensor that receives an output, its rows and their stride."""
+    if x_out is None:
+        x_out = torch.empty(shape, dtype=torch.bfloat16, device=device)
+    elif x_out.dtype != torch.bfloat16 or tuple(x_out.shape) != tuple(shape):
+        raise ValueError(f"{name} must be bfloat16 {tuple(shape)}, got {x_out.dtype} {tuple(x_out.shape)}")
+    cols = shape[-1]
+    rows = x_out.view(-1, cols)  # raises unless the rows are one strided view
+    if (cols > 1 and rows.stride(1) != 1) or (rows.shape[0] > 1 and rows.stride(0) < cols):
+        raise ValueError(f"{name} must hold rows of unit column stride that do not overlap")
+    return x_out, rows, (rows.stride(0) if rows.shape[0] > 1 else cols)
+
+
+def mx_quantize(x: torch.Tensor, bits: int = 8, activation: str | None = None) -> MX:
+    """``x (..., cols)`` (bf16, fp16 or fp32) in microscaled form, ``bits`` 8 or 4: each block's
+    scale is the power of two that brings its largest magnitude to [256, 512) (e4m3) or [4, 8)
+    (e2m1), codes round to nearest even and saturate at 448 or 6, and a block holding an
+    infinity or a NaN is all NaN. ``activation``: "gelu" (the exact one) or "swiglu" (``x (...,
+    2 cols)``: silu of the first half of a row times the second) in float32 on the way."""
+    _check_cuda(x)
+    if x.dtype not in _LOGIT_DTYPES:
+        raise TypeError(f"x must be bfloat16, float16 or float32, got {x.dtype}")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"activation must be None, 'gelu' or 'swiglu', got {activation!r}")
+    _no_gradient("mx_quantize", x)
+    if x.dim() == 0:
+        raise ValueError("x must be (..., cols)")
+    wide = x.shape[-1]
+    if activation == "swiglu" and wide % 2:
+        raise ValueError(f"swiglu takes rows of two halves, got {wide} values")
+    cols = wide // 2 if activation == "swiglu" else wide
+    q = _mx_new((*x.shape[:-1], cols), bits, x.device)
+    if q.codes.shape[0]:
+        r, stride = _plain_rows(x, wide, "x")
+        _mx_call("fm_mx_quantize", x.device, r.data_ptr(), _LOGIT_DTYPES[x.dtype], stride, _ACTIVATIONS[activation],
+                 bits, q.codes.data_ptr(), q.codes.shape[1], q.scales.data_ptr(), q.scales.shape[1], r.shape[0], cols,
+                 _stream(x))
+    return q
+
+
+def mx_dequantize(q: MX, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values of ``q`` (bf16, fp16 or fp32) in its shape: exact in float32 and, for scales
+    above 2^-117, in bfloat16; float16 rounds to nearest and overflows to infinity."""
+    _check_cuda(q.codes, q.scales)
+    if dtype not in _LOGIT_DTYPES:
+        raise TypeError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
+    held = _mx_args(q, "q")
+    out = torch.empty(q.shape, dtype=dtype, device=q.codes.device)
+    if q.rows:
+        _mx_call("fm_mx_dequantize", out.device, *_mx_ptrs(held), q.bits, out.data_ptr(), _LOGIT_DTYPES[dtype], q.cols,
+                 q.rows, q.cols, _stream(out))
+    return out
+
+
+def mx_linear(x: torch.Tensor | MX, weight: MX, bias: torch.Tensor | None = None,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """``x weight^T + bias`` for ``weight (n, k)`` in microscaled 4 bits, on the block-scaled
+    matrix instructions: ``(..., n)`` bf16, accumulated in float32 and rounded once. ``x (...,
+    k)``: microscaled in 8 or 4 bits, or bf16, which the call quantizes to 8 bits
+    (:func:`mx_quantize`). ``bias (n,)`` bf16. ``out (..., n)`` bf16 receives the result."""
+    quantized = isinstance(x, MX)
+    device = _check_cuda(x.codes if quantized else x, x.scales if quantized else None, weight.codes, weight.scales,
+                         bias, out)
+    if weight.bits != 4 or len(weight.shape) != 2:
+        raise ValueError(f"weight must be (n, k) in 4 bits, got {weight.shape} in {weight.bits}")
+    n, k = weight.shape
+    if x.shape[-1:] != (k,):
+        raise ValueError(f"x {tuple(x.shape)} does not match a weight of {k} columns")
+    w = _mx_args(weight, "weight")
+    lead = tuple(x.shape[:-1])
+    if quantized:
+        rows, x_bits, held = x.rows, x.bits, _mx_args(x, "x")
+        xa = _mx_ptrs(held)
+    else:
+        if x.dtype is not torch.bfloat16:
+            raise TypeError(f"x must be bfloat16 or microscaled, got {x.dtype}")
+        _no_gradient("mx_linear", x, bias)
+        held, stride = _plain_rows(x, k, "x")
+        rows, x_bits, xa = held.shape[0], 16, [held.data_ptr(), stride, None, 0]
+    if bias is not None:
+        if bias.dtype is not torch.bfloat16 or tuple(bias.shape) != (n,):
+            raise ValueError(f"bias must be bfloat16 ({n},), got {bias.dtype} {tuple(bias.shape)}")
+        _no_gradient("mx_linear", bias)
+        bias = bias.contiguous()
+    if out is None:
+        out = torch.empty(*lead, n, dtype=torch.bfloat16, device=device)
+        out_rows, stride = out, n
+    else:
+        out, out_rows, stride = _bf16_out(out, (*lead, n), device, "out")
+    if rows and n:
+        nbytes = int(_native.lib().fm_mx_linear_workspace_bytes(rows, n, k, x_bits))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        _mx_call("fm_mx_linear", device, xa[0], x_bits, xa[1], xa[2], xa[3], *_mx_ptrs(w), _ptr(bias),
+                 out_rows.data_ptr(), stride, rows, n, k, _ptr(ws), nbytes, _stream(out))
+    return out
+
+
+def rms_norm_mx(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.Tensor | None = None,
+                x_out: torch.Tensor | None = None, bits: int = 8) -> tuple[torch.Tensor | None, MX]:
+    """A root-mean-square norm with the residual's addition in front and microscaled output:
+    ``s = x + residual`` (float32; ``x`` without one), the stream ``x' = s`` in bf16 and ``s *
+    rsqrt(mean(s^2) + eps) * weight`` in 8 (or 4) bits, rounded once from float32. ``x``,
+    ``residual (..., cols)`` bf16, ``weight (cols,)``; ``x_out`` (may be ``x`` or ``residual``)
+    receives ``x'``. Returns ``(x', q)``, ``x'`` None without a residual."""
+    device = _check_cuda(x, weight, residual, x_out)
+    _no_gradient("rms_norm_mx", x, weight, residual)
+    cols = _norm_cols(x)
+    if weight.numel() != cols:
+        raise ValueError(f"weight holds {weight.numel()} values, a row {cols}")
+    if residual is not None and (residual.dtype != torch.bfloat16 or residual.shape != x.shape):
+        raise ValueError(f"residual must be bfloat16 {tuple(x.shape)}, got {residual.dtype} {tuple(residual.shape)}")
+    if residual is None and x_out is not None:
+        raise ValueError("x_out is the sum of x and a residual: give one")
+    q = _mx_new(tuple(x.shape), bits, device)
+    xr, xs = _plain_rows(x, cols, "x")
+    rr, rs, orows, os_ = None, 0, None, 0
+    if residual is not None:
+        rr, rs = _plain_rows(residual, cols, "residual")
+        x_out, orows, os_ = _bf16_out(x_out, tuple(x.shape), device, "x_out")
+    weight = _f32(weight)
+    if xr.shape[0]:
+        _mx_call("fm_rms_norm_mx", device, xr.data_ptr(), xs, _ptr(rr), rs, weight.data_ptr(), float(eps),
+                 _ptr(orows), os_, bits, q.codes.data_ptr(), q.codes.shape[1], q.scales.data_ptr(), q.scales.shape[1],
+                 xr.shape[0], cols, _stream(x))
+    return x_out, q
+
+
+def _norm_cols(x: torch.Tensor) -> int:
+    if x.dtype != torch.bfloat16 or x.dim() == 0:
+        raise TypeError(f"x must be bfloat16 (..., cols), got {x.dtype} {tuple(x.shape)}")
+    if not 0 < x.shape[-1] <= MX_NORM_COLS:
+        raise ValueError(f"rows of {x.shape[-1]} values: the norms take 1 to {MX_NORM_COLS}")
+    return x.shape[-1]
+
+
+def adaln_residual_mx(
+    x: torch.Tensor,
+    y: torch.Tensor | None,
+    gate: torch.Tensor | None,
+    modulation: tuple[torch.Tensor, torch.Tensor],
+    eps: float,
+    x_out: torch.Tensor | None = None,
+    gate_per_row: bool = False,
+    bits: int = 8,
+) -> tuple[torch.Tensor | None, MX]:
+    """:func:`adaln_residual` with microscaled output for a projection by :func:`mx_linear`:
+    ``s = x + gate * y`` (float32; ``x`` for ``y`` None), the stream ``x' = s`` in bf16, and
+    ``LN(s) * (1 + scale) + shift`` for ``modulation = (scale, shift)`` in 8 (or 4) bits,
+    nothing rounded in between. ``x``/``y (..., cols)`` bf16, or ``x (cols,)``: one row shared
+    by every row of ``y``; ``gate``, ``scale``, ``shift (cols,)`` bf16 (``gate_per_row``: one
+    gate value per row). ``x_out`` (may be ``x``) receives ``x'``. Returns ``(x', q)``, ``x'``
+    None without a residual."""
+    if modulation is None:
+        raise ValueError("a microscaled output needs its modulation (adaln_residual serves the residual alone)")
+    device = _check_cuda(x, y, gate, x_out, *modulation)
+    _no_gradient("adaln_residual_mx", x, y, gate, *modulation)
+    cols = _norm_cols(x)
+    shared = x.dim() == 1 and y is not None
+    shape = tuple(y.shape if shared else x.shape)
+    rows = math.prod(shape[:-1])
+    yr, ys, g, orows, os_ = None, 0, None, None, 0
+    if y is not None:
+        if gate is None:
+            raise ValueError("a residual needs its gate")
+        if y.dtype != torch.bfloat16 or y.shape[-1:] != (cols,) or (not shared and y.shape != x.shape):
+            raise ValueError(f"y {y.dtype} {tuple(y.shape)} does not match x {tuple(x.shape)}")
+        yr, ys = _plain_rows(y, cols, "y")
+        g = _mx_vec(gate, rows, "gate (one per row)") if gate_per_row else _mx_vec(gate, cols, "gate")
+        if shared and x_out is not None and x_out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
+            raise ValueError("x_out may not share the storage of a shared x row")
+        x_out, orows, os_ = _bf16_out(x_out, shape, device, "x_out")
+    elif x_out is not None:
+        raise ValueError("x_out is the sum of x and a gated y: give one")
+    sc, sh = _mx_vec(modulation[0], cols, "scale"), _mx_vec(modulation[1], cols, "shift")
+    xr, xs = _plain_rows(x, cols, "x")
+    q = _mx_new(shape, bits, device)
+    if rows:
+        _mx_call("fm_adaln_residual_mx", device, xr.data_ptr(), 0 if shared else xs, _ptr(yr), ys, _ptr(g),
+                 int(gate_per_row), sc.data_ptr(), sh.data_ptr(), _ptr(orows), os_, float(eps), bits,
+                 q.codes.data_ptr(), q.codes.shape[1], q.scales.data_ptr(), q.scales.shape[1], rows, cols, _stream(x))
+    return x_out, q
+
+
+def _mx_vec(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
+    if t.dtype != torch.bfloat16 or t.numel() != n:
+        raise ValueError(f"{name} must hold {n} bfloat16 values, got {t.dtype} {tuple(t.shape)}")
+    return t.reshape(n).contiguous()
 
 
 def noise_rows(z: torch.Tensor, eigvals: torch.Tensor, eps: float, gain: float,

@@ -475,6 +475,61 @@ int fm_state_update(float *state, int64_t rows, int64_t vocab, int64_t state_str
                     int64_t logits_stride, double start, double end, void *stream);
 
 /* ---------------------------------------------------------------------------------
+ * Microscaled rows: a drafter whose weights are held in 4 bits. No counterpart in the
+ * reference, whose drafters are bf16 throughout; drafts are verified, so the weights'
+ * precision costs acceptance and never correctness.
+ *
+ * The format is OCP microscaling. A block of 32 consecutive values of a row has one scale
+ * byte b = max(floor(log2 max|v|) - emax + 127, 0), emax 8 for 8-bit (e4m3) and 2 for 4-bit
+ * (e2m1) codes; a code is v / 2^(b - 127) rounded to nearest, ties to even, saturated at 448
+ * or 6. A block that holds an infinity or a NaN has the byte 255 (NaN): all of it reads back,
+ * and every product with it, as NaN. Stored rows hold pad(cols) codes, cols rounded up to a
+ * multiple of 128, the padding the codes of zeros: codes (rows, pad) bytes for 8 bits or
+ * (rows, pad / 2) for 4, the even column in a byte's low half; scales (rows, pad / 32).
+ * Code rows are 16-byte aligned with strides of multiples of 16 bytes, scale rows 4-byte
+ * aligned with strides of multiples of 4. Unless said otherwise strides are in elements (codes
+ * and scales: bytes), rows of other tensors may be aligned to their values alone, and cols
+ * is at most 2^26.
+ */
+/* x (rows, cols) of dtype 0 bf16, 1 fp16, 2 fp32 to codes and scales of `bits` 8 or 4, with
+ * activation 1 (x Phi(x), the exact GELU) or 2 (x holds (rows, 2 cols): silu of the first
+ * half of a row times its second half) applied in fp32 on the way, 0 none. */
+int fm_mx_quantize(const void *x, int32_t dtype, int64_t x_stride, int32_t activation, int32_t bits, void *codes,
+                   int64_t codes_stride, void *scales, int64_t scales_stride, int64_t rows, int64_t cols,
+                   void *stream);
+/* The values that codes and scales stand for, out (rows, cols) of dtype 0 bf16, 1 fp16, 2
+ * fp32 (exact in fp32, and in bf16 but for its subnormals; fp16 rounds to nearest). */
+int fm_mx_dequantize(const void *codes, int64_t codes_stride, const void *scales, int64_t scales_stride,
+                     int32_t bits, void *out, int32_t dtype, int64_t out_stride, int64_t rows, int64_t cols,
+                     void *stream);
+/* out (rows, n) bf16 = x w^T (+ bias (n,) bf16 or NULL), accumulated in fp32 and rounded once.
+ * w: 4-bit rows (n, k). x_bits 8 or 4: x holds codes, x_scales its scales; x_bits 16: x is
+ * bf16 (rows, k), quantized to 8 bits in the call (x_scales is not read). rows, n and k at
+ * most 2^26. The workspace (16-byte aligned) holds fm_mx_linear_workspace_bytes(rows, n, k,
+ * x_bits) bytes; concurrent calls must not share it. */
+size_t fm_mx_linear_workspace_bytes(int64_t rows, int64_t n, int64_t k, int32_t x_bits);
+int fm_mx_linear(const void *x, int32_t x_bits, int64_t x_stride, const void *x_scales, int64_t x_scales_stride,
+                 const void *w, int64_t w_stride, const void *w_scales, int64_t w_scales_stride, const void *bias,
+                 void *out, int64_t out_stride, int64_t rows, int64_t n, int64_t k, void *workspace,
+                 size_t workspace_bytes, void *stream);
+/* s = x + residual (fp32; s = x without one), x_out = s in bf16, codes and scales of
+ * s * rsqrt(mean(s^2) + eps) * weight. x, residual, x_out: bf16 rows (x_out goes with a
+ * residual and may be x or the residual); weight fp32 (cols,). cols at most 16384. */
+int fm_rms_norm_mx(const void *x, int64_t x_stride, const void *residual, int64_t residual_stride,
+                   const float *weight, float eps, void *x_out, int64_t x_out_stride, int32_t bits, void *codes,
+                   int64_t codes_stride, void *scales, int64_t scales_stride, int64_t rows, int32_t cols,
+                   void *stream);
+/* fm_adaln_residual with microscaled output: s = x + gate * y (fp32; s = x for y NULL), x_out
+ * = s in bf16, codes and scales of (s - mean) * rsqrt(var + eps) * (1 + scale) + shift, var
+ * biased, nothing rounded in between. x, y, x_out: bf16 rows (x_stride 0: one row for all;
+ * x_out, which goes with y, may be x or y); gate: bf16 (cols,), or one value per row with
+ * gate_per_row; scale, shift: bf16 (cols,). cols at most 16384. */
+int fm_adaln_residual_mx(const void *x, int64_t x_stride, const void *y, int64_t y_stride, const void *gate,
+                         int32_t gate_per_row, const void *scale, const void *shift, void *x_out,
+                         int64_t x_out_stride, float eps, int32_t bits, void *codes, int64_t codes_stride,
+                         void *scales, int64_t scales_stride, int64_t rows, int32_t cols, void *stream);
+
+/* ---------------------------------------------------------------------------------
  * Measurement hook. No reference counterpart: it lets a benchmark time the main
  * split-KV attention kernel alone with HIP events on the stream it runs on, without
  * changing the work any call does. While enabled, every attention call records an

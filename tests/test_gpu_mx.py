@@ -1,0 +1,384 @@
+"""Microscaled rows on the GPU (flashmap_amd.ops.mx_*, rms_norm_mx, adaln_residual_mx) against
+float64 (oracle/mx.py).
+
+Quantization of a tensor's own values is one rounding of exact quotients: codes and scales are
+equal to the oracle's. Where a value is computed before it is quantized (an activation, a
+norm) it is off by its float32 error, which moves a code only past a midpoint: the codes must
+lie between the oracle's for the value less and plus that error. A product's bound counts the
+bf16 rounding (2^-8) and what the matrix instruction drops of products far below the largest
+of a step (measured at most 2^-17 of the absolute sum; 2^-15 allowed)."""
+
+import pytest
+import torch
+
+from _inputs import gen
+from flashmap_amd import ops
+from oracle import mx
+
+pytestmark = pytest.mark.gpu
+
+
+def _cpu(q: ops.MX):
+    """(codes one per value, scales) on the CPU, padding included."""
+    return mx.unpack(q.codes.cpu(), q.bits), q.scales.cpu()
+
+
+def _activations(rows, cols, seed, dtype=torch.bfloat16):
+    g = gen(seed)
+    return (torch.randn(rows, cols, generator=g) * torch.exp(torch.randn(cols, generator=g))).to(dtype)
+
+
+def _between(q: ops.MX, v: torch.Tensor, tol: torch.Tensor) -> None:
+    """Every code of ``q`` is the code of some value within ``tol`` of ``v`` (float64)."""
+    code, scale = _cpu(q)
+    got = mx.values(code, scale, q.bits)
+    (lc, ls), (hc, hs) = mx.quantize(v - tol, q.bits), mx.quantize(v + tol, q.bits)
+    down, up = mx.quantize(v.abs() - tol, q.bits)[1], mx.quantize(v.abs() + tol, q.bits)[1]
+    assert ((scale >= down.minimum(up)) & (scale <= down.maximum(up))).all(), "a scale away from its block's maximum"
+    lo, hi = mx.values(lc, scale.minimum(ls), q.bits), mx.values(hc, scale.maximum(hs), q.bits)
+    same = ((ls == scale) & (hs == scale)).repeat_interleave(32, 1)
+    inside = (got >= lo) & (got <= hi)
+    assert inside[same].all(), f"{int((~inside & same).sum())} codes outside their interval"
+    # where the error moves the block's maximum over a power of two: within a code of it
+    step = 2.0 ** (scale.double() - 127).repeat_interleave(32, 1) * (32 if q.bits == 8 else 2)
+    full = torch.zeros_like(got)
+    full[:, : v.shape[1]] = v
+    assert ((got - full).abs() <= step)[~same].all()
+
+
+SIZES = [(1, 1), (3, 31), (2, 32), (5, 33), (17, 127), (1, 128), (4, 129), (33, 200), (7, 2056), (3, 20480)]
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,cols", SIZES)
+def test_quantize_is_exact(dev, rows, cols, dtype, bits):
+    print(f"mx_quantize {rows} x {cols} {dtype} bits={bits}", flush=True)
+    x = _activations(rows, cols, rows + cols, dtype)
+    q = ops.mx_quantize(x.to(dev), bits)
+    code, scale = _cpu(q)
+    wc, ws = mx.quantize(x, bits)
+    assert q.shape == (rows, cols) and torch.equal(scale, ws) and torch.equal(code, wc)
+    back = ops.mx_dequantize(q, torch.float32)
+    assert torch.equal(back.cpu().double(), mx.values(wc, ws, bits)[:, :cols])
+    for other in (torch.bfloat16, torch.float16):
+        assert torch.equal(ops.mx_dequantize(q, other).cpu(), back.cpu().to(other))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_quantize_edges(dev, bits):
+    """Midpoints, the largest and smallest floats, infinities and NaN, zeros of both signs."""
+    grid = torch.tensor(mx.E4M3 if bits == 8 else mx.E2M1)
+    over = grid[-1:] * torch.tensor([1.01, 1.03, 1.06, 1.13])
+    mids = torch.cat([grid, (grid[1:] + grid[:-1]) / 2, over])
+    v = torch.cat([mids, -mids])
+    v = torch.cat([v, torch.zeros(-len(v) % 32)])
+    top = torch.full((32,), float(grid[-1]))
+    rows = [torch.cat([v * 2.0 ** e, top * 2.0 ** e]) for e in (0, -5, 17, -100, 100)]
+    n = len(rows[0])
+    special = torch.zeros(6, n)
+    special[0, 5], special[0, 40] = float("inf"), float("nan")
+    special[1, :] = -0.0
+    special[2, ::2] = torch.finfo(torch.float32).max
+    special[3, :] = torch.linspace(-1, 1, n) * 2.0 ** -118
+    special[4, 0::32], special[4, 1::32] = 2.0 ** -126, -(2.0 ** -127)
+    special[5, 3], special[5, 7] = -float("inf"), 2.0 ** -149
+    # a scale of 2^e puts each block's maximum on the grid's top: the grid's own points and midpoints
+    x = torch.cat([torch.stack(rows), special])
+    x[:, 0::32] = torch.where(x[:, 0::32].abs() < x[:, -1:].abs(), x[:, -1:], x[:, 0::32])
+    q = ops.mx_quantize(x.to(dev), bits)
+    wc, ws = mx.quantize(x, bits)
+    code, scale = _cpu(q)
+    assert torch.equal(scale, ws)
+    fine = (ws != 255).repeat_interleave(32, 1)
+    assert torch.equal(code[fine], wc[fine])
+    back = ops.mx_dequantize(q, torch.float32).cpu().double()
+    torch.testing.assert_close(back, mx.values(wc, ws, bits)[:, :n], rtol=0, atol=0, equal_nan=True)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("activation", ["gelu", "swiglu"])
+@pytest.mark.parametrize("rows,cols,dtype", [(3, 33, torch.float32), (16, 8192, torch.bfloat16),
+                                             (5, 200, torch.float16), (1, 1, torch.bfloat16), (9, 260, torch.float32)])
+def test_activation(dev, rows, cols, dtype, activation, bits):
+    x = _activations(rows, cols * (2 if activation == "swiglu" else 1), 5 * cols, dtype).clamp(-9, 9)
+    want = mx.gelu(x) if activation == "gelu" else mx.swiglu(x)
+    # erfc(z) moves by 2 z^2 of its argument's relative error, z^2 = x^2 / 2; exp(-g) by g
+    tol = 2.0 ** -22 * (8 + x.double()[:, :cols] ** 2) * want.abs()
+    _between(ops.mx_quantize(x.to(dev), bits, activation), want, tol)
+
+
+def test_layouts(dev):
+    """Leading dimensions, strided and unaligned rows, expanded rows, no rows."""
+    wide = _activations(12, 520, 3).to(dev)
+    want = ops.mx_quantize(wide[:, :256].contiguous())
+    for x in (wide[:, :256], torch.cat([wide.new_zeros(1), wide[:, :256].reshape(-1)])[1:].view(12, 256),
+              wide[:, :256].t().contiguous().t(), wide[:, :256].reshape(3, 4, 256)):
+        q = ops.mx_quantize(x)
+        assert q.shape == tuple(x.shape) and torch.equal(q.codes, want.codes) and torch.equal(q.scales, want.scales)
+    odd = ops.mx_quantize(wide[:, 3:260])
+    assert torch.equal(_cpu(odd)[0], mx.quantize(wide[:, 3:260].cpu(), 8)[0])
+    one = ops.mx_quantize(wide[:1, :256].expand(12, 256))
+    assert torch.equal(one.codes, want.codes[:1].expand(12, -1))
+    empty = ops.mx_quantize(wide[:0])
+    assert empty.rows == 0 and ops.mx_dequantize(empty).shape == (0, 520)
+    assert ops.mx_linear(empty, ops.mx_quantize(wide, 4)).shape == (0, 12)
+    assert ops.mx_quantize(wide[0]).shape == (520,)
+
+
+def _x_of(kind, x):
+    """What the product is given and the float64 values that it stands for."""
+    if kind == "bf16":
+        return x, mx.values(*mx.quantize(x.cpu(), 8), 8)
+    q = ops.mx_quantize(x, kind)
+    return q, mx.values(*_cpu(q), kind)
+
+
+def _check_product(got, xv, wv, bias):
+    ref = xv @ wv.T + (0 if bias is None else bias.cpu().double())
+    total = xv.abs() @ wv.abs().T + (0 if bias is None else bias.cpu().double().abs())
+    err = (got.cpu().double() - ref).abs()
+    bad = err > 2.0 ** -8 * ref.abs() + 2.0 ** -15 * total
+    assert not bad.any(), f"{int(bad.sum())} results off, by up to {(err / total)[bad].max():.2e} of the absolute sum"
+
+
+@pytest.mark.parametrize("kind", ["bf16", 8, 4])
+@pytest.mark.parametrize("rows,n,k", [
+    (1, 1, 1), (1, 17, 32), (3, 15, 33), (16, 16, 128), (17, 33, 160), (16, 300, 2048), (31, 257, 129), (32, 64, 1000),
+    (33, 100, 4096), (64, 130, 640), (65, 127, 256), (100, 1000, 384), (128, 128, 512), (129, 300, 2048),
+    (255, 257, 1152), (256, 512, 1024), (300, 513, 896), (600, 260, 130), (1, 5000, 2048), (16, 9000, 512)])
+def test_linear(dev, rows, n, k, kind):
+    print(f"mx_linear rows={rows} n={n} k={k} x={kind}", flush=True)
+    x = _activations(rows, k, rows + n + k).to(dev)
+    w = ops.mx_quantize(torch.randn(n, k, generator=gen(n)).to(dev) / k ** 0.5, 4)
+    bias = torch.randn(n, generator=gen(k)).bfloat16().to(dev) if (rows + n) % 2 else None
+    given, xv = _x_of(kind, x)
+    got = ops.mx_linear(given, w, bias)
+    assert got.shape == (rows, n) and got.dtype == torch.bfloat16
+    _check_product(got, xv, mx.values(*_cpu(w), 4), bias)
+
+
+@pytest.mark.parametrize("kind", ["bf16", 8, 4])
+@pytest.mark.parametrize("rows", [2, 40, 300])
+def test_linear_layouts(dev, rows, kind):
+    """Leading dimensions, a strided x and out, an out that already holds values around it."""
+    n, k = 100, 300
+    base = _activations(rows, k + 20, 7).to(dev)
+    w = ops.mx_quantize(torch.randn(n, k, generator=gen(1)).to(dev), 4)
+    x = base[:, 5:5 + k]
+    given = x if kind == "bf16" else ops.mx_quantize(x, kind)
+    want = ops.mx_linear(x.contiguous() if kind == "bf16" else given, w)
+    buf = torch.full((rows, n + 9), 7.0, dtype=torch.bfloat16, device=dev)
+    got = ops.mx_linear(given, w, out=buf[:, 3:3 + n])
+    assert got.data_ptr() == buf[:, 3:].data_ptr() and torch.equal(got, want)
+    assert (buf[:, :3] == 7).all() and (buf[:, 3 + n:] == 7).all()
+    lead = given.view(2, rows // 2) if kind != "bf16" else x.reshape(2, rows // 2, k)
+    assert torch.equal(ops.mx_linear(lead, w).view(rows, n), want)
+    # rows of a wider code buffer, and a weight cut out of a larger one
+    if kind != "bf16":
+        wider = torch.zeros(rows, given.codes.shape[1] + 48, dtype=torch.uint8, device=dev)
+        wider[:, 16:16 + given.codes.shape[1]] = given.codes
+        cut = ops.MX(wider[:, 16:16 + given.codes.shape[1]], given.scales, given.bits, given.shape)
+        assert torch.equal(ops.mx_linear(cut, w), want)
+    part = ops.MX(w.codes[30:90], w.scales[30:90], 4, (60, k))
+    assert torch.equal(ops.mx_linear(given, part), want[:, 30:90])
+
+
+@pytest.mark.parametrize("kind", ["bf16", 8, 4])
+@pytest.mark.parametrize("rows", [3, 70, 260])
+def test_linear_not_finite(dev, rows, kind):
+    """A block with an infinity or a NaN makes its row's (or column's) results NaN and no others."""
+    n, k = 90, 416
+    x, wv = _activations(rows, k, 1), torch.randn(n, k, generator=gen(2))
+    x[1, 77], x[2, 3] = float("nan"), float("inf")
+    wv[5, 400], wv[89, 0] = -float("inf"), float("nan")
+    w = ops.mx_quantize(wv.to(dev), 4)
+    given, xv = _x_of(kind, x.to(dev))
+    got = ops.mx_linear(given, w).cpu()
+    bad = torch.isnan(xv).any(1)[:, None] | torch.isnan(mx.values(*_cpu(w), 4)).any(1)[None]
+    assert torch.equal(torch.isnan(got), bad) and bad[:3].float().sum() == n * 2 + 2
+
+
+@pytest.mark.parametrize("kind", ["bf16", 8])
+def test_linear_extreme_scales(dev, kind):
+    """Rows of 2^100 and 2^-100 beside each other: products stay finite where the result is."""
+    rows, n, k = 20, 40, 256
+    x = torch.randn(rows, k, generator=gen(1)) * 2.0 ** torch.linspace(-100, 100, rows)[:, None]
+    w = ops.mx_quantize((torch.randn(n, k, generator=gen(2)) * 2.0 ** -20).to(dev), 4)
+    given, xv = _x_of(kind, x.bfloat16().to(dev))
+    _check_product(ops.mx_linear(given, w), xv, mx.values(*_cpu(w), 4), None)
+
+
+NORM_SIZES = [(1, 1), (5, 33), (3, 129), (16, 512), (33, 2048), (7, 2056), (2, 4100), (9, 8192), (2, 16384)]
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("with_residual", [False, True])
+@pytest.mark.parametrize("rows,cols", NORM_SIZES)
+def test_rms_norm(dev, rows, cols, with_residual, bits):
+    print(f"rms_norm_mx {rows} x {cols} residual={with_residual} bits={bits}", flush=True)
+    g = gen(rows + cols)
+    x, w = _activations(rows, cols, cols), 0.5 + torch.rand(cols, generator=g)
+    res = torch.randn(rows, cols, generator=g).bfloat16() if with_residual else None
+    stream, q = ops.rms_norm_mx(x.to(dev), w.to(dev), 1e-6, None if res is None else res.to(dev))
+    if bits == 4:
+        q = ops.rms_norm_mx(x.to(dev), w.to(dev), 1e-6, None if res is None else res.to(dev), bits=4)[1]
+    s, want = mx.rms_norm(x, res, w, 1e-6)
+    # a thread's 64 squares and the join of 256 threads: 76 roundings of positive terms, half of
+    # it by the root; the sum s, the root and two products
+    tol = want.abs() * (38 + 8) * 2.0 ** -24
+    if res is not None:
+        tol = tol + 2.0 ** -24 * (x.double().abs() + res.double().abs()) * (want / s).abs().nan_to_num(0, 0, 0)
+        assert ((stream.cpu().double() - s).abs() <= 2.0 ** -8 * s.abs() + 2.0 ** -24 * s.abs()).all()
+    else:
+        assert stream is None
+    _between(q, want, tol)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("part", ["norm", "residual", "per_row", "shared"])
+@pytest.mark.parametrize("rows,cols", NORM_SIZES)
+def test_adaln(dev, rows, cols, part, bits):
+    print(f"adaln_residual_mx {rows} x {cols} {part} bits={bits}", flush=True)
+    g = gen(rows + cols)
+    x = (_activations(rows, cols, cols) + 0.25)
+    y = torch.randn(rows, cols, generator=g).bfloat16()
+    gate, scale, shift = (0.3 * torch.randn(3, cols, generator=g)).bfloat16().unbind(0)
+    gr = gate
+    if part == "per_row":
+        gate = torch.randn(rows, generator=g).bfloat16()
+        gr = gate[:, None]
+    if part == "shared":
+        x = x[0]
+    given_y = None if part == "norm" else y
+    stream, q = ops.adaln_residual_mx(x.to(dev), None if given_y is None else y.to(dev), gate.to(dev),
+                                      (scale.to(dev), shift.to(dev)), 1e-6, gate_per_row=part == "per_row", bits=bits)
+    xs = x.expand(rows, cols) if part == "shared" else x
+    s, want = mx.adaln(xs, given_y, gr, scale, shift, 1e-6)
+    err_s = 2.0 ** -24 * s.abs()  # the fused multiply-add's rounding
+    if given_y is not None:
+        assert ((stream.cpu().double() - s).abs() <= 2.0 ** -8 * s.abs() + err_s).all()
+    # the mean of a thread's 64 values and the join of 256 threads: 76 roundings of the absolute
+    # sum; the centred value takes its error and its own, the root half of 80 roundings
+    mean_err = 76 * 2.0 ** -24 * s.abs().mean(-1, keepdim=True)
+    c = (s - s.mean(-1, keepdim=True)).abs()
+    rstd = 1 / torch.sqrt((c * c).mean(-1, keepdim=True) + 1e-6)
+    centre = err_s + mean_err + 2.0 ** -24 * c
+    root = 44 * 2.0 ** -24 + (centre * c + centre ** 2).mean(-1, keepdim=True) * rstd ** 2
+    one = (1 + scale.double()).abs()
+    tol = one * rstd * (centre + c * (root + 4 * 2.0 ** -24)) + 2.0 ** -24 * want.abs()
+    _between(q, want, tol)
+
+
+def test_norms_in_place_and_strided(dev):
+    rows, cols = 12, 264
+    wide = _activations(rows, cols + 33, 4).to(dev)
+    x, y = wide[:, 1:1 + cols], torch.randn(rows, cols, generator=gen(1)).bfloat16().to(dev)
+    v = [t.to(dev) for t in (0.3 * torch.randn(3, cols, generator=gen(2))).bfloat16().unbind(0)]
+    w = torch.rand(cols, generator=gen(3)).to(dev)
+    for call in (lambda a, o: ops.rms_norm_mx(a, w, 1e-5, y, x_out=o),
+                 lambda a, o: ops.adaln_residual_mx(a, y, v[0], (v[1], v[2]), 1e-5, x_out=o)):
+        stream, q = call(x.contiguous(), None)
+        s2, q2 = call(x, None)  # rows at odd addresses
+        assert torch.equal(s2, stream) and torch.equal(q2.codes, q.codes) and torch.equal(q2.scales, q.scales)
+        held = wide.clone()
+        s3, q3 = call(held[:, 1:1 + cols], held[:, 1:1 + cols])
+        assert s3.data_ptr() == held[:, 1:].data_ptr() and torch.equal(s3, stream) and torch.equal(q3.codes, q.codes)
+        assert torch.equal(held[:, 0], wide[:, 0]) and torch.equal(held[:, 1 + cols:], wide[:, 1 + cols:])
+
+
+def test_norm_rows_that_are_not_finite(dev):
+    """A NaN or an infinity in a row makes that row NaN and leaves the others."""
+    x = torch.randn(5, 200, generator=gen(1)).bfloat16()
+    x[1, 3], x[3, 190] = float("nan"), float("inf")
+    v = torch.zeros(200).bfloat16().to(dev)
+    for q in (ops.rms_norm_mx(x.to(dev), torch.ones(200, device=dev), 1e-6)[1],
+              ops.adaln_residual_mx(x.to(dev), None, None, (v, v), 1e-6)[1]):
+        bad = torch.isnan(ops.mx_dequantize(q)).cpu()
+        assert bad[1].all() and bad[[0, 2, 4]].sum() == 0
+        # an infinite sum of squares: the finite values' quotients are 0, the infinity's NaN
+        assert bad[3, 190] and (bad[3].all() or not bad[3, :160].any())
+
+
+def test_two_streams_and_a_graph(dev):
+    """Calls on a stream of their own, two captured graphs side by side, replays with eager work
+    between them."""
+    n, k = 300, 1000
+    w = ops.mx_quantize(torch.randn(n, k, generator=gen(1)).to(dev), 4)
+    xs = [_activations(r, k, r).to(dev) for r in (16, 200)]
+    want = [ops.mx_linear(x, w) for x in xs]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = [ops.mx_linear(x, w) for x in xs]
+    torch.cuda.current_stream().wait_stream(stream)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graphs, outs = [], []
+    for x in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(ops.mx_linear(x, w))
+        graphs.append(g)
+    for _ in range(3):
+        for x in xs:
+            x.mul_(-0.5)
+        for g in graphs:
+            g.replay()
+        again = [ops.mx_linear(x, w) for x in xs]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, again))
+
+
+def test_mlp_of_a_layer(dev):
+    """The operators in a row, as a layer's last sublayer runs them: each step against float64
+    on what the step before it gave."""
+    rows, dim, hidden = 48, 256, 800
+    g = gen(11)
+    x, y = _activations(rows, dim, 1).to(dev), torch.randn(rows, dim, generator=g).bfloat16().to(dev)
+    gate, scale, shift = (t.to(dev) for t in (0.3 * torch.randn(3, dim, generator=g)).bfloat16().unbind(0))
+    fc1 = ops.mx_quantize((torch.randn(hidden, dim, generator=g) / 16).to(dev), 4)
+    fc2 = ops.mx_quantize((torch.randn(dim, hidden, generator=g) / 28).to(dev), 4)
+    b1 = torch.randn(hidden, generator=g).bfloat16().to(dev)
+    stream, h = ops.adaln_residual_mx(x, y, gate, (scale, shift), 1e-6)
+    up = ops.mx_linear(h, fc1, b1)
+    mid = ops.mx_quantize(up, activation="gelu")
+    out = ops.mx_linear(mid, fc2)
+    _check_product(up, mx.values(*_cpu(h), 8), mx.values(*_cpu(fc1), 4), b1)
+    want = mx.gelu(up.cpu())
+    _between(mid, want, 2.0 ** -22 * (8 + up.cpu().double() ** 2) * want.abs())
+    _check_product(out, mx.values(*_cpu(mid), 8), mx.values(*_cpu(fc2), 4), None)
+    s, norm = mx.adaln(*(t.cpu() for t in (x, y, gate, scale, shift)), 1e-6)
+    # end to end: e4m3 activations (2^-4 each at most) in front of both products
+    ref = mx.gelu(norm @ mx.values(*_cpu(fc1), 4)[:, :dim].T + b1.cpu().double())
+    ref = ref @ mx.values(*_cpu(fc2), 4)[:, :hidden].T
+    assert float((out.cpu().double() - ref).norm() / ref.norm()) < 2.0 ** -4
+    assert stream.shape == x.shape
+
+
+def test_rows_far_into_memory(dev):
+    """Weights and outputs whose last rows lie past 2^32 bytes and 2^32 values."""
+    n, k = (1 << 20) + 100, 8200
+    pad = -(-k // 128) * 128
+    seeded = torch.Generator(dev).manual_seed(1)
+    codes = torch.randint(0, 256, (n, pad // 2), dtype=torch.uint8, device=dev, generator=seeded)
+    codes[:, k // 2:] = 0
+    scales = torch.randint(120, 130, (n, pad // 32), dtype=torch.uint8, device=dev)
+    assert codes.numel() > 1 << 32
+    w = ops.MX(codes, scales, 4, (n, k))
+    last = ops.MX(codes[-200:], scales[-200:], 4, (200, k))
+    for rows in (1, 20, 300):
+        x = ops.mx_quantize(_activations(rows, k, rows).to(dev))
+        part = ops.mx_linear(x, last)
+        _check_product(part, mx.values(*_cpu(x), 8), mx.values(*_cpu(last), 4), None)
+        assert torch.equal(ops.mx_linear(x, w)[:, -200:], part)
+    # 4-bit rows as the many: x's rows far into memory too
+    few = ops.MX(codes[:40], scales[:40], 4, (40, k))
+    _check_product(ops.mx_linear(w, few)[-200:], mx.values(*_cpu(last), 4), mx.values(*_cpu(few), 4), None)
+    back = ops.mx_dequantize(w)
+    assert back.numel() > 1 << 32
+    want = mx.values(mx.unpack(codes[-3:].cpu(), 4), scales[-3:].cpu(), 4)[:, :k]
+    assert torch.equal(back[-3:].cpu().double(), want)
+    again = ops.mx_quantize(back[-1000:], 8)
+    assert torch.equal(ops.mx_dequantize(again), back[-1000:])  # e2m1 values are e4m3 values
+    far = ops.mx_quantize(back, 8)
+    assert torch.equal(far.codes[-1000:], again.codes) and torch.equal(far.scales[-1000:], again.scales)
