@@ -10,6 +10,7 @@ call raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from dataclasses import dataclass
 
@@ -1317,6 +1318,7 @@ MX_BLOCK = 32  # values that share a scale
 MX_PAD = 128  # stored rows hold a multiple of this many values
 MX_MAX = 1 << 26  # rows, columns
 MX_NORM_COLS = 16384
+MX_BF16_ROWS = 16  # bf16 rows that the product's kernel quantizes itself
 _ACTIVATIONS = {None: 0, "gelu": 1, "swiglu": 2}
 
 
@@ -1386,7 +1388,8 @@ def _mx_bytes(t: torch.Tensor, unit: int) -> tuple[torch.Tensor, int]:
     """``t`` as byte rows aligned to ``unit`` that do not overlap (a copy if needed), and their
     stride (a lone row's is whatever its tensor was cut from; the kernels never step by it)."""
     rows, width = t.shape
-    if t.data_ptr() % unit or t.stride(1) != 1 or (rows > 1 and (t.stride(0) % unit or t.stride(0) < width)):
+    stride = t.stride(0)
+    if t.data_ptr() % unit or t.stride(1) != 1 or (rows > 1 and (stride % unit or not width <= stride < 1 << 24)):
         t = t.clone(memory_format=torch.contiguous_format)
     return t, t.stride(0) if rows > 1 else width
 
@@ -1475,6 +1478,11 @@ def mx_dequantize(q: MX, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     return out
 
 
+@functools.lru_cache(maxsize=4096)
+def _mx_workspace_bytes(rows: int, n: int, k: int, x_bits: int) -> int:
+    return int(_native.lib().fm_mx_linear_workspace_bytes(rows, n, k, x_bits))
+
+
 def mx_linear(x: torch.Tensor | MX, weight: MX, bias: torch.Tensor | None = None,
               out: torch.Tensor | None = None) -> torch.Tensor:
     """``x weight^T + bias`` for ``weight (n, k)`` in microscaled 4 bits, on the block-scaled
@@ -1499,7 +1507,13 @@ def mx_linear(x: torch.Tensor | MX, weight: MX, bias: torch.Tensor | None = None
             raise TypeError(f"x must be bfloat16 or microscaled, got {x.dtype}")
         _no_gradient("mx_linear", x, bias)
         held, stride = _plain_rows(x, k, "x")
-        rows, x_bits, xa = held.shape[0], 16, [held.data_ptr(), stride, None, 0]
+        rows = held.shape[0]
+        if rows <= MX_BF16_ROWS and k % 8 == 0 and stride % 8 == 0 and held.data_ptr() % 16 == 0:
+            x_bits, xa = 16, [held.data_ptr(), stride, None, 0]
+        else:
+            q = mx_quantize(held)
+            x_bits, held = 8, _mx_args(q, "x")
+            xa = _mx_ptrs(held)
     if bias is not None:
         if bias.dtype is not torch.bfloat16 or tuple(bias.shape) != (n,):
             raise ValueError(f"bias must be bfloat16 ({n},), got {bias.dtype} {tuple(bias.shape)}")
@@ -1511,7 +1525,7 @@ def mx_linear(x: torch.Tensor | MX, weight: MX, bias: torch.Tensor | None = None
     else:
         out, out_rows, stride = _bf16_out(out, (*lead, n), device, "out")
     if rows and n:
-        nbytes = int(_native.lib().fm_mx_linear_workspace_bytes(rows, n, k, x_bits))
+        nbytes = _mx_workspace_bytes(rows, n, k, x_bits)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         _mx_call("fm_mx_linear", device, xa[0], x_bits, xa[1], xa[2], xa[3], *_mx_ptrs(w), _ptr(bias),
                  out_rows.data_ptr(), stride, rows, n, k, _ptr(ws), nbytes, _stream(out))

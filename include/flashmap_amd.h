@@ -503,10 +503,13 @@ int fm_mx_dequantize(const void *codes, int64_t codes_stride, const void *scales
                      int32_t bits, void *out, int32_t dtype, int64_t out_stride, int64_t rows, int64_t cols,
                      void *stream);
 /* out (rows, n) bf16 = x w^T (+ bias (n,) bf16 or NULL), accumulated in fp32 and rounded once.
- * w: 4-bit rows (n, k). x_bits 8 or 4: x holds codes, x_scales its scales; x_bits 16: x is
- * bf16 (rows, k), quantized to 8 bits in the call (x_scales is not read). rows, n and k at
- * most 2^26. The workspace (16-byte aligned) holds fm_mx_linear_workspace_bytes(rows, n, k,
- * x_bits) bytes; concurrent calls must not share it. */
+ * w: 4-bit rows (n, k). x_bits 8 or 4: x holds codes, x_scales its scales. x_bits 16: x is
+ * bf16 (rows, k) and the kernel quantizes it to 8 bits as fm_mx_quantize does (x_scales is not
+ * read): at most 16 rows, 16-byte aligned with a stride of a multiple of 8 values, k a
+ * multiple of 8; others call fm_mx_quantize first. rows and n at most 2^26, k at most 2^22,
+ * strides of codes and scales below 2^24 bytes. The workspace (16-byte aligned) holds
+ * fm_mx_linear_workspace_bytes(rows, n, k, x_bits) bytes (0: none is needed); concurrent calls
+ * must not share it. */
 size_t fm_mx_linear_workspace_bytes(int64_t rows, int64_t n, int64_t k, int32_t x_bits);
 int fm_mx_linear(const void *x, int32_t x_bits, int64_t x_stride, const void *x_scales, int64_t x_scales_stride,
                  const void *w, int64_t w_stride, const void *w_scales, int64_t w_scales_stride, const void *bias,

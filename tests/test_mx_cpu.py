@@ -41,8 +41,7 @@ def test_sizes(cols, pad):
             q.view(2, 2)
         with pytest.raises(TypeError, match="bytes"):
             q.to(BF)
-    assert _native.lib().fm_mx_linear_workspace_bytes(3, 5, cols, 16) == 3 * (pad + pad // 32)
-    assert _native.lib().fm_mx_linear_workspace_bytes(0, 5, cols, 16) == 0
+    assert _native.lib().fm_mx_linear_workspace_bytes(0, 5, cols, 8) == 0
 
 
 def test_quantize_refuses(host):
@@ -177,8 +176,13 @@ def test_entries_refuse_what_they_cannot_launch():
     _fails("x: 16-byte", inv, *lin(xsc=None))
     _fails("out rows", inv, *lin(os=7))
     _fails("at most 2\\^26", unsup, *lin(n=(1 << 26) + 1, os=1 << 27))
-    _fails("workspace", _native.FM_ERR_WORKSPACE, *lin(xb=16, xs=64))
-    _fails("workspace", _native.FM_ERR_WORKSPACE, *lin(xb=16, xs=64, wk=at, wb=4 * 132 - 1))
+    _fails("at most 2\\^22", unsup, *lin(k=(1 << 22) + 1))
+    _fails("below 2\\^24", inv, *lin(xs=1 << 24))
+    _fails("below 2\\^24", inv, *lin(ws=1 << 24))
+    _fails("at most 16 rows", unsup, *lin(xb=16, xs=64, rows=17))
+    _fails("multiple of 8", unsup, *lin(xb=16, xs=64, k=63))
+    _fails("bf16 x", inv, *lin(xb=16, xs=60, k=56))
+    _fails("bf16 x", inv, *lin(xb=16, xs=64, x=at + 8))
     assert _native.call(*lin(x=None, rows=0)) is None
     f = ctypes.c_float(1e-6)
     _fails("at most 16384", unsup, "fm_rms_norm_mx", at, 64, None, 0, at, f, None, 0, 8, at, 128, at, 4, 4, 16385, None)
