@@ -8,10 +8,11 @@
 //   e2m1  16 bytes, the codes of k = 32 g .. 32 g + 31
 //   e4m3  32 bytes, the codes of k = 16 g .. 16 g + 15 and of k = 64 + 16 g .. 64 + 16 g + 15
 //   scale one byte, that of row r's block k = 32 g .. 32 g + 31, for either format
-// (checked lane by lane against the formula). Sums of e2m1 products are exact until they pass
-// 24 bits; with an e4m3 operand the instruction aligns a step's 128 products to the largest
-// of them and drops what lies about 2^-17 below it (measured, sums of 128 to 65536 products:
-// 4e-6 to 9e-6 of the result; the rounding to bf16 is 2^-9 on average).
+// (checked lane by lane against the formula). Its sums, probed with single products: groups of
+// 8 products are aligned to the group's largest, cut below 2^-13 of its power of two (an e2m1
+// product spans less and is exact), and the groups and steps added as floats. With an e4m3
+// operand that costs 4e-6 to 9e-6 of a result (hidden states with outlying channels, sums of
+// 128 to 65536 products), against 2^-9 for its rounding to bf16 and 2^-5 for the operand's own.
 //
 // Rows are padded with zeros to multiples of 128 values, so the loops over k have no tail.
 #include <stdint.h>
@@ -34,6 +35,8 @@ struct MxLinearArgs {
   int32_t n;
   int32_t k, steps;  // steps: of 128 along k
   int32_t vec_out;  // rows of out may be written 16 bytes at a time
+  float *part;  // NULL, or the sums of a part of k: (parts, rows, part_stride) fp32
+  int64_t part_stride;
 };
 
 // D(16x16 f32) += A(16x128 e2m1) * B(128x16 e4m3 or e2m1), block scales in byte 0 of sa, sb.
@@ -45,6 +48,12 @@ __device__ __forceinline__ f32x4_t mfma_mx(const i32x8_t &a, const i32x8_t &b, f
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 4, 0, sa, 0, sb);
 }
 
+// The same with the scales in byte OP.
+template <int XBITS, int OP>
+__device__ __forceinline__ f32x4_t mfma_mx_op(const i32x8_t &a, const i32x8_t &b, f32x4_t c, int sa, int sb) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, XBITS == 8 ? 0 : 4, OP, sa, OP, sb);
+}
+
 __device__ __forceinline__ i32x8_t operand(u32x4_t lo) {
   return i32x8_t{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], 0, 0, 0, 0};
 }
@@ -52,7 +61,42 @@ __device__ __forceinline__ i32x8_t operand(u32x4_t lo, u32x4_t hi) {
   return i32x8_t{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
 }
 
-// -------------------------------------------------------------------- few rows: streaming
+// ------------------------------------------------------------------------- loads into LDS
+
+// One 16-byte-per-lane load straight into LDS: lane l's bytes go to lds + 16 l. Inline asm, so
+// that the compiler, which cannot tell the stages apart, does not wait for the loads in
+// flight before every LDS read; the waits are counted by hand (wait_vm before the barrier
+// that publishes a stage).
+typedef __attribute__((address_space(3))) char lds_char_t;
+__device__ __forceinline__ void dma16(const uint8_t *base, uint32_t offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(lds), "v"(offset), "s"(base)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void dma4(const uint8_t *base, uint32_t offset, uint32_t lds) {  // 4 bytes a lane
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
+               :
+               : "s"(lds), "v"(offset), "s"(base)
+               : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  static_assert(N >= 0 && N < 64, "vmcnt holds 6 bits");
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+
+// Where a row's 16-byte pieces lie in LDS. A load's neighbouring lanes take a row's neighbouring
+// pieces (whole 64- or 128-byte segments: with a row a lane every lane's 16 bytes are a request
+// of their own), so a stage holds rows of 4 or 8 pieces, piece c of row r at place c ^ swizzle(r).
+// ds_read_b128 serves 16 lanes at a time, and not neighbours: lanes 0-3, 12-15, 20-23, 24-27,
+// then the other 16 of the lower half, then the upper half alike (measured by which lanes'
+// conflicts add up). The 16 rows of an operand read are then all different, half of them one
+// piece on; with these places they fall on all 64 banks.
+__device__ __forceinline__ int swizzle4(int r) { return r >> 3 ? 3 : 0; }
+__device__ __forceinline__ int swizzle8(int r) { return r >> 1 ^ ((r >> 2 ^ r >> 3) & 1); }
+
+// ------------------------------------------------------------- few rows: the reduction split
 
 // 128 values of 16 rows in bf16 (lane (r, g): k = 16 g .. 16 g + 15 in v[0], v[1] and 64 + 16 g
 // .. in v[2], v[3]) as the 8-bit operand and its scale, bit for bit what fm_mx_quantize
@@ -210,24 +254,167 @@ static int launch_rows(const MxLinearArgs &a, hipStream_t stream) {
   return FM_OK;
 }
 
-// ------------------------------------------------------------------------ many rows: tiles
+// ----------------------------------------------------------- few rows, many columns: streams
 
-// One 16-byte-per-lane load straight into LDS: lane l's bytes go to lds + 16 l. Inline asm, so
-// that the compiler, which cannot tell the stages apart, does not wait for the loads in
-// flight before every LDS read; the waits are counted by hand (wait_vm before the barrier
-// that publishes a stage).
-typedef __attribute__((address_space(3))) char lds_char_t;
-__device__ __forceinline__ void dma16(const uint8_t *base, uint32_t offset, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-               :
-               : "s"(lds), "v"(offset), "s"(base)
-               : "memory", "m0");
+// Weights larger than what is in flight at once (a head over the vocabulary): a wavefront
+// streams whole 16-row blocks of W through a ring of its own in LDS, D groups of four steps
+// deep, and needs nobody: x, up to 16 MB rows of it, lies in LDS for the workgroup's whole
+// life, quantized once. A group: 16 rows of 256 bytes, as four loads of eight 128-byte
+// segments, and their scales, 16 bytes a row.
+template <int XBITS, int MB, int WAVES, int D>
+struct Stream {
+  static constexpr int GROUP = 4096 + 256, RING = D * GROUP;
+  static constexpr int XSTEP = MB * 16 * (XBITS == 4 ? 64 : 128);  // bytes of a step of x
+  static size_t lds(int32_t steps) { return WAVES * RING + (size_t)steps * XSTEP + (size_t)((steps + 3) / 4) * MB * 256; }
+};
+
+template <int XBITS, int MB, int WAVES, int D>
+__global__ __launch_bounds__(64 * WAVES) void mx_linear_stream_kernel(const MxLinearArgs a) {
+  using T = Stream<XBITS, MB, WAVES, D>;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int lane = threadIdx.x & 63, wave = wave_id();
+  const int r = lane & 15, g = lane >> 4;
+  const int at4 = 64 * r + 16 * (g ^ swizzle4(r));
+  const int at8 = 128 * r + 16 * (g ^ swizzle8(r)), at8h = at8 ^ 64;
+  char *const xl = lds + WAVES * T::RING, *const xsl = xl + a.steps * T::XSTEP;
+  for (int32_t s = wave; s < a.steps; s += WAVES) {
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+      const int64_t m = 16 * i + r < a.rows ? 16 * i + r : a.rows - 1;
+      i32x8_t codes;
+      int scale;
+      if constexpr (XBITS == 16) {
+        u32x4_t v[4];
+#pragma unroll
+        for (int l = 0; l < 4; ++l) {
+          const int32_t k = 128 * s + 16 * g + 64 * (l >> 1) + 8 * (l & 1);  // zeros past the row's end
+          v[l] = k < a.k ? load16(a.x + m * a.xs + 2 * (int64_t)k) : u32x4_t{0, 0, 0, 0};
+        }
+        quantize_operand(v, g, codes, scale);
+      } else {
+        const uint8_t *x = a.x + m * a.xs + (XBITS == 8 ? 128 : 64) * (int64_t)s + 16 * g;
+        codes = XBITS == 8 ? operand(load16(x), load16(x + 64)) : operand(load16(x));
+        scale = a.xsc[m * a.xss + 4 * (int64_t)s + g];
+      }
+      char *const to = xl + s * T::XSTEP + i * (T::XSTEP / MB);
+      store16(to + (XBITS == 4 ? at4 : at8), u32x4_t{(uint32_t)codes[0], (uint32_t)codes[1], (uint32_t)codes[2], (uint32_t)codes[3]});
+      if constexpr (XBITS != 4)
+        store16(to + at8h, u32x4_t{(uint32_t)codes[4], (uint32_t)codes[5], (uint32_t)codes[6], (uint32_t)codes[7]});
+      xsl[((s >> 2) * MB + i) * 256 + 16 * r + 4 * g + (s & 3)] = (char)scale;
+    }
+  }
+  __syncthreads();
+
+  const int32_t groups = (a.steps + 3) >> 2, blocks = (a.n + 15) >> 4;
+  const int64_t waves = (int64_t)gridDim.x * WAVES, id = (int64_t)blockIdx.x * WAVES + wave;
+  const int32_t b0 = (int32_t)(blocks * id / waves), b1 = (int32_t)(blocks * (id + 1) / waves);
+  if (b0 == b1) return;
+  const uint32_t ring = (uint32_t)(uintptr_t)(lds_char_t *)lds + wave * T::RING;
+  const int64_t total = (int64_t)(b1 - b0) * groups;
+  // The next group to load: block lb, group lg. Pieces past the row's end repeat its last ones.
+  int32_t lb = b0, lg = 0, lslot = 0;
+  const int32_t wlast = 64 * a.steps - 16, slast = 4 * a.steps - 4;
+  auto issue = [&]() {
+    const uint32_t to = ring + lslot * T::GROUP;
+    const uint8_t *w = a.w + (int64_t)(16 * lb) * a.ws, *sc = a.wsc + (int64_t)(16 * lb) * a.wss;
+    const int32_t last = a.n - 1 - 16 * lb;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int row = 8 * (u & 1) + (lane >> 3), piece = (lane & 7) ^ swizzle8(row);
+      const int32_t at = 256 * lg + 128 * (u >> 1) + 16 * piece;
+      dma16(w, (uint32_t)((row < last ? row : last) * (int32_t)a.ws + (at < wlast ? at : wlast)), to + 1024 * u);
+    }
+    const int row = lane >> 2;
+    const int32_t at = 16 * lg + 4 * (lane & 3);
+    dma4(sc, (uint32_t)((row < last ? row : last) * (int32_t)a.wss + (at < slast ? at : slast)), to + 4096);
+    if (++lg == groups) lg = 0, ++lb;
+    lslot = lslot == D - 1 ? 0 : lslot + 1;
+  };
+#pragma unroll
+  for (int d = 0; d < D; ++d)
+    if (d < total) issue();
+  const uint32_t pick = 0x0400u + 0x0101u * (uint32_t)g;
+  f32x4_t acc[MB];
+#pragma unroll
+  for (int i = 0; i < MB; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  int32_t block = b0, grp = 0, slot = 0;
+  for (int64_t t = 0; t < total; ++t) {
+    // In flight behind this group: up to D - 1 groups, 5 loads each (and results being stored,
+    // which only make the wait longer).
+    if (t + D <= total)
+      wait_vm<5 * (D - 1)>();
+    else
+      wait_vm<0>();
+    const char *wl = lds + wave * T::RING + slot * T::GROUP;
+    const u32x4_t d = *(const u32x4_t *)(wl + 4096 + 16 * r);
+    const uint32_t a01 = __builtin_amdgcn_perm(d[1], d[0], pick), a23 = __builtin_amdgcn_perm(d[3], d[2], pick);
+    const int sw = (int)__builtin_amdgcn_perm(a23, a01, 0x05040100);
+    int sx[MB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i) sx[i] = *(const int *)(xsl + (grp * MB + i) * 256 + 16 * r + 4 * g);
+    auto step = [&](auto jc) {
+      constexpr int J = decltype(jc)::value;
+      const int32_t s = 4 * grp + J;
+      if (s >= a.steps) return;
+      const i32x8_t wf = operand(load16(wl + 2048 * (J >> 1) + (J & 1 ? at8h : at8)));
+      const char *x = xl + s * T::XSTEP;
+#pragma unroll
+      for (int i = 0; i < MB; ++i) {
+        const char *xi = x + i * (T::XSTEP / MB);
+        i32x8_t xf;
+        if constexpr (XBITS == 4)
+          xf = operand(load16(xi + at4));
+        else
+          xf = operand(load16(xi + at8), load16(xi + at8h));
+        acc[i] = mfma_mx_op<XBITS == 4 ? 4 : 8, J>(wf, xf, acc[i], sw, sx[i]);
+      }
+    };
+    step(std::integral_constant<int, 0>{});
+    step(std::integral_constant<int, 1>{});
+    step(std::integral_constant<int, 2>{});
+    step(std::integral_constant<int, 3>{});
+    // The slot has been read (its values are operands by now): the group D on takes it.
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (t + D < total) issue();
+    slot = slot == D - 1 ? 0 : slot + 1;
+    if (++grp == groups) {
+      // Lane: row m of out, columns n .. n + 3.
+      const int32_t n = 16 * block + 4 * g;
+#pragma unroll
+      for (int i = 0; i < MB; ++i) {
+        const int32_t m = 16 * i + r;
+        if (m < a.rows) {
+          uint16_t *dst = a.out + m * a.os + n;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (a.bias != nullptr && n + q < a.n) acc[i][q] += bf16_to_f32(a.bias[n + q]);
+          if (a.vec_out && n + 4 <= a.n) {
+            *reinterpret_cast<u32x2_t *>(dst) = u32x2_t{pack_bf16x2(acc[i][0], acc[i][1]), pack_bf16x2(acc[i][2], acc[i][3])};
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (n + q < a.n) dst[q] = (uint16_t)(pack_bf16x2(acc[i][q], 0.f) & 0xffffu);
+          }
+        }
+        acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      }
+      grp = 0, ++block;
+    }
+  }
 }
-template <int N>
-__device__ __forceinline__ void wait_vm() {
-  static_assert(N >= 0 && N < 64, "vmcnt holds 6 bits");
-  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+
+template <int XBITS, int MB, int WAVES, int D>
+static int launch_stream(const MxLinearArgs &a, hipStream_t stream) {
+  DeviceInfo info;
+  const int rc = device_info(&info);
+  if (rc != FM_OK) return rc;
+  mx_linear_stream_kernel<XBITS, MB, WAVES, D>
+      <<<dim3((unsigned)info.cus), dim3(64 * WAVES), Stream<XBITS, MB, WAVES, D>::lds(a.steps), stream>>>(a);
+  FM_CHECK_HIP(hipGetLastError());
+  return FM_OK;
 }
+
+// ------------------------------------------------------------------------ many rows: tiles
 
 template <int XBITS, int BM, int BN, int WM, int WN>
 struct Tile {
@@ -243,25 +430,10 @@ struct Tile {
   static_assert(SW <= WAVES, "a row a lane");
 };
 
-// Where a row's 16-byte pieces lie in LDS. A load's neighbouring lanes take a row's neighbouring
-// pieces (whole 64- or 128-byte segments: with a row a lane every lane's 16 bytes are a request
-// of their own), so a stage holds rows of 4 or 8 pieces, piece c of row r at place c ^ swizzle(r).
-// ds_read_b128 serves 16 lanes at a time, and not neighbours: lanes 0-3, 12-15, 20-23, 24-27,
-// then the other 16 of the lower half, then the upper half alike (measured by which lanes'
-// conflicts add up). The 16 rows of an operand read are then all different, half of them one
-// piece on; with these places they fall on all 64 banks.
-__device__ __forceinline__ int swizzle4(int r) { return r >> 3 ? 3 : 0; }
-__device__ __forceinline__ int swizzle8(int r) { return r >> 1 ^ ((r >> 2 ^ r >> 3) & 1); }
-
 // The row of W (in its 32-row group pair) that block f holds at index r: lane group g of the
 // accumulators then holds 8 consecutive columns of out in blocks 2 p and 2 p + 1, which are
 // stored 16 bytes at a time, 64 consecutive bytes a row.
 __device__ __forceinline__ int w_row(int f, int r) { return 32 * (f >> 1) + 8 * (r >> 2) + 4 * (f & 1) + (r & 3); }
-
-template <int XBITS, int OP>
-__device__ __forceinline__ f32x4_t mfma_mx_op(const i32x8_t &a, const i32x8_t &b, f32x4_t c, int sa, int sb) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, XBITS == 8 ? 0 : 4, OP, sa, OP, sb);
-}
 
 template <int XBITS, int BM, int BN, int WM, int WN, bool TURNS>
 __global__ __launch_bounds__(64 * WM * WN, 2) void mx_linear_tile_kernel(const MxLinearArgs a,
@@ -287,8 +459,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx_linear_tile_kernel(const M
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_char_t *)lds;
   const uint32_t sc0 = lds0 + T::STAGES * T::STAGE;
   // This wavefront's units: x's first, then W's. Rows past the end read the last one.
-  // Offsets from the tile's first row stay below 2^32 (k is at most 2^22, rows at most 256).
-  const uint8_t *xbase = a.x + m0 * a.xs, *wbase = a.w + (int64_t)n0 * a.ws;
+  // This workgroup's part of k, in whole chunks of four steps.
+  const int32_t chunks_all = (a.steps + 3) >> 2;
+  const int32_t first = 4 * (int32_t)((int64_t)chunks_all * blockIdx.y / gridDim.y);
+  const int32_t end = 4 * (int32_t)((int64_t)chunks_all * (blockIdx.y + 1) / gridDim.y);
+  const int32_t steps = (end < a.steps ? end : a.steps) - first;
+  // Offsets from the tile's first row stay below 2^32 (strides are below 2^24, rows at most 256).
+  const uint8_t *xbase = a.x + m0 * a.xs + (XBITS == 8 ? 128 : 64) * (int64_t)first;
+  const uint8_t *wbase = a.w + (int64_t)n0 * a.ws + 64 * (int64_t)first;
   const int32_t mlast = (int32_t)(a.rows - 1 - m0 < BM ? a.rows - 1 - m0 : BM - 1);
   const int32_t nlast = a.n - 1 - n0 < BN ? a.n - 1 - n0 : BN - 1;
   uint32_t src[T::PER];
@@ -309,10 +487,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx_linear_tile_kernel(const M
   const int at8 = 128 * r + 16 * (g ^ swizzle8(r)), at8h = at8 ^ 64;
   // Four steps' scales of a row at once, x's rows, then W's, 64 rows a wavefront. The last
   // chunk's 16 bytes end with the row: they hold `back` steps of the chunk before it first.
-  const int32_t steps = a.steps, back = -steps & 3;
+  const int32_t back = -steps & 3;
   static_assert(BM % 64 == 0, "a wavefront's rows are all x's or all W's");
   const bool of_x = 64 * wave < BM;
-  const uint8_t *sbase = of_x ? a.xsc + m0 * a.xss : a.wsc + (int64_t)n0 * a.wss;
+  const uint8_t *sbase = (of_x ? a.xsc + m0 * a.xss : a.wsc + (int64_t)n0 * a.wss) + 4 * (int64_t)first;
   uint32_t ssrc;
   {
     const int row = 64 * wave + lane - (of_x ? 0 : BM);
@@ -455,7 +633,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx_linear_tile_kernel(const M
     const int32_t n = n0 + 32 * (wn * (T::NF / 2) + p) + 8 * g;
     float b[8];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) b[q] = a.bias != nullptr && n + q < a.n ? bf16_to_f32(a.bias[n + q]) : 0.f;
+    for (int q = 0; q < 8; ++q) b[q] = a.part == nullptr && a.bias != nullptr && n + q < a.n ? bf16_to_f32(a.bias[n + q]) : 0.f;
 #pragma unroll
     for (int i = 0; i < T::MF; ++i) {
       const int64_t m = m0 + 16 * (wm * T::MF + i) + r;
@@ -463,6 +641,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx_linear_tile_kernel(const M
       float v[8];
 #pragma unroll
       for (int q = 0; q < 4; ++q) v[q] = acc[2 * p][i][q] + b[q], v[4 + q] = acc[2 * p + 1][i][q] + b[4 + q];
+      if (a.part != nullptr) {  // padded to whole groups of 8 columns
+        if (n < a.n) {
+          float *p = a.part + (blockIdx.y * a.rows + m) * a.part_stride + n;
+          *reinterpret_cast<f32x4_t *>(p) = f32x4_t{v[0], v[1], v[2], v[3]};
+          *reinterpret_cast<f32x4_t *>(p + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
+        }
+        continue;
+      }
       uint16_t *dst = a.out + m * a.os + n;
       if (vec && n + 8 <= a.n) {
         store16(dst, u32x4_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
@@ -476,18 +662,50 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx_linear_tile_kernel(const M
   }
 }
 
+// The parts' sums, in their order, plus the bias: 8 columns a thread.
+__global__ __launch_bounds__(256) void mx_linear_join_kernel(const MxLinearArgs a, const int32_t parts, const uint32_t groups) {
+  const uint32_t item = blockIdx.x * 256 + threadIdx.x, m = item / groups;
+  if (m >= a.rows) return;
+  const int32_t n = 8 * (int32_t)(item - m * groups);
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const float *p = a.part + m * a.part_stride + n;
+  for (int32_t z = 0; z < parts; ++z, p += a.rows * a.part_stride) {
+    const f32x4_t lo = *reinterpret_cast<const f32x4_t *>(p), hi = *reinterpret_cast<const f32x4_t *>(p + 4);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] += lo[q], v[4 + q] += hi[q];
+  }
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    if (a.bias != nullptr && n + q < a.n) v[q] += bf16_to_f32(a.bias[n + q]);
+  uint16_t *dst = a.out + m * a.os + n;
+  if (a.vec_out && n + 8 <= a.n) {
+    store16(dst, u32x4_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])});
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (n + q < a.n) dst[q] = (uint16_t)(pack_bf16x2(v[q], 0.f) & 0xffffu);
+  }
+}
+
+// `parts` > 1: a.part holds parts * rows * part_stride floats (rows at most 2^22 / tiles of n).
 template <int XBITS, int BM, int BN, int WM, int WN, bool TURNS>
-static int launch_tiles(const MxLinearArgs &a, hipStream_t stream) {
+static int launch_tiles(const MxLinearArgs &a, int32_t parts, hipStream_t stream) {
   const int64_t tm = (a.rows + BM - 1) / BM, tn = ((int64_t)a.n + BN - 1) / BN;
   // At most 2^22 workgroups a launch: slices of whole groups of row tiles.
   const int64_t most = (1 << 22) / tn < 8 ? 8 : (1 << 22) / tn / 8 * 8;
   for (int64_t first = 0; first < tm; first += most) {
-    MxLinearArgs part = a;
+    MxLinearArgs slice = a;
     const int64_t rows = a.rows - first * BM, here = tm - first < most ? tm - first : most;
-    part.x += first * BM * a.xs, part.xsc += first * BM * a.xss, part.out += first * BM * a.os;
-    part.rows = rows < here * BM ? rows : here * BM;
+    slice.x += first * BM * a.xs, slice.xsc += first * BM * a.xss, slice.out += first * BM * a.os;
+    slice.rows = rows < here * BM ? rows : here * BM;
+    if (parts == 1) slice.part = nullptr;
     mx_linear_tile_kernel<XBITS, BM, BN, WM, WN, TURNS>
-        <<<dim3((unsigned)(here * tn)), dim3(64 * WM * WN), 0, stream>>>(part, (int32_t)here, (int32_t)tn);
+        <<<dim3((unsigned)(here * tn), (unsigned)parts), dim3(64 * WM * WN), 0, stream>>>(slice, (int32_t)here, (int32_t)tn);
+    FM_CHECK_HIP(hipGetLastError());
+  }
+  if (parts > 1) {
+    const uint32_t groups = (uint32_t)(a.part_stride / 8);
+    mx_linear_join_kernel<<<dim3((unsigned)((a.rows * groups + 255) / 256)), dim3(256), 0, stream>>>(a, parts, groups);
     FM_CHECK_HIP(hipGetLastError());
   }
   return FM_OK;
@@ -495,10 +713,75 @@ static int launch_tiles(const MxLinearArgs &a, hipStream_t stream) {
 
 static bool aligned(const void *p, int64_t n) { return ((uintptr_t)p % (uintptr_t)n) == 0; }
 
+// Which kernel a product runs on, by its sizes (MI355X: 256 CUs).
+struct MxPlan {
+  enum Kind { ROWS, STREAM, TILES } kind;
+  int bm, bn;     // tiles
+  int32_t parts;  // of k
+};
+
+constexpr size_t LDS_BYTES = 160 * 1024;
+constexpr int STREAM_WAVES = 8, STREAM_GROUPS = 2;
+
+template <int XBITS>
+static bool streams(int32_t steps) {
+  return Stream<XBITS, 1, STREAM_WAVES, STREAM_GROUPS>::lds(steps) <= LDS_BYTES;
+}
+
+// Measured, us, weights from HBM, x in 8 bits (bf16 x: the same order):
+//   16 rows, k 2048:  n 4096  rows 5.2, stream 6.4, tiles 8.1;  n 8192  6.7, 7.1, 8.9
+//                     n 12288 9.6, 7.4, 9.2;  n 151936 54.6, 37.7, 43.7
+//   16 rows, n 2048:  k 4096  rows 7.2, stream 9.5, tiles 9.2;  k 8192 11.7, -, 11.2;  k 20480 27.0, -, 16.0
+//   more rows, tiles of 64 x 64, 64 x 128, 128 x 128 and 256 x 256:
+//     64 x 2048 -> 2048 7.8, 9.4, 12.7, -;  64 x 2048 -> 24576 12.8, 11.6, 14.4, -;  1024 x 8192 -> 2048 29.1, 28.4, 43, 76
+//     1024 x 2048 -> 8192 27.1, 24.2, 21.4, 29;  512 x 8192 -> 8192 -, 49.8, 46.3, 79;  4096 x 2048 -> 4096 53, 45, 38, 34.5
+//     300 x 2048 -> 151936 (a last row tile of 44) -, 136, 137, 168
+//   k in parts of at least 2048 values, tiles of 64 x 64: 64 x 8192 -> 2048 1 part 29, 2 14.7, 4 11.9, 8 11.9;
+//     64 x 20480 -> 2048 4 parts 22, 8 16.5, 16 19.1;  64 x 2048 -> 2048 1 part 7.8, 4 8.8
+static MxPlan plan_of(int64_t rows, int64_t n, int64_t k, int32_t x_bits) {
+  const int32_t steps = (int32_t)(mx_padded(k) / MX_PAD);
+  if (rows <= 16) {
+    const bool fits = x_bits == 4 ? streams<4>(steps) : streams<8>(steps);
+    if (n > 8192 && fits) return {MxPlan::STREAM, 0, 0, 1};
+    if (x_bits == 16 || (k < 8192 && n <= 8192)) return {MxPlan::ROWS, 0, 0, 1};
+  }
+  // A tile size is worth taking if it fills the chip and its last row tile is not mostly air.
+  auto fills = [&](int64_t bm, int64_t bn, int64_t least, double full) {
+    const int64_t tiles = ((rows + bm - 1) / bm) * ((n + bn - 1) / bn);
+    return tiles >= least && (double)(rows * n) >= full * (double)(tiles * bm * bn);
+  };
+  if (fills(256, 256, 192, 0.8)) return {MxPlan::TILES, 256, 256, 1};
+  if (fills(128, 128, 256, 0.75)) return {MxPlan::TILES, 128, 128, 1};
+  if (fills(64, 128, 192, 0.0)) return {MxPlan::TILES, 64, 128, 1};
+  const int64_t tiles = ((rows + 63) / 64) * ((n + 63) / 64);
+  int64_t parts = steps / 16 < 512 / tiles ? steps / 16 : 512 / tiles;
+  parts = parts > 8 ? 8 : parts < 1 ? 1 : parts;
+  return {MxPlan::TILES, 64, 64, (int32_t)parts};
+}
+
+static int64_t part_stride(int64_t n) { return (n + 7) / 8 * 8; }
+
+template <int XBITS>
+static int run_plan(const MxPlan &plan, const MxLinearArgs &a, hipStream_t stream) {
+  if (plan.kind == MxPlan::STREAM) return launch_stream<XBITS, 1, STREAM_WAVES, STREAM_GROUPS>(a, stream);
+  if (plan.kind == MxPlan::ROWS)
+    return a.n <= 4096 ? launch_rows<XBITS, 1, 1, 8>(a, stream) : launch_rows<XBITS, 1, 2, 8>(a, stream);
+  if constexpr (XBITS != 16) {
+    if (plan.bm == 256) return launch_tiles<XBITS, 256, 256, 4, 2, true>(a, 1, stream);
+    if (plan.bm == 128) return launch_tiles<XBITS, 128, 128, 2, 2, false>(a, 1, stream);
+    if (plan.bn == 128) return launch_tiles<XBITS, 64, 128, 1, 4, false>(a, 1, stream);
+    return launch_tiles<XBITS, 64, 64, 2, 2, false>(a, plan.parts, stream);
+  }
+  return fail(FM_ERR_UNSUPPORTED, "bf16 x of more than %d rows", MX_BF16_ROWS);
+}
+
 }  // namespace fm
 
 extern "C" size_t fm_mx_linear_workspace_bytes(int64_t rows, int64_t n, int64_t k, int32_t x_bits) {
-  return 0;
+  using namespace fm;
+  if (rows <= 0 || n <= 0 || k <= 0 || k > 1 << 22 || n > 1 << 26 || rows > 1 << 26) return 0;
+  const MxPlan plan = plan_of(rows, n, k, x_bits);
+  return plan.parts == 1 ? 0 : (size_t)(plan.parts * rows * part_stride(n)) * sizeof(float);
 }
 
 extern "C" int fm_mx_linear(const void *x, int32_t x_bits, int64_t x_stride, const void *x_scales,
@@ -536,30 +819,14 @@ extern "C" int fm_mx_linear(const void *x, int32_t x_bits, int64_t x_stride, con
                "x: 16-byte aligned rows of %lld bytes, 4-byte aligned scales of %lld", (long long)(kp * x_bits / 8),
                (long long)(kp / MX_BLOCK));
   }
+  const MxPlan plan = plan_of(rows, n, k, x_bits);
+  const size_t need = fm_mx_linear_workspace_bytes(rows, n, k, x_bits);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
+    return fail(FM_ERR_WORKSPACE, "workspace of %zu bytes, need %zu (16-byte aligned)", workspace_bytes, need);
   const MxLinearArgs a{(const uint8_t *)x, (const uint8_t *)x_scales, (const uint8_t *)w, (const uint8_t *)w_scales,
                        (const uint16_t *)bias, (uint16_t *)out, x_bits == 16 ? 2 * x_stride : x_stride, x_scales_stride,
                        w_stride, w_scales_stride, out_stride, rows, (int32_t)n, (int32_t)k, (int32_t)(kp / MX_PAD),
-                       aligned(out, 16) && out_stride % 8 == 0};
+                       aligned(out, 16) && out_stride % 8 == 0, (float *)workspace, part_stride(n)};
   const hipStream_t st = (hipStream_t)stream;
-  if (rows > 64) {
-    const bool large = ((rows + 255) / 256) * ((n + 255) / 256) >= 256;
-    if (x_bits == 8) return large ? launch_tiles<8, 256, 256, 4, 2, true>(a, st) : launch_tiles<8, 128, 128, 2, 2, false>(a, st);
-    return large ? launch_tiles<4, 256, 256, 4, 2, true>(a, st) : launch_tiles<4, 128, 128, 2, 2, false>(a, st);
-  }
-  auto few = [&](auto xb) {
-    constexpr int XB = decltype(xb)::value;
-    if (rows <= 16) {
-      if (n <= 16 * 256) return launch_rows<XB, 1, 1, 16>(a, st);
-      if (n <= 64 * 256) return launch_rows<XB, 1, 2, 8>(a, st);
-      return launch_rows<XB, 1, 4, 4>(a, st);
-    }
-    if constexpr (XB != 16) {
-      if (rows <= 32) return launch_rows<XB, 2, 2, 4>(a, st);
-      return launch_rows<XB, 4, 2, 4>(a, st);
-    }
-    return (int)FM_ERR_UNSUPPORTED;
-  };
-  return x_bits == 16 ? few(std::integral_constant<int, 16>{})
-         : x_bits == 8 ? few(std::integral_constant<int, 8>{})
-                       : few(std::integral_constant<int, 4>{});
+  return x_bits == 16 ? run_plan<16>(plan, a, st) : x_bits == 8 ? run_plan<8>(plan, a, st) : run_plan<4>(plan, a, st);
 }

@@ -1369,54 +1369,76 @@ def _mx_new(shape: tuple, bits: int, device: torch.device) -> MX:
               torch.empty(rows, pad // MX_BLOCK, dtype=torch.uint8, device=device), bits, tuple(shape))
 
 
-def _mx_args(q: MX, name: str) -> list:
-    """(codes, stride, scales, stride) of rows as the kernels read them."""
-    codes, scales = q.codes, q.scales
-    pad = -(-q.cols // MX_PAD) * MX_PAD
-    rows = q.rows
-    if q.bits not in (4, 8) or codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8:
+def _mx_new_args(q: MX) -> tuple:
+    """(codes, stride, scales, stride) of rows that :func:`_mx_new` made."""
+    return q.codes.data_ptr(), q.codes.shape[1], q.scales.data_ptr(), q.scales.shape[1]
+
+
+def _mx_args(q: MX, name: str) -> tuple:
+    """(codes, stride, scales, stride) of rows as the kernels read them, and what holds them."""
+    codes, scales, bits, shape = q.codes, q.scales, q.bits, q.shape
+    cols = shape[-1]
+    rows = shape[0] if len(shape) == 2 else math.prod(shape[:-1])
+    pad = -(-cols // MX_PAD) * MX_PAD
+    if bits not in (4, 8) or codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8:
         raise TypeError(f"{name} must hold uint8 codes of 4 or 8 bits and uint8 scales")
-    if not 0 < q.cols <= MX_MAX or rows > MX_MAX:
-        raise ValueError(f"{name}: 1 to 2^26 columns and at most 2^26 rows, got {rows} x {q.cols}")
-    if tuple(codes.shape) != (rows, pad * q.bits // 8) or tuple(scales.shape) != (rows, pad // MX_BLOCK):
-        raise ValueError(f"{name} of shape {q.shape} in {q.bits} bits holds codes ({rows}, {pad * q.bits // 8}) and "
-                         f"scales ({rows}, {pad // MX_BLOCK}); got {tuple(codes.shape)} and {tuple(scales.shape)}")
-    return [*_mx_bytes(codes, 16), *_mx_bytes(scales, 4)]
+    if not 0 < cols <= MX_MAX or rows > MX_MAX:
+        raise ValueError(f"{name}: 1 to 2^26 columns and at most 2^26 rows, got {rows} x {cols}")
+    if codes.shape != (rows, pad * bits // 8) or scales.shape != (rows, pad // MX_BLOCK):
+        raise ValueError(f"{name} of shape {shape} in {bits} bits holds codes ({rows}, {pad * bits // 8}) and scales "
+                         f"({rows}, {pad // MX_BLOCK}); got {tuple(codes.shape)} and {tuple(scales.shape)}")
+    codes, cs = _mx_bytes(codes, 16)
+    scales, ss = _mx_bytes(scales, 4)
+    return codes.data_ptr(), cs, scales.data_ptr(), ss, (codes, scales)
 
 
 def _mx_bytes(t: torch.Tensor, unit: int) -> tuple[torch.Tensor, int]:
     """``t`` as byte rows aligned to ``unit`` that do not overlap (a copy if needed), and their
     stride (a lone row's is whatever its tensor was cut from; the kernels never step by it)."""
     rows, width = t.shape
-    stride = t.stride(0)
-    if t.data_ptr() % unit or t.stride(1) != 1 or (rows > 1 and (stride % unit or not width <= stride < 1 << 24)):
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t, t.stride(0) if rows > 1 else width
+    stride, step = t.stride()
+    if t.data_ptr() % unit or step != 1 or (rows > 1 and (stride % unit or not width <= stride < 1 << 24)):
+        t, stride = t.clone(memory_format=torch.contiguous_format), width
+    return t, stride if rows > 1 else width
 
 
-def _mx_ptrs(args: list) -> list:
-    return [args[0].data_ptr(), args[1], args[2].data_ptr(), args[3]]
+def _mx_device(first: torch.Tensor, *others: torch.Tensor | None) -> int:
+    """The index of the device that the tensors share (:func:`_check_cuda` says what does not)."""
+    index = first.get_device()
+    if index >= 0:
+        for t in others:
+            if t is not None and t.get_device() != index:
+                break
+        else:
+            return index
+    _check_cuda(first, *others)
+    return index
 
 
-def _mx_call(name: str, device: torch.device, *args) -> None:
-    """``call`` with ``device`` current (the kernels are launched there)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        call(name, *args)
+def _mx_call(name: str, index: int, *args) -> None:
+    """``call`` on the current stream of device ``index``, with that device current."""
+    if index == torch._C._cuda_getDevice():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            call(name, *args)
+        with torch.cuda.device(index):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _no_gradient(name: str, *tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or on detached tensors")
 
 
 def _plain_rows(t: torch.Tensor, cols: int, name: str) -> tuple[torch.Tensor, int]:
-    """``t (..., cols)`` as ``(rows, cols)`` with unit column stride (a copy where the leading
-    dimensions do not flatten to one stride of at least a row) and that stride."""
+    """A tensor that starts where the rows of ``t (..., cols)`` do, its columns in unit stride,
+    and the rows' stride (a copy where the leading dimensions do not flatten to one stride of
+    at least a row)."""
     if t.dim() == 0 or t.shape[-1] != cols:
         raise ValueError(f"{name} must be (..., {cols}), got {tuple(t.shape)}")
+    if t.is_contiguous():
+        return t, cols
     r = t.reshape(-1, cols)
     if (cols > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and r.stride(0) < cols):
         r = r.contiguous()
@@ -1425,13 +1447,15 @@ def _plain_rows(t: torch.Tensor, cols: int, name: str) -> tuple[torch.Tensor, in
 
 def _bf16_out(x_out: torch.Tensor | None, shape: tuple, device: torch.device,
               name: str) -> tuple[torch.Tensor, torch.Tensor, int]:
-    """The bf16 tensor that receives an output, its rows and their stride."""
+    """The bf16 tensor that receives an output, one that starts where its rows do, and their
+    stride."""
     if x_out is None:
         x_out = torch.empty(shape, dtype=torch.bfloat16, device=device)
-    elif x_out.dtype != torch.bfloat16 or tuple(x_out.shape) != tuple(shape):
+        return x_out, x_out, shape[-1]
+    if x_out.dtype != torch.bfloat16 or tuple(x_out.shape) != tuple(shape):
         raise ValueError(f"{name} must be bfloat16 {tuple(shape)}, got {x_out.dtype} {tuple(x_out.shape)}")
     cols = shape[-1]
-    rows = x_out.view(-1, cols)  # raises unless the rows are one strided view
+    rows = x_out.view(-1, cols) if x_out.numel() else x_out.reshape(-1, max(cols, 1))  # one strided view, or it raises
     if (cols > 1 and rows.stride(1) != 1) or (rows.shape[0] > 1 and rows.stride(0) < cols):
         raise ValueError(f"{name} must hold rows of unit column stride that do not overlap")
     return x_out, rows, (rows.stride(0) if rows.shape[0] > 1 else cols)
@@ -1443,38 +1467,39 @@ def mx_quantize(x: torch.Tensor, bits: int = 8, activation: str | None = None) -
     (e2m1), codes round to nearest even and saturate at 448 or 6, and a block holding an
     infinity or a NaN is all NaN. ``activation``: "gelu" (the exact one) or "swiglu" (``x (...,
     2 cols)``: silu of the first half of a row times the second) in float32 on the way."""
-    _check_cuda(x)
-    if x.dtype not in _LOGIT_DTYPES:
+    index = _mx_device(x)
+    dtype = _LOGIT_DTYPES.get(x.dtype)
+    if dtype is None:
         raise TypeError(f"x must be bfloat16, float16 or float32, got {x.dtype}")
-    if activation not in _ACTIVATIONS:
+    kind = _ACTIVATIONS.get(activation)
+    if kind is None:
         raise ValueError(f"activation must be None, 'gelu' or 'swiglu', got {activation!r}")
     _no_gradient("mx_quantize", x)
     if x.dim() == 0:
         raise ValueError("x must be (..., cols)")
     wide = x.shape[-1]
-    if activation == "swiglu" and wide % 2:
+    if kind == 2 and wide % 2:
         raise ValueError(f"swiglu takes rows of two halves, got {wide} values")
-    cols = wide // 2 if activation == "swiglu" else wide
+    cols = wide // 2 if kind == 2 else wide
     q = _mx_new((*x.shape[:-1], cols), bits, x.device)
-    if q.codes.shape[0]:
+    rows = q.codes.shape[0]
+    if rows:
         r, stride = _plain_rows(x, wide, "x")
-        _mx_call("fm_mx_quantize", x.device, r.data_ptr(), _LOGIT_DTYPES[x.dtype], stride, _ACTIVATIONS[activation],
-                 bits, q.codes.data_ptr(), q.codes.shape[1], q.scales.data_ptr(), q.scales.shape[1], r.shape[0], cols,
-                 _stream(x))
+        _mx_call("fm_mx_quantize", index, r.data_ptr(), dtype, stride, kind, bits, *_mx_new_args(q), rows, cols)
     return q
 
 
 def mx_dequantize(q: MX, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values of ``q`` (bf16, fp16 or fp32) in its shape: exact in float32 and, for scales
     above 2^-117, in bfloat16; float16 rounds to nearest and overflows to infinity."""
-    _check_cuda(q.codes, q.scales)
+    index = _mx_device(q.codes, q.scales)
     if dtype not in _LOGIT_DTYPES:
         raise TypeError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
-    held = _mx_args(q, "q")
+    *held, keep = _mx_args(q, "q")
     out = torch.empty(q.shape, dtype=dtype, device=q.codes.device)
-    if q.rows:
-        _mx_call("fm_mx_dequantize", out.device, *_mx_ptrs(held), q.bits, out.data_ptr(), _LOGIT_DTYPES[dtype], q.cols,
-                 q.rows, q.cols, _stream(out))
+    if keep[0].shape[0]:
+        _mx_call("fm_mx_dequantize", index, *held, q.bits, out.data_ptr(), _LOGIT_DTYPES[dtype], q.cols,
+                 keep[0].shape[0], q.cols)
     return out
 
 
@@ -1488,47 +1513,49 @@ def mx_linear(x: torch.Tensor | MX, weight: MX, bias: torch.Tensor | None = None
     """``x weight^T + bias`` for ``weight (n, k)`` in microscaled 4 bits, on the block-scaled
     matrix instructions: ``(..., n)`` bf16, accumulated in float32 and rounded once. ``x (...,
     k)``: microscaled in 8 or 4 bits, or bf16, which the call quantizes to 8 bits
-    (:func:`mx_quantize`). ``bias (n,)`` bf16. ``out (..., n)`` bf16 receives the result."""
+    (:func:`mx_quantize`). ``bias (n,)`` bf16. ``out (..., n)`` bf16 receives the result. The
+    kernel goes by the sizes, and with it the order of the sums over ``k``: a row's results may
+    differ in their last place between calls of different row counts or widths."""
     quantized = isinstance(x, MX)
-    device = _check_cuda(x.codes if quantized else x, x.scales if quantized else None, weight.codes, weight.scales,
-                         bias, out)
+    index = _mx_device(weight.codes, weight.scales, x.codes if quantized else x, x.scales if quantized else None, bias,
+                       out)
     if weight.bits != 4 or len(weight.shape) != 2:
         raise ValueError(f"weight must be (n, k) in 4 bits, got {weight.shape} in {weight.bits}")
     n, k = weight.shape
-    if x.shape[-1:] != (k,):
-        raise ValueError(f"x {tuple(x.shape)} does not match a weight of {k} columns")
-    w = _mx_args(weight, "weight")
-    lead = tuple(x.shape[:-1])
+    shape = x.shape
+    if not shape or shape[-1] != k:
+        raise ValueError(f"x {tuple(shape)} does not match a weight of {k} columns")
+    *w, keep_w = _mx_args(weight, "weight")
+    lead = tuple(shape[:-1])
+    rows = math.prod(lead)
     if quantized:
-        rows, x_bits, held = x.rows, x.bits, _mx_args(x, "x")
-        xa = _mx_ptrs(held)
+        x_bits = x.bits
+        xp, xs, xsp, xss, keep_x = _mx_args(x, "x")
     else:
         if x.dtype is not torch.bfloat16:
             raise TypeError(f"x must be bfloat16 or microscaled, got {x.dtype}")
         _no_gradient("mx_linear", x, bias)
-        held, stride = _plain_rows(x, k, "x")
-        rows = held.shape[0]
-        if rows <= MX_BF16_ROWS and k % 8 == 0 and stride % 8 == 0 and held.data_ptr() % 16 == 0:
-            x_bits, xa = 16, [held.data_ptr(), stride, None, 0]
+        keep_x, xs = _plain_rows(x, k, "x")
+        xp = keep_x.data_ptr()
+        # the rows that the kernel quantizes itself; past these sums and columns a call of its own
+        # is cheaper (16 rows, us: 8192 -> 2048 15.6 / 14, 20480 -> 2048 33.7 / 19)
+        if (rows <= MX_BF16_ROWS and k % 8 == 0 and xs % 8 == 0 and xp % 16 == 0
+                and (k < 8192 if n <= 8192 else k <= 5632)):
+            x_bits, xsp, xss = 16, None, 0
         else:
-            q = mx_quantize(held)
-            x_bits, held = 8, _mx_args(q, "x")
-            xa = _mx_ptrs(held)
+            x_bits, keep_x = 8, mx_quantize(x)
+            xp, xs, xsp, xss = _mx_new_args(keep_x)
     if bias is not None:
-        if bias.dtype is not torch.bfloat16 or tuple(bias.shape) != (n,):
+        if bias.dtype is not torch.bfloat16 or bias.shape != (n,):
             raise ValueError(f"bias must be bfloat16 ({n},), got {bias.dtype} {tuple(bias.shape)}")
         _no_gradient("mx_linear", bias)
         bias = bias.contiguous()
-    if out is None:
-        out = torch.empty(*lead, n, dtype=torch.bfloat16, device=device)
-        out_rows, stride = out, n
-    else:
-        out, out_rows, stride = _bf16_out(out, (*lead, n), device, "out")
+    out, out_rows, stride = _bf16_out(out, (*lead, n), weight.codes.device, "out")
     if rows and n:
         nbytes = _mx_workspace_bytes(rows, n, k, x_bits)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        _mx_call("fm_mx_linear", device, xa[0], x_bits, xa[1], xa[2], xa[3], *_mx_ptrs(w), _ptr(bias),
-                 out_rows.data_ptr(), stride, rows, n, k, _ptr(ws), nbytes, _stream(out))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=out.device) if nbytes else None
+        _mx_call("fm_mx_linear", index, xp, x_bits, xs, xsp, xss, *w, _ptr(bias), out_rows.data_ptr(), stride, rows, n,
+                 k, _ptr(ws), nbytes)
     return out
 
 
@@ -1539,35 +1566,38 @@ def rms_norm_mx(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: tor
     rsqrt(mean(s^2) + eps) * weight`` in 8 (or 4) bits, rounded once from float32. ``x``,
     ``residual (..., cols)`` bf16, ``weight (cols,)``; ``x_out`` (may be ``x`` or ``residual``)
     receives ``x'``. Returns ``(x', q)``, ``x'`` None without a residual."""
-    device = _check_cuda(x, weight, residual, x_out)
+    index = _mx_device(x, weight, residual, x_out)
     _no_gradient("rms_norm_mx", x, weight, residual)
     cols = _norm_cols(x)
     if weight.numel() != cols:
         raise ValueError(f"weight holds {weight.numel()} values, a row {cols}")
-    if residual is not None and (residual.dtype != torch.bfloat16 or residual.shape != x.shape):
-        raise ValueError(f"residual must be bfloat16 {tuple(x.shape)}, got {residual.dtype} {tuple(residual.shape)}")
-    if residual is None and x_out is not None:
-        raise ValueError("x_out is the sum of x and a residual: give one")
-    q = _mx_new(tuple(x.shape), bits, device)
+    device = x.device
+    shape = tuple(x.shape)
+    q = _mx_new(shape, bits, device)
     xr, xs = _plain_rows(x, cols, "x")
     rr, rs, orows, os_ = None, 0, None, 0
     if residual is not None:
+        if residual.dtype != torch.bfloat16 or residual.shape != x.shape:
+            raise ValueError(f"residual must be bfloat16 {shape}, got {residual.dtype} {tuple(residual.shape)}")
         rr, rs = _plain_rows(residual, cols, "residual")
-        x_out, orows, os_ = _bf16_out(x_out, tuple(x.shape), device, "x_out")
+        x_out, orows, os_ = _bf16_out(x_out, shape, device, "x_out")
+    elif x_out is not None:
+        raise ValueError("x_out is the sum of x and a residual: give one")
     weight = _f32(weight)
-    if xr.shape[0]:
-        _mx_call("fm_rms_norm_mx", device, xr.data_ptr(), xs, _ptr(rr), rs, weight.data_ptr(), float(eps),
-                 _ptr(orows), os_, bits, q.codes.data_ptr(), q.codes.shape[1], q.scales.data_ptr(), q.scales.shape[1],
-                 xr.shape[0], cols, _stream(x))
+    rows = q.codes.shape[0]
+    if rows:
+        _mx_call("fm_rms_norm_mx", index, xr.data_ptr(), xs, _ptr(rr), rs, weight.data_ptr(), eps, _ptr(orows), os_,
+                 bits, *_mx_new_args(q), rows, cols)
     return x_out, q
 
 
 def _norm_cols(x: torch.Tensor) -> int:
-    if x.dtype != torch.bfloat16 or x.dim() == 0:
+    if x.dtype is not torch.bfloat16 or x.dim() == 0:
         raise TypeError(f"x must be bfloat16 (..., cols), got {x.dtype} {tuple(x.shape)}")
-    if not 0 < x.shape[-1] <= MX_NORM_COLS:
-        raise ValueError(f"rows of {x.shape[-1]} values: the norms take 1 to {MX_NORM_COLS}")
-    return x.shape[-1]
+    cols = x.shape[-1]
+    if not 0 < cols <= MX_NORM_COLS:
+        raise ValueError(f"rows of {cols} values: the norms take 1 to {MX_NORM_COLS}")
+    return cols
 
 
 def adaln_residual_mx(
@@ -1585,43 +1615,45 @@ def adaln_residual_mx(
     ``LN(s) * (1 + scale) + shift`` for ``modulation = (scale, shift)`` in 8 (or 4) bits,
     nothing rounded in between. ``x``/``y (..., cols)`` bf16, or ``x (cols,)``: one row shared
     by every row of ``y``; ``gate``, ``scale``, ``shift (cols,)`` bf16 (``gate_per_row``: one
-    gate value per row). ``x_out`` (may be ``x``) receives ``x'``. Returns ``(x', q)``, ``x'``
-    None without a residual."""
+    gate value per row). ``x_out`` (may be ``x`` or ``y``) receives ``x'``. Returns ``(x', q)``,
+    ``x'`` None without a residual."""
     if modulation is None:
         raise ValueError("a microscaled output needs its modulation (adaln_residual serves the residual alone)")
-    device = _check_cuda(x, y, gate, x_out, *modulation)
-    _no_gradient("adaln_residual_mx", x, y, gate, *modulation)
+    scale, shift = modulation
+    index = _mx_device(x, y, scale, shift, x_out, None if y is None else gate)
+    _no_gradient("adaln_residual_mx", x, y, scale, shift, None if y is None else gate)
     cols = _norm_cols(x)
     shared = x.dim() == 1 and y is not None
     shape = tuple(y.shape if shared else x.shape)
-    rows = math.prod(shape[:-1])
+    device = x.device
     yr, ys, g, orows, os_ = None, 0, None, None, 0
     if y is not None:
         if gate is None:
             raise ValueError("a residual needs its gate")
-        if y.dtype != torch.bfloat16 or y.shape[-1:] != (cols,) or (not shared and y.shape != x.shape):
+        if y.dtype is not torch.bfloat16 or y.shape[-1:] != (cols,) or (not shared and y.shape != x.shape):
             raise ValueError(f"y {y.dtype} {tuple(y.shape)} does not match x {tuple(x.shape)}")
         yr, ys = _plain_rows(y, cols, "y")
-        g = _mx_vec(gate, rows, "gate (one per row)") if gate_per_row else _mx_vec(gate, cols, "gate")
+        g = _mx_vec(gate, math.prod(shape[:-1]), "gate (one per row)") if gate_per_row else _mx_vec(gate, cols, "gate")
         if shared and x_out is not None and x_out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
             raise ValueError("x_out may not share the storage of a shared x row")
         x_out, orows, os_ = _bf16_out(x_out, shape, device, "x_out")
     elif x_out is not None:
         raise ValueError("x_out is the sum of x and a gated y: give one")
-    sc, sh = _mx_vec(modulation[0], cols, "scale"), _mx_vec(modulation[1], cols, "shift")
+    sc, sh = _mx_vec(scale, cols, "scale"), _mx_vec(shift, cols, "shift")
     xr, xs = _plain_rows(x, cols, "x")
     q = _mx_new(shape, bits, device)
+    rows = q.codes.shape[0]
     if rows:
-        _mx_call("fm_adaln_residual_mx", device, xr.data_ptr(), 0 if shared else xs, _ptr(yr), ys, _ptr(g),
-                 int(gate_per_row), sc.data_ptr(), sh.data_ptr(), _ptr(orows), os_, float(eps), bits,
-                 q.codes.data_ptr(), q.codes.shape[1], q.scales.data_ptr(), q.scales.shape[1], rows, cols, _stream(x))
+        _mx_call("fm_adaln_residual_mx", index, xr.data_ptr(), 0 if shared else xs, _ptr(yr), ys, _ptr(g),
+                 int(gate_per_row), sc.data_ptr(), sh.data_ptr(), _ptr(orows), os_, eps, bits, *_mx_new_args(q), rows,
+                 cols)
     return x_out, q
 
 
 def _mx_vec(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
-    if t.dtype != torch.bfloat16 or t.numel() != n:
+    if t.dtype is not torch.bfloat16 or t.numel() != n:
         raise ValueError(f"{name} must hold {n} bfloat16 values, got {t.dtype} {tuple(t.shape)}")
-    return t.reshape(n).contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def noise_rows(z: torch.Tensor, eigvals: torch.Tensor, eps: float, gain: float,

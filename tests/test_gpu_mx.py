@@ -5,8 +5,14 @@ Quantization of a tensor's own values is one rounding of exact quotients: codes 
 equal to the oracle's. Where a value is computed before it is quantized (an activation, a
 norm) it is off by its float32 error, which moves a code only past a midpoint: the codes must
 lie between the oracle's for the value less and plus that error. A product's bound counts the
-bf16 rounding (2^-8) and what the matrix instruction drops of products far below the largest
-of a step (measured at most 2^-17 of the absolute sum; 2^-15 allowed)."""
+bf16 rounding (2^-8 of the result) and what the sums lose of their absolute sum: 2^-15 for the
+float32 sums of groups, steps and parts (probed with single products: a term is cut below 2^-20
+of the largest of the 16 groups of a step, 16 2^-20; 160 steps and 8 parts of 2^-23 each), and
+with an 8-bit operand 7 2^-13 < 2^-10 more: the instruction adds the 8 products of a group after
+cutting each below 2^-13 of the power of two of the group's largest (probed likewise), so that 7
+of them lose less than 2^-13 of the largest, and the largest is at most the group's absolute
+sum. Products within 2^12 of each other lose nothing there, which
+``test_linear_of_even_magnitudes`` holds the kernels to."""
 
 import pytest
 import torch
@@ -134,11 +140,11 @@ def _x_of(kind, x):
     return q, mx.values(*_cpu(q), kind)
 
 
-def _check_product(got, xv, wv, bias):
+def _check_product(got, xv, wv, bias, sums=2.0 ** -15 + 2.0 ** -10):
     ref = xv @ wv.T + (0 if bias is None else bias.cpu().double())
     total = xv.abs() @ wv.abs().T + (0 if bias is None else bias.cpu().double().abs())
     err = (got.cpu().double() - ref).abs()
-    bad = err > 2.0 ** -8 * ref.abs() + 2.0 ** -15 * total
+    bad = err > 2.0 ** -8 * ref.abs() + sums * total
     assert not bad.any(), f"{int(bad.sum())} results off, by up to {(err / total)[bad].max():.2e} of the absolute sum"
 
 
@@ -146,7 +152,13 @@ def _check_product(got, xv, wv, bias):
 @pytest.mark.parametrize("rows,n,k", [
     (1, 1, 1), (1, 17, 32), (3, 15, 33), (16, 16, 128), (17, 33, 160), (16, 300, 2048), (31, 257, 129), (32, 64, 1000),
     (33, 100, 4096), (64, 130, 640), (65, 127, 256), (100, 1000, 384), (128, 128, 512), (129, 300, 2048),
-    (255, 257, 1152), (256, 512, 1024), (300, 513, 896), (600, 260, 130), (1, 5000, 2048), (16, 9000, 512)])
+    (255, 257, 1152), (256, 512, 1024), (300, 513, 896), (600, 260, 130), (1, 5000, 2048), (16, 9000, 512),
+    # a stream of columns: groups that end early, odd columns, the longest rows that lie in LDS
+    (16, 8200, 128), (1, 9001, 700), (7, 12288, 1408), (16, 8193, 5632), (3, 8300, 10880),
+    # few rows, long sums, in parts: whole ones and a last one of less than a chunk
+    (5, 100, 8192), (16, 70, 20480), (33, 64, 8320), (64, 200, 4224), (130, 72, 6272),
+    # tiles of 128 and 256, more than the chip holds at once and not
+    (2048, 2048, 256), (1920, 2500, 384), (3300, 4100, 128), (2048, 6144, 640), (4096, 4096, 200)])
 def test_linear(dev, rows, n, k, kind):
     print(f"mx_linear rows={rows} n={n} k={k} x={kind}", flush=True)
     x = _activations(rows, k, rows + n + k).to(dev)
@@ -155,7 +167,21 @@ def test_linear(dev, rows, n, k, kind):
     given, xv = _x_of(kind, x)
     got = ops.mx_linear(given, w, bias)
     assert got.shape == (rows, n) and got.dtype == torch.bfloat16
-    _check_product(got, xv, mx.values(*_cpu(w), 4), bias)
+    _check_product(got, xv, mx.values(*_cpu(w), 4), bias, 2.0 ** -15 + (0 if kind == 4 else 2.0 ** -10))
+
+
+@pytest.mark.parametrize("kind", ["bf16", 8])
+@pytest.mark.parametrize("rows,n,k", [(1, 300, 2048), (16, 5000, 1000), (13, 9000, 5632), (16, 100, 20480),
+                                      (40, 70, 8320), (130, 1500, 384), (1024, 2048, 512), (2048, 6200, 640)])
+def test_linear_of_even_magnitudes(dev, rows, n, k, kind):
+    """x of magnitudes from 1 to 2 within each block: codes of one or two binades, products
+    (with the weights' 0.5 to 6) within 2^6 of each other, nothing lost in the groups."""
+    g = gen(rows + k)
+    x = (1 + torch.rand(rows, k, generator=g)) * torch.randint(0, 2, (rows, k), generator=g).mul(2).sub(1)
+    x = x * torch.randint(-6, 7, (rows, -(-k // 32)), generator=g).float().exp2().repeat_interleave(32, 1)[:, :k]
+    w = ops.mx_quantize(torch.randn(n, k, generator=g).to(dev), 4)
+    given, xv = _x_of(kind, x.bfloat16().to(dev))
+    _check_product(ops.mx_linear(given, w), xv, mx.values(*_cpu(w), 4), None, 2.0 ** -15)
 
 
 @pytest.mark.parametrize("kind", ["bf16", 8, 4])
@@ -368,9 +394,7 @@ def test_rows_far_into_memory(dev):
     last = ops.MX(codes[-200:], scales[-200:], 4, (200, k))
     for rows in (1, 20, 300):
         x = ops.mx_quantize(_activations(rows, k, rows).to(dev))
-        part = ops.mx_linear(x, last)
-        _check_product(part, mx.values(*_cpu(x), 8), mx.values(*_cpu(last), 4), None)
-        assert torch.equal(ops.mx_linear(x, w)[:, -200:], part)
+        _check_product(ops.mx_linear(x, w)[:, -200:], mx.values(*_cpu(x), 8), mx.values(*_cpu(last), 4), None)
     # 4-bit rows as the many: x's rows far into memory too
     few = ops.MX(codes[:40], scales[:40], 4, (40, k))
     _check_product(ops.mx_linear(w, few)[-200:], mx.values(*_cpu(last), 4), mx.values(*_cpu(few), 4), None)
