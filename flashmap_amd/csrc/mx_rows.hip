@@ -96,6 +96,20 @@ __device__ __forceinline__ void store_block(const float (&v)[8], int32_t c, uint
   if ((c & 31) == 0) scales[c >> 5] = (uint8_t)byte;
 }
 
+// item / chunks for item < 2^30 and 16 <= chunks <= 2^23, by a multiplication: with 2^l >= chunks
+// and magic = floor(2^(30 + l) / chunks) + 1 the quotient is off by less than 2^-l <= 1 / chunks,
+// and never past the next integer.
+struct RowOf {
+  uint32_t magic, shift;
+  explicit RowOf(uint32_t chunks) {
+    shift = 0;
+    while ((1u << shift) < chunks) ++shift;
+    magic = (uint32_t)(((uint64_t)1 << (30 + shift)) / chunks + 1);
+    shift -= 2;
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t item) const { return __umulhi(item, magic) >> shift; }
+};
+
 // -------------------------------------------------------------------------- quantization
 
 struct QuantArgs {
@@ -105,19 +119,53 @@ struct QuantArgs {
   int64_t rows;
   int32_t cols;
   uint32_t chunks;  // 8-value chunks of a stored row
+  RowOf row_of;
   int32_t vec;
 };
 
 enum { ACT_NONE = 0, ACT_GELU = 1, ACT_SWIGLU = 2 };
 
-// x Phi(x) from erfc, which keeps its relative accuracy for negative x.
-__device__ __forceinline__ float gelu(float x) { return 0.5f * x * erfcf(x * -0.70710678f); }
-__device__ __forceinline__ float swiglu(float gate, float up) { return gate / (1.f + expf(-gate)) * up; }
+// x Phi(x) = max(x, 0) - h, h = |x| / 2 erfc(|x| / sqrt 2): nothing cancels (h is at most half of
+// |x|). erfc(z) = exp(-z^2) erfcx(z), and erfcx(a / sqrt 2) / 2 is a polynomial in 1 / (1 + 0.23 a),
+// fitted to 5e-8 of its value for a up to 14.5 (least squares in Chebyshev polynomials,
+// reweighted towards the largest relative error). h comes to 4e-7 of its value for |x| below 4
+// (beyond, the exponent's rounding adds 1e-8 x^2), and for no bf16 x does that move the result
+// past a midpoint of a code. A third of erfcf's instructions, which bounded the pass (1024 x 8192,
+// 25 MB: 14.9 us). Infinities and NaN give NaN; h is 0 where it is below 2^-126 (x < -13).
+__device__ __forceinline__ float gelu(float x) {
+#pragma clang fp contract(off)
+  const float a = fabsf(x);
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.23f, a, 1.f));
+  float p = -0.0784958884f;
+  p = __builtin_fmaf(p, t, 0.290552796f);
+  p = __builtin_fmaf(p, t, -0.278415741f);
+  p = __builtin_fmaf(p, t, 0.301807729f);
+  p = __builtin_fmaf(p, t, -0.0331565229f);
+  p = __builtin_fmaf(p, t, 0.119617817f);
+  p = __builtin_fmaf(p, t, 0.0857352587f);
+  p = __builtin_fmaf(p, t, 0.0923825472f);
+  p = __builtin_fmaf(p, t, -2.80193462e-5f);
+  const float e = __builtin_amdgcn_exp2f(a * a * -0.721347520f);  // exp(-a^2 / 2)
+  return fmaxf(x, 0.f) - a * (e * p);
+}
+// gate / (1 + exp(-gate)) * up: the exponential as above, the quotient by a refined reciprocal.
+// From gate = -88 on the result is 0.
+__device__ __forceinline__ float swiglu(float gate, float up) {
+#pragma clang fp contract(off)
+  const float y = fminf(-gate, 88.f);
+  const float u = y * 1.44269504f;
+  const float r = __builtin_fmaf(y, 1.92596299e-8f, __builtin_fmaf(y, 1.44269504f, -u));
+  const float e = __builtin_amdgcn_exp2f(u);
+  const float d = 1.f + __builtin_fmaf(e * 0.693147182f, r, e);
+  float q = __builtin_amdgcn_rcpf(d);
+  q = __builtin_fmaf(__builtin_fmaf(-d, q, 1.f), q, q);
+  return gate * up * q;
+}
 
 template <typename T, int BITS, int ACT>
 __global__ __launch_bounds__(ROW_THREADS) void mx_quantize_kernel(const QuantArgs a) {
   const uint32_t item = blockIdx.x * ROW_THREADS + threadIdx.x;
-  const uint32_t row = item / a.chunks;
+  const uint32_t row = a.row_of(item);
   if (row >= a.rows) return;  // chunks of a row are a multiple of 16: whole quads leave
   const int32_t c = 8 * (int32_t)(item - row * a.chunks);
   const T *x = (const T *)a.x + row * a.xs;
@@ -144,13 +192,14 @@ struct DequantArgs {
   int64_t rows;
   int32_t cols;
   uint32_t chunks;
+  RowOf row_of;
   int32_t vec;
 };
 
 template <typename T, int BITS>
 __global__ __launch_bounds__(ROW_THREADS) void mx_dequantize_kernel(const DequantArgs a) {
   const uint32_t item = blockIdx.x * ROW_THREADS + threadIdx.x;
-  const uint32_t row = item / a.chunks;
+  const uint32_t row = a.row_of(item);
   if (row >= a.rows) return;
   const int32_t c = 8 * (int32_t)(item - row * a.chunks);
   if (c >= a.cols) return;
@@ -199,15 +248,20 @@ struct NormArgs {
   float eps;
 };
 
-// The sum over a row's TPR threads, the same bits in all of them.
+// The sum over a wavefront, the same bits in every lane.
+__device__ __forceinline__ float wave_sum(float v) {
+  v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x128, 0xf, 0xf, true));  // row_ror 8
+  v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x124, 0xf, 0xf, true));
+  v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x122, 0xf, 0xf, true));
+  v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x121, 0xf, 0xf, true));
+  return sum_over_groups(v);
+}
+// The sum over a row's TPR threads; lds: a place of its own per sum.
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float *lds) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+  v = wave_sum(v);
   if constexpr (TPR > 64) {
-    const int wave = wave_id();
-    __syncthreads();  // the last sum has been read
-    if ((threadIdx.x & 63) == 0) lds[wave] = v;
+    if ((threadIdx.x & 63) == 0) lds[wave_id()] = v;
     __syncthreads();
     v = 0.f;
 #pragma unroll
@@ -216,14 +270,23 @@ __device__ __forceinline__ float row_sum(float v, float *lds) {
   return v;
 }
 
-template <int TPR, int NCH, bool RMS, int BITS>
+// EARLY: the row-independent operands are loaded with the row, not after its statistics (one
+// round trip less, for as many registers).
+template <int TPR, int NCH, bool RMS, int BITS, bool EARLY>
 __global__ __launch_bounds__(ROW_THREADS) void mx_norm_kernel(const NormArgs a) {
-  __shared__ float lds[ROW_THREADS / 64];
+  __shared__ float lds[2][ROW_THREADS / 64];
   const int t = threadIdx.x % TPR;
   const int64_t row = (int64_t)blockIdx.x * (ROW_THREADS / TPR) + threadIdx.x / TPR;
   if (row >= a.rows) return;  // a whole wavefront, and with TPR 256 a whole workgroup
-  float v[NCH][8];
-  float sum = 0.f;
+  float v[NCH][8], p[EARLY ? NCH : 1][8], q[EARLY && !RMS ? NCH : 1][8];
+  auto operands = [&](int32_t c, float (&pc)[8], float (&qc)[8]) {
+    if constexpr (RMS) {
+      load8(a.weight, c, a.cols, a.vec_p != 0, pc);
+    } else {
+      load8((const bf16_raw *)a.scale, c, a.cols, a.vec_p != 0, pc);
+      load8((const bf16_raw *)a.shift, c, a.cols, a.vec_p != 0, qc);
+    }
+  };
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
     const int32_t c = 8 * (t + TPR * i);
@@ -245,16 +308,22 @@ __global__ __launch_bounds__(ROW_THREADS) void mx_norm_kernel(const NormArgs a) 
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] = __builtin_fmaf(g[j], y[j], v[i][j]);
       }
-      if (a.x_out != nullptr && c < a.cols) store8_bf16(a.x_out + row * a.xos, c, a.cols, a.vec_o != 0, v[i]);
     }
+    if constexpr (EARLY) operands(c, p[i], q[RMS ? 0 : i]);
+  }
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < NCH; ++i) {
+    const int32_t c = 8 * (t + TPR * i);
+    if (a.x_out != nullptr && c < a.cols) store8_bf16(a.x_out + row * a.xos, c, a.cols, a.vec_o != 0, v[i]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) sum += RMS ? v[i][j] * v[i][j] : v[i][j];
   }
   const float n = (float)a.cols;
-  sum = row_sum<TPR>(sum, lds);
+  sum = row_sum<TPR>(sum, lds[0]);
   float mean = 0.f;
   if constexpr (!RMS) {
-    mean = sum / n;
+    mean = __fdiv_rn(sum, n);
     sum = 0.f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i)
@@ -263,24 +332,23 @@ __global__ __launch_bounds__(ROW_THREADS) void mx_norm_kernel(const NormArgs a) 
         const float d = 8 * (t + TPR * i) + j < a.cols ? v[i][j] - mean : 0.f;
         sum += d * d;
       }
-    sum = row_sum<TPR>(sum, lds);
+    sum = row_sum<TPR>(sum, lds[1]);
   }
-  const float r = rsqrtf(sum / n + a.eps);
+  // Rounded correctly: an ulp here moves every value of the row, and codes past their midpoints.
+  const float r = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(sum, n) + a.eps));
 #pragma unroll
   for (int i = 0; i < NCH; ++i) {
     const int32_t c = 8 * (t + TPR * i);
     if (c >= 8 * (int32_t)a.chunks) break;  // whole quads: chunks is a multiple of 16
-    float p[8], q[8];
+    if constexpr (!EARLY) operands(c, p[0], q[0]);
+    float(&pc)[8] = p[EARLY ? i : 0], (&qc)[8] = q[EARLY && !RMS ? i : 0];
     if constexpr (RMS) {
-      load8(a.weight, c, a.cols, a.vec_p != 0, p);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] *= r * p[j];
+      for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * r * pc[j];
     } else {
-      load8((const bf16_raw *)a.scale, c, a.cols, a.vec_p != 0, p);
-      load8((const bf16_raw *)a.shift, c, a.cols, a.vec_p != 0, q);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        v[i][j] = c + j < a.cols ? __builtin_fmaf((v[i][j] - mean) * r, 1.f + p[j], q[j]) : 0.f;
+        v[i][j] = c + j < a.cols ? __builtin_fmaf((v[i][j] - mean) * r, 1.f + pc[j], qc[j]) : 0.f;
     }
     store_block<BITS>(v[i], c, a.codes + row * a.cs, a.scales + row * a.ss);
   }
@@ -323,8 +391,8 @@ static void by_dtype(int32_t dtype, F f) {
 }
 
 static int launch_norm(const NormArgs &base, bool rms, int32_t bits, hipStream_t stream) {
-  // A wavefront a row while it holds the row in 4 chunks a lane, else a workgroup.
-  const int tpr = base.chunks <= 256 ? 64 : 256;
+  // Rows of up to 512 values: a wavefront each; longer ones: a workgroup each.
+  const int tpr = base.chunks <= 64 ? 64 : 256;
   const int nch = (int)((base.chunks + tpr - 1) / tpr);
   return by_slices(base.rows, tpr, [&](int64_t first, int64_t rows) {
     NormArgs a = base;
@@ -338,7 +406,8 @@ static int launch_norm(const NormArgs &base, bool rms, int32_t bits, hipStream_t
     const int per = ROW_THREADS / tpr;
     const dim3 grid((unsigned)((rows + per - 1) / per));
     auto go = [&](auto t, auto c, auto r, auto b) {
-      mx_norm_kernel<decltype(t)::value, decltype(c)::value, decltype(r)::value, decltype(b)::value>
+      constexpr int NCH = decltype(c)::value;
+      mx_norm_kernel<decltype(t)::value, NCH, decltype(r)::value, decltype(b)::value, NCH <= 2>
           <<<grid, dim3(ROW_THREADS), 0, stream>>>(a);
     };
     auto with_bits = [&](auto t, auto c, auto r) {
@@ -353,21 +422,16 @@ static int launch_norm(const NormArgs &base, bool rms, int32_t bits, hipStream_t
       else
         with_bits(t, c, std::false_type{});
     };
-    if (tpr == 64) {
-      if (nch == 1)
-        with_kind(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
-      else if (nch == 2)
-        with_kind(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
-      else
-        with_kind(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
-    } else {
-      if (nch <= 2)
-        with_kind(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
-      else if (nch <= 4)
-        with_kind(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
-      else
-        with_kind(std::integral_constant<int, 256>{}, std::integral_constant<int, 8>{});
-    }
+    if (tpr == 64)
+      with_kind(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
+    else if (nch <= 1)
+      with_kind(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{});
+    else if (nch <= 2)
+      with_kind(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
+    else if (nch <= 4)
+      with_kind(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
+    else
+      with_kind(std::integral_constant<int, 256>{}, std::integral_constant<int, 8>{});
   });
 }
 
@@ -395,7 +459,7 @@ extern "C" int fm_mx_quantize(const void *x, int32_t dtype, int64_t x_stride, in
       typedef decltype(tag) T;
       QuantArgs a{(const T *)x + first * x_stride, (uint8_t *)codes + first * codes_stride,
                   (uint8_t *)scales + first * scales_stride, x_stride, codes_stride, scales_stride, n, (int32_t)cols,
-                  (uint32_t)chunks, vec_rows(x, x_stride, size)};
+                  (uint32_t)chunks, RowOf((uint32_t)chunks), vec_rows(x, x_stride, size)};
       const dim3 grid((unsigned)((n * chunks + ROW_THREADS - 1) / ROW_THREADS));
       auto go = [&](auto b, auto act) {
         mx_quantize_kernel<T, decltype(b)::value, decltype(act)::value>
@@ -437,7 +501,7 @@ extern "C" int fm_mx_dequantize(const void *codes, int64_t codes_stride, const v
       typedef decltype(tag) T;
       DequantArgs a{(const uint8_t *)codes + first * codes_stride, (const uint8_t *)scales + first * scales_stride,
                     (T *)out + first * out_stride, codes_stride, scales_stride, out_stride, n, (int32_t)cols,
-                    (uint32_t)chunks, vec_rows(out, out_stride, size)};
+                    (uint32_t)chunks, RowOf((uint32_t)chunks), vec_rows(out, out_stride, size)};
       const dim3 grid((unsigned)((n * chunks + ROW_THREADS - 1) / ROW_THREADS));
       if (bits == 8)
         mx_dequantize_kernel<T, 8><<<grid, dim3(ROW_THREADS), 0, (hipStream_t)stream>>>(a);
