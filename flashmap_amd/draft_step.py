@@ -28,6 +28,13 @@ row kernels (``ops.state_embed_rows``: posterior and state as the embedding GEMM
 operand; ``ops.state_update``: the jump head's softmax and the update, in place).
 Inputs are explicit (what vLLM's forward context supplies): anchors and their positions
 and slots, the noise, the caches, the block table. bf16 only.
+
+With ``mx`` the step's projections and head are held in microscaled 4 bits (a quarter of the
+bytes, which is what a step of few requests waits for) and their inputs in 8: the norms write
+them so (``ops.adaln_residual_mx``, ``ops.rms_norm_mx``), the MLP's activation is applied on the
+way into them (``ops.mx_quantize``), and the products are ``ops.mx_linear``. Drafts are verified,
+so that this costs acceptance and never correctness. The several-jump state's embedding stays
+bf16.
 """
 
 from __future__ import annotations
@@ -39,7 +46,32 @@ from . import ops
 from .drafter import FlashMapDraftModel, jump_times
 from .fold import fold_head, fold_noise
 
-__all__ = ["DraftStep"]
+__all__ = ["DraftStep", "MXLayer", "product"]
+
+
+def product(x, weight, bias: torch.Tensor | None = None) -> torch.Tensor:
+    """``x weight^T + bias`` for a weight in bf16 or in microscaled 4 bits."""
+    return ops.mx_linear(x, weight, bias) if isinstance(weight, ops.MX) else ops.linear(x, weight, bias)
+
+
+class MXLayer:
+    """A DiT layer's projections in microscaled 4 bits; ``qkv`` the self-attention's joined
+    q/k/v weight. The biases stay bf16."""
+
+    def __init__(self, layer, qkv: torch.Tensor):
+        weights = (qkv, layer.self_attn.o_proj.weight, layer.cross_attn.q_proj.weight, layer.cross_attn.o_proj.weight)
+        self.qkv, self.self_o, self.cross_q, self.cross_o = (ops.mx_quantize(w, 4) for w in weights)
+        mlp = layer.mlp
+        self.activation = mlp.mlp_type
+        up, down = (mlp.gate_up_proj, mlp.down_proj) if self.activation == "swiglu" else (mlp.fc1, mlp.fc2)
+        self.up, self.up_bias = ops.mx_quantize(up.weight, 4), up.bias
+        self.down, self.down_bias = ops.mx_quantize(down.weight, 4), down.bias
+
+    def mlp(self, h) -> torch.Tensor:
+        """The layer's MLP (flashmap/modeling_flashmap.py:150-170), the activation applied as its
+        values go to 8 bits."""
+        up = ops.mx_linear(h, self.up, self.up_bias)
+        return ops.mx_linear(ops.mx_quantize(up, 8, self.activation), self.down, self.down_bias)
 
 
 def _split_k(a: torch.Tensor, w: torch.Tensor, splits: int = 4) -> torch.Tensor:
@@ -72,11 +104,13 @@ class DraftStep:
     rows); ``hot_ids``: the draft vocabulary's token ids when the drafter has a state
     vocabulary (``draft_ids``) or vLLM restricts it (``d2t``), else None; ``num_steps``:
     the jumps per draft (the drafter's configured count when None; the config's
-    ``jump_grids`` must hold a grid for it)."""
+    ``jump_grids`` must hold a grid for it); ``mx``: hold the projections and the head in
+    microscaled 4 bits."""
 
     @torch.no_grad()
     def __init__(self, model: FlashMapDraftModel, embed_tokens: torch.Tensor, lm_head: torch.Tensor,
-                 max_model_len: int, hot_ids: torch.Tensor | None = None, num_steps: int | None = None):
+                 max_model_len: int, hot_ids: torch.Tensor | None = None, num_steps: int | None = None,
+                 mx: bool = False):
         cfg = model.config
         if model.dtype != torch.bfloat16:
             raise TypeError("the draft step's kernels are bf16: move the drafter to torch.bfloat16")
@@ -131,6 +165,18 @@ class DraftStep:
             self.jump_head = ((self.head_weight, self.head_bias) if hot_ids is None or state_vocab
                               else fold_head(lm_head, model.head.weight, model.head.bias))
         self.scale = self.head_dim ** -0.5
+        self.mx_layers = self.mx_fc = self.mx_anchor = self.mx_embed = None
+        if mx:
+            self.mx_layers = [MXLayer(layer, qkv) for layer, qkv in zip(layers, self.self_qkv)]
+            self.self_qkv = [layer.qkv for layer in self.mx_layers]
+            self.mx_fc, self.mx_anchor = (ops.mx_quantize(p.weight, 4) for p in (model.fc, model.anchor_proj))
+            self.mx_embed = ops.mx_quantize(model.x_embed.weight, 4) if self.num_steps > 1 else None
+            shared = self.jump_head is not None and self.jump_head[0] is self.head_weight
+            self.context_kv_weight, self.noise_embed, self.head_weight = (
+                ops.mx_quantize(w, 4) for w in (self.context_kv_weight, self.noise_embed, self.head_weight))
+            if self.jump_head is not None:
+                self.jump_head = (self.head_weight if shared else ops.mx_quantize(self.jump_head[0], 4),
+                                  self.jump_head[1])
 
     @property
     def noise_columns(self) -> int:
@@ -152,10 +198,11 @@ class DraftStep:
         return bases, (c0.stride(0), c0.stride(1), c0.stride(2), c0.shape[-1] // 2), c0.shape[2]
 
     @torch.no_grad()
-    def write_rows(self, rows: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, layout) -> None:
-        """Keys and values of context rows ``(tokens, dim)`` for every layer: one GEMM over
-        the layers' K/V weights and one writer launch (flashmap/vllm/model.py:735-777)."""
-        kv = F.linear(rows, self.context_kv_weight)
+    def write_rows(self, rows, positions: torch.Tensor, slots: torch.Tensor, layout) -> None:
+        """Keys and values of context rows ``(tokens, dim)`` (bf16, or microscaled where the
+        weights are) for every layer: one GEMM over the layers' K/V weights and one writer launch
+        (flashmap/vllm/model.py:735-777)."""
+        kv = F.linear(rows, self.context_kv_weight) if self.mx_layers is None else product(rows, self.context_kv_weight)
         bases, strides, page = layout
         ops.write_context_kv(kv.view(rows.shape[0], len(self.model.layers), 2, self.heads, self.head_dim),
                              positions, slots, self.context_k_norm, self.rope, bases, strides, page, self.k_eps)
@@ -164,7 +211,12 @@ class DraftStep:
     def write_context(self, states: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, layout) -> None:
         """The target's hidden states ``(tokens, n_layers * H)`` at ``positions``, stored
         at ``slots`` (precompute_and_store_context_kv, flashmap/vllm/model.py:759-767)."""
-        self.write_rows(self.model.hidden_norm(F.linear(states, self.model.fc.weight)), positions, slots, layout)
+        norm = self.model.hidden_norm
+        if self.mx_layers is None:
+            rows = norm(F.linear(states, self.model.fc.weight))
+        else:
+            rows = ops.rms_norm_mx(ops.mx_linear(states, self.mx_fc), norm.weight, norm.eps)[1]
+        self.write_rows(rows, positions, slots, layout)
 
     # -- the step --------------------------------------------------------------------
 
@@ -184,7 +236,12 @@ class DraftStep:
             raise ValueError(f"the noise must be float32 ({batch * k}, {self.noise_columns}), "
                              f"got {z.dtype} {tuple(z.shape)}")
         layout = layout or self.cache_layout(caches)
-        anchor_rows = model.anchor_norm(model.anchor_proj(F.embedding(anchors, self.embed_weight)))
+        anchor_rows = F.embedding(anchors, self.embed_weight)
+        if self.mx_layers is None:
+            anchor_rows = model.anchor_norm(model.anchor_proj(anchor_rows))
+        else:
+            anchor_rows = ops.mx_linear(anchor_rows, self.mx_anchor, model.anchor_proj.bias)
+            anchor_rows = ops.rms_norm_mx(anchor_rows, model.anchor_norm.weight, model.anchor_norm.eps)[1]
         self.write_rows(anchor_rows, anchor_positions, anchor_slots, layout)
         seqused_k = (anchor_positions + 1).to(torch.int32)
         if plan is None:
@@ -194,10 +251,9 @@ class DraftStep:
                   torch.arange(0, batch * k + 1, k, dtype=torch.int32, device=anchors.device))
         if self.num_steps == 1:
             z16, row_scale = ops.noise_rows(z, self.noise_eigvals, self.noise_eps, self.noise_gains[0])
-            noise = F.linear(z16, self.noise_embed)
+            noise = F.linear(z16, self.noise_embed) if self.mx_layers is None else product(z16, self.noise_embed)
             eps = model.layers[0].self_attn_adaln.eps if len(model.layers) else model.final_adaln.eps
-            hidden, h = ops.adaln_residual(self.first_hidden, noise, row_scale, self._first_norm(0), eps,
-                                           gate_per_row=True)
+            hidden, h = self._norm(0)(self.first_hidden, noise, row_scale, self._first_norm(0), eps, gate_per_row=True)
             return self._dit(hidden, h, 0, attend)
         # The state is updated in place between the jumps: a copy of the caller's noise,
         # in rows padded to a multiple of 4 values (the row kernels' 16-byte chunks).
@@ -208,11 +264,17 @@ class DraftStep:
         for step, (start, _, end) in enumerate(self.jumps):
             hidden = self._embed_state(state, step)
             eps = model.layers[0].self_attn_adaln.eps if len(model.layers) else model.final_adaln.eps
-            h = ops.adaln_residual(hidden, None, None, self._first_norm(step), eps)[1]
+            h = self._norm(0)(hidden, None, None, self._first_norm(step), eps)[1]
             h = self._dit(hidden, h, step, attend)
             if step + 1 < self.num_steps:
-                ops.state_update(state, F.linear(h, *self.jump_head), start, end)
+                logits = F.linear(h, *self.jump_head) if self.mx_layers is None else product(h, *self.jump_head)
+                ops.state_update(state, logits, start, end)
         return h
+
+    def _norm(self, layer: int):
+        """The norm in front of layer ``layer``'s projections: microscaled output where its
+        weights are; the final norm's (behind the last layer) is bf16."""
+        return ops.adaln_residual if self.mx_layers is None or layer >= len(self.mx_layers) else ops.adaln_residual_mx
 
     def _first_norm(self, step: int):
         """``(scale, shift)`` of the norm the jump's DiT input goes through first."""
@@ -235,6 +297,8 @@ class DraftStep:
             posterior_emb, state_emb = both.split(state.shape[0])
             posterior = model.state_norm(posterior_emb)
         embedded = (self.noise_gains[step] * model.noise_norm(state_emb)).to(weight.dtype)
+        if self.mx_embed is not None:
+            return ops.mx_linear(posterior + embedded, self.mx_embed, model.x_embed.bias)
         return model.x_embed(posterior + embedded)
 
     def _dit(self, hidden: torch.Tensor, h: torch.Tensor, step: int, attend) -> torch.Tensor:
@@ -248,29 +312,31 @@ class DraftStep:
         for i, layer in enumerate(model.layers):
             (_, _, g_self), (c_scale, c_shift, g_cross), (m_scale, m_shift, g_mlp) = mods[i]
             self_qn, self_kn, cross_qn = self.norms[i]
-            attn = ops.block_self_attention(ops.linear(h, self.self_qkv[i]).view(batch, k, 3, heads, hd),
+            held = None if self.mx_layers is None else self.mx_layers[i]
+            attn = ops.block_self_attention(product(h, self.self_qkv[i]).view(batch, k, 3, heads, hd),
                                             self_qn, self_kn, self.rope, slot_positions, layer.self_attn.q_norm.eps)
-            y = ops.linear(attn.view(tokens, self.dim), layer.self_attn.o_proj.weight)
-            hidden, h = ops.adaln_residual(hidden, y, g_self, (c_scale, c_shift), layer.cross_attn_adaln.eps,
-                                           x_out=hidden)
-            query = ops.linear(h, layer.cross_attn.q_proj.weight).view(tokens, heads, hd)
+            y = product(attn.view(tokens, self.dim), held.self_o if held else layer.self_attn.o_proj.weight)
+            hidden, h = self._norm(i)(hidden, y, g_self, (c_scale, c_shift), layer.cross_attn_adaln.eps, x_out=hidden)
+            query = product(h, held.cross_q if held else layer.cross_attn.q_proj.weight).view(tokens, heads, hd)
             prologue = ops.Prologue(cross_qn, self.rope, slot_positions, layer.cross_attn.q_norm.eps)
             ctx = ops.block_attention_paged(query, caches[i], cu, seqused_k, block_table, k, self.max_model_len,
                                             self.scale, prologue=prologue, plan=plan)
-            y = ops.linear(ctx.view(tokens, self.dim), layer.cross_attn.o_proj.weight)
-            hidden, h = ops.adaln_residual(hidden, y, g_cross, (m_scale, m_shift), layer.mlp_adaln.eps, x_out=hidden)
-            y = layer.mlp(h)
+            y = product(ctx.view(tokens, self.dim), held.cross_o if held else layer.cross_attn.o_proj.weight)
+            hidden, h = self._norm(i)(hidden, y, g_cross, (m_scale, m_shift), layer.mlp_adaln.eps, x_out=hidden)
+            y = held.mlp(h) if held else layer.mlp(h)
             if i + 1 < len(model.layers):
                 nxt, eps = mods[i + 1][0][:2], model.layers[i + 1].self_attn_adaln.eps
             else:
                 nxt, eps = self.final_mods[step], model.final_adaln.eps
-            hidden, h = ops.adaln_residual(hidden, y, g_mlp, nxt, eps, x_out=hidden)
+            hidden, h = self._norm(i + 1)(hidden, y, g_mlp, nxt, eps, x_out=hidden)
         return h  # without layers: the first norm, which is then the final one
 
     def logits(self, hidden: torch.Tensor) -> torch.Tensor:
         """Draft logits over the draft vocabulary (compute_draft_logits,
         flashmap/vllm/model.py:1039-1041)."""
-        return F.linear(hidden, self.head_weight, self.head_bias)
+        if self.mx_layers is None:
+            return F.linear(hidden, self.head_weight, self.head_bias)
+        return product(hidden, self.head_weight, self.head_bias)
 
     def greedy(self, hidden: torch.Tensor) -> torch.Tensor:
         """Greedy draft tokens ``(rows,)`` as target token ids (``split_argmax`` on the

@@ -25,6 +25,9 @@ kernel of this library:
 The plugin's drafts of several jumps go through its jump bank (flashmap/sglang/
 jump_bank.py), a different scheme from the vLLM plugin's vocabulary-sized state; this
 step takes one jump. GEMMs are hipBLASLt through torch; bf16 only.
+
+With ``mx`` the projections and the head are held in microscaled 4 bits and their inputs go to
+8 on the way out of the norms and activations, as in ``flashmap_amd.draft_step``.
 """
 
 from __future__ import annotations
@@ -33,6 +36,7 @@ import torch
 import torch.nn.functional as F
 
 from . import ops
+from .draft_step import MXLayer, product
 from .drafter import FlashMapDraftModel, jump_times
 from .fold import fold_head, fold_noise
 from .sglang import rope_freqs
@@ -45,11 +49,12 @@ class SGLangDraftStep:
     drafter (bf16, on the GPU); ``embed_tokens`` / ``lm_head``: the target's ``(V, H)``
     weights; ``max_positions``: the positions the pool writer's rotary table covers (the
     server's longest request plus a block); ``hot_ids``: the draft vocabulary's token ids
-    (a drafter's ``draft_ids``), else None."""
+    (a drafter's ``draft_ids``), else None; ``mx``: hold the projections and the head in
+    microscaled 4 bits."""
 
     @torch.no_grad()
     def __init__(self, model: FlashMapDraftModel, embed_tokens: torch.Tensor, lm_head: torch.Tensor,
-                 max_positions: int, hot_ids: torch.Tensor | None = None):
+                 max_positions: int, hot_ids: torch.Tensor | None = None, mx: bool = False):
         cfg = model.config
         if model.dtype != torch.bfloat16:
             raise TypeError("the draft step's kernels are bf16: move the drafter to torch.bfloat16")
@@ -89,6 +94,13 @@ class SGLangDraftStep:
         self.writer_rope = ops.rope_from_cat(self.cos_sin)
         self.head_weight, self.head_bias = fold_head(lm_head, model.head.weight, model.head.bias, hot_ids)
         self.scale = self.head_dim ** -0.5
+        self.mx_layers = self.mx_fc = self.mx_anchor = None
+        if mx:
+            self.mx_layers = [MXLayer(layer, qkv) for layer, qkv in zip(layers, self.self_qkv)]
+            self.self_qkv = [layer.qkv for layer in self.mx_layers]
+            self.mx_fc, self.mx_anchor, self.ctx_kv_weight, self.noise_embed, self.head_weight = (
+                ops.mx_quantize(w, 4) for w in (model.fc.weight, model.anchor_proj.weight, self.ctx_kv_weight,
+                                                self.noise_embed, self.head_weight))
 
     # -- the context -----------------------------------------------------------------
 
@@ -105,10 +117,11 @@ class SGLangDraftStep:
                             dtype=torch.int64, device=k_bufs[0].device)
 
     @torch.no_grad()
-    def write_rows(self, rows: torch.Tensor, positions: torch.Tensor, locs: torch.Tensor, meta: torch.Tensor) -> None:
-        """Every layer's keys (k-normed, rotated) and values of ``rows (tokens, dim)``,
-        stored at pool rows ``locs`` (``_kv_write``, flashmap/sglang/model.py:746-766)."""
-        kv = F.linear(rows, self.ctx_kv_weight)
+    def write_rows(self, rows, positions: torch.Tensor, locs: torch.Tensor, meta: torch.Tensor) -> None:
+        """Every layer's keys (k-normed, rotated) and values of ``rows (tokens, dim)`` (bf16, or
+        microscaled where the weights are), stored at pool rows ``locs`` (``_kv_write``,
+        flashmap/sglang/model.py:746-766)."""
+        kv = F.linear(rows, self.ctx_kv_weight) if self.mx_layers is None else product(rows, self.ctx_kv_weight)
         ops.write_context_kv_pool(kv, meta, self.k_norms, self.writer_rope, positions, locs, len(self.model.layers),
                                   self.dim, self.head_dim, self.k_eps)
 
@@ -117,7 +130,12 @@ class SGLangDraftStep:
                       meta: torch.Tensor) -> None:
         """The target's hidden states ``(tokens, n_layers * H)`` at ``positions``, stored at
         pool rows ``locs`` (``write_target_hidden_kv``, flashmap/sglang/model.py:700-744)."""
-        self.write_rows(self.model.hidden_norm(F.linear(states, self.model.fc.weight)), positions, locs, meta)
+        norm = self.model.hidden_norm
+        if self.mx_layers is None:
+            rows = norm(F.linear(states, self.model.fc.weight))
+        else:
+            rows = ops.rms_norm_mx(ops.mx_linear(states, self.mx_fc), norm.weight, norm.eps)[1]
+        self.write_rows(rows, positions, locs, meta)
 
     # -- the step --------------------------------------------------------------------
 
@@ -138,7 +156,12 @@ class SGLangDraftStep:
             raise ValueError(f"the noise must be float32 ({blocks * k}, {self.noise_embed.shape[1]}), "
                              f"got {z.dtype} {tuple(z.shape)}")
         meta = self.pool_meta(k_bufs, v_bufs) if meta is None else meta
-        anchor_rows = model.anchor_norm(model.anchor_proj(F.embedding(anchors, self.embed_weight)))
+        anchor_rows = F.embedding(anchors, self.embed_weight)
+        if self.mx_layers is None:
+            anchor_rows = model.anchor_norm(model.anchor_proj(anchor_rows))
+        else:
+            anchor_rows = ops.mx_linear(anchor_rows, self.mx_anchor, model.anchor_proj.bias)
+            anchor_rows = ops.rms_norm_mx(anchor_rows, model.anchor_norm.weight, model.anchor_norm.eps)[1]
         self.write_rows(anchor_rows, anchor_positions, anchor_locs, meta)
         cache_seqlens = (anchor_positions + 1).to(torch.int32)
         if plan is None:
@@ -150,39 +173,44 @@ class SGLangDraftStep:
             freqs = freqs.repeat_interleave(n_cand, dim=0)
         rope = ops.rope_from_table(freqs.reshape(blocks * k, self.head_dim // 2, 2).contiguous())
         z16, row_scale = ops.noise_rows(z, self.noise_eigvals, self.noise_eps, self.noise_gain)
-        noise = F.linear(z16, self.noise_embed)
+        noise = F.linear(z16, self.noise_embed) if self.mx_layers is None else product(z16, self.noise_embed)
         mods = self.layer_mods
         first = mods[0][0] if mods else self.final_mod
         eps = model.layers[0].self_attn_adaln.eps if mods else model.final_adaln.eps
-        hidden, h = ops.adaln_residual(self.first_hidden, noise, row_scale, (first[0], first[1]), eps,
-                                       gate_per_row=True)
+        # in front of a layer's projections: microscaled where its weights are; the final norm's bf16
+        norm = ops.adaln_residual if self.mx_layers is None else ops.adaln_residual_mx
+        hidden, h = (norm if mods else ops.adaln_residual)(self.first_hidden, noise, row_scale, (first[0], first[1]),
+                                                           eps, gate_per_row=True)
         heads, hd, tokens = self.heads, self.head_dim, blocks * k
         for i, layer in enumerate(model.layers):
             (_, _, g_self), (c_scale, c_shift, g_cross), (m_scale, m_shift, g_mlp) = mods[i]
             self_qn, self_kn, cross_qn = self.norms[i]
-            attn = ops.block_self_attention(ops.linear(h, self.self_qkv[i]).view(blocks, k, 3, heads, hd),
+            held = None if self.mx_layers is None else self.mx_layers[i]
+            attn = ops.block_self_attention(product(h, self.self_qkv[i]).view(blocks, k, 3, heads, hd),
                                             self_qn, self_kn, rope, None, layer.self_attn.q_norm.eps)
-            y = ops.linear(attn.view(tokens, self.dim), layer.self_attn.o_proj.weight)
-            hidden, h = ops.adaln_residual(hidden, y, g_self, (c_scale, c_shift), layer.cross_attn_adaln.eps,
-                                           x_out=hidden)
-            query = ops.linear(h, layer.cross_attn.q_proj.weight).view(requests, n_cand * k, heads, hd)
+            y = product(attn.view(tokens, self.dim), held.self_o if held else layer.self_attn.o_proj.weight)
+            hidden, h = norm(hidden, y, g_self, (c_scale, c_shift), layer.cross_attn_adaln.eps, x_out=hidden)
+            query = product(h, held.cross_q if held else layer.cross_attn.q_proj.weight)
+            query = query.view(requests, n_cand * k, heads, hd)
             prologue = ops.Prologue(cross_qn, rope, None, layer.cross_attn.q_norm.eps)
             ctx = ops.block_attention_token_paged(query, k_bufs[i], v_bufs[i], cache_seqlens, page_table,
                                                   self.scale, prologue=prologue, plan=plan)
-            y = ops.linear(ctx.view(tokens, self.dim), layer.cross_attn.o_proj.weight)
-            hidden, h = ops.adaln_residual(hidden, y, g_cross, (m_scale, m_shift), layer.mlp_adaln.eps, x_out=hidden)
-            y = layer.mlp(h)
+            y = product(ctx.view(tokens, self.dim), held.cross_o if held else layer.cross_attn.o_proj.weight)
+            hidden, h = norm(hidden, y, g_cross, (m_scale, m_shift), layer.mlp_adaln.eps, x_out=hidden)
+            y = held.mlp(h) if held else layer.mlp(h)
             if i + 1 < len(model.layers):
-                nxt, eps = mods[i + 1][0][:2], model.layers[i + 1].self_attn_adaln.eps
+                nxt, eps, follow = mods[i + 1][0][:2], model.layers[i + 1].self_attn_adaln.eps, norm
             else:
-                nxt, eps = self.final_mod, model.final_adaln.eps
-            hidden, h = ops.adaln_residual(hidden, y, g_mlp, nxt, eps, x_out=hidden)
+                nxt, eps, follow = self.final_mod, model.final_adaln.eps, ops.adaln_residual
+            hidden, h = follow(hidden, y, g_mlp, nxt, eps, x_out=hidden)
         return h
 
     def logits(self, hidden: torch.Tensor) -> torch.Tensor:
         """Draft-vocabulary logits (``head_logits``, the folded head,
         flashmap/sglang/model.py:511-513)."""
-        return F.linear(hidden, self.head_weight, self.head_bias)
+        if self.mx_layers is None:
+            return F.linear(hidden, self.head_weight, self.head_bias)
+        return product(hidden, self.head_weight, self.head_bias)
 
     def sample(self, hidden: torch.Tensor, temperatures: torch.Tensor, greedy: torch.Tensor,
                seed: torch.Tensor) -> torch.Tensor:

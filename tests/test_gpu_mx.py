@@ -1,55 +1,17 @@
 """Microscaled rows on the GPU (flashmap_amd.ops.mx_*, rms_norm_mx, adaln_residual_mx) against
-float64 (oracle/mx.py).
-
-Quantization of a tensor's own values is one rounding of exact quotients: codes and scales are
-equal to the oracle's. Where a value is computed before it is quantized (an activation, a
-norm) it is off by its float32 error, which moves a code only past a midpoint: the codes must
-lie between the oracle's for the value less and plus that error. A product's bound counts the
-bf16 rounding (2^-8 of the result) and what the sums lose of their absolute sum: 2^-15 for the
-float32 sums of groups, steps and parts (probed with single products: a term is cut below 2^-20
-of the largest of the 16 groups of a step, 16 2^-20; 160 steps and 8 parts of 2^-23 each), and
-with an 8-bit operand 7 2^-13 < 2^-10 more: the instruction adds the 8 products of a group after
-cutting each below 2^-13 of the power of two of the group's largest (probed likewise), so that 7
-of them lose less than 2^-13 of the largest, and the largest is at most the group's absolute
-sum. Products within 2^12 of each other lose nothing there, which
-``test_linear_of_even_magnitudes`` holds the kernels to."""
+float64 (oracle/mx.py), with the bounds of _mx_checks.py; quantization of a tensor's own values is
+one rounding of exact quotients, and its codes and scales are equal to the oracle's."""
 
 import pytest
 import torch
 
 from _inputs import gen
+from _mx_checks import (activations, check_activation, check_adaln, check_product, check_rms_norm, codes_of,
+                        operand)
 from flashmap_amd import ops
 from oracle import mx
 
 pytestmark = pytest.mark.gpu
-
-
-def _cpu(q: ops.MX):
-    """(codes one per value, scales) on the CPU, padding included."""
-    return mx.unpack(q.codes.cpu(), q.bits), q.scales.cpu()
-
-
-def _activations(rows, cols, seed, dtype=torch.bfloat16):
-    g = gen(seed)
-    return (torch.randn(rows, cols, generator=g) * torch.exp(torch.randn(cols, generator=g))).to(dtype)
-
-
-def _between(q: ops.MX, v: torch.Tensor, tol: torch.Tensor) -> None:
-    """Every code of ``q`` is the code of some value within ``tol`` of ``v`` (float64)."""
-    code, scale = _cpu(q)
-    got = mx.values(code, scale, q.bits)
-    (lc, ls), (hc, hs) = mx.quantize(v - tol, q.bits), mx.quantize(v + tol, q.bits)
-    down, up = mx.quantize(v.abs() - tol, q.bits)[1], mx.quantize(v.abs() + tol, q.bits)[1]
-    assert ((scale >= down.minimum(up)) & (scale <= down.maximum(up))).all(), "a scale away from its block's maximum"
-    lo, hi = mx.values(lc, scale.minimum(ls), q.bits), mx.values(hc, scale.maximum(hs), q.bits)
-    same = ((ls == scale) & (hs == scale)).repeat_interleave(32, 1)
-    inside = (got >= lo) & (got <= hi)
-    assert inside[same].all(), f"{int((~inside & same).sum())} codes outside their interval"
-    # where the error moves the block's maximum over a power of two: within a code of it
-    step = 2.0 ** (scale.double() - 127).repeat_interleave(32, 1) * (32 if q.bits == 8 else 2)
-    full = torch.zeros_like(got)
-    full[:, : v.shape[1]] = v
-    assert ((got - full).abs() <= step)[~same].all()
 
 
 SIZES = [(1, 1), (3, 31), (2, 32), (5, 33), (17, 127), (1, 128), (4, 129), (33, 200), (7, 2056), (3, 20480)]
@@ -60,9 +22,9 @@ SIZES = [(1, 1), (3, 31), (2, 32), (5, 33), (17, 127), (1, 128), (4, 129), (33, 
 @pytest.mark.parametrize("rows,cols", SIZES)
 def test_quantize_is_exact(dev, rows, cols, dtype, bits):
     print(f"mx_quantize {rows} x {cols} {dtype} bits={bits}", flush=True)
-    x = _activations(rows, cols, rows + cols, dtype)
+    x = activations(rows, cols, rows + cols, dtype)
     q = ops.mx_quantize(x.to(dev), bits)
-    code, scale = _cpu(q)
+    code, scale = codes_of(q)
     wc, ws = mx.quantize(x, bits)
     assert q.shape == (rows, cols) and torch.equal(scale, ws) and torch.equal(code, wc)
     back = ops.mx_dequantize(q, torch.float32)
@@ -94,7 +56,7 @@ def test_quantize_edges(dev, bits):
     x[:, 0::32] = torch.where(x[:, 0::32].abs() < x[:, -1:].abs(), x[:, -1:], x[:, 0::32])
     q = ops.mx_quantize(x.to(dev), bits)
     wc, ws = mx.quantize(x, bits)
-    code, scale = _cpu(q)
+    code, scale = codes_of(q)
     assert torch.equal(scale, ws)
     fine = (ws != 255).repeat_interleave(32, 1)
     assert torch.equal(code[fine], wc[fine])
@@ -107,45 +69,26 @@ def test_quantize_edges(dev, bits):
 @pytest.mark.parametrize("rows,cols,dtype", [(3, 33, torch.float32), (16, 8192, torch.bfloat16),
                                              (5, 200, torch.float16), (1, 1, torch.bfloat16), (9, 260, torch.float32)])
 def test_activation(dev, rows, cols, dtype, activation, bits):
-    x = _activations(rows, cols * (2 if activation == "swiglu" else 1), 5 * cols, dtype).clamp(-9, 9)
-    want = mx.gelu(x) if activation == "gelu" else mx.swiglu(x)
-    # erfc(z) moves by 2 z^2 of its argument's relative error, z^2 = x^2 / 2; exp(-g) by g
-    tol = 2.0 ** -22 * (8 + x.double()[:, :cols] ** 2) * want.abs()
-    _between(ops.mx_quantize(x.to(dev), bits, activation), want, tol)
+    x = activations(rows, cols * (2 if activation == "swiglu" else 1), 5 * cols, dtype).clamp(-9, 9)
+    check_activation(ops.mx_quantize(x.to(dev), bits, activation), x, activation)
 
 
 def test_layouts(dev):
     """Leading dimensions, strided and unaligned rows, expanded rows, no rows."""
-    wide = _activations(12, 520, 3).to(dev)
+    wide = activations(12, 520, 3).to(dev)
     want = ops.mx_quantize(wide[:, :256].contiguous())
     for x in (wide[:, :256], torch.cat([wide.new_zeros(1), wide[:, :256].reshape(-1)])[1:].view(12, 256),
               wide[:, :256].t().contiguous().t(), wide[:, :256].reshape(3, 4, 256)):
         q = ops.mx_quantize(x)
         assert q.shape == tuple(x.shape) and torch.equal(q.codes, want.codes) and torch.equal(q.scales, want.scales)
     odd = ops.mx_quantize(wide[:, 3:260])
-    assert torch.equal(_cpu(odd)[0], mx.quantize(wide[:, 3:260].cpu(), 8)[0])
+    assert torch.equal(codes_of(odd)[0], mx.quantize(wide[:, 3:260].cpu(), 8)[0])
     one = ops.mx_quantize(wide[:1, :256].expand(12, 256))
     assert torch.equal(one.codes, want.codes[:1].expand(12, -1))
     empty = ops.mx_quantize(wide[:0])
     assert empty.rows == 0 and ops.mx_dequantize(empty).shape == (0, 520)
     assert ops.mx_linear(empty, ops.mx_quantize(wide, 4)).shape == (0, 12)
     assert ops.mx_quantize(wide[0]).shape == (520,)
-
-
-def _x_of(kind, x):
-    """What the product is given and the float64 values that it stands for."""
-    if kind == "bf16":
-        return x, mx.values(*mx.quantize(x.cpu(), 8), 8)
-    q = ops.mx_quantize(x, kind)
-    return q, mx.values(*_cpu(q), kind)
-
-
-def _check_product(got, xv, wv, bias, sums=2.0 ** -15 + 2.0 ** -10):
-    ref = xv @ wv.T + (0 if bias is None else bias.cpu().double())
-    total = xv.abs() @ wv.abs().T + (0 if bias is None else bias.cpu().double().abs())
-    err = (got.cpu().double() - ref).abs()
-    bad = err > 2.0 ** -8 * ref.abs() + sums * total
-    assert not bad.any(), f"{int(bad.sum())} results off, by up to {(err / total)[bad].max():.2e} of the absolute sum"
 
 
 @pytest.mark.parametrize("kind", ["bf16", 8, 4])
@@ -161,13 +104,13 @@ def _check_product(got, xv, wv, bias, sums=2.0 ** -15 + 2.0 ** -10):
     (2048, 2048, 256), (1920, 2500, 384), (3300, 4100, 128), (2048, 6144, 640), (4096, 4096, 200)])
 def test_linear(dev, rows, n, k, kind):
     print(f"mx_linear rows={rows} n={n} k={k} x={kind}", flush=True)
-    x = _activations(rows, k, rows + n + k).to(dev)
+    x = activations(rows, k, rows + n + k).to(dev)
     w = ops.mx_quantize(torch.randn(n, k, generator=gen(n)).to(dev) / k ** 0.5, 4)
     bias = torch.randn(n, generator=gen(k)).bfloat16().to(dev) if (rows + n) % 2 else None
-    given, xv = _x_of(kind, x)
+    given, xv = operand(kind, x)
     got = ops.mx_linear(given, w, bias)
     assert got.shape == (rows, n) and got.dtype == torch.bfloat16
-    _check_product(got, xv, mx.values(*_cpu(w), 4), bias, 2.0 ** -15 + (0 if kind == 4 else 2.0 ** -10))
+    check_product(got, xv, mx.values(*codes_of(w), 4), bias, 2.0 ** -15 + (0 if kind == 4 else 2.0 ** -10))
 
 
 @pytest.mark.parametrize("kind", ["bf16", 8])
@@ -180,8 +123,8 @@ def test_linear_of_even_magnitudes(dev, rows, n, k, kind):
     x = (1 + torch.rand(rows, k, generator=g)) * torch.randint(0, 2, (rows, k), generator=g).mul(2).sub(1)
     x = x * torch.randint(-6, 7, (rows, -(-k // 32)), generator=g).float().exp2().repeat_interleave(32, 1)[:, :k]
     w = ops.mx_quantize(torch.randn(n, k, generator=g).to(dev), 4)
-    given, xv = _x_of(kind, x.bfloat16().to(dev))
-    _check_product(ops.mx_linear(given, w), xv, mx.values(*_cpu(w), 4), None, 2.0 ** -15)
+    given, xv = operand(kind, x.bfloat16().to(dev))
+    check_product(ops.mx_linear(given, w), xv, mx.values(*codes_of(w), 4), None, 2.0 ** -15)
 
 
 @pytest.mark.parametrize("kind", ["bf16", 8, 4])
@@ -189,7 +132,7 @@ def test_linear_of_even_magnitudes(dev, rows, n, k, kind):
 def test_linear_layouts(dev, rows, kind):
     """Leading dimensions, a strided x and out, an out that already holds values around it."""
     n, k = 100, 300
-    base = _activations(rows, k + 20, 7).to(dev)
+    base = activations(rows, k + 20, 7).to(dev)
     w = ops.mx_quantize(torch.randn(n, k, generator=gen(1)).to(dev), 4)
     x = base[:, 5:5 + k]
     given = x if kind == "bf16" else ops.mx_quantize(x, kind)
@@ -215,13 +158,13 @@ def test_linear_layouts(dev, rows, kind):
 def test_linear_not_finite(dev, rows, kind):
     """A block with an infinity or a NaN makes its row's (or column's) results NaN and no others."""
     n, k = 90, 416
-    x, wv = _activations(rows, k, 1), torch.randn(n, k, generator=gen(2))
+    x, wv = activations(rows, k, 1), torch.randn(n, k, generator=gen(2))
     x[1, 77], x[2, 3] = float("nan"), float("inf")
     wv[5, 400], wv[89, 0] = -float("inf"), float("nan")
     w = ops.mx_quantize(wv.to(dev), 4)
-    given, xv = _x_of(kind, x.to(dev))
+    given, xv = operand(kind, x.to(dev))
     got = ops.mx_linear(given, w).cpu()
-    bad = torch.isnan(xv).any(1)[:, None] | torch.isnan(mx.values(*_cpu(w), 4)).any(1)[None]
+    bad = torch.isnan(xv).any(1)[:, None] | torch.isnan(mx.values(*codes_of(w), 4)).any(1)[None]
     assert torch.equal(torch.isnan(got), bad) and bad[:3].float().sum() == n * 2 + 2
 
 
@@ -231,8 +174,8 @@ def test_linear_extreme_scales(dev, kind):
     rows, n, k = 20, 40, 256
     x = torch.randn(rows, k, generator=gen(1)) * 2.0 ** torch.linspace(-100, 100, rows)[:, None]
     w = ops.mx_quantize((torch.randn(n, k, generator=gen(2)) * 2.0 ** -20).to(dev), 4)
-    given, xv = _x_of(kind, x.bfloat16().to(dev))
-    _check_product(ops.mx_linear(given, w), xv, mx.values(*_cpu(w), 4), None)
+    given, xv = operand(kind, x.bfloat16().to(dev))
+    check_product(ops.mx_linear(given, w), xv, mx.values(*codes_of(w), 4), None)
 
 
 NORM_SIZES = [(1, 1), (5, 33), (3, 129), (16, 512), (33, 2048), (7, 2056), (2, 4100), (9, 8192), (2, 16384)]
@@ -244,21 +187,13 @@ NORM_SIZES = [(1, 1), (5, 33), (3, 129), (16, 512), (33, 2048), (7, 2056), (2, 4
 def test_rms_norm(dev, rows, cols, with_residual, bits):
     print(f"rms_norm_mx {rows} x {cols} residual={with_residual} bits={bits}", flush=True)
     g = gen(rows + cols)
-    x, w = _activations(rows, cols, cols), 0.5 + torch.rand(cols, generator=g)
+    x, w = activations(rows, cols, cols), 0.5 + torch.rand(cols, generator=g)
     res = torch.randn(rows, cols, generator=g).bfloat16() if with_residual else None
     stream, q = ops.rms_norm_mx(x.to(dev), w.to(dev), 1e-6, None if res is None else res.to(dev))
     if bits == 4:
         q = ops.rms_norm_mx(x.to(dev), w.to(dev), 1e-6, None if res is None else res.to(dev), bits=4)[1]
-    s, want = mx.rms_norm(x, res, w, 1e-6)
-    # a thread's 64 squares and the join of 256 threads: 76 roundings of positive terms, half of
-    # it by the root; the sum s, the root and two products
-    tol = want.abs() * (38 + 8) * 2.0 ** -24
-    if res is not None:
-        tol = tol + 2.0 ** -24 * (x.double().abs() + res.double().abs()) * (want / s).abs().nan_to_num(0, 0, 0)
-        assert ((stream.cpu().double() - s).abs() <= 2.0 ** -8 * s.abs() + 2.0 ** -24 * s.abs()).all()
-    else:
-        assert stream is None
-    _between(q, want, tol)
+    assert (stream is None) == (res is None)
+    check_rms_norm(stream, q, x, res, w, 1e-6)
 
 
 @pytest.mark.parametrize("bits", [8, 4])
@@ -267,7 +202,7 @@ def test_rms_norm(dev, rows, cols, with_residual, bits):
 def test_adaln(dev, rows, cols, part, bits):
     print(f"adaln_residual_mx {rows} x {cols} {part} bits={bits}", flush=True)
     g = gen(rows + cols)
-    x = (_activations(rows, cols, cols) + 0.25)
+    x = (activations(rows, cols, cols) + 0.25)
     y = torch.randn(rows, cols, generator=g).bfloat16()
     gate, scale, shift = (0.3 * torch.randn(3, cols, generator=g)).bfloat16().unbind(0)
     gr = gate
@@ -280,25 +215,12 @@ def test_adaln(dev, rows, cols, part, bits):
     stream, q = ops.adaln_residual_mx(x.to(dev), None if given_y is None else y.to(dev), gate.to(dev),
                                       (scale.to(dev), shift.to(dev)), 1e-6, gate_per_row=part == "per_row", bits=bits)
     xs = x.expand(rows, cols) if part == "shared" else x
-    s, want = mx.adaln(xs, given_y, gr, scale, shift, 1e-6)
-    err_s = 2.0 ** -24 * s.abs()  # the fused multiply-add's rounding
-    if given_y is not None:
-        assert ((stream.cpu().double() - s).abs() <= 2.0 ** -8 * s.abs() + err_s).all()
-    # the mean of a thread's 64 values and the join of 256 threads: 76 roundings of the absolute
-    # sum; the centred value takes its error and its own, the root half of 80 roundings
-    mean_err = 76 * 2.0 ** -24 * s.abs().mean(-1, keepdim=True)
-    c = (s - s.mean(-1, keepdim=True)).abs()
-    rstd = 1 / torch.sqrt((c * c).mean(-1, keepdim=True) + 1e-6)
-    centre = err_s + mean_err + 2.0 ** -24 * c
-    root = 44 * 2.0 ** -24 + (centre * c + centre ** 2).mean(-1, keepdim=True) * rstd ** 2
-    one = (1 + scale.double()).abs()
-    tol = one * rstd * (centre + c * (root + 4 * 2.0 ** -24)) + 2.0 ** -24 * want.abs()
-    _between(q, want, tol)
+    check_adaln(stream, q, xs, given_y, gr, scale, shift, 1e-6)
 
 
 def test_norms_in_place_and_strided(dev):
     rows, cols = 12, 264
-    wide = _activations(rows, cols + 33, 4).to(dev)
+    wide = activations(rows, cols + 33, 4).to(dev)
     x, y = wide[:, 1:1 + cols], torch.randn(rows, cols, generator=gen(1)).bfloat16().to(dev)
     v = [t.to(dev) for t in (0.3 * torch.randn(3, cols, generator=gen(2))).bfloat16().unbind(0)]
     w = torch.rand(cols, generator=gen(3)).to(dev)
@@ -331,7 +253,7 @@ def test_two_streams_and_a_graph(dev):
     between them."""
     n, k = 300, 1000
     w = ops.mx_quantize(torch.randn(n, k, generator=gen(1)).to(dev), 4)
-    xs = [_activations(r, k, r).to(dev) for r in (16, 200)]
+    xs = [activations(r, k, r).to(dev) for r in (16, 200)]
     want = [ops.mx_linear(x, w) for x in xs]
     stream = torch.cuda.Stream()
     stream.wait_stream(torch.cuda.current_stream())
@@ -360,7 +282,7 @@ def test_mlp_of_a_layer(dev):
     on what the step before it gave."""
     rows, dim, hidden = 48, 256, 800
     g = gen(11)
-    x, y = _activations(rows, dim, 1).to(dev), torch.randn(rows, dim, generator=g).bfloat16().to(dev)
+    x, y = activations(rows, dim, 1).to(dev), torch.randn(rows, dim, generator=g).bfloat16().to(dev)
     gate, scale, shift = (t.to(dev) for t in (0.3 * torch.randn(3, dim, generator=g)).bfloat16().unbind(0))
     fc1 = ops.mx_quantize((torch.randn(hidden, dim, generator=g) / 16).to(dev), 4)
     fc2 = ops.mx_quantize((torch.randn(dim, hidden, generator=g) / 28).to(dev), 4)
@@ -369,14 +291,13 @@ def test_mlp_of_a_layer(dev):
     up = ops.mx_linear(h, fc1, b1)
     mid = ops.mx_quantize(up, activation="gelu")
     out = ops.mx_linear(mid, fc2)
-    _check_product(up, mx.values(*_cpu(h), 8), mx.values(*_cpu(fc1), 4), b1)
-    want = mx.gelu(up.cpu())
-    _between(mid, want, 2.0 ** -22 * (8 + up.cpu().double() ** 2) * want.abs())
-    _check_product(out, mx.values(*_cpu(mid), 8), mx.values(*_cpu(fc2), 4), None)
+    check_product(up, mx.values(*codes_of(h), 8), mx.values(*codes_of(fc1), 4), b1)
+    check_activation(mid, up.cpu(), "gelu")
+    check_product(out, mx.values(*codes_of(mid), 8), mx.values(*codes_of(fc2), 4), None)
     s, norm = mx.adaln(*(t.cpu() for t in (x, y, gate, scale, shift)), 1e-6)
     # end to end: e4m3 activations (2^-4 each at most) in front of both products
-    ref = mx.gelu(norm @ mx.values(*_cpu(fc1), 4)[:, :dim].T + b1.cpu().double())
-    ref = ref @ mx.values(*_cpu(fc2), 4)[:, :hidden].T
+    ref = mx.gelu(norm @ mx.values(*codes_of(fc1), 4)[:, :dim].T + b1.cpu().double())
+    ref = ref @ mx.values(*codes_of(fc2), 4)[:, :hidden].T
     assert float((out.cpu().double() - ref).norm() / ref.norm()) < 2.0 ** -4
     assert stream.shape == x.shape
 
@@ -393,11 +314,11 @@ def test_rows_far_into_memory(dev):
     w = ops.MX(codes, scales, 4, (n, k))
     last = ops.MX(codes[-200:], scales[-200:], 4, (200, k))
     for rows in (1, 20, 300):
-        x = ops.mx_quantize(_activations(rows, k, rows).to(dev))
-        _check_product(ops.mx_linear(x, w)[:, -200:], mx.values(*_cpu(x), 8), mx.values(*_cpu(last), 4), None)
+        x = ops.mx_quantize(activations(rows, k, rows).to(dev))
+        check_product(ops.mx_linear(x, w)[:, -200:], mx.values(*codes_of(x), 8), mx.values(*codes_of(last), 4), None)
     # 4-bit rows as the many: x's rows far into memory too
     few = ops.MX(codes[:40], scales[:40], 4, (40, k))
-    _check_product(ops.mx_linear(w, few)[-200:], mx.values(*_cpu(last), 4), mx.values(*_cpu(few), 4), None)
+    check_product(ops.mx_linear(w, few)[-200:], mx.values(*codes_of(last), 4), mx.values(*codes_of(few), 4), None)
     back = ops.mx_dequantize(w)
     assert back.numel() > 1 << 32
     want = mx.values(mx.unpack(codes[-3:].cpu(), 4), scales[-3:].cpu(), 4)[:, :k]
