@@ -1461,6 +1461,23 @@ def _bf16_out(x_out: torch.Tensor | None, shape: tuple, device: torch.device,
     return x_out, rows, (rows.stride(0) if rows.shape[0] > 1 else cols)
 
 
+def _apart(name: str, out: torch.Tensor, out_stride: int, rows: int, cols: int, *others: tuple) -> None:
+    """Refuse a given output whose rows share bytes with rows that are read: ``others``
+    (tensor, stride, rows, cols, whether the very same rows may be given: each is read before
+    it is written)."""
+    size = out.element_size()
+    begin, step, width = out.data_ptr(), out_stride * size, cols * size
+    end = begin + (rows - 1) * step + width
+    for t, stride, count, wide, same in others:
+        size = t.element_size()
+        first, by, w = t.data_ptr(), stride * size, wide * size
+        if first >= end or first + (count - 1) * by + w <= begin or (same and first == begin and by == step):
+            continue
+        at = (first - begin) % step
+        if by != step or at < width or at + w > step:
+            raise ValueError(f"{name} overlaps rows that the call reads")
+
+
 def mx_quantize(x: torch.Tensor, bits: int = 8, activation: str | None = None) -> MX:
     """``x (..., cols)`` (bf16, fp16 or fp32) in microscaled form, ``bits`` 8 or 4: each block's
     scale is the power of two that brings its largest magnitude to [256, 512) (e4m3) or [4, 8)
@@ -1531,12 +1548,14 @@ def mx_linear(x: torch.Tensor | MX, weight: MX, bias: torch.Tensor | None = None
     if quantized:
         x_bits = x.bits
         xp, xs, xsp, xss, keep_x = _mx_args(x, "x")
+        read = keep_x[0], xs, rows, keep_x[0].shape[1], False
     else:
         if x.dtype is not torch.bfloat16:
             raise TypeError(f"x must be bfloat16 or microscaled, got {x.dtype}")
         _no_gradient("mx_linear", x, bias)
         keep_x, xs = _plain_rows(x, k, "x")
         xp = keep_x.data_ptr()
+        read = keep_x, xs, rows, k, False
         # the rows that the kernel quantizes itself; past these sums and columns a call of its own
         # is cheaper (16 rows, us: 8192 -> 2048 15.6 / 14, 20480 -> 2048 33.7 / 19)
         if (rows <= MX_BF16_ROWS and k % 8 == 0 and xs % 8 == 0 and xp % 16 == 0
@@ -1550,8 +1569,11 @@ def mx_linear(x: torch.Tensor | MX, weight: MX, bias: torch.Tensor | None = None
             raise ValueError(f"bias must be bfloat16 ({n},), got {bias.dtype} {tuple(bias.shape)}")
         _no_gradient("mx_linear", bias)
         bias = bias.contiguous()
+    given = out is not None
     out, out_rows, stride = _bf16_out(out, (*lead, n), weight.codes.device, "out")
     if rows and n:
+        if given:
+            _apart("out", out_rows, stride, rows, n, read)
         nbytes = _mx_workspace_bytes(rows, n, k, x_bits)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=out.device) if nbytes else None
         _mx_call("fm_mx_linear", index, xp, x_bits, xs, xsp, xss, *w, _ptr(bias), out_rows.data_ptr(), stride, rows, n,
@@ -1580,7 +1602,10 @@ def rms_norm_mx(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: tor
         if residual.dtype != torch.bfloat16 or residual.shape != x.shape:
             raise ValueError(f"residual must be bfloat16 {shape}, got {residual.dtype} {tuple(residual.shape)}")
         rr, rs = _plain_rows(residual, cols, "residual")
+        given, rows = x_out is not None, q.codes.shape[0]
         x_out, orows, os_ = _bf16_out(x_out, shape, device, "x_out")
+        if given and rows:
+            _apart("x_out", orows, os_, rows, cols, (xr, xs, rows, cols, True), (rr, rs, rows, cols, True))
     elif x_out is not None:
         raise ValueError("x_out is the sum of x and a residual: give one")
     weight = _f32(weight)
@@ -1636,6 +1661,7 @@ def adaln_residual_mx(
         g = _mx_vec(gate, math.prod(shape[:-1]), "gate (one per row)") if gate_per_row else _mx_vec(gate, cols, "gate")
         if shared and x_out is not None and x_out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
             raise ValueError("x_out may not share the storage of a shared x row")
+        given = x_out is not None
         x_out, orows, os_ = _bf16_out(x_out, shape, device, "x_out")
     elif x_out is not None:
         raise ValueError("x_out is the sum of x and a gated y: give one")
@@ -1643,6 +1669,9 @@ def adaln_residual_mx(
     xr, xs = _plain_rows(x, cols, "x")
     q = _mx_new(shape, bits, device)
     rows = q.codes.shape[0]
+    if rows and y is not None and given:
+        _apart("x_out", orows, os_, rows, cols, (xr, xs, 1 if shared else rows, cols, not shared),
+               (yr, ys, rows, cols, True))
     if rows:
         _mx_call("fm_adaln_residual_mx", index, xr.data_ptr(), 0 if shared else xs, _ptr(yr), ys, _ptr(g),
                  int(gate_per_row), sc.data_ptr(), sh.data_ptr(), _ptr(orows), os_, eps, bits, *_mx_new_args(q), rows,

@@ -327,3 +327,34 @@ def test_rows_far_into_memory(dev):
     assert torch.equal(ops.mx_dequantize(again), back[-1000:])  # e2m1 values are e4m3 values
     far = ops.mx_quantize(back, 8)
     assert torch.equal(far.codes[-1000:], again.codes) and torch.equal(far.scales[-1000:], again.scales)
+
+
+def test_outputs_that_overlap_inputs(dev):
+    """An output over rows that the call reads is refused, but for the very same rows of a norm,
+    whose results equal those into a tensor of their own."""
+    buf = activations(34, 256, 5, torch.bfloat16).to(dev)
+    x, y = buf[:16, :128], buf[:16, 128:]
+    w = ops.mx_quantize(activations(128, 128, 6, torch.bfloat16).to(dev), 4)
+    for rows in (16, 17):
+        read = buf[:rows, :128]
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.mx_linear(read, w, out=read)
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.mx_linear(read, w, out=buf[1:rows + 1, :128])
+        want = ops.mx_linear(read, w)
+        side = buf.clone()
+        assert torch.equal(ops.mx_linear(side[:rows, :128], w, out=side[:rows, 128:]), want)
+        assert torch.equal(side[:, :128], buf[:, :128]) and torch.equal(side[rows:], buf[rows:])
+    v = buf[33, :128].clone()
+    for call in (lambda a, b, out: ops.rms_norm_mx(a, v, 1e-6, residual=b, x_out=out),
+                 lambda a, b, out: ops.adaln_residual_mx(a, b, v, (v, v), 1e-6, x_out=out)):
+        with pytest.raises(ValueError, match="overlaps"):
+            call(x, y, buf[1:17, :128])
+        with pytest.raises(ValueError, match="overlaps"):
+            call(x, y, buf[:16, 64:192])
+        s, q = call(x, y, None)
+        for half in (slice(0, 128), slice(128, 256)):
+            own = buf.clone()
+            t, p = call(own[:16, :128], own[:16, 128:], own[:16, half])
+            assert torch.equal(t, s) and torch.equal(p.codes, q.codes) and torch.equal(p.scales, q.scales)
+            assert torch.equal(own[16:], buf[16:])

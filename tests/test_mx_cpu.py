@@ -192,3 +192,30 @@ def test_entries_refuse_what_they_cannot_launch():
            4, 64, None)
     _fails("shared x row", inv, "fm_adaln_residual_mx", at, 0, at, 64, at, 0, at, at, at, 64, f, 8, at, 128, at, 4, 4,
            64, None)
+
+
+def test_outputs_over_rows_that_are_read():
+    """ops._apart: rows of one buffer side by side and the very same rows pass, others do not."""
+    from flashmap_amd import ops
+
+    buf = torch.zeros(40, 64, dtype=torch.bfloat16)
+    x = buf[:16, :32]
+    for name, out, same, refused in (
+        ("beside", buf[:16, 32:], False, False),
+        ("the same, read first", x, True, False),
+        ("the same, read by others", x, False, True),
+        ("behind", buf[16:32, :32], False, False),
+        ("a row on", buf[1:17, :32], True, True),
+        ("some columns on", buf[:16, 16:48], True, True),
+        ("from one row's end into the next", buf.view(-1)[48:48 + 16 * 64].view(16, 64)[:, :32], False, True),
+        ("another stride", buf.view(-1)[: 16 * 32].view(16, 32), True, True),
+    ):
+        args = ("out", out, out.stride(0), 16, 32, (x, 64, 16, 32, same))
+        if refused:
+            with pytest.raises(ValueError, match="overlaps rows"):
+                ops._apart(*args)
+        else:
+            ops._apart(*args)
+    ops._apart("out", buf[1:2], 64, 1, 64, (buf[0:1], 64, 1, 64, False))
+    with pytest.raises(ValueError):
+        ops._apart("out", buf[0:1, 8:], 56, 1, 56, (buf[0:1], 64, 1, 64, False))
