@@ -142,7 +142,9 @@ __device__ __forceinline__ void quantize_operand(const u32x4_t (&v)[4], int g, i
 }
 
 // A workgroup owns 16 NB rows of W against 16 MB rows of x; its wavefronts split k and meet in
-// LDS in a fixed order. XBITS 16: x in bf16, quantized in registers.
+// LDS in a fixed order. XBITS 16: x in bf16, quantized in registers. Bound: latency (a launch, the
+// loads of a wavefront's share of k, all in flight at once, and the join): 1 x 2048 -> 2048 4.7 us,
+// 16 x 2048 -> 8192 7.6 us, 9.3 MB.
 template <int XBITS, int MB, int NB, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void mx_linear_rows_kernel(const MxLinearArgs a) {
   __shared__ f32x4_t part[WAVES][NB * MB][64];
@@ -260,7 +262,8 @@ static int launch_rows(const MxLinearArgs &a, hipStream_t stream) {
 // streams whole 16-row blocks of W through a ring of its own in LDS, D groups of four steps
 // deep, and needs nobody: x, up to 16 MB rows of it, lies in LDS for the workgroup's whole
 // life, quantized once. A group: 16 rows of 256 bytes, as four loads of eight 128-byte
-// segments, and their scales, 16 bytes a row.
+// segments, and their scales, 16 bytes a row. Bound: HBM; 16 x 2048 -> 151936, 170 MB, 38 to 41 us,
+// 4.1 to 4.4 TB/s (with a workgroup per 16 columns and k split, 54.6 us).
 template <int XBITS, int MB, int WAVES, int D>
 struct Stream {
   static constexpr int GROUP = 4096 + 256, RING = D * GROUP;

@@ -162,6 +162,10 @@ __device__ __forceinline__ float swiglu(float gate, float up) {
   return gate * up * q;
 }
 
+// A thread per 8 values, no loop: every load of the call is in flight at once, and the rows need
+// nothing of each other. Bound: HBM without an activation (24576 x 2048 bf16 to 4 bits and back
+// 48.7 us, 5.2 TB/s, a copy's rate), VALU issue with GELU (1024 x 8192 bf16 to 8 bits 10.1 us, 2.5
+// TB/s, 32 instructions a value).
 template <typename T, int BITS, int ACT>
 __global__ __launch_bounds__(ROW_THREADS) void mx_quantize_kernel(const QuantArgs a) {
   const uint32_t item = blockIdx.x * ROW_THREADS + threadIdx.x;
@@ -270,6 +274,11 @@ __device__ __forceinline__ float row_sum(float v, float *lds) {
   return v;
 }
 
+// s = x + y or x + gate y, the stream; then s rsqrt(mean s^2 + eps) weight (RMS), or the LayerNorm
+// (s - mean) rsqrt(var + eps) (1 + scale) + shift, its variance of the differences from the mean.
+// TPR threads a row, NCH 8-value pieces each, held in registers between the one read and the one
+// write. Bound: HBM for many rows (8192 x 4096 with a residual 49.6 us, 4.8 TB/s), a launch and a
+// round trip for few (16 x 2048 4.0 us, 1024 x 2048 6.4 us).
 // EARLY: the row-independent operands are loaded with the row, not after its statistics (one
 // round trip less, for as many registers).
 template <int TPR, int NCH, bool RMS, int BITS, bool EARLY>
