@@ -815,13 +815,32 @@ static int run_plan(const MxPlan &plan, const MxLinearArgs &a, hipStream_t strea
   return fail(FM_ERR_UNSUPPORTED, "bf16 x of more than %d rows", MX_BF16_ROWS);
 }
 
+// Whether the kernel quantizes bf16 rows itself. Past these sums and columns a pass of its own in
+// front is cheaper (16 rows, us: 8192 -> 2048 15.6 / 14, 20480 -> 2048 33.7 / 19), and so it is for
+// more rows, where every workgroup would quantize them again.
+static bool quantizes(int64_t rows, int64_t n, int64_t k) {
+  return rows <= MX_BF16_ROWS && k % 8 == 0 && (n <= 8192 ? k < 8192 : k <= 5632);
+}
+
+// The workspace: the sums of parts of k, then bf16 rows as 8-bit codes and scales.
+struct MxWorkspace {
+  size_t parts, codes, scales;  // bytes
+};
+static MxWorkspace workspace_of(int64_t rows, int64_t n, int64_t k, int32_t x_bits) {
+  const bool first = x_bits == 16 && !quantizes(rows, n, k);
+  const MxPlan plan = plan_of(rows, n, k, first ? 8 : x_bits);
+  const int64_t kp = mx_padded(k);
+  return {plan.parts == 1 ? 0 : (size_t)(plan.parts * rows * part_stride(n)) * sizeof(float),
+          first ? (size_t)(rows * kp) : 0, first ? (size_t)(rows * kp / MX_BLOCK) : 0};
+}
+
 }  // namespace fm
 
 extern "C" size_t fm_mx_linear_workspace_bytes(int64_t rows, int64_t n, int64_t k, int32_t x_bits) {
   using namespace fm;
   if (rows <= 0 || n <= 0 || k <= 0 || k > 1 << 22 || n > 1 << 26 || rows > 1 << 26) return 0;
-  const MxPlan plan = plan_of(rows, n, k, x_bits);
-  return plan.parts == 1 ? 0 : (size_t)(plan.parts * rows * part_stride(n)) * sizeof(float);
+  const MxWorkspace ws = workspace_of(rows, n, k, x_bits);
+  return ws.parts + ws.codes + ws.scales;
 }
 
 extern "C" int fm_mx_linear(const void *x, int32_t x_bits, int64_t x_stride, const void *x_scales,
@@ -847,22 +866,26 @@ extern "C" int fm_mx_linear(const void *x, int32_t x_bits, int64_t x_stride, con
              "rows of codes and scales: strides below 2^24 bytes");
   FM_REQUIRE(aligned(out, 2) && aligned(bias, 2) && (rows == 1 || out_stride >= n), "out rows must cover %lld values",
              (long long)n);
-  if (x_bits == 16) {
-    if (rows > MX_BF16_ROWS || k % 8 != 0)
-      return fail(FM_ERR_UNSUPPORTED, "bf16 x of %lld rows of %lld: at most %d rows, a multiple of 8 values",
-                  (long long)rows, (long long)k, MX_BF16_ROWS);
+  if (x_bits == 16 && quantizes(rows, n, k)) {
     FM_REQUIRE(aligned(x, 16) && x_stride % 8 == 0 && (rows == 1 || x_stride >= k),
                "bf16 x: 16-byte aligned rows, a stride of a multiple of 8 values");
-  } else {
+  } else if (x_bits != 16) {
     FM_REQUIRE(x_scales && aligned(x, 16) && x_stride % 16 == 0 && x_stride >= kp * x_bits / 8 && aligned(x_scales, 4) &&
                    x_scales_stride % 4 == 0 && x_scales_stride >= kp / MX_BLOCK,
                "x: 16-byte aligned rows of %lld bytes, 4-byte aligned scales of %lld", (long long)(kp * x_bits / 8),
                (long long)(kp / MX_BLOCK));
   }
-  const MxPlan plan = plan_of(rows, n, k, x_bits);
-  const size_t need = fm_mx_linear_workspace_bytes(rows, n, k, x_bits);
+  const MxWorkspace ws = workspace_of(rows, n, k, x_bits);
+  const size_t need = ws.parts + ws.codes + ws.scales;
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(FM_ERR_WORKSPACE, "workspace of %zu bytes, need %zu (16-byte aligned)", workspace_bytes, need);
+  if (ws.codes > 0) {
+    uint8_t *codes = (uint8_t *)workspace + ws.parts, *scales = codes + ws.codes;
+    const int rc = fm_mx_quantize(x, 0, x_stride, 0, 8, codes, kp, scales, kp / MX_BLOCK, rows, k, stream);
+    if (rc != FM_OK) return rc;
+    x = codes, x_bits = 8, x_stride = kp, x_scales = scales, x_scales_stride = kp / MX_BLOCK;
+  }
+  const MxPlan plan = plan_of(rows, n, k, x_bits);
   const MxLinearArgs a{(const uint8_t *)x, (const uint8_t *)x_scales, (const uint8_t *)w, (const uint8_t *)w_scales,
                        (const uint16_t *)bias, (uint16_t *)out, x_bits == 16 ? 2 * x_stride : x_stride, x_scales_stride,
                        w_stride, w_scales_stride, out_stride, rows, (int32_t)n, (int32_t)k, (int32_t)(kp / MX_PAD),

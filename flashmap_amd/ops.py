@@ -1318,7 +1318,6 @@ MX_BLOCK = 32  # values that share a scale
 MX_PAD = 128  # stored rows hold a multiple of this many values
 MX_MAX = 1 << 26  # rows, columns
 MX_NORM_COLS = 16384
-MX_BF16_ROWS = 16  # bf16 rows that the product's kernel quantizes itself
 _ACTIVATIONS = {None: 0, "gelu": 1, "swiglu": 2}
 
 
@@ -1556,12 +1555,8 @@ def mx_linear(x: torch.Tensor | MX, weight: MX, bias: torch.Tensor | None = None
         keep_x, xs = _plain_rows(x, k, "x")
         xp = keep_x.data_ptr()
         read = keep_x, xs, rows, k, False
-        # the rows that the kernel quantizes itself; past these sums and columns a call of its own
-        # is cheaper (16 rows, us: 8192 -> 2048 15.6 / 14, 20480 -> 2048 33.7 / 19)
-        if (rows <= MX_BF16_ROWS and k % 8 == 0 and xs % 8 == 0 and xp % 16 == 0
-                and (k < 8192 if n <= 8192 else k <= 5632)):
-            x_bits, xsp, xss = 16, None, 0
-        else:
+        x_bits, xsp, xss = 16, None, 0
+        if (xs % 8 or xp % 16) and not _mx_workspace_bytes(rows, n, k, 16):  # not as the product's kernel reads them
             x_bits, keep_x = 8, mx_quantize(x)
             xp, xs, xsp, xss = _mx_new_args(keep_x)
     if bias is not None:

@@ -504,10 +504,11 @@ int fm_mx_dequantize(const void *codes, int64_t codes_stride, const void *scales
                      void *stream);
 /* out (rows, n) bf16 = x w^T (+ bias (n,) bf16 or NULL), accumulated in fp32 and rounded once.
  * w: 4-bit rows (n, k). x_bits 8 or 4: x holds codes, x_scales its scales. x_bits 16: x is
- * bf16 (rows, k) and the kernel quantizes it to 8 bits as fm_mx_quantize does (x_scales is not
- * read): at most 16 rows, 16-byte aligned with a stride of a multiple of 8 values, k a
- * multiple of 8; others call fm_mx_quantize first. rows and n at most 2^26, k at most 2^22,
- * strides of codes and scales below 2^24 bytes. The workspace (16-byte aligned) holds
+ * bf16 (rows, k) and is quantized to 8 bits as fm_mx_quantize does (x_scales is not read):
+ * by a pass in front, or, where that call needs no workspace, in the product's kernel, which
+ * takes 16-byte aligned rows with a stride of a multiple of 8 values. rows and n at most
+ * 2^26, k at most 2^22, strides of codes and scales below 2^24 bytes. out must not overlap
+ * what is read. The workspace (16-byte aligned) holds
  * fm_mx_linear_workspace_bytes(rows, n, k, x_bits) bytes (0: none is needed); concurrent calls
  * must not share it. */
 size_t fm_mx_linear_workspace_bytes(int64_t rows, int64_t n, int64_t k, int32_t x_bits);

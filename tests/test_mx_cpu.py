@@ -179,8 +179,19 @@ def test_entries_refuse_what_they_cannot_launch():
     _fails("at most 2\\^22", unsup, *lin(k=(1 << 22) + 1))
     _fails("below 2\\^24", inv, *lin(xs=1 << 24))
     _fails("below 2\\^24", inv, *lin(ws=1 << 24))
-    _fails("at most 16 rows", unsup, *lin(xb=16, xs=64, rows=17))
-    _fails("multiple of 8", unsup, *lin(xb=16, xs=64, k=63))
+    # bf16 rows that the product's kernel does not quantize itself need room for their codes
+    lib = _native.lib()
+    for rows, n, k in ((17, 8, 64), (4, 8, 63), (16, 8, 8192), (16, 8200, 5640)):
+        pad = -(-k // 128) * 128
+        need = lib.fm_mx_linear_workspace_bytes(rows, n, k, 8) + rows * pad * 33 // 32
+        assert lib.fm_mx_linear_workspace_bytes(rows, n, k, 16) == need
+        w = dict(xb=16, xs=k, ws=pad // 2, wss=pad // 32, os=n, rows=rows, n=n, k=k)
+        _fails(f"workspace of 0 bytes, need {need}", _native.FM_ERR_WORKSPACE, *lin(**w))
+        _fails("workspace of", _native.FM_ERR_WORKSPACE, *lin(**w, wk=at, wb=need - 1))
+        _fails("workspace of", _native.FM_ERR_WORKSPACE, *lin(**w, wk=at + 8, wb=need))
+        _fails("overlap", inv, *lin(**dict(w, xs=k - 1), wk=at, wb=need))
+    for rows, n, k in ((16, 8, 8184), (16, 8200, 5632), (1, 8192, 8)):
+        assert lib.fm_mx_linear_workspace_bytes(rows, n, k, 16) == 0
     _fails("bf16 x", inv, *lin(xb=16, xs=60, k=56))
     _fails("bf16 x", inv, *lin(xb=16, xs=64, x=at + 8))
     assert _native.call(*lin(x=None, rows=0)) is None
