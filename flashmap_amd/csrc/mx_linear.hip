@@ -34,7 +34,7 @@ struct MxLinearArgs {
   int64_t rows;
   int32_t n;
   int32_t k, steps;  // steps: of 128 along k
-  int32_t vec_out;  // rows of out may be written 16 bytes at a time
+  int32_t out_unit;  // values of out that may be written at once: 8, 4, 2 or 1
   float *part;  // NULL, or the sums of a part of k: (parts, rows, part_stride) fp32
   int64_t part_stride;
 };
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(64 * WAVES) void mx_linear_rows_kernel(const MxLine
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (a.bias != nullptr && n + i < a.n) sum[i] += bf16_to_f32(a.bias[n + i]);
-    if (a.vec_out && n + 4 <= a.n) {
+    if (a.out_unit >= 4 && n + 4 <= a.n) {
       *reinterpret_cast<u32x2_t *>(dst) = u32x2_t{pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3])};
     } else {
 #pragma unroll
@@ -391,7 +391,7 @@ __global__ __launch_bounds__(64 * WAVES) void mx_linear_stream_kernel(const MxLi
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             if (a.bias != nullptr && n + q < a.n) acc[i][q] += bf16_to_f32(a.bias[n + q]);
-          if (a.vec_out && n + 4 <= a.n) {
+          if (a.out_unit >= 4 && n + 4 <= a.n) {
             *reinterpret_cast<u32x2_t *>(dst) = u32x2_t{pack_bf16x2(acc[i][0], acc[i][1]), pack_bf16x2(acc[i][2], acc[i][3])};
           } else {
 #pragma unroll
@@ -640,14 +640,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx_linear_tile_kernel(const M
   }
   if (TURNS ? !late : a.part == nullptr) barrier();  // nobody reads the stages any more
 
-  // Lane (r, g) holds row m of out, 8 columns from 8 g on in each 32-column group.
+  // Lane (r, g) holds row m of out, 8 columns from 8 g on in each 32-column group. (Found anew,
+  // not kept in registers through the loop.)
+  int out_lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(out_lane));
+  const int out_r = out_lane & 15, out_g = out_lane >> 4;
   if (a.part != nullptr) {  // rows padded to whole groups of 8 columns
 #pragma unroll
     for (int p = 0; p < T::NF / 2; ++p) {
-      const int32_t n = n0 + 32 * (wn * (T::NF / 2) + p) + 8 * g;
+      const int32_t n = n0 + 32 * (wn * (T::NF / 2) + p) + 8 * out_g;
 #pragma unroll
       for (int i = 0; i < T::MF; ++i) {
-        const int64_t m = m0 + 16 * (wm * T::MF + i) + r;
+        const int64_t m = m0 + 16 * (wm * T::MF + i) + out_r;
         if (m >= a.rows || n >= a.n) continue;
         float *to = a.part + (blockIdx.y * a.rows + m) * a.part_stride + n;
         *reinterpret_cast<f32x4_t *>(to) = acc[2 * p][i];
@@ -662,7 +666,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx_linear_tile_kernel(const M
   constexpr int PIECES = BN / 8, ROWS = 64 / PIECES;
 #pragma unroll
   for (int p = 0; p < T::NF / 2; ++p) {
-    const int piece = 4 * (wn * (T::NF / 2) + p) + g;
+    const int piece = 4 * (wn * (T::NF / 2) + p) + out_g;
     const int32_t n = n0 + 8 * piece;
     float b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (a.bias != nullptr) {
@@ -672,34 +676,60 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx_linear_tile_kernel(const M
 #pragma unroll
     for (int i = 0; i < T::MF; ++i) {
       const f32x4_t lo = acc[2 * p][i], hi = acc[2 * p + 1][i];
-      const int row = 16 * (wm * T::MF + i) + r;
-      store16(lds + 2 * BN * row + 16 * (piece ^ (r & 7)),
+      const int row = 16 * (wm * T::MF + i) + out_r;
+      store16(lds + 2 * BN * row + 16 * (piece ^ (out_r & 7)),
               u32x4_t{pack_bf16x2(lo[0] + b[0], lo[1] + b[1]), pack_bf16x2(lo[2] + b[2], lo[3] + b[3]),
                       pack_bf16x2(hi[0] + b[4], hi[1] + b[5]), pack_bf16x2(hi[2] + b[6], hi[3] + b[7])});
     }
   }
   barrier();
-  const int piece = lane % PIECES;
-  const int32_t n = n0 + 8 * piece;
-  const bool vec = a.vec_out != 0 && n + 8 <= a.n;
+  if (a.out_unit == 8) {
+    const int piece = out_lane % PIECES;
+    const int32_t n = n0 + 8 * piece;
 #pragma unroll
-  for (int q = 0; q < BM / T::WAVES / ROWS; ++q) {
-    const int row = (q * T::WAVES + wave) * ROWS + lane / PIECES;
-    if (m0 + row >= a.rows) continue;
-    const u32x4_t v = load16(lds + 2 * BN * row + 16 * (piece ^ (row & 7)));
-    uint16_t *dst = a.out + (m0 + row) * a.os + n;
-    if (vec) {
-      // Tiles this large are chosen for results that no cache holds.
-      if (BM == 256)
-        store16_nt(dst, v);
-      else
-        store16(dst, v);
-    } else {
+    for (int q = 0; q < BM / T::WAVES / ROWS; ++q) {
+      const int row = (q * T::WAVES + wave) * ROWS + out_lane / PIECES;
+      if (m0 + row >= a.rows) continue;
+      const u32x4_t v = load16(lds + 2 * BN * row + 16 * (piece ^ (row & 7)));
+      uint16_t *dst = a.out + (m0 + row) * a.os + n;
+      if (n + 8 <= a.n) {
+        // Tiles this large are chosen for results that no cache holds.
+        if (BM == 256)
+          store16_nt(dst, v);
+        else
+          store16(dst, v);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (n + e < a.n) dst[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+        for (int e = 0; e < 8; ++e)
+          if (n + e < a.n) dst[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+      }
     }
+    return;
   }
+  // Rows that are not 16-byte aligned: as many values a lane as they allow, neighbouring lanes'
+  // side by side.
+  auto loose = [&](auto type) {
+    typedef decltype(type) U;
+    constexpr int W = sizeof(U) / 2;
+    for (int q = wave; q < BM * BN / (64 * W); q += T::WAVES) {
+      const int at = W * (64 * q + out_lane), row = at / BN, c = at % BN;
+      const int32_t n = n0 + c;
+      if (m0 + row >= a.rows || n >= a.n) continue;
+      const U v = *reinterpret_cast<const U *>(lds + 2 * BN * row + 16 * ((c >> 3) ^ (row & 7)) + 2 * (c & 7));
+      uint16_t *dst = a.out + (m0 + row) * a.os + n;
+      if (n + W <= a.n) {
+        *reinterpret_cast<U *>(dst) = v;
+      } else {
+        for (int e = 0; n + e < a.n; ++e) dst[e] = (uint16_t)(v >> (16 * e));
+      }
+    }
+  };
+  if (a.out_unit == 4)
+    loose((uint64_t)0);
+  else if (a.out_unit == 2)
+    loose((uint32_t)0);
+  else
+    loose((uint16_t)0);
 }
 
 // The parts' sums, in their order, plus the bias: 8 columns a thread.
@@ -718,7 +748,7 @@ __global__ __launch_bounds__(256) void mx_linear_join_kernel(const MxLinearArgs 
   for (int q = 0; q < 8; ++q)
     if (a.bias != nullptr && n + q < a.n) v[q] += bf16_to_f32(a.bias[n + q]);
   uint16_t *dst = a.out + m * a.os + n;
-  if (a.vec_out && n + 8 <= a.n) {
+  if (a.out_unit == 8 && n + 8 <= a.n) {
     store16(dst, u32x4_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])});
   } else {
 #pragma unroll
@@ -761,6 +791,7 @@ struct MxPlan {
 };
 
 constexpr size_t LDS_BYTES = 160 * 1024;
+constexpr int64_t CUS = 256;
 constexpr int STREAM_WAVES = 8, STREAM_GROUPS = 2;
 
 template <int XBITS>
@@ -807,7 +838,28 @@ static int run_plan(const MxPlan &plan, const MxLinearArgs &a, hipStream_t strea
   if (plan.kind == MxPlan::ROWS)
     return a.n <= 4096 ? launch_rows<XBITS, 1, 1, 8>(a, stream) : launch_rows<XBITS, 1, 2, 8>(a, stream);
   if constexpr (XBITS != 16) {
-    if (plan.bm == 256) return launch_tiles<XBITS, 256, 256, 4, 2, true>(a, 1, stream);
+    if (plan.bm == 256) {
+      // A tile a CU: where the last round is for few, its columns' tiles go to a launch of smaller
+      // ones. Measured, 1024 to 4096 rows, 1 / 4 / 9 whole rounds and a last one of
+      //   16 tiles  8-bit x -23 / -8 / -2 %, 4-bit x -18 / -8 / -1 %;  48   -13 / -5 / -2, -9 / -4 / +1
+      //   80        -5 / -3 / -2, -1 / -1 / +1;  112  -3 / -1 / -1, +3 / 0 / +3;  144 and more  +3 and more
+      const int64_t tm = (a.rows + 255) / 256, tn = ((int64_t)a.n + 255) / 256, last = tm * tn % CUS;
+      const int64_t moved = (last + tm - 1) / tm;
+      const int64_t most = XBITS == 8 ? 96 : tm * tn < 8 * CUS ? 64 : 0;
+      if (tm * tn > CUS && last > 0 && last <= most && moved < tn) {
+        MxLinearArgs body = a, tail = a;
+        body.n = (int32_t)(256 * (tn - moved)), tail.n = a.n - body.n;
+        tail.w += body.n * a.ws, tail.wsc += body.n * a.wss, tail.out += body.n;
+        if (a.bias != nullptr) tail.bias += body.n;
+        const int rc = launch_tiles<XBITS, 256, 256, 4, 2, true>(body, 1, stream);
+        if (rc != FM_OK) return rc;
+        MxPlan rest = plan_of(a.rows, tail.n, a.k, XBITS);
+        rest.parts = 1;
+        return rest.bm == 256 ? launch_tiles<XBITS, 256, 256, 4, 2, true>(tail, 1, stream)
+                              : run_plan<XBITS>(rest, tail, stream);
+      }
+      return launch_tiles<XBITS, 256, 256, 4, 2, true>(a, 1, stream);
+    }
     if (plan.bm == 128) return launch_tiles<XBITS, 128, 128, 2, 2, false>(a, 1, stream);
     if (plan.bn == 128) return launch_tiles<XBITS, 64, 128, 1, 4, false>(a, 1, stream);
     return launch_tiles<XBITS, 64, 64, 2, 2, false>(a, plan.parts, stream);
@@ -820,6 +872,12 @@ static int run_plan(const MxPlan &plan, const MxLinearArgs &a, hipStream_t strea
 // more rows, where every workgroup would quantize them again.
 static bool quantizes(int64_t rows, int64_t n, int64_t k) {
   return rows <= MX_BF16_ROWS && k % 8 == 0 && (n <= 8192 ? k < 8192 : k <= 5632);
+}
+
+static int32_t out_unit(const void *out, int64_t stride) {
+  for (int32_t unit = 8; unit > 1; unit /= 2)
+    if (aligned(out, 2 * unit) && stride % unit == 0) return unit;
+  return 1;
 }
 
 // The workspace: the sums of parts of k, then bf16 rows as 8-bit codes and scales.
@@ -889,7 +947,7 @@ extern "C" int fm_mx_linear(const void *x, int32_t x_bits, int64_t x_stride, con
   const MxLinearArgs a{(const uint8_t *)x, (const uint8_t *)x_scales, (const uint8_t *)w, (const uint8_t *)w_scales,
                        (const uint16_t *)bias, (uint16_t *)out, x_bits == 16 ? 2 * x_stride : x_stride, x_scales_stride,
                        w_stride, w_scales_stride, out_stride, rows, (int32_t)n, (int32_t)k, (int32_t)(kp / MX_PAD),
-                       aligned(out, 16) && out_stride % 8 == 0, (float *)workspace, part_stride(n)};
+                       out_unit(out, out_stride), (float *)workspace, part_stride(n)};
   const hipStream_t st = (hipStream_t)stream;
   return x_bits == 16 ? run_plan<16>(plan, a, st) : x_bits == 8 ? run_plan<8>(plan, a, st) : run_plan<4>(plan, a, st);
 }

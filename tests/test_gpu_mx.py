@@ -358,3 +358,37 @@ def test_outputs_that_overlap_inputs(dev):
             t, p = call(own[:16, :128], own[:16, 128:], own[:16, half])
             assert torch.equal(t, s) and torch.equal(p.codes, q.codes) and torch.equal(p.scales, q.scales)
             assert torch.equal(own[16:], buf[16:])
+
+
+@pytest.mark.parametrize("kind", [8, 4])
+@pytest.mark.parametrize("rows,n,k,stride", [
+    (4096, 4160, 128, 4160), (4100, 4200, 256, 4204), (1024, 16900, 128, 16902), (2050, 8193, 384, 8193),
+    (1024, 16640, 640, 16640)])
+def test_linear_last_round(dev, rows, n, k, stride, kind):
+    """More tiles of 256 x 256 than the chip holds at once, the last ones few (their columns go
+    to smaller tiles) and rows of out aligned to 16, 8, 4 and 2 bytes."""
+    print(f"mx_linear rows={rows} n={n} k={k} x={kind} stride={stride}", flush=True)
+    x = activations(rows, k, rows + n).to(dev)
+    w = ops.mx_quantize(torch.randn(n, k, generator=gen(n)).to(dev) / k ** 0.5, 4)
+    bias = torch.randn(n, generator=gen(k)).bfloat16().to(dev)
+    given, xv = operand(kind, x)
+    buf = torch.full((rows, stride), 7.0, dtype=torch.bfloat16, device=dev)
+    got = ops.mx_linear(given, w, bias, out=buf[:, :n])
+    check_product(got, xv, mx.values(*codes_of(w), 4), bias, 2.0 ** -15 + (0 if kind == 4 else 2.0 ** -10))
+    assert (buf[:, n:] == 7).all()
+
+
+@pytest.mark.parametrize("rows,n", [(20, 70), (70, 130), (300, 513), (1500, 2500)])
+@pytest.mark.parametrize("stride", [0, 1, 2, 4])
+def test_linear_rows_of_any_alignment(dev, rows, n, stride):
+    """The same bits whatever the alignment of out's rows, and nothing written between them."""
+    k = 300
+    w = ops.mx_quantize(torch.randn(n, k, generator=gen(1)).to(dev), 4)
+    x = ops.mx_quantize(activations(rows, k, n).to(dev))
+    want = ops.mx_linear(x, w)
+    wide = -(-n // 8) * 8 + 8 + stride
+    for first in (0, stride):
+        buf = torch.full((rows, wide), 7.0, dtype=torch.bfloat16, device=dev)
+        got = ops.mx_linear(x, w, out=buf[:, first:first + n])
+        assert torch.equal(got, want)
+        assert (buf[:, :first] == 7).all() and (buf[:, first + n:] == 7).all()
