@@ -424,8 +424,9 @@ static int launch_stream(const MxLinearArgs &a, hipStream_t stream) {
 // instruction, and at 256 x 256 both are busy alike. Bound, large products: the instruction,
 // whose clock falls under it (random codes, nothing but the instruction on every SIMD: 17.5 ns
 // with 8-bit x, 10.1 ns with 4-bit x, 3.8 and 6.6 PFLOP/s). Reached at 4096 x 20480 -> 4096: 252
-// and 188 us, 2.7 and 3.65 PFLOP/s; results add 20 us per 134 MB (1024 x 2048 -> 151936 of 8-bit
-// x 292 us, 8192 x 2048 -> 24576 of 4-bit x 258 us). Small products (1024 x 8192 -> 2048: 28 us)
+// and 188 us, 2.7 and 3.65 PFLOP/s; storing results takes 25 us per 100 MB (with k = 128), partly
+// beside other tiles' products (1024 x 2048 -> 151936 of 8-bit x 290 us, 8192 x 2048 -> 24576 of
+// 4-bit x 265 us). Small products (1024 x 8192 -> 2048: 28 us)
 // are bound by a step's way through a workgroup, 0.41 us for 8 instructions a wavefront,
 // whatever the number of workgroups.
 // Measured and not taken: a persistent grid that starts the next tile's loads before this one's
