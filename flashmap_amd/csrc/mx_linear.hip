@@ -419,16 +419,15 @@ static int launch_stream(const MxLinearArgs &a, hipStream_t stream) {
 
 // ------------------------------------------------------------------------ many rows: tiles
 //
-// Steps of 128 along k, three stages in LDS: a tile's operands are read from LDS once a
-// wavefront, so 16 BM BN / (wavefronts' rows and columns) decides between LDS and the matrix
-// instruction, and at 256 x 256 both are busy alike. Bound, large products: the instruction,
-// whose clock falls under it (random codes, nothing but the instruction on every SIMD: 17.5 ns
-// with 8-bit x, 10.1 ns with 4-bit x, 3.8 and 6.6 PFLOP/s). Reached at 4096 x 20480 -> 4096: 252
-// and 188 us, 2.7 and 3.65 PFLOP/s; storing results takes 25 us per 100 MB (with k = 128), partly
-// beside other tiles' products (1024 x 2048 -> 151936 of 8-bit x 290 us, 8192 x 2048 -> 24576 of
-// 4-bit x 265 us). Small products (1024 x 8192 -> 2048: 28 us)
-// are bound by a step's way through a workgroup, 0.41 us for 8 instructions a wavefront,
-// whatever the number of workgroups.
+// Steps of 128 along k, three stages in LDS. A wavefront reads its rows and columns of a stage and
+// multiplies all of one by all of the other, so larger shares need fewer bytes of LDS a product;
+// at 256 x 256 LDS and the matrix instruction are busy alike. Bound, large products: the
+// instruction, whose clock falls under it (random codes, nothing but the instruction on every
+// SIMD: 17.5 ns with 8-bit x, 10.1 ns with 4-bit x, 3.8 and 6.6 PFLOP/s). Reached at 4096 x 20480
+// -> 4096: 252 and 188 us, 2.7 and 3.65 PFLOP/s; storing results takes 25 us per 100 MB (with k =
+// 128), partly beside other tiles' products (1024 x 2048 -> 151936 of 8-bit x 290 us, 8192 x 2048
+// -> 24576 of 4-bit x 265 us). Small products (1024 x 8192 -> 2048: 28 us) are bound by a step's way
+// through a workgroup, 0.41 us for 8 instructions a wavefront, however many workgroups run.
 // Measured and not taken: a persistent grid that starts the next tile's loads before this one's
 // stores (1 % either way; the stores count among the loads awaited), four and more stages (+6 %
 // at 256 x 256, none below), 4-bit rows read two steps at a time in whole cache lines (4-bit x
