@@ -148,18 +148,39 @@ __device__ __forceinline__ float gelu(float x) {
   const float e = __builtin_amdgcn_exp2f(a * a * -0.721347520f);  // exp(-a^2 / 2)
   return fmaxf(x, 0.f) - a * (e * p);
 }
-// gate / (1 + exp(-gate)) * up: the exponential as above, the quotient by a refined reciprocal.
-// From gate = -88 on the result is 0.
+// gate / (1 + exp(-gate)) * up for gate from -87 on: the exponential with what its argument lost
+// put back, the quotient by a refined reciprocal. The quotient is at most 1 in magnitude of gate
+// and a normal float, so that only the result overflows. (A gate past 104 has the quotient 1.)
 __device__ __forceinline__ float swiglu(float gate, float up) {
 #pragma clang fp contract(off)
-  const float y = fminf(-gate, 88.f);
+  const float y = fmaxf(-gate, -104.f);
   const float u = y * 1.44269504f;
   const float r = __builtin_fmaf(y, 1.92596299e-8f, __builtin_fmaf(y, 1.44269504f, -u));
   const float e = __builtin_amdgcn_exp2f(u);
   const float d = 1.f + __builtin_fmaf(e * 0.693147182f, r, e);
   float q = __builtin_amdgcn_rcpf(d);
   q = __builtin_fmaf(__builtin_fmaf(-d, q, 1.f), q, q);
-  return gate * up * q;
+  return gate * q * up;
+}
+// The gates whose quotient is subnormal (or whose gate times quotient may be) while the result
+// need not be: mantissas are multiplied and exponents added, for negative gates as gate
+// exp(gate) / (1 + exp(gate)) * up with exp(-|gate|) = 2^n e, e from 0.7 to 1.42. -200 stands
+// for what lies below it: with any up the result is below half of the smallest float. -inf gives
+// NaN, as -inf times 0 does. Taken for every value this makes 1024 x 8192 13.5 us instead of 10.1
+// (without it 9.6).
+__device__ __forceinline__ bool swiglu_is_wide(float gate) { return gate < -87.f || fabsf(gate) < 0x1p-100f; }
+__device__ __forceinline__ float swiglu_wide(float gate, float up) {
+#pragma clang fp contract(off)
+  const float g = gate < -200.f ? (gate - gate) - 200.f : gate;
+  const float y = fminf(fabsf(gate), 200.f);
+  const float u = y * -1.44269504f;
+  const float r = __builtin_fmaf(y, -1.92596299e-8f, __builtin_fmaf(y, -1.44269504f, -u));
+  const float n = rintf(u);
+  const float p = __builtin_amdgcn_exp2f(u - n);
+  const float e = __builtin_fmaf(p * 0.693147182f, r, p);
+  const float d = 1.f + __builtin_ldexpf(e, (int)n);
+  const float v = __builtin_amdgcn_frexp_mantf(g) * __builtin_amdgcn_frexp_mantf(up) * __fdiv_rn(gate < 0.f ? e : 1.f, d);
+  return __builtin_ldexpf(v, __builtin_amdgcn_frexp_expf(g) + __builtin_amdgcn_frexp_expf(up) + (gate < 0.f ? (int)n : 0));
 }
 
 // A thread per 8 values, no loop: every load of the call is in flight at once, and the rows need
@@ -179,10 +200,19 @@ __global__ __launch_bounds__(ROW_THREADS) void mx_quantize_kernel(const QuantArg
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = gelu(v[i]);
   } else if constexpr (ACT == ACT_SWIGLU) {
-    float u[8];
+    float u[8], w[8], low = 0.f, least = 1.f;
     load8(x + a.cols, c, a.cols, a.vec != 0 && a.cols % 8 == 0, u);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = swiglu(v[i], u[i]);
+    for (int i = 0; i < 8; ++i) {
+      low = fminf(low, v[i]), least = fminf(least, fabsf(v[i]));
+      w[i] = swiglu(v[i], u[i]);
+    }
+    if (c < a.cols && (low < -87.f || least < 0x1p-100f)) {  // rare
+      for (int i = 0; i < 8; ++i)
+        if (swiglu_is_wide(v[i])) w[i] = swiglu_wide(v[i], u[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = w[i];
   }
   store_block<BITS>(v, c, a.codes + row * a.cs, a.scales + row * a.ss);
 }

@@ -1,0 +1,48 @@
+"""The activations on the way to microscaled rows over everything that their inputs' types hold,
+each value in a block of its own, against float64 (oracle/mx.py)."""
+
+import pytest
+import torch
+
+from _mx_checks import codes_of
+from flashmap_amd import ops
+from oracle import mx
+
+pytestmark = pytest.mark.gpu
+
+
+def _check_alone(code, scale, bits, v, off):
+    """Rows of one value each: what is stored lies between what is stored for the value less and plus
+    its error (a block of one value stores a value that never falls as the value rises, its
+    saturation below a power of two included)."""
+    got = mx.values(code, scale, bits)
+    lo, hi = (mx.values(*mx.quantize(w, bits), bits) for w in (v - off, v + off))
+    bad = (got < lo) | (got > hi) | torch.isnan(got)
+    rows = torch.nonzero(bad.any(1))[:5, 0]
+    assert not bad.any(), f"{int(bad.any(1).sum())} values off: " + ", ".join(f"{v[r, 0]:.9g} gave {got[r, 0]:.9g}" for r in rows)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_swiglu_over_the_whole_range(dev, dtype, bits):
+    """Gates and factors of every size, each pair in a block of its own: the result counts, whatever
+    the gate's exponential or the product of the two does by itself. A few roundings of the
+    exponential, the quotient and three products: 16 of 2^-24, and half of the smallest float where
+    the result is subnormal. Where float32 cannot hold it the block is NaN, as where an input is
+    not finite."""
+    sizes = [0.0, 1e-40, 1e-30, 1e-3, 0.5, 1.0, 9.0, 50.0, 80.0, 87.0, 87.3, 87.5, 88.0, 88.5, 89.0, 95.0, 103.0, 104.0,
+             120.0, 140.0, 199.0, 201.0, 1e3, 1e4, 1e9, 1e30, 2.4e38, 3e38, float("inf")]
+    gates = torch.tensor([s * v for v in sizes for s in (1, -1)] + [float("nan")])
+    ups = torch.tensor([1e-40, 1e-30, 1e-10, -1.0, 300.0, -1e9, 1e30, 1e37, 3e38, 0.0, float("inf"), float("nan")])
+    pairs = torch.cartesian_prod(gates, ups)
+    x = torch.zeros(len(pairs), 64)
+    x[:, 0], x[:, 32] = pairs[:, 0], pairs[:, 1]
+    x = x.to(dtype)
+    q = ops.mx_quantize(x.to(dev), bits, "swiglu")
+    want = mx.swiglu(x)
+    want[~torch.isfinite(want.float())] = float("nan")
+    bad = torch.isnan(want[:, 0])
+    code, scale = codes_of(q)
+    wrong = (scale[:, 0] == 255) != bad
+    assert not wrong.any(), f"{int(wrong.sum())} pairs: " + str([x[i, [0, 32]].tolist() for i in torch.nonzero(wrong)[:5, 0]])
+    _check_alone(code[~bad], scale[~bad], bits, want[~bad], 2.0 ** -20 * want[~bad].abs() + 2.0 ** -150)
