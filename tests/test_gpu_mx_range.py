@@ -46,3 +46,26 @@ def test_swiglu_over_the_whole_range(dev, dtype, bits):
     wrong = (scale[:, 0] == 255) != bad
     assert not wrong.any(), f"{int(wrong.sum())} pairs: " + str([x[i, [0, 32]].tolist() for i in torch.nonzero(wrong)[:5, 0]])
     _check_alone(code[~bad], scale[~bad], bits, want[~bad], 2.0 ** -20 * want[~bad].abs() + 2.0 ** -150)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gelu_over_the_whole_range(dev, dtype, bits):
+    """Every bf16 value (in float32 too, with values between them): x Phi(x) = max(x, 0) - h, h = |x| / 2
+    erfc(|x| / sqrt 2), where h moves by x^2 of its argument's relative error and is 0 below 2^-126, and
+    the difference is rounded once. NaN for what is not finite."""
+    x = torch.arange(1 << 16, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)[:, None].to(dtype)
+    if dtype == torch.float32:
+        x = torch.cat([x, torch.linspace(-16, 16, 65537)[:, None]])
+    q = ops.mx_quantize(x.to(dev), bits, "gelu")
+    fine = torch.isfinite(x[:, 0])
+    code, scale = codes_of(q)
+    assert (scale[~fine, 0] == 255).all()
+    v, want = x[fine].double(), mx.gelu(x[fine])
+    h = 0.5 * v.abs() * torch.special.erfc(v.abs() / 2.0 ** 0.5)
+    off = 2.0 ** -22 * (8 + v.clamp(-20, 20) ** 2) * h + 2.0 ** -24 * want.abs() + 2.0 ** -126
+    _check_alone(code[fine], scale[fine], bits, want, off)
+    best = mx.quantize(want.float(), bits)
+    differ = ((code[fine] != best[0]).any(1) | (scale[fine] != best[1]).any(1)) & (want[:, 0].abs() > 2.0 ** -126)
+    print(f"gelu {dtype} bits={bits}: {int(differ.sum())} of {len(v)} codes are not those of the value rounded to float32, "
+          f"at x from {x[fine][differ].abs().min():.3g}" if differ.any() else "gelu: all codes as rounded", flush=True)
