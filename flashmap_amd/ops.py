@@ -1460,10 +1460,11 @@ def _bf16_out(x_out: torch.Tensor | None, shape: tuple, device: torch.device,
     return x_out, rows, (rows.stride(0) if rows.shape[0] > 1 else cols)
 
 
-def _apart(name: str, out: torch.Tensor, out_stride: int, rows: int, cols: int, *others: tuple) -> None:
-    """Refuse a given output whose rows share bytes with rows that are read: ``others``
-    (tensor, stride, rows, cols, whether the very same rows may be given: each is read before
-    it is written)."""
+def _apart(name: str, out: torch.Tensor, out_stride: int, rows: int, cols: int, *others: tuple,
+           vectors: tuple = ()) -> None:
+    """Refuse a given output whose rows share bytes with what is read: rows, ``others`` (tensor,
+    stride, rows, cols, whether the very same rows may be given: each is read before it is
+    written), and contiguous ``vectors`` (or None)."""
     size = out.element_size()
     begin, step, width = out.data_ptr(), out_stride * size, cols * size
     end = begin + (rows - 1) * step + width
@@ -1475,6 +1476,20 @@ def _apart(name: str, out: torch.Tensor, out_stride: int, rows: int, cols: int, 
         at = (first - begin) % step
         if by != step or at < width or at + w > step:
             raise ValueError(f"{name} overlaps rows that the call reads")
+    for t in vectors:
+        if t is None:
+            continue
+        first, w = t.data_ptr(), t.nbytes
+        if first < end and first + w > begin:
+            at = (first - begin) % step
+            if at < width or at + w > step:
+                raise ValueError(f"{name} overlaps a vector that the call reads")
+
+
+def _mx_read(args: tuple, keep: tuple) -> tuple:
+    """The rows that :func:`_mx_args` gave ``(codes, stride, scales, stride)`` of and holds, as
+    :func:`_apart` takes them."""
+    return tuple((t, stride, *t.shape, False) for t, stride in zip(keep, (args[1], args[3])))
 
 
 def mx_quantize(x: torch.Tensor, bits: int = 8, activation: str | None = None) -> MX:
@@ -1547,14 +1562,13 @@ def mx_linear(x: torch.Tensor | MX, weight: MX, bias: torch.Tensor | None = None
     if quantized:
         x_bits = x.bits
         xp, xs, xsp, xss, keep_x = _mx_args(x, "x")
-        read = keep_x[0], xs, rows, keep_x[0].shape[1], False
     else:
         if x.dtype is not torch.bfloat16:
             raise TypeError(f"x must be bfloat16 or microscaled, got {x.dtype}")
         _no_gradient("mx_linear", x, bias)
         keep_x, xs = _plain_rows(x, k, "x")
         xp = keep_x.data_ptr()
-        read = keep_x, xs, rows, k, False
+        x_rows, x_stride = keep_x, xs
         x_bits, xsp, xss = 16, None, 0
         if (xs % 8 or xp % 16) and not _mx_workspace_bytes(rows, n, k, 16):  # not as the product's kernel reads them
             x_bits, keep_x = 8, mx_quantize(x)
@@ -1568,7 +1582,8 @@ def mx_linear(x: torch.Tensor | MX, weight: MX, bias: torch.Tensor | None = None
     out, out_rows, stride = _bf16_out(out, (*lead, n), weight.codes.device, "out")
     if rows and n:
         if given:
-            _apart("out", out_rows, stride, rows, n, read)
+            read = _mx_read((xp, xs, xsp, xss), keep_x) if quantized else ((x_rows, x_stride, rows, k, False),)
+            _apart("out", out_rows, stride, rows, n, *read, *_mx_read(w, keep_w), vectors=(bias,))
         nbytes = _mx_workspace_bytes(rows, n, k, x_bits)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=out.device) if nbytes else None
         _mx_call("fm_mx_linear", index, xp, x_bits, xs, xsp, xss, *w, _ptr(bias), out_rows.data_ptr(), stride, rows, n,
@@ -1590,6 +1605,7 @@ def rms_norm_mx(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: tor
         raise ValueError(f"weight holds {weight.numel()} values, a row {cols}")
     device = x.device
     shape = tuple(x.shape)
+    weight = _f32(weight)
     q = _mx_new(shape, bits, device)
     xr, xs = _plain_rows(x, cols, "x")
     rr, rs, orows, os_ = None, 0, None, 0
@@ -1600,10 +1616,10 @@ def rms_norm_mx(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: tor
         given, rows = x_out is not None, q.codes.shape[0]
         x_out, orows, os_ = _bf16_out(x_out, shape, device, "x_out")
         if given and rows:
-            _apart("x_out", orows, os_, rows, cols, (xr, xs, rows, cols, True), (rr, rs, rows, cols, True))
+            _apart("x_out", orows, os_, rows, cols, (xr, xs, rows, cols, True), (rr, rs, rows, cols, True),
+                   vectors=(weight,))
     elif x_out is not None:
         raise ValueError("x_out is the sum of x and a residual: give one")
-    weight = _f32(weight)
     rows = q.codes.shape[0]
     if rows:
         _mx_call("fm_rms_norm_mx", index, xr.data_ptr(), xs, _ptr(rr), rs, weight.data_ptr(), eps, _ptr(orows), os_,
@@ -1666,7 +1682,7 @@ def adaln_residual_mx(
     rows = q.codes.shape[0]
     if rows and y is not None and given:
         _apart("x_out", orows, os_, rows, cols, (xr, xs, 1 if shared else rows, cols, not shared),
-               (yr, ys, rows, cols, True))
+               (yr, ys, rows, cols, True), vectors=(g, sc, sh))
     if rows:
         _mx_call("fm_adaln_residual_mx", index, xr.data_ptr(), 0 if shared else xs, _ptr(yr), ys, _ptr(g),
                  int(gate_per_row), sc.data_ptr(), sh.data_ptr(), _ptr(orows), os_, eps, bits, *_mx_new_args(q), rows,
