@@ -62,7 +62,7 @@ class MXLayer:
         weights = (qkv, layer.self_attn.o_proj.weight, layer.cross_attn.q_proj.weight, layer.cross_attn.o_proj.weight)
         self.qkv, self.self_o, self.cross_q, self.cross_o = (ops.mx_quantize(w, 4) for w in weights)
         mlp = layer.mlp
-        self.activation = mlp.mlp_type
+        self.activation = "swiglu" if mlp.mlp_type == "swiglu" else "gelu"  # as the module takes its type
         up, down = (mlp.gate_up_proj, mlp.down_proj) if self.activation == "swiglu" else (mlp.fc1, mlp.fc2)
         self.up, self.up_bias = ops.mx_quantize(up.weight, 4), up.bias
         self.down, self.down_bias = ops.mx_quantize(down.weight, 4), down.bias
