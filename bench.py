@@ -561,6 +561,8 @@ def _flushed(call, args, dev, flush_mb: int = 512) -> dict:
 # (Algorithm 8) carry a state over the whole vocabulary between them and run the DiT, and
 # so every layer's cross-attention, twice.
 DRAFT_STEP_WORKLOADS = {
+    "draft-step-8b-b1": (1, 1024, 1024, 1, {}),
+    "draft-step-8b-b4": (4, 1024, 1024, 1, {}),
     "draft-step-8b-b64": (64, 256, 8192, 1, {}),
     "draft-step-8b-b64-2jump": (64, 256, 8192, 2, {}),
 }
@@ -593,7 +595,7 @@ def run_draft_step(args, dev) -> dict:
     gd = torch.Generator(device=dev).manual_seed(0)
     embed = torch.randn(cfg.vocab_size, cfg.target_hidden_size, generator=gd, device=dev).bfloat16()
     lm_head = (torch.randn(cfg.vocab_size, cfg.target_hidden_size, generator=gd, device=dev) / 64).bfloat16()
-    step = DraftStep(model, embed, lm_head, max_model_len=hi + cfg.block_size + 1, num_steps=jumps)
+    step = DraftStep(model, embed, lm_head, max_model_len=hi + cfg.block_size + 1, num_steps=jumps, mx=args.mx)
     heads, hd = step.heads, step.head_dim
     caches = []
     for _ in model.layers:
@@ -630,10 +632,12 @@ def run_draft_step(args, dev) -> dict:
     result = {
         "metric": f"{jumps}-jump draft step µs/step (anchor write, " + (
             "noise read-out" if jumps == 1 else "state embedding and update") + f", {jumps} x 6 DiT layers, "
-                  "folded head, argmax), 8B drafter, K=16, batch 64, ctx 256–8k, 1 GPU",
+                  f"folded head, argmax), 8B drafter, K=16, batch {batch}, ctx "
+                  + ("256–8k" if (lo, hi) == (256, 8192) else f"{lo}") + _mx_words(args) + ", 1 GPU",
         "value": round(ms * 1e3, 2), "unit": "us/step", "n_gpus": 1, "steps": args.steps, "warmup": args.warmup,
         "ms_per_step": round(ms, 5), "higher_is_better": False, "scaling": "weak", "vs_baseline": None,
-        "dtype": "bf16", "data": "synthetic: random-init drafter and target embedding / LM head, random paged K/V, "
+        "dtype": _step_dtype(args),
+        "data": "synthetic: random-init drafter and target embedding / LM head, random paged K/V, "
                                  "seeded draw of lengths and block table (C3's)",
         "config": {"workload": args.workload, "batch": batch, "jumps": jumps, "hidden": dim, "heads": heads,
                    "head_dim": hd, "layers": layers, "intermediate": inter, "mlp": cfg.mlp_type, "vocab": vocab,
@@ -651,6 +655,14 @@ def run_draft_step(args, dev) -> dict:
     if not args.no_cpu_baseline:
         result["cpu_baseline"] = draft_step_cpu_baseline(step, lm_head, lens, anchors.cpu(), z.cpu(), args.cpu_budget)
     return result
+
+
+def _mx_words(args) -> str:
+    return ", projections and head on microscaled 4-bit weights" if args.mx else ""
+
+
+def _step_dtype(args) -> str:
+    return "mxfp4 weights x mxfp8 rows, bf16 elsewhere" if args.mx else "bf16"
 
 
 def draft_step_cpu_baseline(step, lm_head, lens, anchors, z, budget_s) -> dict:
@@ -725,7 +737,7 @@ def run_sglang_step(args, dev) -> dict:
     gd = torch.Generator(device=dev).manual_seed(0)
     embed = torch.randn(cfg.vocab_size, cfg.target_hidden_size, generator=gd, device=dev).bfloat16()
     lm_head = (torch.randn(cfg.vocab_size, cfg.target_hidden_size, generator=gd, device=dev) / 64).bfloat16()
-    step = SGLangDraftStep(model, embed, lm_head, max_positions=hi + cfg.block_size + 1)
+    step = SGLangDraftStep(model, embed, lm_head, max_positions=hi + cfg.block_size + 1, mx=args.mx)
     heads, hd, k = step.heads, step.head_dim, cfg.block_size
     k_bufs, v_bufs = [], []
     for _ in model.layers:
@@ -759,10 +771,11 @@ def run_sglang_step(args, dev) -> dict:
         + 2 * requests * (th * dim + 2 * layers * dim * dim)
     result = {
         "metric": f"SGLang one-jump draft step µs/step ({n_cand} candidate(s) per request: anchor write, noise "
-                  "read-out, 6 DiT layers, folded head, sampler), 8B drafter, 1 GPU",
+                  "read-out, 6 DiT layers, folded head, sampler), 8B drafter" + _mx_words(args) + ", 1 GPU",
         "value": round(ms * 1e3, 2), "unit": "us/step", "n_gpus": 1, "steps": args.steps, "warmup": args.warmup,
         "ms_per_step": round(ms, 5), "higher_is_better": False, "scaling": "weak", "vs_baseline": None,
-        "dtype": "bf16", "data": "synthetic: random-init drafter and target embedding / LM head, random pools, "
+        "dtype": _step_dtype(args),
+        "data": "synthetic: random-init drafter and target embedding / LM head, random pools, "
                                  "seeded draw of lengths and pool rows",
         "config": {"workload": args.workload, "requests": requests, "candidates": n_cand, "hidden": dim,
                    "heads": heads, "head_dim": hd, "layers": layers, "intermediate": inter, "mlp": cfg.mlp_type,
@@ -1218,6 +1231,8 @@ def main() -> int:
                     + sorted(VIRTUAL_WORKLOADS) + sorted(TREE_WORKLOADS) + sorted(TREE_FP8_WORKLOADS)
                     + sorted(SELECT_WORKLOADS) + sorted(KERNEL_WORKLOADS)
                     + sorted(CONTIG_WORKLOADS) + sorted(DRAFT_STEP_WORKLOADS) + sorted(SGLANG_STEP_WORKLOADS))
+    ap.add_argument("--mx", action="store_true",
+                    help="the draft steps' projections and head on microscaled 4-bit weights")
     ap.add_argument("--no-cpu-baseline", action="store_true")
     ap.add_argument("--cpu-budget", type=float, default=12.0)
     ap.add_argument("--settle-ms", type=float, default=100.0,
@@ -1228,6 +1243,8 @@ def main() -> int:
     ap.add_argument("--calibrate-copy", type=int, default=0,
                     help="only run N copies of a 1 GiB buffer (HBM counter calibration)")
     args = ap.parse_args()
+    if args.mx and args.workload not in DRAFT_STEP_WORKLOADS and args.workload not in SGLANG_STEP_WORKLOADS:
+        ap.error(f"--mx: {args.workload} has no projections (the draft steps have)")
     if args.gpus != 1:
         print(json.dumps({"error": "this benchmark runs on one GPU; the hot path is measured per GPU "
                           "(multi-GPU sharding is a design note, not a measured configuration)"}))

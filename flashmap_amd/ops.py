@@ -1464,7 +1464,7 @@ def _apart(name: str, out: torch.Tensor, out_stride: int, rows: int, cols: int, 
            vectors: tuple = ()) -> None:
     """Refuse a given output whose rows share bytes with what is read: rows, ``others`` (tensor,
     stride, rows, cols, whether the very same rows may be given: each is read before it is
-    written), and contiguous ``vectors`` (or None)."""
+    written), and ``vectors`` (address, bytes)."""
     size = out.element_size()
     begin, step, width = out.data_ptr(), out_stride * size, cols * size
     end = begin + (rows - 1) * step + width
@@ -1476,10 +1476,7 @@ def _apart(name: str, out: torch.Tensor, out_stride: int, rows: int, cols: int, 
         at = (first - begin) % step
         if by != step or at < width or at + w > step:
             raise ValueError(f"{name} overlaps rows that the call reads")
-    for t in vectors:
-        if t is None:
-            continue
-        first, w = t.data_ptr(), t.nbytes
+    for first, w in vectors:
         if first < end and first + w > begin:
             at = (first - begin) % step
             if at < width or at + w > step:
@@ -1583,7 +1580,8 @@ def mx_linear(x: torch.Tensor | MX, weight: MX, bias: torch.Tensor | None = None
     if rows and n:
         if given:
             read = _mx_read((xp, xs, xsp, xss), keep_x) if quantized else ((x_rows, x_stride, rows, k, False),)
-            _apart("out", out_rows, stride, rows, n, *read, *_mx_read(w, keep_w), vectors=(bias,))
+            _apart("out", out_rows, stride, rows, n, *read, *_mx_read(w, keep_w),
+                   vectors=() if bias is None else ((bias.data_ptr(), 2 * n),))
         nbytes = _mx_workspace_bytes(rows, n, k, x_bits)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=out.device) if nbytes else None
         _mx_call("fm_mx_linear", index, xp, x_bits, xs, xsp, xss, *w, _ptr(bias), out_rows.data_ptr(), stride, rows, n,
@@ -1617,7 +1615,7 @@ def rms_norm_mx(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: tor
         x_out, orows, os_ = _bf16_out(x_out, shape, device, "x_out")
         if given and rows:
             _apart("x_out", orows, os_, rows, cols, (xr, xs, rows, cols, True), (rr, rs, rows, cols, True),
-                   vectors=(weight,))
+                   vectors=((weight.data_ptr(), 4 * cols),))
     elif x_out is not None:
         raise ValueError("x_out is the sum of x and a residual: give one")
     rows = q.codes.shape[0]
@@ -1677,15 +1675,17 @@ def adaln_residual_mx(
     elif x_out is not None:
         raise ValueError("x_out is the sum of x and a gated y: give one")
     sc, sh = _mx_vec(scale, cols, "scale"), _mx_vec(shift, cols, "shift")
+    gp, scp, shp = _ptr(g), sc.data_ptr(), sh.data_ptr()
     xr, xs = _plain_rows(x, cols, "x")
     q = _mx_new(shape, bits, device)
     rows = q.codes.shape[0]
     if rows and y is not None and given:
         _apart("x_out", orows, os_, rows, cols, (xr, xs, 1 if shared else rows, cols, not shared),
-               (yr, ys, rows, cols, True), vectors=(g, sc, sh))
+               (yr, ys, rows, cols, True),
+               vectors=((gp, 2 * (rows if gate_per_row else cols)), (scp, 2 * cols), (shp, 2 * cols)))
     if rows:
-        _mx_call("fm_adaln_residual_mx", index, xr.data_ptr(), 0 if shared else xs, _ptr(yr), ys, _ptr(g),
-                 int(gate_per_row), sc.data_ptr(), sh.data_ptr(), _ptr(orows), os_, eps, bits, *_mx_new_args(q), rows,
+        _mx_call("fm_adaln_residual_mx", index, xr.data_ptr(), 0 if shared else xs, _ptr(yr), ys, gp,
+                 int(gate_per_row), scp, shp, _ptr(orows), os_, eps, bits, *_mx_new_args(q), rows,
                  cols)
     return x_out, q
 
