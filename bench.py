@@ -559,7 +559,7 @@ def _flushed(call, args, dev, flush_mb: int = 512) -> dict:
 # (hidden 2048, 16 heads of 128, 6 layers, GELU MLP 8192) over a Qwen3-8B target (hidden
 # 4096, vocabulary 151936); contexts drawn as C3's, paged in 16-token blocks. Two jumps
 # (Algorithm 8) carry a state over the whole vocabulary between them and run the DiT, and
-# so every layer's cross-attention, twice.
+# so every layer's cross-attention, twice. b1 and b4: one user and four, 1024 positions each.
 DRAFT_STEP_WORKLOADS = {
     "draft-step-8b-b1": (1, 1024, 1024, 1, {}),
     "draft-step-8b-b4": (4, 1024, 1024, 1, {}),
