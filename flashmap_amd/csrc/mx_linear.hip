@@ -143,8 +143,8 @@ __device__ __forceinline__ void quantize_operand(const u32x4_t (&v)[4], int g, i
 
 // A workgroup owns 16 NB rows of W against 16 MB rows of x; its wavefronts split k and meet in
 // LDS in a fixed order. XBITS 16: x in bf16, quantized in registers. Bound: latency (a launch, the
-// loads of a wavefront's share of k, all in flight at once, and the join): 1 x 2048 -> 2048 4.7 us,
-// 16 x 2048 -> 8192 7.6 us, 9.3 MB.
+// loads of a wavefront's share of k, all in flight at once, and the join): 1 x 2048 -> 2048 3.8 us,
+// 16 x 2048 -> 8192 6.5 us, 9.3 MB.
 template <int XBITS, int MB, int NB, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void mx_linear_rows_kernel(const MxLinearArgs a) {
   __shared__ f32x4_t part[WAVES][NB * MB][64];
@@ -262,8 +262,8 @@ static int launch_rows(const MxLinearArgs &a, hipStream_t stream) {
 // streams whole 16-row blocks of W through a ring of its own in LDS, D groups of four steps
 // deep, and needs nobody: x, up to 16 MB rows of it, lies in LDS for the workgroup's whole
 // life, quantized once. A group: 16 rows of 256 bytes, as four loads of eight 128-byte
-// segments, and their scales, 16 bytes a row. Bound: HBM; 16 x 2048 -> 151936, 170 MB, 38 to 41 us,
-// 4.1 to 4.4 TB/s (with a workgroup per 16 columns and k split, 54.6 us).
+// segments, and their scales, 16 bytes a row. Bound: HBM; 16 x 2048 -> 151936, 170 MB, 37 to 38 us,
+// 4.4 to 4.6 TB/s (with a workgroup per 16 columns and k split, 61.5 us).
 template <int XBITS, int MB, int WAVES, int D>
 struct Stream {
   static constexpr int GROUP = 4096 + 256, RING = D * GROUP;
@@ -425,8 +425,8 @@ static int launch_stream(const MxLinearArgs &a, hipStream_t stream) {
 // instruction, whose clock falls under it (random codes, nothing but the instruction on every
 // SIMD: 17.5 ns with 8-bit x, 10.1 ns with 4-bit x, 3.8 and 6.6 PFLOP/s). Reached at 4096 x 20480
 // -> 4096: 252 and 188 us, 2.7 and 3.65 PFLOP/s; storing results takes 25 us per 100 MB (with k =
-// 128), partly beside other tiles' products (1024 x 2048 -> 151936 of 8-bit x 290 us, 8192 x 2048
-// -> 24576 of 4-bit x 265 us). Small products (1024 x 8192 -> 2048: 28 us) are bound by a step's way
+// 128), partly beside other tiles' products (1024 x 2048 -> 151936 of 8-bit x 284 us, 8192 x 2048
+// -> 24576 of 8-bit x 326 us, of 4-bit x 254 us). Small products (1024 x 8192 -> 2048: 25 to 28 us) are bound by a step's way
 // through a workgroup, 0.41 us for 8 instructions a wavefront, however many workgroups run.
 // Measured and not taken: a persistent grid that starts the next tile's loads before this one's
 // stores (1 % either way; the stores count among the loads awaited), four and more stages (+6 %
@@ -799,16 +799,17 @@ static bool streams(int32_t steps) {
   return Stream<XBITS, 1, STREAM_WAVES, STREAM_GROUPS>::lds(steps) <= LDS_BYTES;
 }
 
-// Measured, us, weights from HBM, x in 8 bits (bf16 x: the same order):
-//   16 rows, k 2048:  n 4096  rows 5.2, stream 6.4, tiles 8.1;  n 8192  6.7, 7.1, 8.9
-//                     n 12288 9.6, 7.4, 9.2;  n 151936 54.6, 37.7, 43.7
-//   16 rows, n 2048:  k 4096  rows 7.2, stream 9.5, tiles 9.2;  k 8192 11.7, -, 11.2;  k 20480 27.0, -, 16.0
+// Measured, us, weights from HBM (copies past the caches in turn, in a graph), x in 8 bits (bf16 x:
+// the same order):
+//   16 rows, k 2048:  n 4096  rows 4.9, stream 6.4, tiles 8.1;  n 8192  6.4, 7.1, 8.8
+//                     n 12288 9.4, 7.4, 8.9;  n 151936 61.5, 36.8, 37.7
+//   16 rows, n 2048:  k 4096  rows 7.0, stream 9.5, tiles 10.6;  k 8192 11.5, -, 12.1;  k 20480 26.9, -, 15.1
 //   more rows, tiles of 64 x 64, 64 x 128, 128 x 128 and 256 x 256:
-//     64 x 2048 -> 2048 7.8, 9.4, 12.7, -;  64 x 2048 -> 24576 12.8, 11.6, 14.4, -;  1024 x 8192 -> 2048 29.1, 28.4, 43, 76
-//     1024 x 2048 -> 8192 27.1, 24.2, 21.4, 29;  512 x 8192 -> 8192 -, 49.8, 46.3, 79;  4096 x 2048 -> 4096 53, 45, 38, 34.5
-//     300 x 2048 -> 151936 (a last row tile of 44) -, 136, 137, 168
-//   k in parts of at least 2048 values, tiles of 64 x 64: 64 x 8192 -> 2048 1 part 29, 2 14.7, 4 11.9, 8 11.9;
-//     64 x 20480 -> 2048 4 parts 22, 8 16.5, 16 19.1;  64 x 2048 -> 2048 1 part 7.8, 4 8.8
+//     64 x 2048 -> 2048 6.9, 8.5, 11.7, 22;  64 x 2048 -> 24576 11.8, 10.8, 13.0, 23;  1024 x 8192 -> 2048 29.6, 27.9, 38.6, 73
+//     1024 x 2048 -> 8192 27.9, 24.4, 21.6, 25.1;  512 x 8192 -> 8192 56, 46.8, 40.1, 74;  4096 x 2048 -> 4096 51, 43, 38.3, 30.6
+//     300 x 2048 -> 151936 (a last row tile of 44) 150, 123, 124, 137
+//   k in parts of at least 2048 values, tiles of 64 x 64: 64 x 8192 -> 2048 1 part 25.0, 2 17.7, 4 12.7, 8 12.1;
+//     64 x 20480 -> 2048 4 parts 21.2, 8 15.7, 16 18.5;  64 x 2048 -> 2048 1 part 6.9, 4 7.9
 static MxPlan plan_of(int64_t rows, int64_t n, int64_t k, int32_t x_bits) {
   const int32_t steps = (int32_t)(mx_padded(k) / MX_PAD);
   if (rows <= 16) {
@@ -867,9 +868,10 @@ static int run_plan(const MxPlan &plan, const MxLinearArgs &a, hipStream_t strea
   return fail(FM_ERR_UNSUPPORTED, "bf16 x of more than %d rows", MX_BF16_ROWS);
 }
 
-// Whether the kernel quantizes bf16 rows itself. Past these sums and columns a pass of its own in
-// front is cheaper (16 rows, us: 8192 -> 2048 15.6 / 14, 20480 -> 2048 33.7 / 19), and so it is for
-// more rows, where every workgroup would quantize them again.
+// Whether the kernel quantizes bf16 rows itself: for longer sums a pass of its own in front is
+// cheaper (16 rows, us: 8192 -> 2048 15.6 / 14, 20480 -> 2048 33.7 / 19), and so it is for more rows,
+// where every workgroup would quantize them again. With more than 8192 columns 5632 values are the
+// longest rows that lie in LDS beside the streams' rings.
 static bool quantizes(int64_t rows, int64_t n, int64_t k) {
   return rows <= MX_BF16_ROWS && k % 8 == 0 && (n <= 8192 ? k < 8192 : k <= 5632);
 }

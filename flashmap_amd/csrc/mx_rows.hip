@@ -128,12 +128,12 @@ enum { ACT_NONE = 0, ACT_GELU = 1, ACT_SWIGLU = 2 };
 // x Phi(x) = max(x, 0) - h, h = |x| / 2 erfc(|x| / sqrt 2): nothing cancels (h is at most half of
 // |x|). erfc(z) = exp(-z^2) erfcx(z), and erfcx(a / sqrt 2) / 2 is a polynomial in 1 / (1 + 0.23 a),
 // fitted to 5e-8 of its value for a up to 14.5 (least squares in Chebyshev polynomials,
-// reweighted towards the largest relative error). Over all bf16 x h comes to 5.4e-7 of its value for
-// |x| below 4 and 3.8e-6 below 13.2 (the rounding of the exponential's argument, which grows with
-// x^2); beyond it is 0 (the exponential is below 2^-126). 16 of the 65280 finite bf16 x get another
-// e4m3 code than the value rounded to float32 has, 5 another e2m1 code: a midpoint lies between the
-// two. A third of erfcf's instructions, which bounded the pass (1024 x 8192,
-// 25 MB: 14.9 us). Infinities and NaN give NaN.
+// reweighted towards the largest relative error). Over all bf16 x, with a correctly rounded
+// reciprocal and exponential, h comes to 5.4e-7 of its value for |x| below 4 and 3.8e-6 below 13.2
+// (the rounding of the exponential's argument, which grows with x^2); beyond it is 0 (the
+// exponential is below 2^-126). 16 of the 65280 finite bf16 x get another e4m3 code than the value
+// rounded to float32 has, 5 another e2m1 code: a midpoint lies between the two. A third of erfcf's
+// instructions, which bounded the pass (1024 x 8192, 25 MB: 14.9 us). Infinities and NaN give NaN.
 __device__ __forceinline__ float gelu(float x) {
 #pragma clang fp contract(off)
   const float a = fabsf(x);
@@ -168,8 +168,8 @@ __device__ __forceinline__ float swiglu(float gate, float up) {
 // need not be: mantissas are multiplied and exponents added, for negative gates as gate
 // exp(gate) / (1 + exp(gate)) * up with exp(-|gate|) = 2^n e, e from 0.7 to 1.42. -200 stands
 // for what lies below it: with any up the result is below half of the smallest float. -inf gives
-// NaN, as -inf times 0 does. Taken for every value this makes 1024 x 8192 13.5 us instead of 10.1
-// (without it 9.6).
+// NaN, as -inf times 0 does. Taken for every value this makes the pass a third longer (1024 x 8192);
+// where no gate needs it the test for it is 5 %.
 __device__ __forceinline__ bool swiglu_is_wide(float gate) { return gate < -87.f || fabsf(gate) < 0x1p-100f; }
 __device__ __forceinline__ float swiglu_wide(float gate, float up) {
 #pragma clang fp contract(off)
@@ -187,8 +187,8 @@ __device__ __forceinline__ float swiglu_wide(float gate, float up) {
 
 // A thread per 8 values, no loop: every load of the call is in flight at once, and the rows need
 // nothing of each other. Bound: HBM without an activation (24576 x 2048 bf16 to 4 bits and back
-// 48.7 us, 5.2 TB/s, a copy's rate), VALU issue with GELU (1024 x 8192 bf16 to 8 bits 10.1 us, 2.5
-// TB/s, 32 instructions a value).
+// 42.5 us, 6.0 TB/s, a copy's rate at this size) and with SwiGLU (1024 x 8192 bf16 8.8 us, 4.8 TB/s), VALU
+// issue with GELU (1024 x 8192 bf16 to 8 bits 8.6 us, 2.9 TB/s, 32 instructions a value).
 template <typename T, int BITS, int ACT>
 __global__ __launch_bounds__(ROW_THREADS) void mx_quantize_kernel(const QuantArgs a) {
   const uint32_t item = blockIdx.x * ROW_THREADS + threadIdx.x;
@@ -232,6 +232,8 @@ struct DequantArgs {
   int32_t vec;
 };
 
+// Bound: HBM to bf16 (24576 x 2048 of 4 bits 19.7 us, 6.5 TB/s); fp16 and fp32 leave value by value, 62
+// and 121 us, 2 TB/s.
 template <typename T, int BITS>
 __global__ __launch_bounds__(ROW_THREADS) void mx_dequantize_kernel(const DequantArgs a) {
   const uint32_t item = blockIdx.x * ROW_THREADS + threadIdx.x;
@@ -309,8 +311,8 @@ __device__ __forceinline__ float row_sum(float v, float *lds) {
 // s = x + y or x + gate y, the stream; then s rsqrt(mean s^2 + eps) weight (RMS), or the LayerNorm
 // (s - mean) rsqrt(var + eps) (1 + scale) + shift, its variance of the differences from the mean.
 // TPR threads a row, NCH 8-value pieces each, held in registers between the one read and the one
-// write. Bound: HBM for many rows (8192 x 4096 with a residual 49.6 us, 4.8 TB/s), a launch and a
-// round trip for few (16 x 2048 4.0 us, 1024 x 2048 6.4 us).
+// write. Bound: HBM for many rows (8192 x 4096 with a residual 42.3 us, 5.6 TB/s), a launch and a
+// round trip for few (16 x 2048 3.0 us, 1024 x 2048 5.3 us).
 // EARLY: the row-independent operands are loaded with the row, not after its statistics (one
 // round trip less, for as many registers).
 template <int TPR, int NCH, bool RMS, int BITS, bool EARLY>

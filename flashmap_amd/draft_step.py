@@ -29,9 +29,9 @@ operand; ``ops.state_update``: the jump head's softmax and the update, in place)
 Inputs are explicit (what vLLM's forward context supplies): anchors and their positions
 and slots, the noise, the caches, the block table. bf16 only.
 
-With ``mx`` the step's projections and head are held in microscaled 4 bits (a quarter of the
-bytes, which is what a step of few requests waits for) and their inputs in 8: the norms write
-them so (``ops.adaln_residual_mx``, ``ops.rms_norm_mx``), the MLP's activation is applied on the
+With ``mx`` the step reads its projections and head in microscaled 4 bits (a quarter of the
+bytes, which is what a step of few requests waits for), from copies made when the step is; the
+drafter's own weights stay as they are. Their inputs are held in 8: the norms write them so (``ops.adaln_residual_mx``, ``ops.rms_norm_mx``), the MLP's activation is applied on the
 way into them (``ops.mx_quantize``), and the products are ``ops.mx_linear``. Drafts are verified,
 so that this costs acceptance and never correctness. The several-jump state's embedding stays
 bf16.
@@ -104,8 +104,8 @@ class DraftStep:
     rows); ``hot_ids``: the draft vocabulary's token ids when the drafter has a state
     vocabulary (``draft_ids``) or vLLM restricts it (``d2t``), else None; ``num_steps``:
     the jumps per draft (the drafter's configured count when None; the config's
-    ``jump_grids`` must hold a grid for it); ``mx``: hold the projections and the head in
-    microscaled 4 bits."""
+    ``jump_grids`` must hold a grid for it); ``mx``: the projections and the head are read
+    from copies in microscaled 4 bits, made here."""
 
     @torch.no_grad()
     def __init__(self, model: FlashMapDraftModel, embed_tokens: torch.Tensor, lm_head: torch.Tensor,

@@ -1494,7 +1494,8 @@ def mx_quantize(x: torch.Tensor, bits: int = 8, activation: str | None = None) -
     scale is the power of two that brings its largest magnitude to [256, 512) (e4m3) or [4, 8)
     (e2m1), codes round to nearest even and saturate at 448 or 6, and a block holding an
     infinity or a NaN is all NaN. ``activation``: "gelu" (the exact one) or "swiglu" (``x (...,
-    2 cols)``: silu of the first half of a row times the second) in float32 on the way."""
+    2 cols)``: silu of the first half of a row times the second) in float32 on the way; a result
+    that float32 cannot hold is infinite, one below 2^-126 may be 0."""
     index = _mx_device(x)
     dtype = _LOGIT_DTYPES.get(x.dtype)
     if dtype is None:

@@ -26,8 +26,8 @@ The plugin's drafts of several jumps go through its jump bank (flashmap/sglang/
 jump_bank.py), a different scheme from the vLLM plugin's vocabulary-sized state; this
 step takes one jump. GEMMs are hipBLASLt through torch; bf16 only.
 
-With ``mx`` the projections and the head are held in microscaled 4 bits and their inputs go to
-8 on the way out of the norms and activations, as in ``flashmap_amd.draft_step``.
+With ``mx`` the projections and the head are read from copies in microscaled 4 bits and their
+inputs go to 8 on the way out of the norms and activations, as in ``flashmap_amd.draft_step``.
 """
 
 from __future__ import annotations
@@ -49,8 +49,8 @@ class SGLangDraftStep:
     drafter (bf16, on the GPU); ``embed_tokens`` / ``lm_head``: the target's ``(V, H)``
     weights; ``max_positions``: the positions the pool writer's rotary table covers (the
     server's longest request plus a block); ``hot_ids``: the draft vocabulary's token ids
-    (a drafter's ``draft_ids``), else None; ``mx``: hold the projections and the head in
-    microscaled 4 bits."""
+    (a drafter's ``draft_ids``), else None; ``mx``: the projections and the head are read
+    from copies in microscaled 4 bits, made here."""
 
     @torch.no_grad()
     def __init__(self, model: FlashMapDraftModel, embed_tokens: torch.Tensor, lm_head: torch.Tensor,
