@@ -12,7 +12,8 @@
 // 8 products are aligned to the group's largest, cut below 2^-13 of its power of two (an e2m1
 // product spans less and is exact), and the groups and steps added as floats. With an e4m3
 // operand that costs 4e-6 to 9e-6 of a result (hidden states with outlying channels, sums of
-// 128 to 65536 products), against 2^-9 for its rounding to bf16 and 2^-5 for the operand's own.
+// 128 to 65536 products) and at most 3e-5 of the absolute sum (sums made to cancel; 6e-7 in the
+// mean), against 2^-9 for its rounding to bf16 and 2^-5 for the operand's own.
 //
 // Rows are padded with zeros to multiples of 128 values, so the loops over k have no tail.
 #include <stdint.h>

@@ -1,5 +1,6 @@
-"""The activations on the way to microscaled rows over everything that their inputs' types hold,
-each value in a block of its own, against float64 (oracle/mx.py)."""
+"""Microscaled operators where their accuracy shows: the activations over everything that their
+inputs' types hold, each value in a block of its own, and products whose sums cancel, against
+float64 (oracle/mx.py)."""
 
 import pytest
 import torch
@@ -69,3 +70,31 @@ def test_gelu_over_the_whole_range(dev, dtype, bits):
     differ = ((code[fine] != best[0]).any(1) | (scale[fine] != best[1]).any(1)) & (want[:, 0].abs() > 2.0 ** -126)
     print(f"gelu {dtype} bits={bits}: {int(differ.sum())} of {len(v)} codes are not those of the value rounded to float32, "
           f"at x from {x[fine][differ].abs().min():.3g}" if differ.any() else "gelu: all codes as rounded", flush=True)
+
+
+@pytest.mark.parametrize("kind", ["bf16", 8, 4])
+@pytest.mark.parametrize("rows,n,k", [(1, 48, 2048), (16, 40, 1024), (40, 70, 2048), (130, 64, 512)])
+def test_sums_that_cancel(dev, rows, n, k, kind):
+    """What the product's sums lose, not hidden by the rounding of a result of the sum's size: the
+    second half of k holds the first half's values again, negated and in another order, and one
+    column of its own. Per step of 128 the 16 groups of 8 products lose at most 7 2^-13 of each
+    group's largest product, together of the step's 16 largest (nothing with 4-bit rows); the
+    float32 sums 2^-15 of the absolute sum."""
+    g = torch.Generator().manual_seed(rows + k)
+    half = k // 2
+    order = torch.cat([32 * b + torch.randperm(32, generator=g) for b in torch.randperm(half // 32, generator=g)])
+    x = torch.randn(rows, half, generator=g) * torch.exp(torch.randn(half, generator=g))
+    w = torch.randn(n, half, generator=g)
+    x, w = torch.cat([x, -x[:, order]], 1).bfloat16(), torch.cat([w, w[:, order]], 1)
+    x[:, -1] *= 1.25
+    weight = ops.mx_quantize(w.to(dev), 4)
+    given = x.to(dev) if kind == "bf16" else ops.mx_quantize(x.to(dev), kind)
+    xv = mx.values(*(mx.quantize(x, 8) if kind == "bf16" else codes_of(given)), 4 if kind == 4 else 8)
+    products = xv[:, None] * mx.values(*codes_of(weight), 4)[None]
+    ref, size = products.sum(-1), products.abs().sum(-1)
+    lost = 0 if kind == 4 else 7 * 2.0 ** -13 * products.abs().view(rows, n, -1, 128).topk(16, -1).values.sum((-1, -2))
+    err = (ops.mx_linear(given, weight).cpu().double() - ref).abs()
+    over = (err - 2.0 ** -8 * ref.abs()).clamp(min=0) / size
+    print(f"mx_linear rows={rows} n={n} k={k} x={kind}: sums of {float((ref.abs() / size).median()):.2e} of their absolute "
+          f"sum, off by {float(over.max()):.1e} of it at most, {float(over.mean()):.1e} in the mean", flush=True)
+    assert (err <= 2.0 ** -8 * ref.abs() + lost + 2.0 ** -15 * size).all()
