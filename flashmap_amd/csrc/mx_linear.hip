@@ -142,40 +142,35 @@ __device__ __forceinline__ void quantize_operand(const u32x4_t (&v)[4], int g, i
   scale = (int)(g & 1 ? swapped[1] : swapped[0]);
 }
 
-// A workgroup owns 16 NB rows of W against 16 MB rows of x; its wavefronts split k and meet in
+// A workgroup owns 16 NB rows of W against up to 16 rows of x; its wavefronts split k and meet in
 // LDS in a fixed order. XBITS 16: x in bf16, quantized in registers. Bound: latency (a launch, the
 // loads of a wavefront's share of k, all in flight at once, and the join): 1 x 2048 -> 2048 3.8 us,
 // 16 x 2048 -> 8192 6.5 us, 9.3 MB.
-template <int XBITS, int MB, int NB, int WAVES>
+template <int XBITS, int NB, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void mx_linear_rows_kernel(const MxLinearArgs a) {
-  __shared__ f32x4_t part[WAVES][NB * MB][64];
+  __shared__ f32x4_t part[WAVES][NB][64];
   constexpr int XL = XBITS == 16 ? 4 : XBITS == 8 ? 2 : 1;  // 16-byte loads of x a step
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int r = lane & 15, g = lane >> 4;
   const int32_t n0 = (int32_t)blockIdx.x * 16 * NB;
   const int32_t s0 = (int32_t)((int64_t)a.steps * wave / WAVES), s1 = (int32_t)((int64_t)a.steps * (wave + 1) / WAVES);
   // Rows past the end read the last one: their results are not stored.
-  const uint8_t *w[NB], *wsc[NB], *x[MB], *xsc[MB];
+  const uint8_t *w[NB], *wsc[NB];
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
     const int64_t n = n0 + 16 * j + r < a.n ? n0 + 16 * j + r : a.n - 1;
     w[j] = a.w + n * a.ws + 16 * g, wsc[j] = a.wsc + n * a.wss + g;
   }
+  const int64_t row = r < a.rows ? r : a.rows - 1;
+  const uint8_t *const x = a.x + row * a.xs + (XBITS == 16 ? 32 : 16) * g;
+  const uint8_t *const xsc = XBITS == 16 ? nullptr : a.xsc + row * a.xss + g;
+  f32x4_t acc[NB];
 #pragma unroll
-  for (int i = 0; i < MB; ++i) {
-    const int64_t m = 16 * i + r < a.rows ? 16 * i + r : a.rows - 1;
-    x[i] = a.x + m * a.xs + (XBITS == 16 ? 32 : 16) * g;
-    xsc[i] = XBITS == 16 ? nullptr : a.xsc + m * a.xss + g;
-  }
-  f32x4_t acc[NB][MB];
-#pragma unroll
-  for (int j = 0; j < NB; ++j)
-#pragma unroll
-    for (int i = 0; i < MB; ++i) acc[j][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < NB; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   auto take = [&](auto group, int32_t s) {  // steps s .. s + G - 1, all their loads in flight at once
     constexpr int G = decltype(group)::value;
-    u32x4_t wf[G][NB], xf[G][MB][XL];
-    int sw[G][NB], sx[G][MB];
+    u32x4_t wf[G][NB], xf[G][XL];
+    int sw[G][NB], sx[G];
 #pragma unroll
     for (int t = 0; t < G; ++t) {
       const int64_t at = s + t;
@@ -185,38 +180,32 @@ __global__ __launch_bounds__(64 * WAVES) void mx_linear_rows_kernel(const MxLine
 #pragma unroll
     for (int t = 0; t < G; ++t) {
       const int64_t at = s + t;
+      if constexpr (XBITS == 16) {
+        // k is a multiple of 8: a 16-byte load past the row's end is zeros
+        const int32_t k0 = 128 * (int32_t)at + 16 * g;
 #pragma unroll
-      for (int i = 0; i < MB; ++i) {
-        if constexpr (XBITS == 16) {
-          // k is a multiple of 8: a 16-byte load past the row's end is zeros
-          const int32_t k0 = 128 * (int32_t)at + 16 * g;
-#pragma unroll
-          for (int l = 0; l < 4; ++l) {
-            const int o = 64 * (l >> 1) + 8 * (l & 1);
-            xf[t][i][l] = k0 + o < a.k ? load16(x[i] + 256 * at + 2 * o) : u32x4_t{0, 0, 0, 0};
-          }
-        } else {
-#pragma unroll
-          for (int l = 0; l < XL; ++l) xf[t][i][l] = load16(x[i] + 64 * XL * at + 64 * l);
-          sx[t][i] = xsc[i][4 * at];
+        for (int l = 0; l < 4; ++l) {
+          const int o = 64 * (l >> 1) + 8 * (l & 1);
+          xf[t][l] = k0 + o < a.k ? load16(x + 256 * at + 2 * o) : u32x4_t{0, 0, 0, 0};
         }
+      } else {
+#pragma unroll
+        for (int l = 0; l < XL; ++l) xf[t][l] = load16(x + 64 * XL * at + 64 * l);
+        sx[t] = xsc[4 * at];
       }
     }
 #pragma unroll
     for (int t = 0; t < G; ++t) {
+      i32x8_t xo;
+      if constexpr (XBITS == 16)
+        quantize_operand(xf[t], g, xo, sx[t]);
+      else if constexpr (XBITS == 8)
+        xo = operand(xf[t][0], xf[t][1]);
+      else
+        xo = operand(xf[t][0]);
 #pragma unroll
-      for (int i = 0; i < MB; ++i) {
-        i32x8_t xo;
-        if constexpr (XBITS == 16)
-          quantize_operand(xf[t][i], g, xo, sx[t][i]);
-        else if constexpr (XBITS == 8)
-          xo = operand(xf[t][i][0], xf[t][i][1]);
-        else
-          xo = operand(xf[t][i][0]);
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-          acc[j][i] = mfma_mx<XBITS == 4 ? 4 : 8>(operand(wf[t][j]), xo, acc[j][i], sw[t][j], sx[t][i]);
-      }
+      for (int j = 0; j < NB; ++j)
+        acc[j] = mfma_mx<XBITS == 4 ? 4 : 8>(operand(wf[t][j]), xo, acc[j], sw[t][j], sx[t]);
     }
   };
   int32_t s = s0;
@@ -224,18 +213,16 @@ __global__ __launch_bounds__(64 * WAVES) void mx_linear_rows_kernel(const MxLine
   if (s1 - s & 2) take(std::integral_constant<int, 2>{}, s), s += 2;
   if (s1 - s & 1) take(std::integral_constant<int, 1>{}, s);
 #pragma unroll
-  for (int j = 0; j < NB; ++j)
-#pragma unroll
-    for (int i = 0; i < MB; ++i) part[wave][j * MB + i][lane] = acc[j][i];
+  for (int j = 0; j < NB; ++j) part[wave][j][lane] = acc[j];
   __syncthreads();
-  for (int b = wave; b < NB * MB; b += WAVES) {
+  for (int b = wave; b < NB; b += WAVES) {
     f32x4_t sum = part[0][b][lane];
 #pragma unroll
     for (int q = 1; q < WAVES; ++q) sum += part[q][b][lane];
-    // Lane: row m of out, columns n .. n + 3.
-    const int32_t m = 16 * (b % MB) + r, n = n0 + 16 * (b / MB) + 4 * g;
-    if (m >= a.rows) continue;
-    uint16_t *dst = a.out + m * a.os + n;
+    // Lane: row r of out, columns n .. n + 3.
+    const int32_t n = n0 + 16 * b + 4 * g;
+    if (r >= a.rows) continue;
+    uint16_t *dst = a.out + r * a.os + n;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (a.bias != nullptr && n + i < a.n) sum[i] += bf16_to_f32(a.bias[n + i]);
@@ -249,10 +236,10 @@ __global__ __launch_bounds__(64 * WAVES) void mx_linear_rows_kernel(const MxLine
   }
 }
 
-template <int XBITS, int MB, int NB, int WAVES>
+template <int XBITS, int NB, int WAVES>
 static int launch_rows(const MxLinearArgs &a, hipStream_t stream) {
   const unsigned tiles = (unsigned)((a.n + 16 * NB - 1) / (16 * NB));
-  mx_linear_rows_kernel<XBITS, MB, NB, WAVES><<<dim3(tiles), dim3(64 * WAVES), 0, stream>>>(a);
+  mx_linear_rows_kernel<XBITS, NB, WAVES><<<dim3(tiles), dim3(64 * WAVES), 0, stream>>>(a);
   FM_CHECK_HIP(hipGetLastError());
   return FM_OK;
 }
@@ -261,51 +248,48 @@ static int launch_rows(const MxLinearArgs &a, hipStream_t stream) {
 
 // Weights larger than what is in flight at once (a head over the vocabulary): a wavefront
 // streams whole 16-row blocks of W through a ring of its own in LDS, D groups of four steps
-// deep, and needs nobody: x, up to 16 MB rows of it, lies in LDS for the workgroup's whole
+// deep, and needs nobody: x, up to 16 rows of it, lies in LDS for the workgroup's whole
 // life, quantized once. A group: 16 rows of 256 bytes, as four loads of eight 128-byte
 // segments, and their scales, 16 bytes a row. Bound: HBM; 16 x 2048 -> 151936, 170 MB, 37 to 38 us,
 // 4.4 to 4.6 TB/s (with a workgroup per 16 columns and k split, 61.5 us).
-template <int XBITS, int MB, int WAVES, int D>
+template <int XBITS, int WAVES, int D>
 struct Stream {
   static constexpr int GROUP = 4096 + 256, RING = D * GROUP;
-  static constexpr int XSTEP = MB * 16 * (XBITS == 4 ? 64 : 128);  // bytes of a step of x
-  static size_t lds(int32_t steps) { return WAVES * RING + (size_t)steps * XSTEP + (size_t)((steps + 3) / 4) * MB * 256; }
+  static constexpr int XSTEP = 16 * (XBITS == 4 ? 64 : 128);  // bytes of a step of x
+  static size_t lds(int32_t steps) { return WAVES * RING + (size_t)steps * XSTEP + (size_t)((steps + 3) / 4) * 256; }
 };
 
-template <int XBITS, int MB, int WAVES, int D>
+template <int XBITS, int WAVES, int D>
 __global__ __launch_bounds__(64 * WAVES) void mx_linear_stream_kernel(const MxLinearArgs a) {
-  using T = Stream<XBITS, MB, WAVES, D>;
+  using T = Stream<XBITS, WAVES, D>;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int r = lane & 15, g = lane >> 4;
   const int at4 = 64 * r + 16 * (g ^ swizzle4(r));
   const int at8 = 128 * r + 16 * (g ^ swizzle8(r)), at8h = at8 ^ 64;
   char *const xl = lds + WAVES * T::RING, *const xsl = xl + a.steps * T::XSTEP;
+  const int64_t row = r < a.rows ? r : a.rows - 1;
   for (int32_t s = wave; s < a.steps; s += WAVES) {
+    i32x8_t codes;
+    int scale;
+    if constexpr (XBITS == 16) {
+      u32x4_t v[4];
 #pragma unroll
-    for (int i = 0; i < MB; ++i) {
-      const int64_t m = 16 * i + r < a.rows ? 16 * i + r : a.rows - 1;
-      i32x8_t codes;
-      int scale;
-      if constexpr (XBITS == 16) {
-        u32x4_t v[4];
-#pragma unroll
-        for (int l = 0; l < 4; ++l) {
-          const int32_t k = 128 * s + 16 * g + 64 * (l >> 1) + 8 * (l & 1);  // zeros past the row's end
-          v[l] = k < a.k ? load16(a.x + m * a.xs + 2 * (int64_t)k) : u32x4_t{0, 0, 0, 0};
-        }
-        quantize_operand(v, g, codes, scale);
-      } else {
-        const uint8_t *x = a.x + m * a.xs + (XBITS == 8 ? 128 : 64) * (int64_t)s + 16 * g;
-        codes = XBITS == 8 ? operand(load16(x), load16(x + 64)) : operand(load16(x));
-        scale = a.xsc[m * a.xss + 4 * (int64_t)s + g];
+      for (int l = 0; l < 4; ++l) {
+        const int32_t k = 128 * s + 16 * g + 64 * (l >> 1) + 8 * (l & 1);  // zeros past the row's end
+        v[l] = k < a.k ? load16(a.x + row * a.xs + 2 * (int64_t)k) : u32x4_t{0, 0, 0, 0};
       }
-      char *const to = xl + s * T::XSTEP + i * (T::XSTEP / MB);
-      store16(to + (XBITS == 4 ? at4 : at8), u32x4_t{(uint32_t)codes[0], (uint32_t)codes[1], (uint32_t)codes[2], (uint32_t)codes[3]});
-      if constexpr (XBITS != 4)
-        store16(to + at8h, u32x4_t{(uint32_t)codes[4], (uint32_t)codes[5], (uint32_t)codes[6], (uint32_t)codes[7]});
-      xsl[((s >> 2) * MB + i) * 256 + 16 * r + 4 * g + (s & 3)] = (char)scale;
+      quantize_operand(v, g, codes, scale);
+    } else {
+      const uint8_t *x = a.x + row * a.xs + (XBITS == 8 ? 128 : 64) * (int64_t)s + 16 * g;
+      codes = XBITS == 8 ? operand(load16(x), load16(x + 64)) : operand(load16(x));
+      scale = a.xsc[row * a.xss + 4 * (int64_t)s + g];
     }
+    char *const to = xl + s * T::XSTEP;
+    store16(to + (XBITS == 4 ? at4 : at8), u32x4_t{(uint32_t)codes[0], (uint32_t)codes[1], (uint32_t)codes[2], (uint32_t)codes[3]});
+    if constexpr (XBITS != 4)
+      store16(to + at8h, u32x4_t{(uint32_t)codes[4], (uint32_t)codes[5], (uint32_t)codes[6], (uint32_t)codes[7]});
+    xsl[(s >> 2) * 256 + 16 * r + 4 * g + (s & 3)] = (char)scale;
   }
   __syncthreads();
 
@@ -338,9 +322,7 @@ __global__ __launch_bounds__(64 * WAVES) void mx_linear_stream_kernel(const MxLi
   for (int d = 0; d < D; ++d)
     if (d < total) issue();
   const uint32_t pick = 0x0400u + 0x0101u * (uint32_t)g;
-  f32x4_t acc[MB];
-#pragma unroll
-  for (int i = 0; i < MB; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
   int32_t block = b0, grp = 0, slot = 0;
   for (int64_t t = 0; t < total; ++t) {
     // In flight behind this group: up to D - 1 groups, 5 loads each (and results being stored,
@@ -353,25 +335,19 @@ __global__ __launch_bounds__(64 * WAVES) void mx_linear_stream_kernel(const MxLi
     const u32x4_t d = *(const u32x4_t *)(wl + 4096 + 16 * r);
     const uint32_t a01 = __builtin_amdgcn_perm(d[1], d[0], pick), a23 = __builtin_amdgcn_perm(d[3], d[2], pick);
     const int sw = (int)__builtin_amdgcn_perm(a23, a01, 0x05040100);
-    int sx[MB];
-#pragma unroll
-    for (int i = 0; i < MB; ++i) sx[i] = *(const int *)(xsl + (grp * MB + i) * 256 + 16 * r + 4 * g);
+    const int sx = *(const int *)(xsl + grp * 256 + 16 * r + 4 * g);
     auto step = [&](auto jc) {
       constexpr int J = decltype(jc)::value;
       const int32_t s = 4 * grp + J;
       if (s >= a.steps) return;
       const i32x8_t wf = operand(load16(wl + 2048 * (J >> 1) + (J & 1 ? at8h : at8)));
       const char *x = xl + s * T::XSTEP;
-#pragma unroll
-      for (int i = 0; i < MB; ++i) {
-        const char *xi = x + i * (T::XSTEP / MB);
-        i32x8_t xf;
-        if constexpr (XBITS == 4)
-          xf = operand(load16(xi + at4));
-        else
-          xf = operand(load16(xi + at8), load16(xi + at8h));
-        acc[i] = mfma_mx_op<XBITS == 4 ? 4 : 8, J>(wf, xf, acc[i], sw, sx[i]);
-      }
+      i32x8_t xf;
+      if constexpr (XBITS == 4)
+        xf = operand(load16(x + at4));
+      else
+        xf = operand(load16(x + at8), load16(x + at8h));
+      acc = mfma_mx_op<XBITS == 4 ? 4 : 8, J>(wf, xf, acc, sw, sx);
     };
     step(std::integral_constant<int, 0>{});
     step(std::integral_constant<int, 1>{});
@@ -382,38 +358,34 @@ __global__ __launch_bounds__(64 * WAVES) void mx_linear_stream_kernel(const MxLi
     if (t + D < total) issue();
     slot = slot == D - 1 ? 0 : slot + 1;
     if (++grp == groups) {
-      // Lane: row m of out, columns n .. n + 3.
+      // Lane: row r of out, columns n .. n + 3.
       const int32_t n = 16 * block + 4 * g;
+      if (r < a.rows) {
+        uint16_t *dst = a.out + r * a.os + n;
 #pragma unroll
-      for (int i = 0; i < MB; ++i) {
-        const int32_t m = 16 * i + r;
-        if (m < a.rows) {
-          uint16_t *dst = a.out + m * a.os + n;
+        for (int q = 0; q < 4; ++q)
+          if (a.bias != nullptr && n + q < a.n) acc[q] += bf16_to_f32(a.bias[n + q]);
+        if (a.out_unit >= 4 && n + 4 <= a.n) {
+          *reinterpret_cast<u32x2_t *>(dst) = u32x2_t{pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
+        } else {
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            if (a.bias != nullptr && n + q < a.n) acc[i][q] += bf16_to_f32(a.bias[n + q]);
-          if (a.out_unit >= 4 && n + 4 <= a.n) {
-            *reinterpret_cast<u32x2_t *>(dst) = u32x2_t{pack_bf16x2(acc[i][0], acc[i][1]), pack_bf16x2(acc[i][2], acc[i][3])};
-          } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (n + q < a.n) dst[q] = (uint16_t)(pack_bf16x2(acc[i][q], 0.f) & 0xffffu);
-          }
+            if (n + q < a.n) dst[q] = (uint16_t)(pack_bf16x2(acc[q], 0.f) & 0xffffu);
         }
-        acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
       }
+      acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
       grp = 0, ++block;
     }
   }
 }
 
-template <int XBITS, int MB, int WAVES, int D>
+template <int XBITS, int WAVES, int D>
 static int launch_stream(const MxLinearArgs &a, hipStream_t stream) {
   DeviceInfo info;
   const int rc = device_info(&info);
   if (rc != FM_OK) return rc;
-  mx_linear_stream_kernel<XBITS, MB, WAVES, D>
-      <<<dim3((unsigned)info.cus), dim3(64 * WAVES), Stream<XBITS, MB, WAVES, D>::lds(a.steps), stream>>>(a);
+  mx_linear_stream_kernel<XBITS, WAVES, D>
+      <<<dim3((unsigned)info.cus), dim3(64 * WAVES), Stream<XBITS, WAVES, D>::lds(a.steps), stream>>>(a);
   FM_CHECK_HIP(hipGetLastError());
   return FM_OK;
 }
@@ -797,7 +769,7 @@ constexpr int STREAM_WAVES = 8, STREAM_GROUPS = 2;
 
 template <int XBITS>
 static bool streams(int32_t steps) {
-  return Stream<XBITS, 1, STREAM_WAVES, STREAM_GROUPS>::lds(steps) <= LDS_BYTES;
+  return Stream<XBITS, STREAM_WAVES, STREAM_GROUPS>::lds(steps) <= LDS_BYTES;
 }
 
 // Measured, us, weights from HBM (copies past the caches in turn, in a graph), x in 8 bits (bf16 x:
@@ -836,9 +808,9 @@ static int64_t part_stride(int64_t n) { return (n + 7) / 8 * 8; }
 
 template <int XBITS>
 static int run_plan(const MxPlan &plan, const MxLinearArgs &a, hipStream_t stream) {
-  if (plan.kind == MxPlan::STREAM) return launch_stream<XBITS, 1, STREAM_WAVES, STREAM_GROUPS>(a, stream);
+  if (plan.kind == MxPlan::STREAM) return launch_stream<XBITS, STREAM_WAVES, STREAM_GROUPS>(a, stream);
   if (plan.kind == MxPlan::ROWS)
-    return a.n <= 4096 ? launch_rows<XBITS, 1, 1, 8>(a, stream) : launch_rows<XBITS, 1, 2, 8>(a, stream);
+    return a.n <= 4096 ? launch_rows<XBITS, 1, 8>(a, stream) : launch_rows<XBITS, 2, 8>(a, stream);
   if constexpr (XBITS != 16) {
     if (plan.bm == 256) {
       // A tile a CU: where the last round is for few, its columns' tiles go to a launch of smaller
