@@ -117,6 +117,17 @@ SIGNATURES: dict[str, tuple] = {
     "fm_adaln_residual_mx": (
         c_int, [P, I64, P, I64, P, I32, P, P, P, I64, F32, I32, P, I64, P, I64, I64, I32, P]
     ),
+    "fm_write_context_kv_mx": (
+        c_int, [P, I64, I32, I32, I32, P, P, P, *_ROPE, P, P, I64, I64, I64, I32, F32, P]
+    ),
+    "fm_block_attn_paged_mx_workspace_bytes": (c_size_t, [I32, I32, I32, I32]),
+    "fm_block_attn_paged_mx": (
+        c_int,
+        [P, I64, I64, I64, P, I64, I64, P, P, I64, P, I64, I64, I32, P, I64, I64, P, I32, I32, I32, I32, I32, I32, F32,
+         *_PROLOGUE, P, c_size_t, P],
+    ),
+    "fm_log_probs_workspace_bytes": (c_size_t, [I64, I64, I32]),
+    "fm_log_probs_rows": (c_int, [P, I32, I64, I64, I64, P, P, I32, P, P, P, P, P, P, c_size_t, P]),
     "fm_profile_enable": (c_int, [c_int]),
     "fm_clock_probe": (c_int, [P, ctypes.c_uint64, P]),
     "fm_profile_read": (c_int, [ctypes.POINTER(c_double), ctypes.POINTER(c_int64)]),

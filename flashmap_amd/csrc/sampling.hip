@@ -22,8 +22,8 @@
 #include <math.h>
 #include <stdint.h>
 
-#include "fm_device.h"
 #include "fm_host.h"
+#include "logits_device.h"
 
 namespace fm {
 
@@ -32,8 +32,6 @@ constexpr int SEL_THREADS = 256;
 // flight per wavefront (1024 x 151936 bf16 logits in 64 us against 71 us with 32 per thread).
 constexpr int SEL_TILE = 16384;
 constexpr int NOISE_COLS = 1024;  // columns per workgroup of seeded normals (4 per thread)
-
-enum LogitType { LOGITS_BF16 = 0, LOGITS_F16 = 1, LOGITS_F32 = 2 };
 
 __device__ __forceinline__ void philox4x32_10(uint32_t (&c)[4], uint32_t k0, uint32_t k1) {
 #pragma unroll
@@ -231,73 +229,6 @@ __device__ __forceinline__ int32_t ordered(float f) {
 }
 __device__ __forceinline__ float unordered(int32_t i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
 
-// Eight consecutive logits as they are stored (few registers while a tile is in flight).
-template <int TY>
-struct Chunk {
-  static constexpr int WORDS = TY == LOGITS_F32 ? 8 : 4, PER_WORD = 8 / WORDS;
-  uint32_t w[WORDS];
-  // The compiler takes the words as new from here on: the logits decoded before are not
-  // kept for a later pass over them (32 registers, which would spill).
-  __device__ __forceinline__ void forget() {
-#pragma unroll
-    for (int q = 0; q < WORDS; ++q) asm volatile("" : "+v"(w[q]));
-  }
-  __device__ __forceinline__ float at(int j) const {
-    const uint32_t v = w[j / PER_WORD];
-    if (TY == LOGITS_F32) return __uint_as_float(v);
-    if (TY == LOGITS_BF16) return j & 1 ? bf16_hi(v) : bf16_lo(v);
-    return j & 1 ? f16_hi(v) : f16_lo(v);
-  }
-  // -inf in the place of logit j.
-  __device__ __forceinline__ void drop(int j) {
-    uint32_t &v = w[j / PER_WORD];
-    if (TY == LOGITS_F32)
-      v = 0xFF800000u;
-    else
-      v = j & 1 ? (v & 0xFFFFu) | (TY == LOGITS_BF16 ? 0xFF800000u : 0xFC000000u)
-                : (v & 0xFFFF0000u) | (TY == LOGITS_BF16 ? 0xFF80u : 0xFC00u);
-  }
-};
-
-// A row as 16-byte granules from the one its first logit lies in: `skip` logits of that
-// granule come before the row, and the last granule may end past it. Loads are of whole
-// granules with a logit of the row in them (no allocation ends inside one); the logits
-// around the row are dropped after the load.
-template <int TY>
-struct RowView {
-  static constexpr int ES = TY == LOGITS_F32 ? 4 : 2;
-  const char *from;
-  uint32_t skip, vocab, last;  // last: the row's last granule
-  __device__ __forceinline__ RowView(const SelectArgs &a, int64_t row) {
-    const char *src = a.logits + row * a.row_bytes;
-    skip = (uint32_t)((uintptr_t)src & 15) / ES;
-    from = src - skip * ES;
-    vocab = (uint32_t)a.vocab;
-    last = (uint32_t)(((uint64_t)skip + vocab - 1) * ES / 16);
-  }
-  // Chunk g: the logits of columns 8 g - skip to 8 g - skip + 7.
-  __device__ __forceinline__ Chunk<TY> chunk(uint32_t g) const {
-    Chunk<TY> c;
-#pragma unroll
-    for (int h = 0; h < ES / 2; ++h) {
-      const uint32_t n = g * (ES / 2) + h;
-      const u32x4_t v = load16(from + 16 * (uint64_t)(n < last ? n : last));
-#pragma unroll
-      for (int q = 0; q < 4; ++q) c.w[4 * h + q] = v[q];
-    }
-    return c;
-  }
-  // Whether some of n chunks from g on reach past either end.
-  __device__ __forceinline__ bool edge(uint32_t g, uint32_t n) const {
-    return (g == 0 && skip != 0) || 8 * ((uint64_t)g + n) > (uint64_t)skip + vocab;
-  }
-  __device__ __forceinline__ void trim(Chunk<TY> &c, uint32_t g) const {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (8 * g - skip + j >= vocab) c.drop(j);
-  }
-};
-
 // The largest of a thread's logits of a tile (NaN aside) and whether one is NaN.
 template <int TY>
 __device__ __forceinline__ float tile_max(Chunk<TY> (&x)[SAMPLE_IT], bool &nan) {
@@ -352,7 +283,7 @@ __global__ __launch_bounds__(THREADS, TY == LOGITS_F32 ? 4 : 8) void sample_part
   __shared__ Pending queues[THREADS / 64][SAMPLE_QUEUE];
   __shared__ int32_t bound;
   const int64_t row = blockIdx.y;
-  const RowView<TY> view(a, row);
+  const RowView<TY> view(a.logits + row * a.row_bytes, a.vocab);
   const uint32_t chunks = (view.skip + view.vocab + 7) / 8, hop = gridDim.x * CHUNKS;
   if (!SEVERAL && chunks <= THREADS) {  // a chunk per thread: every logit drawn for, no bound
     sample_short<TY, THREADS>(a, view, row);

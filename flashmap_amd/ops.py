@@ -12,6 +12,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+from collections.abc import Sequence
 from dataclasses import dataclass
 
 import torch
@@ -20,6 +21,7 @@ from . import _native
 from ._native import call
 
 __all__ = [
+    "LogProbs",
     "MX",
     "Rope",
     "adaln_residual",
@@ -30,10 +32,13 @@ __all__ = [
     "block_attention_contig",
     "block_attention_paged",
     "block_attention_paged_fp8",
+    "block_attention_paged_mx",
     "block_attention_paged_runs",
     "block_attention_token_paged",
     "block_attention_token_paged_fp8",
     "block_self_attention",
+    "log_probs_rows",
+    "mx_cache",
     "mx_dequantize",
     "mx_linear",
     "mx_quantize",
@@ -49,6 +54,7 @@ __all__ = [
     "workspace_for",
     "write_context_kv",
     "write_context_kv_fp8",
+    "write_context_kv_mx",
     "write_context_kv_pool",
     "write_context_kv_pool_fp8",
 ]
@@ -1110,6 +1116,62 @@ def sample_rows(
                    seed.data_ptr())
 
 
+LOG_PROBS_TOP = 32
+
+
+@dataclass(frozen=True)
+class LogProbs:
+    """What :func:`log_probs_rows` says per row: the given token's log probability and its rank (None
+    without tokens), the distribution's entropy, the likeliest tokens and their log probabilities."""
+
+    token: torch.Tensor | None  # (rows,) float32
+    rank: torch.Tensor | None  # (rows,) int64
+    entropy: torch.Tensor  # (rows,) float32
+    top_ids: torch.Tensor  # (rows, top) int64
+    top: torch.Tensor  # (rows, top) float32
+
+
+def log_probs_rows(logits: torch.Tensor, tokens: torch.Tensor | None = None, top: int = 0,
+                   temperatures: torch.Tensor | None = None) -> LogProbs:
+    """Per row of ``logits (rows, vocab)`` (bf16, fp16 or fp32), in one pass over it and with ``p =
+    softmax(logits / temperature)``: ``log p(tokens[row])`` and the token's rank (1 + the number of
+    larger logits), the entropy ``-sum p log p`` in nats, and the ``top`` (at most 32) likeliest tokens
+    with their log probabilities, in falling order, the lower index first among equals, a NaN before
+    any number. ``temperatures (rows,)`` must be positive (None: 1). A token outside the
+    vocabulary (padding) has NaN and rank 0; a row with a NaN or an infinite logit, or of -inf alone,
+    has NaN for every probability. No gradient."""
+    _check_cuda(logits, tokens, temperatures)
+    _no_gradient("log_probs_rows", logits, temperatures)
+    logits = _logits(logits)
+    rows, vocab = logits.shape
+    if not 0 <= top <= LOG_PROBS_TOP or top > max(vocab, 1):
+        raise ValueError(f"top must be 0 to {LOG_PROBS_TOP} and at most the vocabulary, got {top} of {vocab}")
+    if tokens is not None and (tokens.shape != (rows,) or tokens.dtype not in (torch.int32, torch.int64)):
+        raise ValueError(f"tokens must be int64 or int32 ({rows},), got {tokens.dtype} {tuple(tokens.shape)}")
+    if temperatures is not None and (temperatures.shape != (rows,) or not temperatures.is_floating_point()):
+        raise ValueError(f"temperatures must be floating point ({rows},), got {tuple(temperatures.shape)}")
+    device = logits.device
+    floats = torch.empty(rows * (2 + top), dtype=torch.float32, device=device)
+    ints = torch.empty(rows * (1 + top), dtype=torch.int64, device=device)
+    out = LogProbs(None if tokens is None else floats[:rows], None if tokens is None else ints[:rows],
+                   floats[rows:2 * rows], ints[rows:].view(rows, top), floats[2 * rows:].view(rows, top))
+    if rows == 0:
+        return out
+    if vocab == 0:
+        raise ValueError("an empty vocabulary has no probabilities")
+    stride = logits.stride(0) if rows > 1 else vocab
+    if stride < vocab:
+        logits, stride = logits.contiguous(), vocab
+    tokens = None if tokens is None else _i64(tokens)
+    temperatures = None if temperatures is None else _f32(temperatures)
+    nbytes = int(_native.lib().fm_log_probs_workspace_bytes(rows, vocab, top))
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+    _mx_call("fm_log_probs_rows", logits.get_device(), logits.data_ptr(), _LOGIT_DTYPES[logits.dtype], rows, vocab,
+             stride, _ptr(tokens), _ptr(temperatures), top, _ptr(out.token), _ptr(out.rank), out.entropy.data_ptr(),
+             out.top_ids.data_ptr(), out.top.data_ptr(), ws.data_ptr(), nbytes)
+    return out
+
+
 def seeded_normal(
     seeds: torch.Tensor, rows: torch.Tensor, positions: torch.Tensor, n_cols: int, scale: float = 1.0
 ) -> torch.Tensor:
@@ -1348,6 +1410,14 @@ class MX:
         if math.prod(lead) != self.rows:
             raise ValueError(f"{self.rows} rows cannot be viewed as {lead}")
         return MX(self.codes, self.scales, self.bits, (*lead, self.cols))
+
+    def __getitem__(self, index: int) -> "MX":
+        """The part of one index of the leading dimension (a layer of a cache of several)."""
+        if len(self.shape) < 3 or not -self.shape[0] <= index < self.shape[0]:
+            raise IndexError(f"no part {index} of microscaled rows of shape {self.shape}")
+        rows = self.rows // self.shape[0]
+        at = slice(index % self.shape[0] * rows, (index % self.shape[0] + 1) * rows)
+        return MX(self.codes[at], self.scales[at], self.bits, tuple(self.shape[1:]))
 
     def to(self, *args, **kwargs) -> "MX":
         """On another device (``Tensor.to`` of the codes and the scales)."""
@@ -1695,6 +1765,188 @@ def _mx_vec(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
     if t.dtype is not torch.bfloat16 or t.numel() != n:
         raise ValueError(f"{name} must hold {n} bfloat16 values, got {t.dtype} {tuple(t.shape)}")
     return t if t.is_contiguous() else t.contiguous()
+
+
+# ------------------------------------------------------------- a context in microscaled 4 bits
+
+
+def mx_cache(num_blocks: int, kv_heads: int, page: int, head_dim: int, device: torch.device | str = "cuda",
+             layers: int | None = None) -> MX:
+    """An empty context cache in microscaled 4 bits, :class:`MX` rows of ``shape ([layers,] num_blocks,
+    kv_heads, page, 2 head_dim)``: a position's keys, then its values, for one head, as a bf16
+    cache lays them out, in 17/64 of its bytes. ``page`` 1 makes it a pool of positions.
+    :func:`write_context_kv_mx` fills it, :func:`block_attention_paged_mx` reads it,
+    :func:`mx_quantize` (``bits`` 4) makes one of a bf16 cache's rows and :func:`mx_dequantize` the
+    values again (of up to 2^26 rows)."""
+    if head_dim not in (64, 128):
+        raise ValueError(f"head_dim must be 64 or 128, got {head_dim}")
+    lead = (num_blocks, kv_heads, page) if layers is None else (layers, num_blocks, kv_heads, page)
+    if min(lead) < 1:
+        raise ValueError(f"a cache of {lead} rows")
+    rows = math.prod(lead)
+    return MX(torch.zeros(rows, head_dim, dtype=torch.uint8, device=device),
+              torch.zeros(rows, head_dim // 16, dtype=torch.uint8, device=device), 4, (*lead, 2 * head_dim))
+
+
+def _mx_cache_args(cache: MX, dims: int, name: str) -> tuple[int, int, int, int]:
+    """(codes, stride, scales, stride) of a cache of ``dims`` dimensions, which is used in place."""
+    codes, scales, shape = cache.codes, cache.scales, cache.shape
+    if cache.bits != 4 or codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8:
+        raise TypeError(f"{name} must be in microscaled 4 bits (uint8 codes and scales)")
+    if len(shape) != dims or shape[-1] not in (128, 256) or min(shape) < 1:
+        raise ValueError(f"{name} must be ({'layers, ' if dims == 5 else ''}blocks, heads, page, 2 * head_dim) with "
+                         f"head_dim 64 or 128; got {tuple(shape)}")
+    d, rows = shape[-1] // 2, math.prod(shape[:-1])
+    if codes.shape != (rows, d) or scales.shape != (rows, d // 16):
+        raise ValueError(f"{name} of shape {tuple(shape)} holds codes ({rows}, {d}) and scales ({rows}, {d // 16}); got "
+                         f"{tuple(codes.shape)} and {tuple(scales.shape)}")
+    cs, ss = codes.stride(0) if rows > 1 else d, scales.stride(0) if rows > 1 else d // 16
+    if (codes.stride(1) != 1 or scales.stride(1) != 1 or cs < d or ss < d // 16 or cs % 16 or ss % 4
+            or codes.data_ptr() % 16 or scales.data_ptr() % 4):
+        raise ValueError(f"{name}: rows of codes must be 16-byte aligned, of scales 4-byte aligned, and not overlap")
+    return codes.data_ptr(), cs, scales.data_ptr(), ss
+
+
+def write_context_kv_mx(
+    kv: torch.Tensor,
+    positions: torch.Tensor,
+    slots: torch.Tensor,
+    k_norm: torch.Tensor,
+    rope: Rope,
+    caches: MX | Sequence[MX],
+    eps: float,
+) -> None:
+    """k-norm + RoPE + store of ``kv (tokens, layers, 2, heads, D)`` bf16 into caches in microscaled
+    4 bits (:func:`mx_cache`) at ``slots`` (page ``slots[t] // page``, place ``slots[t] % page``; a slot
+    outside the cache, such as a negative one, is skipped, and kept slots must differ): ``caches``
+    one of ``shape (layers, blocks, heads, page, 2D)`` or a ``(blocks, heads, page, 2D)`` per layer, all
+    laid out alike. Keys are normed and rotated in float32, ``(k / sqrt(mean(k^2) + eps)) * k_norm``,
+    and rounded once, to their code. See fm_write_context_kv_mx."""
+    if kv.dim() != 5 or kv.shape[2] != 2:
+        raise ValueError(f"kv must be (tokens, layers, 2, heads, head_dim), got {tuple(kv.shape)}")
+    if kv.dtype is not torch.bfloat16:
+        raise TypeError(f"kv must be bfloat16, got {kv.dtype}")
+    tokens, layers, _, heads, d = kv.shape
+    joined = isinstance(caches, MX)
+    held = [caches] if joined else list(caches)
+    if not held or (caches.shape[0] if joined else len(held)) != layers:
+        raise ValueError(f"kv holds {layers} layers, the caches {caches.shape[0] if joined else len(held)}")
+    index = _mx_device(kv, positions, slots, k_norm, rope.cos, *(t for c in held for t in (c.codes, c.scales)))
+    _no_gradient("write_context_kv_mx", kv, k_norm)
+    args = [_mx_cache_args(c, 5 if joined else 4, "a cache") for c in held]
+    blocks, cache_heads, page, two_d = held[0].shape[-4:]
+    _, cs, _, ss = args[0]
+    if any(c.shape != held[0].shape or a[1] != cs or a[3] != ss for c, a in zip(held, args)):
+        raise ValueError("the layers' caches must share one shape and strides")
+    if cache_heads != heads or two_d != 2 * d:
+        raise ValueError(f"kv of {heads} heads x {d} does not match a cache of {cache_heads} x {two_d // 2}")
+    rope.check(d)
+    if k_norm.numel() != layers * d:
+        raise ValueError(f"k_norm holds {k_norm.numel()} values, expected {layers} x {d}")
+    if positions.shape != (tokens,) or slots.shape != (tokens,):
+        raise ValueError(f"positions and slots must be ({tokens},), got {tuple(positions.shape)} and "
+                         f"{tuple(slots.shape)}")
+    if tokens == 0:
+        return
+    if joined:
+        rows = blocks * heads * page
+        at = [(args[0][0] + i * rows * cs, args[0][2] + i * rows * ss) for i in range(layers)]
+    else:
+        at = [(a[0], a[2]) for a in args]
+    kv, positions, slots, k_norm = kv.contiguous(), _i64(positions), _i64(slots), _f32(k_norm)
+    if kv.data_ptr() % 16:
+        kv = kv.clone()
+    pointers = ctypes.c_void_p * layers
+    _mx_call("fm_write_context_kv_mx", index, kv.data_ptr(), tokens, layers, heads, d, positions.data_ptr(),
+             slots.data_ptr(), k_norm.data_ptr(), *rope.args(), pointers(*(c for c, _ in at)),
+             pointers(*(s for _, s in at)), cs, ss, blocks, page, float(eps))
+
+
+@functools.lru_cache(maxsize=4096)
+def _attn_mx_workspace_bytes(q_len: int, hq: int, hkv: int, d: int, index: int) -> int:
+    with torch.cuda.device(index):
+        return int(_native.lib().fm_block_attn_paged_mx_workspace_bytes(q_len, hq, hkv, d))
+
+
+def block_attention_paged_mx(
+    query: torch.Tensor,
+    cache: MX,
+    cu_seqlens_q: torch.Tensor | None,
+    seqused_k: torch.Tensor,
+    block_table: torch.Tensor,
+    max_seqlen_q: int,
+    max_seqlen_k: int,
+    softmax_scale: float,
+    prologue: Prologue | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """:func:`block_attention_paged` onto a cache in microscaled 4 bits (:func:`mx_cache`,
+    ``(num_blocks, Hkv, page, 2D)``; pages of one position make ``block_table`` a table of positions):
+    ``query (tokens, Hq, D)`` bf16, each request reading its first ``seqused_k[b]`` positions (at most
+    ``max_seqlen_k``), zeros for a request of none. The cache's values enter exactly, the query with its
+    8 bits (a prologue's norm and rotation are float32 in front of that one rounding), scores and sums
+    are float32, probabilities are rounded to bf16. ``out`` (bf16, may be ``query``) receives the
+    result; its rows behind the last request are left alone. The context is cut over the chip by
+    lengths read on the device: a row's result may differ in its last place between calls of other
+    batches."""
+    index = _mx_device(query, cache.codes, cache.scales, cu_seqlens_q, seqused_k, block_table, out)
+    _no_gradient("block_attention_paged_mx", query)
+    if query.dim() != 3:
+        raise ValueError(f"query must be (tokens, heads, head_dim), got {tuple(query.shape)}")
+    tokens, hq, d = query.shape
+    codes, cs, scales, ss = _mx_cache_args(cache, 4, "cache")
+    blocks, hkv, page, two_d = cache.shape
+    if two_d != 2 * d:
+        raise ValueError(f"cache rows hold {two_d} values, expected 2 * {d}")
+    if hq < 1 or hq % hkv:
+        raise ValueError(f"{hq} query heads do not divide into {hkv} KV heads")
+    if blocks * hkv * page >= 1 << 32:
+        raise ValueError(f"a cache of at most 2^32 - 1 rows, got {blocks * hkv * page}")
+    if max_seqlen_q < 0 or max_seqlen_k < 0 or not 0 <= softmax_scale < math.inf:
+        raise ValueError("max_seqlen_q, max_seqlen_k and softmax_scale must be finite and not negative")
+    if seqused_k.dim() != 1:
+        raise ValueError(f"seqused_k must be (requests,), got {tuple(seqused_k.shape)}")
+    batch = seqused_k.shape[0]
+    _check_requests(batch, cu_seqlens_q, tokens, max_seqlen_q, block_table, "block_table", None)
+    if prologue is not None:
+        _mx_device(query, prologue.weight, prologue.rope.cos, prologue.positions)
+        _no_gradient("block_attention_paged_mx", prologue.weight)
+    query = _bf16_rows(query, "query")
+    if out is None:
+        out = torch.empty((tokens, hq, d), dtype=torch.bfloat16, device=query.device)
+    else:
+        if out.dtype is not torch.bfloat16 or out.shape != query.shape:
+            raise ValueError(f"out must be bfloat16 {tuple(query.shape)}, got {out.dtype} {tuple(out.shape)}")
+        if (out.stride(2) != 1 or out.data_ptr() % 16 or out.stride(0) % 8 or out.stride(1) % 8 or out.stride(1) < d
+                or (tokens > 1 and out.stride(0) < (hq - 1) * out.stride(1) + d)):
+            raise ValueError("out must hold 16-byte aligned heads of unit channel stride that do not overlap")
+        same = out.data_ptr() == query.data_ptr() and out.stride() == query.stride()
+        if not same and tokens and _meet(out, query):
+            raise ValueError("out overlaps the query (it may be the query itself)")
+        if tokens and (_meet(out, cache.codes) or _meet(out, cache.scales)):
+            raise ValueError("out overlaps the cache")
+    if batch == 0 or tokens == 0 or max_seqlen_q == 0:
+        return out
+    pro = _prologue_args(prologue, tokens, d)
+    cu = None if cu_seqlens_q is None else _i32(cu_seqlens_q)
+    table = block_table if (block_table.dtype == torch.int32 and block_table.stride(-1) == 1) else _i32(block_table)
+    lens = _i32(seqused_k)
+    nbytes = _attn_mx_workspace_bytes(max_seqlen_q, hq, hkv, d, index)
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=query.device)
+    _mx_call("fm_block_attn_paged_mx", index, query.data_ptr(), tokens, query.stride(0), query.stride(1),
+             out.data_ptr(), out.stride(0), out.stride(1), _ptr(cu), codes, cs, scales, ss, blocks, page,
+             table.data_ptr(), table.stride(0), table.shape[1], lens.data_ptr(), batch, max_seqlen_q, max_seqlen_k, hq,
+             hkv, d, float(softmax_scale), *pro, ws.data_ptr(), nbytes)
+    return out
+
+
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors (not empty) meet."""
+    def span(t):
+        first = t.data_ptr()
+        return first, first + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
 
 
 def noise_rows(z: torch.Tensor, eigvals: torch.Tensor, eps: float, gain: float,

@@ -534,6 +534,69 @@ int fm_adaln_residual_mx(const void *x, int64_t x_stride, const void *y, int64_t
                          void *scales, int64_t scales_stride, int64_t rows, int32_t cols, void *stream);
 
 /* ---------------------------------------------------------------------------------
+ * A context cache in microscaled 4 bits, and attention over it. No reference counterpart (its
+ * caches are bf16 or e4m3; the layout follows vLLM's, flashmap/vllm/model.py:707-733): a cache
+ * is 4-bit microscaled rows (blocks, heads, page_size, 2 head_dim), a position's keys and then
+ * its values for one head: row (block * heads + head) * page_size + position holds head_dim
+ * code bytes and 2 head_dim / 32 scale bytes. Strides of rows are in bytes, codes 16-byte aligned
+ * with strides of multiples of 16, scales 4-byte aligned with strides of multiples of 4. Pages
+ * of one position make it a pool of positions. head_dim in {64, 128}.
+ */
+/* The keys (k-norm, RoPE at positions[t], as fm_write_context_kv but in fp32 from one end to the
+ * other: (k / sqrt(mean(k^2) + eps)) * w, rotated, rounded once, to 4 bits) and values of kv
+ * (tokens, layers, 2, heads, head_dim) bf16 (contiguous, 16-byte aligned) into row slots[t] %
+ * page_size of block slots[t] / page_size of every layer's cache. A slot outside the cache (negative:
+ * padding) is skipped; slots of one call that are kept must differ. codes, scales: HOST arrays of
+ * `layers` device addresses, read during the call. */
+int fm_write_context_kv_mx(const void *kv, int64_t tokens, int32_t layers, int32_t heads, int32_t head_dim,
+                           const int64_t *positions, const int64_t *slots, const float *k_norm_weight,
+                           const float *rope_cos, const float *rope_sin, int64_t rope_row_stride,
+                           int64_t rope_pair_stride, int64_t rope_rows, void *const *codes, void *const *scales,
+                           int64_t row_stride, int64_t scales_stride, int64_t num_blocks, int32_t page_size,
+                           float eps, void *stream);
+/* fm_block_attn_paged over such a cache: q, out (q_tokens, num_q_heads, head_dim) bf16, token t of
+ * sequence b at row cu_seqlens_q[b] + t (b * max_seqlen_q + t without cu_seqlens_q; rows that no
+ * sequence has, and what cu_seqlens_q says past q_tokens, are left alone), each
+ * sequence's positions below min(seqused_k[b], max_seqlen_k, block_table_width * page_size)
+ * through its row of block_table; a page outside the cache is read as page 0. Sequences of
+ * length 0 get zeros. The query's norm and rotation are applied on the way when q_norm_weight
+ * is given, in fp32 as the writer's, and the query enters with 8 significant bits. softmax_scale >= 0; num_blocks * num_kv_heads *
+ * page_size < 2^32. The workspace (16-byte aligned) holds
+ * fm_block_attn_paged_mx_workspace_bytes(...) bytes for the current device; calls that may overlap in time
+ * must not share it. */
+size_t fm_block_attn_paged_mx_workspace_bytes(int32_t max_seqlen_q, int32_t num_q_heads, int32_t num_kv_heads,
+                                              int32_t head_dim);
+int fm_block_attn_paged_mx(const void *q, int64_t q_tokens, int64_t q_stride_token, int64_t q_stride_head,
+                           void *out, int64_t out_stride_token, int64_t out_stride_head, const int32_t *cu_seqlens_q,
+                           const void *codes, int64_t row_stride, const void *scales, int64_t scales_stride,
+                           int64_t num_blocks, int32_t page_size, const int32_t *block_table,
+                           int64_t block_table_stride, int64_t block_table_width, const int32_t *seqused_k,
+                           int32_t batch, int32_t max_seqlen_q, int32_t max_seqlen_k, int32_t num_q_heads,
+                           int32_t num_kv_heads, int32_t head_dim, float softmax_scale,
+                           const float *q_norm_weight, const float *rope_cos, const float *rope_sin,
+                           int64_t rope_row_stride, int64_t rope_pair_stride, int64_t rope_rows,
+                           const int64_t *q_positions, float eps, void *workspace, size_t workspace_bytes,
+                           void *stream);
+
+/* ---------------------------------------------------------------------------------
+ * Per row of logits (rows, vocab) of dtype 0 bf16, 1 fp16, 2 fp32, in one pass: with p =
+ * softmax(logits / temperature) (temperatures fp32 (rows,), positive; NULL: 1)
+ *   token[r] = log p(tokens[r]), rank[r] = 1 + the number of larger logits (tokens int64, NULL:
+ *   neither is written; a token outside the vocabulary: NaN and rank 0),
+ *   entropy[r] = -sum p log p,
+ *   top_ids, top_log_probs (rows, top): the `top` largest logits in falling order, the lower
+ *   index first among equals, a NaN before any number (top at most 32 and the vocabulary).
+ * A row with a NaN or +infinity, or of -infinity alone, has NaN for every probability. No
+ * reference counterpart (its servers take log probabilities from the engine). Workspace (16-byte
+ * aligned): fm_log_probs_workspace_bytes(rows, vocab, top) bytes.
+ */
+size_t fm_log_probs_workspace_bytes(int64_t rows, int64_t vocab, int32_t top);
+int fm_log_probs_rows(const void *logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                      const int64_t *tokens, const float *temperatures, int32_t top, float *token, int64_t *rank,
+                      float *entropy, int64_t *top_ids, float *top_log_probs, void *workspace,
+                      size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------------
  * Measurement hook. No reference counterpart: it lets a benchmark time the main
  * split-KV attention kernel alone with HIP events on the stream it runs on, without
  * changing the work any call does. While enabled, every attention call records an
