@@ -76,19 +76,16 @@ struct MxGeo {
   static constexpr int DMAS = CODES / 1024;               // 16-byte loads a lane of a tile's codes
   static constexpr int LOADS = DMAS + 2;                  // and its scales, and later page ids
   static constexpr int SLOT = CODES + SCALES + 4 * MXA_TILE;
-  static constexpr int NS = RB <= 2 ? 3 : 5;              // tiles in a wavefront's ring
+  static constexpr int NS = 3;                            // tiles in a wavefront's ring
   static constexpr int RING = MXA_WAVES * NS * SLOT;
-  static constexpr int HALVES = RB <= 2 ? 2 : 1;          // parts that a row block is joined in
-  static constexpr int MERGE = MXA_WAVES * 16 * D * 4 / HALVES;
-  static constexpr int QROW = 2 * D + 16;                 // a query row on its way to operands
   static constexpr int QN = D == 128 ? 4 : 2;             // 16-byte operands a lane of a row block's queries
   static constexpr int QOP = QN * 1024 + 128;             // and the bytes of their two scales
-  static constexpr int QBYTES = RB * QOP;
-  static constexpr int STAGE = RB * 16 * QROW;            // shares its place with MERGE
-  static constexpr int SHARED = MERGE > STAGE ? MERGE : STAGE;
+  static constexpr int MERGE = MXA_WAVES * 4 * 1024;      // four fragments of every wavefront
+  static constexpr int SHARED = RB * QOP > MERGE ? RB * QOP : MERGE;  // one after the other
   static constexpr int ML = MXA_WAVES * RB * 16 * 8;
   static constexpr int PRE = (MXA_BATCH + 4) * 4 + MXA_BATCH * 4;
-  static constexpr int SMEM = RING + QBYTES + SHARED + ML + PRE;
+  static constexpr int SMEM = RING + SHARED + ML + PRE;
+  static_assert(SMEM <= 80 * 1024, "two workgroups a CU");
 };
 
 // ------------------------------------------------------------------------------ pieces
@@ -255,28 +252,17 @@ __device__ __forceinline__ void wait_tiles(int32_t behind) {
     wait_tiles<LOADS, MOST - 1>(behind);
 }
 
-template <int N>
-__device__ __forceinline__ void store_bf16(uint16_t *dst, const float (&v)[N]) {  // 2, 4 or 8 of them, aligned
-  if constexpr (N == 8)
-    store16(dst, u32x4_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])});
-  else if constexpr (N == 4)
-    *reinterpret_cast<u32x2_t *>(dst) = u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-  else
-    *reinterpret_cast<uint32_t *>(dst) = pack_bf16x2(v[0], v[1]);
-}
-
 // --------------------------------------------------------------------------- the kernel
 
 template <int D, int RB>
-__global__ __launch_bounds__(64 * MXA_WAVES, RB <= 2 ? 2 : 1) void attn_mx_kernel(const MxAttnArgs a) {
+__global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttnArgs a) {
   using G = MxGeo<D, RB>;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int n = lane & 15, g = lane >> 4;
   char *const ring = lds + wave * G::NS * G::SLOT;
   const uint32_t ring_at = (uint32_t)(uintptr_t)(lds_char_t *)ring;
-  char *const qop = lds + G::RING;
-  char *const shared = qop + G::QBYTES;
+  char *const shared = lds + G::RING, *const qop = shared;
   float *const ml = reinterpret_cast<float *>(shared + G::SHARED);
   int32_t *const pre = reinterpret_cast<int32_t *>(shared + G::SHARED + G::ML);
   int32_t *const len = pre + MXA_BATCH + 4;
@@ -391,7 +377,8 @@ __global__ __launch_bounds__(64 * MXA_WAVES, RB <= 2 ? 2 : 1) void attn_mx_kerne
 #pragma unroll
           for (int i = 0; i < 4; ++i) y[t][2 * i] = bf16_lo(x[t][i]), y[t][2 * i + 1] = bf16_hi(x[t][i]);
       }
-      char *const stage = shared + wave * 16 * G::QROW + n * G::QROW;  // a row: hi, lo
+      // A row's hi and lo codes, 2 D bytes, then all rows in the operands' order in their place.
+      char *const to = qop + wave * G::QOP, *const stage = to + n * 2 * D;
       uint32_t mine = 0;  // the byte of block g
 #pragma unroll
       for (int t = 0; t < D / 32; ++t) {
@@ -405,23 +392,23 @@ __global__ __launch_bounds__(64 * MXA_WAVES, RB <= 2 ? 2 : 1) void attn_mx_kerne
       wave_fence();
       // The operand of lane group g: channels 16 g to 16 g + 15 and, in its second half, 64 on; its
       // scale byte that of channels 32 g on. D 64: hi in the first half, lo in the second.
-      char *const to = qop + wave * G::QOP;
+      u32x4_t op[G::QN];
 #pragma unroll
-      for (int i = 0; i < G::QN; ++i) store16(to + 1024 * i + 16 * lane, load16(stage + 64 * i + 16 * g));
+      for (int i = 0; i < G::QN; ++i) op[i] = load16(stage + 64 * i + 16 * g);
+      wave_fence();
+#pragma unroll
+      for (int i = 0; i < G::QN; ++i) store16(to + 1024 * i + 16 * lane, op[i]);
       const uint32_t low = lo_byte(mine);
       *reinterpret_cast<uint16_t *>(to + G::QN * 1024 + 2 * lane) =
           (uint16_t)(D == 128 ? mine | low << 8 : g < 2 ? mine : low);
     }
     lds_barrier();
     u32x4_t qr[RB <= 2 ? RB : 1][G::QN];
-    int qs[RB];
+    if constexpr (RB <= 2) {
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      qs[rb] = *reinterpret_cast<const uint16_t *>(qop + rb * G::QOP + G::QN * 1024 + 2 * lane);
-      if constexpr (RB <= 2) {
+      for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
         for (int i = 0; i < G::QN; ++i) qr[rb][i] = load16(qop + rb * G::QOP + 1024 * i + 16 * lane);
-      }
     }
 
     f32x4_t o[RB][G::NF];
@@ -446,6 +433,72 @@ __global__ __launch_bounds__(64 * MXA_WAVES, RB <= 2 ? 2 : 1) void attn_mx_kerne
           kf[tb] = load16(slot + place<D>(r, c));
           ks[tb] = *reinterpret_cast<const uint8_t *>(slot + G::CODES + r * (D / 16) + c);
         }
+        u32x4_t p[RB];
+        auto scores = [&](auto from) {  // of two row blocks (or the last one)
+          constexpr int R0 = decltype(from)::value, R1 = R0 + 2 < RB ? R0 + 2 : RB, R = R1 - R0;
+          f32x4_t s[R][2];
+#pragma unroll
+          for (int i = 0; i < R; ++i) {
+            u32x4_t q[G::QN];
+#pragma unroll
+            for (int x = 0; x < G::QN; ++x) {
+              if constexpr (RB <= 2)
+                q[x] = qr[R0 + i][x];
+              else
+                q[x] = load16(qop + (R0 + i) * G::QOP + 1024 * x + 16 * lane);
+            }
+            const int qs = *reinterpret_cast<const uint16_t *>(qop + (R0 + i) * G::QOP + G::QN * 1024 + 2 * lane);
+#pragma unroll
+            for (int tb = 0; tb < 2; ++tb) {
+              s[i][tb] = mfma_k_q(kf[tb], q[0], q[1], f32x4_t{0.f, 0.f, 0.f, 0.f}, ks[tb], qs);
+              if constexpr (D == 128) s[i][tb] = mfma_k_q(kf[tb], q[2], q[3], s[i][tb], ks[tb], qs >> 8);
+            }
+          }
+          if (live < MXA_TILE) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int r = 16 * (j >> 2) + (g & 1) + 8 * (g >> 1) + 2 * (j & 3);
+#pragma unroll
+              for (int i = 0; i < R; ++i)
+                if (r >= live) s[i][j >> 2][j & 3] = -INFINITY;
+            }
+          }
+          float top[R];
+          bool passed = false;
+#pragma unroll
+          for (int i = 0; i < R; ++i) {
+            top[i] = s[i][0][0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) top[i] = fmaxf(top[i], s[i][j >> 2][j & 3]);
+            top[i] *= a.scale_log2;
+            passed |= top[i] > ref[R0 + i] + MXA_SLACK;
+          }
+          if (__ballot(passed) != 0) {
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+              const float m = fmaxf(fmaxf(ref[R0 + i], max_over_groups(top[i])), -3.0e38f);
+              const float f = __builtin_amdgcn_exp2f(ref[R0 + i] - m);
+              ref[R0 + i] = m;
+              sum[R0 + i] *= f;
+#pragma unroll
+              for (int c = 0; c < G::NF; ++c) o[R0 + i][c] *= f;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < R; ++i) {
+            float e[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j >> 2][j & 3], a.scale_log2, -ref[R0 + i]));
+              sum[R0 + i] += e[j];
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) p[R0 + i][c] = pack_bf16x2(e[2 * c], e[2 * c + 1]);
+          }
+        };
+        scores(std::integral_constant<int, 0>{});
+        if constexpr (RB > 2) scores(std::integral_constant<int, 2>{});
+        asm volatile("" : : : "memory");  // the values are read behind the scores: registers
         typedef typename std::conditional<D == 128, uint32_t, uint16_t>::type vword_t;
         uint32_t vw[8];
         float vs[8];
@@ -455,65 +508,6 @@ __global__ __launch_bounds__(64 * MXA_WAVES, RB <= 2 ? 2 : 1) void attn_mx_kerne
           const int c = D == 128 ? n >> 2 : n >> 3, in = D == 128 ? 4 * (n & 3) : 2 * (n & 7);
           vw[j] = *reinterpret_cast<const vword_t *>(slot + place<D>(r, D / 32 + c) + in);
           vs[j] = mx_scale_float(*reinterpret_cast<const uint8_t *>(slot + G::CODES + r * (D / 16) + D / 32 + c));
-        }
-        f32x4_t s[RB][2];
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          u32x4_t q[G::QN];
-#pragma unroll
-          for (int x = 0; x < G::QN; ++x) {
-            if constexpr (RB <= 2)
-              q[x] = qr[rb][x];
-            else
-              q[x] = load16(qop + rb * G::QOP + 1024 * x + 16 * lane);
-          }
-#pragma unroll
-          for (int tb = 0; tb < 2; ++tb) {
-            s[rb][tb] = mfma_k_q(kf[tb], q[0], q[1], f32x4_t{0.f, 0.f, 0.f, 0.f}, ks[tb], qs[rb]);
-            if constexpr (D == 128) s[rb][tb] = mfma_k_q(kf[tb], q[2], q[3], s[rb][tb], ks[tb], qs[rb] >> 8);
-          }
-        }
-        if (live < MXA_TILE) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int r = 16 * (j >> 2) + (g & 1) + 8 * (g >> 1) + 2 * (j & 3);
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb)
-              if (r >= live) s[rb][j >> 2][j & 3] = -INFINITY;
-          }
-        }
-        float top[RB];
-        bool passed = false;
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          top[rb] = s[rb][0][0];
-#pragma unroll
-          for (int j = 1; j < 8; ++j) top[rb] = fmaxf(top[rb], s[rb][j >> 2][j & 3]);
-          top[rb] *= a.scale_log2;
-          passed |= top[rb] > ref[rb] + MXA_SLACK;
-        }
-        if (__ballot(passed) != 0) {
-#pragma unroll
-          for (int rb = 0; rb < RB; ++rb) {
-            const float m = fmaxf(fmaxf(ref[rb], max_over_groups(top[rb])), -3.0e38f);
-            const float f = __builtin_amdgcn_exp2f(ref[rb] - m);
-            ref[rb] = m;
-            sum[rb] *= f;
-#pragma unroll
-            for (int q = 0; q < G::NF; ++q) o[rb][q] *= f;
-          }
-        }
-        u32x4_t p[RB];
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          float e[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][j >> 2][j & 3], a.scale_log2, -ref[rb]));
-            sum[rb] += e[j];
-          }
-#pragma unroll
-          for (int q = 0; q < 4; ++q) p[rb][q] = pack_bf16x2(e[2 * q], e[2 * q + 1]);
         }
         auto channels = [&](auto sel) {  // two of this lane's channels
           constexpr int B = decltype(sel)::value;
@@ -538,8 +532,7 @@ __global__ __launch_bounds__(64 * MXA_WAVES, RB <= 2 ? 2 : 1) void attn_mx_kerne
       if (k + G::NS < count) load_tile();
     }
 
-    // The four wavefronts' parts of the unit together, a row block (or half its channels) at a time.
-    float scale[RB];
+    // The four wavefronts' parts of the unit together, four fragments of each at a time.
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       sum[rb] = sum_over_groups(sum[rb]);
@@ -557,54 +550,48 @@ __global__ __launch_bounds__(64 * MXA_WAVES, RB <= 2 ? 2 : 1) void attn_mx_kerne
 #pragma unroll
       for (int w = 0; w < MXA_WAVES; ++w) l += v[w].y * __builtin_amdgcn_exp2f(v[w].x - m);
     };
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      float m, l;
-      joined(rb * 16 + n, m, l);
-      scale[rb] = __builtin_amdgcn_exp2f(ref[rb] - m);
-    }
     const int64_t part = 2 * share + (k == seg ? 0 : 1);
-    constexpr int FH = G::NF / G::HALVES;  // channels of a thread
-    const int row = threadIdx.x >> 4, dim = threadIdx.x & 15;
+    constexpr int FW = G::NF / 4;  // fragments of a row block that a wavefront joins
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      const int32_t r = row0 + 16 * rb + row, head = r / a.q_len, tok = r - head * a.q_len;
+      const int32_t r = row0 + 16 * rb + n, head = r / a.q_len, tok = r - head * a.q_len;
       const bool live = r < rows && tok < tokens;
       float m, l;
-      joined(rb * 16 + row, m, l);
+      joined(rb * 16 + n, m, l);
+      const float scale = __builtin_amdgcn_exp2f(ref[rb] - m);
+      f32x4_t v[FW];
 #pragma unroll
-      for (int half = 0; half < G::HALVES; ++half) {
-        if (rb + half > 0) lds_barrier();  // the last part has been read
+      for (int h = 0; h < FW; ++h) {
+        lds_barrier();  // the last four fragments (the queries, at first) have been read
 #pragma unroll
-        for (int f = 0; f < FH; ++f)
-          *reinterpret_cast<f32x4_t *>(shared + ((wave * FH + f) * 64 + lane) * 16) = o[rb][half * FH + f] * scale[rb];
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<f32x4_t *>(shared + ((q * MXA_WAVES + wave) * 64 + lane) * 16) = o[rb][q * FW + h] * scale;
         lds_barrier();
-        float v[FH];
+        v[h] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int f = 0; f < FH; ++f) {
-          v[f] = 0.f;
+        for (int w = 0; w < MXA_WAVES; ++w)
+          v[h] += *reinterpret_cast<const f32x4_t *>(shared + ((wave * MXA_WAVES + w) * 64 + lane) * 16);
+      }
+      // Channels (4 g + i) NF + wave FW + h of row n.
+      if (whole) {
+        if (live) {
+          const float inv = 1.f / l;
+          uint16_t *dst = a.o + (token0 + tok) * a.o_st + ((int64_t)cc.h * a.group + head) * a.o_sh + 4 * g * G::NF + wave * FW;
 #pragma unroll
-          for (int w = 0; w < MXA_WAVES; ++w)
-            v[f] += *reinterpret_cast<const float *>(shared + ((w * FH + f) * 64 + row + 16 * (dim >> 2)) * 16 + 4 * (dim & 3));
-        }
-        const int at = dim * G::NF + half * FH;
-        if (whole) {
-          if (live) {
-            const float inv = 1.f / l;
-            uint16_t *dst = a.o + (token0 + tok) * a.o_st + ((int64_t)cc.h * a.group + head) * a.o_sh + at;
-#pragma unroll
-            for (int f = 0; f < FH; ++f) v[f] *= inv;
-            store_bf16<FH>(dst, v);
-          }
-        } else {
-          float *dst = a.part_o + ((part * RB + rb) * 16 + row) * D + at;
-#pragma unroll
-          for (int f = 0; f < FH; ++f) dst[f] = v[f];
-          if (dim == 0 && half == 0) {
-            float *const to = a.part_ml + 2 * ((part * RB + rb) * 16 + row);
-            to[0] = m, to[1] = l;
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t d = pack_bf16x2(v[0][i] * inv, v[FW - 1][i] * inv);
+            if constexpr (FW == 2)
+              *reinterpret_cast<uint32_t *>(dst + i * G::NF) = d;
+            else
+              dst[i * G::NF] = (uint16_t)d;
           }
         }
+      } else {
+        const int64_t at = part * RB + rb;
+#pragma unroll
+        for (int h = 0; h < FW; ++h)
+          *reinterpret_cast<f32x4_t *>(a.part_o + ((at * G::NF + wave * FW + h) * 64 + lane) * 4) = v[h];
+        if (wave == 0 && g == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * (at * 16 + n)) = make_float2(m, l);
       }
     }
     cc.lt += seg - 1;
@@ -613,12 +600,13 @@ __global__ __launch_bounds__(64 * MXA_WAVES, RB <= 2 ? 2 : 1) void attn_mx_kerne
 }
 
 // The units that shares cut, from their parts, and zeros for the sequences without context. A
-// workgroup a 16-row block of a unit, a thread D / 16 channels of a row.
+// workgroup a 16-row block of a unit, laid out as the parts are: a wavefront D / 64 fragments.
 template <int D>
-__global__ __launch_bounds__(256) void attn_mx_join_kernel(const MxAttnArgs a, int rb_unit) {
-  constexpr int C = D / 16;
+__global__ __launch_bounds__(64 * MXA_WAVES) void attn_mx_join_kernel(const MxAttnArgs a, int rb_unit) {
+  constexpr int NF = D / 16, FW = NF / 4;
   __shared__ int32_t sums[2][MXA_WAVES];
   const int lane = threadIdx.x & 63, wave = wave_id();
+  const int n = lane & 15, g = lane >> 4;
   const int64_t ups = (int64_t)a.hkv * a.rgroups;
   const int b = (int)(blockIdx.x / ups), u = (int)(blockIdx.x - b * ups), h = u / a.rgroups, rg = u - h * a.rgroups;
   const int rb = blockIdx.y;
@@ -635,37 +623,39 @@ __global__ __launch_bounds__(256) void attn_mx_join_kernel(const MxAttnArgs a, i
   const int64_t total = ups * all, shares = total < a.shares ? total : a.shares;
   const int32_t steps = steps_of(context_len(a, b));
   const int32_t tokens = tokens_of(a, b);
-  const int row = threadIdx.x >> 4, dim = threadIdx.x & 15;
-  const int32_t r = (rg * rb_unit + rb) * 16 + row, head = r / a.q_len, tok = r - head * a.q_len;
+  const int32_t r = (rg * rb_unit + rb) * 16 + n, head = r / a.q_len, tok = r - head * a.q_len;
   const bool live = r < a.group * a.q_len && tok < tokens;
-  uint16_t *const dst =
-      a.o + (first_token(a, b) + tok) * a.o_st + ((int64_t)h * a.group + head) * a.o_sh + dim * C;
-  float v[C];
+  f32x4_t v[FW];
 #pragma unroll
-  for (int c = 0; c < C; ++c) v[c] = 0.f;
-  if (steps == 0) {
-    if (live) store_bf16<C>(dst, v);
-    return;
+  for (int f = 0; f < FW; ++f) v[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float inv = 0.f;
+  if (steps > 0) {
+    const int64_t s = ups * before + (int64_t)u * steps, e = s + steps;
+    const int64_t w0 = ((s + 1) * shares - 1) / total, w1 = (e * shares - 1) / total;
+    if (w0 == w1) return;
+    float m = -INFINITY, l = 0.f;
+    for (int64_t w = w0; w <= w1; ++w) {
+      const int64_t at = (2 * w + (share_at(w, total, shares) < s ? 1 : 0)) * rb_unit + rb;
+      const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + 2 * (at * 16 + n));
+      const float top = fmaxf(m, ml.x), f0 = __builtin_amdgcn_exp2f(m - top), f1 = __builtin_amdgcn_exp2f(ml.x - top);
+      l = l * f0 + ml.y * f1;
+#pragma unroll
+      for (int f = 0; f < FW; ++f)
+        v[f] = v[f] * f0 + *reinterpret_cast<const f32x4_t *>(a.part_o + ((at * NF + wave * FW + f) * 64 + lane) * 4) * f1;
+      m = top;
+    }
+    inv = 1.f / l;
   }
-  const int64_t s = ups * before + (int64_t)u * steps, e = s + steps;
-  const int64_t w0 = ((s + 1) * shares - 1) / total, w1 = (e * shares - 1) / total;
-  if (w0 == w1 || !live) return;
-  float m = -INFINITY, l = 0.f;
-  for (int64_t w = w0; w <= w1; ++w) {
-    const int64_t part = 2 * w + (share_at(w, total, shares) < s ? 1 : 0);
-    const int64_t at = (part * rb_unit + rb) * 16 + row;
-    const float pm = a.part_ml[2 * at], pl = a.part_ml[2 * at + 1];
-    const float *po = a.part_o + at * D + dim * C;
-    const float top = fmaxf(m, pm), f0 = __builtin_amdgcn_exp2f(m - top), f1 = __builtin_amdgcn_exp2f(pm - top);
-    l = l * f0 + pl * f1;
+  if (!live) return;
+  uint16_t *dst = a.o + (first_token(a, b) + tok) * a.o_st + ((int64_t)h * a.group + head) * a.o_sh + 4 * g * NF + wave * FW;
 #pragma unroll
-    for (int c = 0; c < C; ++c) v[c] = v[c] * f0 + po[c] * f1;
-    m = top;
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t d = pack_bf16x2(v[0][i] * inv, v[FW - 1][i] * inv);
+    if constexpr (FW == 2)
+      *reinterpret_cast<uint32_t *>(dst + i * NF) = d;
+    else
+      dst[i * NF] = (uint16_t)d;
   }
-  const float inv = 1.f / l;
-#pragma unroll
-  for (int c = 0; c < C; ++c) v[c] *= inv;
-  store_bf16<C>(dst, v);
 }
 
 // Row blocks of a unit: up to 4, all units alike where the rows fill more than one.
@@ -678,7 +668,8 @@ static int unit_blocks(int32_t rows, int32_t *rgroups) {
 static int mx_attn_shares(int rb) {
   DeviceInfo info;
   const int cus = device_info(&info) == FM_OK ? info.cus : 256;
-  return rb <= 2 ? 2 * cus : cus;
+  (void)rb;
+  return 2 * cus;
 }
 
 static size_t mx_attn_part_floats(int rb, int d) { return (size_t)2 * mx_attn_shares(rb) * 16 * rb * (d + 2); }
