@@ -38,6 +38,7 @@ constexpr int MXA_WAVES = 4;
 constexpr int MXA_TILE = 32;                     // positions of a wavefront's tile
 constexpr int MXA_STEP = MXA_WAVES * MXA_TILE;   // of a workgroup's step
 constexpr int MXA_BATCH = 256;                   // sequences of one launch: their steps lie in LDS
+constexpr int MXA_UNIT_COST = 6;                 // steps that a unit's start and end cost
 constexpr float MXA_SLACK = 8.f;                 // log2 that scores may pass their row's reference by
 
 struct MxAttnArgs {
@@ -48,10 +49,10 @@ struct MxAttnArgs {
   const int32_t *cu_q;  // NULL: sequence b's tokens start at token0 + b q_len
   int64_t token0, q_tokens;  // q_tokens: rows of q and out; what cu_q says past them is left alone
   int32_t q_len, group, hkv, rgroups;
+  uint32_t q_mul, q_shift;  // n / q_len, as n / page below
   const uint8_t *codes, *scales;
-  int64_t cs, ss;  // row strides, bytes
-  int64_t num_blocks;
-  int32_t page;
+  uint32_t cs16, ss4;  // row strides in 16 and in 4 bytes (the last row's offsets in them below 2^32)
+  uint32_t num_blocks, page, head_rows;  // head_rows: rows of a block, hkv page
   uint32_t page_mul, page_shift;  // n / page = mulhi(2 n, page_mul) >> page_shift for n < 2^31
   const int32_t *table;
   int64_t table_stride;
@@ -65,12 +66,11 @@ struct MxAttnArgs {
   float eps;
   float *part_o;   // (2 shares, 16 RB, D), relative to the row's reference
   float *part_ml;  // (2 shares, 16 RB, 2): the reference (log2) and the sum
-  int32_t shares;
+  int32_t log_shares;
 };
 
 template <int D, int RB>
 struct MxGeo {
-  static constexpr int KB = D / 2;                        // bytes of a row's keys, and of its values
   static constexpr int NF = D / 16;                       // 16-channel fragments
   static constexpr int CODES = MXA_TILE * D, SCALES = MXA_TILE * (D / 16);
   static constexpr int DMAS = CODES / 1024;               // 16-byte loads a lane of a tile's codes
@@ -83,8 +83,8 @@ struct MxGeo {
   static constexpr int MERGE = MXA_WAVES * 4 * 1024;      // four fragments of every wavefront
   static constexpr int SHARED = RB * QOP > MERGE ? RB * QOP : MERGE;  // one after the other
   static constexpr int ML = MXA_WAVES * RB * 16 * 8;
-  static constexpr int PRE = (MXA_BATCH + 4) * 4 + MXA_BATCH * 4;
-  static constexpr int SMEM = RING + SHARED + ML + PRE;
+  static constexpr int LINE = 4 * (MXA_BATCH + 4) * 4;    // the sequences (MxLine)
+  static constexpr int SMEM = RING + SHARED + ML + LINE + 4 * D;
   static_assert(SMEM <= 80 * 1024, "two workgroups a CU");
 };
 
@@ -118,62 +118,92 @@ __device__ __forceinline__ int32_t context_len(const MxAttnArgs &a, int b) {
   return n < 0 ? 0 : n < a.max_len ? n : a.max_len;
 }
 __device__ __forceinline__ int32_t steps_of(int32_t len) { return (len + MXA_STEP - 1) / MXA_STEP; }
-__device__ __forceinline__ int32_t tokens_of(const MxAttnArgs &a, int b) {  // query tokens of sequence b
-  if (a.cu_q == nullptr) return a.q_len;
-  const int64_t first = a.cu_q[b], end = a.cu_q[b + 1], n = (end < a.q_tokens ? end : a.q_tokens) - first;
+// Query tokens [first, stop) of the caller's rows: the first and how many the call takes.
+__device__ __forceinline__ int32_t tokens_in(const MxAttnArgs &a, int64_t first, int64_t stop) {
+  const int64_t n = (stop < a.q_tokens ? stop : a.q_tokens) - first;
   return n < 0 || first < 0 ? 0 : n < a.q_len ? (int32_t)n : a.q_len;
 }
-__device__ __forceinline__ int64_t first_token(const MxAttnArgs &a, int b) {
-  return a.cu_q == nullptr ? a.token0 + (int64_t)b * a.q_len : (int64_t)a.cu_q[b];
+__device__ __forceinline__ int32_t divided(int32_t n, uint32_t mul, uint32_t shift) {  // n < 2^31
+  return (int32_t)(__umulhi((uint32_t)n << 1, mul) >> shift);
 }
 
-// The line's share s: [s total / n, (s + 1) total / n).
-__device__ __forceinline__ int64_t share_at(int64_t s, int64_t total, int64_t n) { return s * total / n; }
+// floor(a / b) for 0 <= a < 2^50, b > 0 and a quotient below 2^24.
+__device__ __forceinline__ int32_t quotient(int64_t a, int64_t b) {
+  int32_t q = (int32_t)((float)a * __builtin_amdgcn_rcpf((float)b));
+  while ((int64_t)q * b > a) --q;
+  while ((int64_t)(q + 1) * b <= a) ++q;
+  return q;
+}
+
+// The line of all units' steps, cut into n shares by cost: a unit counts its steps and, in front of
+// them, c more for its start and end (0 where shares are a few steps). Of 64 requests of 256 to 8192
+// positions the shares that hold the short ones would otherwise take twice the others' time. With fewer
+// steps than shares each is one; else n is 2^log_shares, and share s starts at s total >> log_shares.
+struct MxPlan {
+  int64_t ups, total;
+  int32_t n, c, shift;
+  __device__ __forceinline__ MxPlan(const MxAttnArgs &a, int32_t steps, int32_t sequences) {
+    ups = (int64_t)a.hkv * a.rgroups;
+    const int64_t all = ups * steps;
+    const bool few = all < 1ll << a.log_shares;
+    n = few ? (int32_t)all : 1 << a.log_shares;
+    shift = few ? 0 : a.log_shares;
+    const int64_t fair = few ? 0 : all >> (a.log_shares + 2);
+    c = fair < MXA_UNIT_COST ? (int32_t)fair : MXA_UNIT_COST;
+    total = all + ups * c * sequences;
+  }
+  __device__ __forceinline__ int64_t share(int64_t s) const { return shift ? s * total >> shift : s; }
+  // The share that `at` lies in: the last that starts there or before.
+  __device__ __forceinline__ int32_t share_of(int64_t at) const {
+    return shift ? quotient(((at + 1) << shift) - 1, total) : (int32_t)at;
+  }
+};
 
 // A place on the line: step lt of unit (b, h, rg).
 struct MxCursor {
   int b, h, rg, lt, steps, len;
 };
 
-struct MxLine {  // in LDS: steps of the sequences before b, and their lengths
-  const int32_t *pre, *len;
+// In LDS, by sequence: the steps, and the sequences with steps, before it; its length; its first token.
+struct MxLine {
+  int32_t *pre, *some, *len, *cu;
   __device__ __forceinline__ void load(MxCursor &c) const {
-    c.steps = uniform(pre[c.b + 1] - pre[c.b]);
     c.len = uniform(len[c.b]);
+    c.steps = steps_of(c.len);
   }
 };
 
-__device__ __forceinline__ bool advance(const MxAttnArgs &a, const MxLine &line, MxCursor &c) {  // true: a new unit
-  if (++c.lt < c.steps) return false;
+__device__ __forceinline__ void advance(const MxAttnArgs &a, const MxLine &line, MxCursor &c) {
+  if (++c.lt < c.steps) return;
   c.lt = 0;
-  if (++c.rg < a.rgroups) return true;
+  if (++c.rg < a.rgroups) return;
   c.rg = 0;
-  if (++c.h < a.hkv) return true;
+  if (++c.h < a.hkv) return;
   c.h = 0;
   for (++c.b; c.b < a.batch; ++c.b) {  // sequences without context have no units
     line.load(c);
     if (c.steps > 0) break;
   }
-  return true;
 }
 
-// Where step t of the line lies, the sequences tested 64 at a time.
-__device__ __forceinline__ MxCursor cursor_at(const MxAttnArgs &a, const MxLine &line, int64_t t) {
-  const int64_t ups = (int64_t)a.hkv * a.rgroups;
+// The step at which `at` of the cost line lies, and its number; the sequences are tested 64 at a time.
+__device__ __forceinline__ int64_t locate(const MxAttnArgs &a, const MxPlan &plan, const MxLine &line, int64_t at,
+                                          MxCursor &c) {
   const int lane = threadIdx.x & 63;
   int before = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 64)
-    before += __popcll(__ballot(b0 + lane < a.batch && ups * line.pre[b0 + lane < a.batch ? b0 + lane : 0] <= t));
-  // The last sequence that starts at or before t; those without steps start where the next does.
-  MxCursor c;
-  c.b = uniform(before - 1);
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const int b = b0 + lane < a.batch ? b0 + lane : 0;
+    before += __popcll(__ballot(b0 + lane < a.batch && plan.ups * (line.pre[b] + (int64_t)plan.c * line.some[b]) <= at));
+  }
+  c.b = uniform(before - 1);  // the last that starts there or before: those without steps start where the next does
   line.load(c);
-  const int64_t off = t - ups * uniform(line.pre[c.b]);
-  const int unit = (int)(off / c.steps);
-  c.lt = (int)(off - (int64_t)unit * c.steps);
-  c.h = unit / a.rgroups;
+  const int32_t pre = uniform(line.pre[c.b]);
+  const int64_t off = at - plan.ups * (pre + (int64_t)plan.c * uniform(line.some[c.b]));
+  const int unit = uniform(quotient(off, c.steps + plan.c)), in = (int)(off - (int64_t)unit * (c.steps + plan.c)) - plan.c;
+  c.lt = in > 0 ? in : 0;
+  c.h = a.rgroups == 1 ? unit : unit / a.rgroups;
   c.rg = unit - c.h * a.rgroups;
-  return c;
+  return plan.ups * pre + (int64_t)unit * c.steps + c.lt;
 }
 
 // LDS place of the 16-byte piece c of tile row r: rows of 128 bytes (D 128) or 64. Operand
@@ -194,6 +224,30 @@ __device__ __forceinline__ f32x4_t mfma_k_q(u32x4_t k, u32x4_t q0, u32x4_t q1, f
 }
 
 __device__ __forceinline__ uint32_t lo_byte(uint32_t byte) { return byte == 255u ? 255u : byte - 5; }
+
+// norm_rope_exact where the result is rounded to 8 bits: sums and root in float32 as they come.
+template <int D>
+__device__ __forceinline__ void norm_rope_query(const u32x4_t (&x)[D / 32], const PrologueOps<D> &ops, float eps,
+                                                float (&y)[D / 32][8]) {
+  float ss = 0.f;
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      y[t][2 * q] = bf16_lo(x[t][q]), y[t][2 * q + 1] = bf16_hi(x[t][q]);
+      ss += y[t][2 * q] * y[t][2 * q] + y[t][2 * q + 1] * y[t][2 * q + 1];
+    }
+  ss = sum_over_groups(ss);
+  const float r = __builtin_amdgcn_rsqf(ss * (1.f / D) + eps);
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float e = y[t][2 * q] * r * ops.w[t][2 * q], o = y[t][2 * q + 1] * r * ops.w[t][2 * q + 1];
+      y[t][2 * q] = e * ops.c[t][q] - o * ops.s[t][q];
+      y[t][2 * q + 1] = o * ops.c[t][q] + e * ops.s[t][q];
+    }
+}
 
 // Eight of a block's 32 values in each of a row's four lanes, as two e4m3 operands and the scale byte
 // of the first.
@@ -235,8 +289,29 @@ __device__ __forceinline__ uint32_t widen(uint32_t w, float scale) {
 __device__ __forceinline__ uint32_t both_lo(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ __forceinline__ uint32_t both_hi(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
+// sum + both bf16 values of p (v_dot2_f32_bf16 with ones).
+__device__ __forceinline__ float add_both(uint32_t p, float sum) {
+  typedef __attribute__((ext_vector_type(2))) __bf16 b2_t;
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2_t, p), __builtin_bit_cast(b2_t, 0x3f803f80u), sum, false);
+}
+
 // The float of a scale byte, of which the widening takes the exponent (0: 2^-127; 255: NaN).
 __device__ __forceinline__ float mx_scale_float(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// The sum over the lanes up to this one.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int32_t shifted(int32_t v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int32_t wave_prefix(int32_t v) {
+  v += shifted<0x111, 0xf>(v);  // from the lane 1, 2, 4 and 8 before, in rows of 16
+  v += shifted<0x112, 0xf>(v);
+  v += shifted<0x114, 0xf>(v);
+  v += shifted<0x118, 0xf>(v);
+  v += shifted<0x142, 0xa>(v);  // the row before's last, into rows 1 and 3
+  v += shifted<0x143, 0xc>(v);  // lane 31, into rows 2 and 3
+  return v;
+}
 
 // The workgroup's LDS writes are everybody's; loads in flight go on.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
@@ -264,118 +339,180 @@ __global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttn
   const uint32_t ring_at = (uint32_t)(uintptr_t)(lds_char_t *)ring;
   char *const shared = lds + G::RING, *const qop = shared;
   float *const ml = reinterpret_cast<float *>(shared + G::SHARED);
-  int32_t *const pre = reinterpret_cast<int32_t *>(shared + G::SHARED + G::ML);
-  int32_t *const len = pre + MXA_BATCH + 4;
+  int32_t *const first = reinterpret_cast<int32_t *>(shared + G::SHARED + G::ML);
+  const MxLine line{first, first + (MXA_BATCH + 4), first + 2 * (MXA_BATCH + 4), first + 3 * (MXA_BATCH + 4)};
+  float *const qn_w = reinterpret_cast<float *>(first + 4 * (MXA_BATCH + 4));
 
-  // The steps of the sequences before each: a prefix sum, a sequence a thread.
-  {
-    static_assert(MXA_BATCH == 64 * MXA_WAVES, "a sequence a thread");
-    const int b = threadIdx.x;
+  // The steps before each sequence, and the sequences with steps, by every wavefront for itself (all
+  // write the same): a prefix sum of 64 sequences at a time.
+  int32_t steps_all = 0, some_all = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const int b = b0 + lane;
     const int32_t l = b < a.batch ? context_len(a, b) : 0, s = steps_of(l);
-    int32_t sum = s;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int32_t v = __shfl_up(sum, o);
-      if (lane >= o) sum += v;
-    }
-    int32_t *const totals = reinterpret_cast<int32_t *>(ml);
-    if (lane == 63) totals[wave] = sum;
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) sum += totals[w];
-    len[b] = l;
-    pre[b] = sum - s;
-    if (b == MXA_BATCH - 1) pre[MXA_BATCH] = sum;
-    __syncthreads();
+    if (a.cu_q != nullptr && b < a.batch) line.cu[b] = a.cu_q[b];
+    const int32_t sum = wave_prefix(s) + steps_all;
+    const uint64_t has = __ballot(s > 0);
+    line.len[b] = l;
+    line.pre[b] = sum - s;
+    line.some[b] = some_all + __popcll(has & ((1ull << lane) - 1));
+    steps_all = __builtin_amdgcn_readlane(sum, 63);
+    some_all += __popcll(has);
   }
-  const MxLine line{pre, len};
-  const int64_t total = (int64_t)a.hkv * a.rgroups * uniform(pre[a.batch]);
-  const int64_t shares = total < a.shares ? total : a.shares;
+  if (a.cu_q != nullptr) line.cu[a.batch] = a.cu_q[a.batch];
+  if (a.qn_w != nullptr && threadIdx.x < D) qn_w[threadIdx.x] = a.qn_w[threadIdx.x];
+  wave_fence();
+  const MxPlan plan(a, steps_all, some_all);
   // Neighbouring shares on one XCD (workgroups go to the 8 XCDs in turn): the row groups of a head
   // and the ends of units read the same cache rows.
   const int64_t wg = blockIdx.x, per = gridDim.x >> 3;
   const int64_t share = wg < 8 * per ? (wg & 7) * per + (wg >> 3) : wg;
-  if (share >= shares) return;
-  const int64_t t0 = share_at(share, total, shares), t1 = share_at(share + 1, total, shares);
-  const int32_t count = (int32_t)(t1 - t0);
+  if (share >= plan.n) return;
+  MxCursor cc, ci;
+  const int64_t end = share + 1 < plan.n ? locate(a, plan, line, plan.share(share + 1), ci)
+                                         : plan.ups * steps_all;
+  const int32_t count = uniform((int)(end - locate(a, plan, line, plan.share(share), cc)));
+  if (count == 0) return;  // a part of a unit's start alone
 
+  // ---- the queries: a wavefront holds the 16 rows of its row block on their way from memory
+  const int32_t rows = a.group * a.q_len;  // of a sequence's KV head
+  auto row_token = [&](const MxCursor &c, int rb, int32_t &head) {  // of this lane's row of a row block; -1: none
+    int64_t from = a.token0 + (int64_t)c.b * a.q_len;
+    int32_t tokens = a.q_len;
+    if (a.cu_q != nullptr) {
+      from = uniform(line.cu[c.b]);
+      tokens = tokens_in(a, from, uniform(line.cu[c.b + 1]));
+    }
+    const int32_t r = (c.rg * RB + rb) * 16 + n;
+    head = divided(r, a.q_mul, a.q_shift);
+    const int32_t tok = r - head * a.q_len;
+    return r < rows && tok < tokens ? from + tok : -1;
+  };
+  u32x4_t qx[D / 32];
+  PrologueOps<D> ops;
+  int32_t rope_row = 0;
+  auto fetch_position = [&](const MxCursor &c) {
+    if (a.qn_w == nullptr || wave >= RB) return;
+    int32_t head;
+    const int64_t token = row_token(c, wave, head);
+    int64_t pos = token < 0 ? 0 : token;
+    if (a.q_pos != nullptr) pos = a.q_pos[pos];
+    rope_row = (int32_t)clamp_row(a.rope, pos);
+  };
+  auto fetch_query = [&](const MxCursor &c) {
+    // Whatever the branches below leave out is new here: nothing of the last rows is kept for it.
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) {
+      qx[t] = u32x4_t{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ops.c[t][i] = ops.s[t][i] = 0.f;
+    }
+    if (wave >= RB) return;
+    int32_t head;
+    const int64_t token = row_token(c, wave, head);
+    const bool live = token >= 0;
+    const uint16_t *src = a.q + (live ? token : 0) * a.q_st + ((int64_t)c.h * a.group + (live ? head : 0)) * a.q_sh + 8 * g;
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+      if (live) qx[t] = load16(src + 32 * t);
+    if (a.qn_w != nullptr) load_rope_ops<D>(ops, a.rope, rope_row, g);
+  };
   // ---- the ring. A tile's page ids lie in its slot before its rows are asked for: those of tile
   // t + NS travel with the rows of tile t.
-  const MxCursor start = cursor_at(a, line, t0);
-  MxCursor ci = start, cd = start, cc = start;
+  MxCursor cd = ci = cc;
   int32_t ids_left = count;
-  auto page_of = [&](const MxCursor &c, int32_t &t) {  // of this lane's position, t, of the wavefront's tile
+  auto page_of = [&](const MxCursor &c, uint32_t lane, uint32_t &t) {  // of this lane's position, t, of the tile
     t = c.lt * MXA_STEP + wave * MXA_TILE + (lane & (MXA_TILE - 1));
-    t = t < c.len ? t : c.len - 1;
-    return __umulhi((uint32_t)t << 1, a.page_mul) >> a.page_shift;
+    t = min(t, (uint32_t)c.len - 1);
+    return (uint32_t)divided(t, a.page_mul, a.page_shift);
   };
-  auto load_ids = [&](uint32_t to) {  // of the tile at ci; past the share's end its last tile's again
-    int32_t t;
-    const uint32_t col = page_of(ci, t);
+  auto load_ids = [&](uint32_t to, uint32_t lane) {  // of the tile at ci; past the share's end its last tile's again
+    uint32_t t;
+    const uint32_t col = page_of(ci, lane, t);
     if (lane < MXA_TILE) ring_load4(a.table + (int64_t)ci.b * a.table_stride + col, to + G::CODES + G::SCALES);
     if (--ids_left > 0) advance(a, line, ci);
   };
   int32_t load_at = 0;  // the slot of the tile at cd
-  auto load_tile = [&]() {
-    const uint32_t to = ring_at + load_at;
-    int32_t t;
-    const uint32_t col = page_of(cd, t);
+  // Lane constants of both steps are worked out anew for every tile: kept, they would go to scratch
+  // memory, whose reloads wait for the whole ring.
+  struct Rows {
+    uint32_t at16, at4;  // where this lane's position of the tile lies: codes in 16 bytes, scales in 4
+  };
+  auto find_rows = [&]() {  // of the tile at cd, whose ids lie in its slot
+    uint32_t lane = threadIdx.x & 63, t;
+    asm volatile("" : "+v"(lane));
+    const uint32_t col = page_of(cd, lane, t);
     uint32_t id = *reinterpret_cast<const uint32_t *>(ring + load_at + G::CODES + G::SCALES + 4 * (lane & (MXA_TILE - 1)));
-    ring_read_done();                           // and whoever read this slot's last tile is done
-    id = id < (uint32_t)a.num_blocks ? id : 0;  // a page that the cache does not have: its first
-    const uint32_t row = (id * (uint32_t)a.hkv + cd.h) * (uint32_t)a.page + ((uint32_t)t - col * (uint32_t)a.page);
-    constexpr int LPR = D / 16;  // lanes of a row
+    id = id < a.num_blocks ? id : 0;  // a page that the cache does not have: its first
+    const uint32_t row = id * a.head_rows + (cd.h * a.page + (t - __umul24(col, a.page)));
+    return Rows{row * a.cs16, row * a.ss4};
+  };
+  auto load_tile = [&](const Rows &rows) {
+    const uint32_t to = ring_at + load_at;
+    uint32_t lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    constexpr uint32_t LPR = D / 16;  // lanes of a row
+    const uint32_t r = lane / LPR, piece = lane % LPR ^ (D == 128 ? r >> 1 : r >> 2 & 3);  // as place() says
+    uint32_t from[G::DMAS], scale_from = rows.at4;
+#pragma unroll
+    for (int u = 0; u < G::DMAS; ++u)
+      from[u] = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * (r + u * (64 / LPR)), (int)rows.at16);
+    if constexpr (D == 128) scale_from = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * (lane >> 1), (int)rows.at4);
+    ring_read_done();  // all of them, and whoever read this slot's last tile is done
 #pragma unroll
     for (int u = 0; u < G::DMAS; ++u) {
-      const int r = (64 / LPR) * u + lane / LPR;
-      const uint32_t from = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * r, (int)row);
-      const int piece = (lane % LPR) ^ (D == 128 ? r >> 1 & 7 : r >> 2 & 3);  // as place() says
-      ring_load16(a.codes + (uint64_t)from * (uint64_t)a.cs + 16 * piece, to + 1024 * u);
+      const uint32_t c = D == 128 ? piece ^ (u & 1) << 2 : piece;
+      ring_load16(a.codes + 16 * c + ((uint64_t)from[u] << 4), to + 1024 * u);
     }
-    if constexpr (D == 128) {
-      const uint32_t from = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * (lane >> 1), (int)row);
-      ring_load4(a.scales + (uint64_t)from * (uint64_t)a.ss + 4 * (lane & 1), to + G::CODES);
-    } else {
-      if (lane < MXA_TILE) ring_load4(a.scales + (uint64_t)row * (uint64_t)a.ss, to + G::CODES);
-    }
-    load_ids(to);
+    if (D == 128 || lane < MXA_TILE)
+      ring_load4(a.scales + (D == 128 ? 4 * (lane & 1) : 0) + ((uint64_t)scale_from << 2), to + G::CODES);
+    load_ids(to, lane);
     advance(a, line, cd);
     load_at = load_at == (G::NS - 1) * G::SLOT ? 0 : load_at + G::SLOT;
   };
   const int32_t ahead = count < G::NS ? count : G::NS;
-  for (int32_t i = 0; i < ahead; ++i) load_ids(ring_at + i * G::SLOT);
+  for (int32_t i = 0; i < ahead; ++i) load_ids(ring_at + i * G::SLOT, lane);
+  fetch_position(cc);
   ring_wait<0>();
-  for (int32_t i = 0; i < ahead; ++i) load_tile();
+  fetch_query(cc);
+  for (int32_t i = 0; i < ahead; ++i) load_tile(find_rows());
+
+  // Where this lane's operands lie in a tile: key row row_of(n) and its scale; value dwords of rows
+  // row_of(4 g + i), i the last two bits of what follows, and their scales.
+  const uint32_t key_at = place<D>(row_of(n), D == 128 ? g : g & 1);
+  const uint32_t key_scale_at = G::CODES + row_of(n) * (D / 16) + (D == 128 ? g : g & 1);
+  const uint32_t value_row = (g & 1) + 8 * (g >> 1), value_block = D == 128 ? n >> 2 : n >> 3;
+  uint32_t value_at[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    value_at[i] = place<D>(value_row + 2 * i, D / 32 + value_block) + (D == 128 ? 4 * (n & 3) : 2 * (n & 7));
+  const uint32_t value_scale_at = G::CODES + value_row * (D / 16) + D / 32 + value_block;
 
   // ---- the share, unit by unit
-  const int32_t rows = a.group * a.q_len;  // of a sequence's KV head
-  int32_t read_at = 0;                     // the slot of the tile to take
+  int32_t read_at = 0;  // the slot of the tile to take
   for (int32_t k = 0; k < count;) {
     const int32_t seg = cc.steps - cc.lt < count - k ? cc.steps - cc.lt : count - k;
-    const bool whole = seg == cc.steps;
-    const int32_t row0 = cc.rg * RB * 16, tokens = tokens_of(a, cc.b);
-    const int64_t token0 = first_token(a, cc.b);
+    const int32_t part = 2 * (int32_t)share + (k > 0 ? 1 : 0);  // where the unit's sums go if it is not whole
+    const bool whole = seg == cc.steps, more = k + seg < count;
+    MxCursor next = cc;
+    next.lt += seg - 1;
+    if (more) advance(a, line, next);
 
+    if (more) fetch_position(next);
     // The unit's queries as operands: a wavefront a row block.
     lds_barrier();  // nobody joins the last unit any more
     if (wave < RB) {
-      const int32_t r = row0 + 16 * wave + n, head = r / a.q_len, tok = r - head * a.q_len;
-      const bool live = r < rows && tok < tokens;
-      const int64_t token = live ? token0 + tok : 0;
-      const uint16_t *src = a.q + token * a.q_st + ((int64_t)cc.h * a.group + (live ? head : 0)) * a.q_sh + 8 * g;
-      u32x4_t x[D / 32];
-#pragma unroll
-      for (int t = 0; t < D / 32; ++t) x[t] = live ? load16(src + 32 * t) : u32x4_t{0, 0, 0, 0};
       float y[D / 32][8];
       if (a.qn_w != nullptr) {
-        const int64_t pos = live ? (a.q_pos != nullptr ? a.q_pos[token] : token) : 0;
-        PrologueOps<D> ops;
-        load_prologue_ops<D>(ops, a.qn_w, a.rope, clamp_row(a.rope, pos), g);
-        norm_rope_exact<D>(x, ops, a.eps, y);
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) ops.w[t][i] = qn_w[32 * t + 8 * g + i];
+        norm_rope_query<D>(qx, ops, a.eps, y);
       } else {
 #pragma unroll
         for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) y[t][2 * i] = bf16_lo(x[t][i]), y[t][2 * i + 1] = bf16_hi(x[t][i]);
+          for (int i = 0; i < 4; ++i) y[t][2 * i] = bf16_lo(qx[t][i]), y[t][2 * i + 1] = bf16_hi(qx[t][i]);
       }
       // A row's hi and lo codes, 2 D bytes, then all rows in the operands' order in their place.
       char *const to = qop + wave * G::QOP, *const stage = to + n * 2 * D;
@@ -384,6 +521,8 @@ __global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttn
       for (int t = 0; t < D / 32; ++t) {
         u32x2_t hi, lo;
         uint32_t byte;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[t][i] *= a.scale_log2;
         split_query(y[t], hi, lo, byte);
         mine = t == (g & (D / 32 - 1)) ? byte : mine;
         *reinterpret_cast<u32x2_t *>(stage + 32 * t + 8 * g) = hi;
@@ -411,17 +550,25 @@ __global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttn
         for (int i = 0; i < G::QN; ++i) qr[rb][i] = load16(qop + rb * G::QOP + 1024 * i + 16 * lane);
     }
 
+    // The next unit's positions are there before the tiles: a load that the compiler waits for among
+    // them would wait for the whole ring every time.
+    asm volatile("" : "+v"(rope_row));
     f32x4_t o[RB][G::NF];
-    float ref[RB], sum[RB];
+    f32x4_t minus[RB];  // less a row's reference, four times: what its scores' sums start from
+    float sum[RB];      // of a row's probabilities in this lane
+    bool fresh = true;  // no tile yet
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      ref[rb] = -INFINITY, sum[rb] = 0.f;
+      minus[rb] = f32x4_t{0.f, 0.f, 0.f, 0.f}, sum[rb] = 0.f;
 #pragma unroll
       for (int f = 0; f < G::NF; ++f) o[rb][f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
 
     for (int32_t i = 0; i < seg; ++i, ++k) {
       wait_tiles<G::LOADS, G::NS - 1>(count - k - 1);
+      const bool again = k + G::NS < count;
+      Rows rows{0, 0};
+      if (again) rows = find_rows();
       const int32_t live = cc.len - (cc.lt + i) * MXA_STEP - wave * MXA_TILE;  // positions of the tile
       if (live > 0) {
         const char *const slot = ring + read_at;
@@ -429,85 +576,98 @@ __global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttn
         int ks[2];
 #pragma unroll
         for (int tb = 0; tb < 2; ++tb) {
-          const int r = 16 * tb + row_of(n), c = D == 128 ? g : g & 1;
-          kf[tb] = load16(slot + place<D>(r, c));
-          ks[tb] = *reinterpret_cast<const uint8_t *>(slot + G::CODES + r * (D / 16) + c);
+          kf[tb] = load16(slot + key_at + 16 * D * tb);
+          ks[tb] = *reinterpret_cast<const uint8_t *>(slot + key_scale_at + D * tb);
         }
-        u32x4_t p[RB];
-        auto scores = [&](auto from) {  // of two row blocks (or the last one)
-          constexpr int R0 = decltype(from)::value, R1 = R0 + 2 < RB ? R0 + 2 : RB, R = R1 - R0;
-          f32x4_t s[R][2];
+        // The log2 of row block rb's probabilities: scores less the references. Positions past the context
+        // repeat its last one.
+        auto scores = [&](int rb, f32x4_t (&s)[2]) {
+          u32x4_t q[G::QN];
 #pragma unroll
-          for (int i = 0; i < R; ++i) {
-            u32x4_t q[G::QN];
-#pragma unroll
-            for (int x = 0; x < G::QN; ++x) {
-              if constexpr (RB <= 2)
-                q[x] = qr[R0 + i][x];
-              else
-                q[x] = load16(qop + (R0 + i) * G::QOP + 1024 * x + 16 * lane);
-            }
-            const int qs = *reinterpret_cast<const uint16_t *>(qop + (R0 + i) * G::QOP + G::QN * 1024 + 2 * lane);
-#pragma unroll
-            for (int tb = 0; tb < 2; ++tb) {
-              s[i][tb] = mfma_k_q(kf[tb], q[0], q[1], f32x4_t{0.f, 0.f, 0.f, 0.f}, ks[tb], qs);
-              if constexpr (D == 128) s[i][tb] = mfma_k_q(kf[tb], q[2], q[3], s[i][tb], ks[tb], qs >> 8);
-            }
+          for (int x = 0; x < G::QN; ++x) {
+            if constexpr (RB <= 2)
+              q[x] = qr[rb][x];
+            else
+              q[x] = load16(qop + rb * G::QOP + 1024 * x + 16 * lane);
           }
-          if (live < MXA_TILE) {
+          const int qs = *reinterpret_cast<const uint16_t *>(qop + rb * G::QOP + G::QN * 1024 + 2 * lane);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int r = 16 * (j >> 2) + (g & 1) + 8 * (g >> 1) + 2 * (j & 3);
+          for (int tb = 0; tb < 2; ++tb) s[tb] = mfma_k_q(kf[tb], q[0], q[1], minus[rb], ks[tb], qs);
+          if constexpr (D == 128) {
 #pragma unroll
-              for (int i = 0; i < R; ++i)
-                if (r >= live) s[i][j >> 2][j & 3] = -INFINITY;
-            }
-          }
-          float top[R];
-          bool passed = false;
-#pragma unroll
-          for (int i = 0; i < R; ++i) {
-            top[i] = s[i][0][0];
-#pragma unroll
-            for (int j = 1; j < 8; ++j) top[i] = fmaxf(top[i], s[i][j >> 2][j & 3]);
-            top[i] *= a.scale_log2;
-            passed |= top[i] > ref[R0 + i] + MXA_SLACK;
-          }
-          if (__ballot(passed) != 0) {
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-              const float m = fmaxf(fmaxf(ref[R0 + i], max_over_groups(top[i])), -3.0e38f);
-              const float f = __builtin_amdgcn_exp2f(ref[R0 + i] - m);
-              ref[R0 + i] = m;
-              sum[R0 + i] *= f;
-#pragma unroll
-              for (int c = 0; c < G::NF; ++c) o[R0 + i][c] *= f;
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < R; ++i) {
-            float e[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j >> 2][j & 3], a.scale_log2, -ref[R0 + i]));
-              sum[R0 + i] += e[j];
-            }
-#pragma unroll
-            for (int c = 0; c < 4; ++c) p[R0 + i][c] = pack_bf16x2(e[2 * c], e[2 * c + 1]);
+            for (int tb = 0; tb < 2; ++tb) s[tb] = mfma_k_q(kf[tb], q[2], q[3], s[tb], ks[tb], qs >> 8);
           }
         };
-        scores(std::integral_constant<int, 0>{});
-        if constexpr (RB > 2) scores(std::integral_constant<int, 2>{});
-        asm volatile("" : : : "memory");  // the values are read behind the scores: registers
+        // References of rows that have none yet or are passed by: the tile's largest score, and what
+        // was summed in line with it.
+        auto refer = [&]() {
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) {
+            f32x4_t s[2];
+            scores(rb, s);
+            __builtin_amdgcn_sched_barrier(0);
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) top = fmaxf(fmaxf(top, s[j >> 2][j & 3]), s[j >> 2][(j & 3) + 1]);
+            top = max_over_groups(top);
+            const float by = (fresh ? top > -INFINITY : top >= 1.f) ? top + MXA_SLACK - 1.f : 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) minus[rb][i] -= by;
+            if (!fresh) {
+              const float f = __builtin_amdgcn_exp2f(-by);
+              sum[rb] *= f;
+#pragma unroll
+              for (int c = 0; c < G::NF; ++c) o[rb][c] *= f;
+            }
+          }
+          fresh = false;
+        };
+        u32x4_t p[RB];
+#pragma nounroll
+        for (int told = fresh ? 1 : 0;; told = 2) {
+          if (told) refer();
+          uint32_t any = 0;
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) {
+            f32x4_t s[2];
+            scores(rb, s);
+            float e[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f(s[j >> 2][j & 3]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              p[rb][c] = both_hi(__float_as_uint(e[2 * c]), __float_as_uint(e[2 * c + 1]));
+              any |= p[rb][c];
+            }
+            if (rb & 1) __builtin_amdgcn_sched_barrier(0);  // two row blocks' scores at a time: registers
+          }
+          // The highest exponent bit: a probability of 2 or more, 2^8 times what its row's reference meant.
+          if (told == 2 || __ballot((any & 0x40004000u) != 0) == 0) break;
+        }
+        if (live < MXA_TILE) {
+          int32_t left = live - (int)value_row;
+          asm volatile("" : "+v"(left));  // the comparisons stay in here
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int r = 16 * (c >> 1) + 4 * (c & 1);
+            const uint32_t kept = (r < left ? 0xffffu : 0u) | (r + 2 < left ? 0xffff0000u : 0u);
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) p[rb][c] &= kept;
+          }
+        }
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) sum[rb] = add_both(p[rb][c], sum[rb]);
+        __builtin_amdgcn_sched_barrier(0);  // the values are read behind the scores: registers
         typedef typename std::conditional<D == 128, uint32_t, uint16_t>::type vword_t;
         uint32_t vw[8];
         float vs[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int r = 16 * (j >> 2) + (g & 1) + 8 * (g >> 1) + 2 * (j & 3);
-          const int c = D == 128 ? n >> 2 : n >> 3, in = D == 128 ? 4 * (n & 3) : 2 * (n & 7);
-          vw[j] = *reinterpret_cast<const vword_t *>(slot + place<D>(r, D / 32 + c) + in);
-          vs[j] = mx_scale_float(*reinterpret_cast<const uint8_t *>(slot + G::CODES + r * (D / 16) + D / 32 + c));
+          const int i = j & 3, tb = j >> 2;
+          vw[j] = *reinterpret_cast<const vword_t *>(slot + value_at[i] + 16 * D * tb);
+          vs[j] = mx_scale_float(*reinterpret_cast<const uint8_t *>(slot + value_scale_at + (D / 16) * (16 * tb + 2 * i)));
         }
         auto channels = [&](auto sel) {  // two of this lane's channels
           constexpr int B = decltype(sel)::value;
@@ -529,43 +689,41 @@ __global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttn
         }
       }
       read_at = read_at == (G::NS - 1) * G::SLOT ? 0 : read_at + G::SLOT;
-      if (k + G::NS < count) load_tile();
+      if (again) load_tile(rows);
     }
 
+    fetch_query(more ? next : cc);  // on its way while this unit is joined
     // The four wavefronts' parts of the unit together, four fragments of each at a time.
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       sum[rb] = sum_over_groups(sum[rb]);
-      if (g == 0) *reinterpret_cast<float2 *>(ml + 2 * ((wave * RB + rb) * 16 + n)) = make_float2(ref[rb], sum[rb]);
+      if (g == 0) *reinterpret_cast<float2 *>(ml + 2 * ((wave * RB + rb) * 16 + n)) = make_float2(fresh ? -INFINITY : -minus[rb][0], sum[rb]);
     }
-    lds_barrier();
-    auto joined = [&](int row, float &m, float &l) {  // a row's reference and sum over the wavefronts
+    lds_barrier();  // and the queries have been read: their place takes the fragments
+    float scale[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {  // a row's reference and sum over the wavefronts
       float2 v[MXA_WAVES];
 #pragma unroll
-      for (int w = 0; w < MXA_WAVES; ++w) v[w] = *reinterpret_cast<const float2 *>(ml + 2 * (w * RB * 16 + row));
-      m = v[0].x;
+      for (int w = 0; w < MXA_WAVES; ++w) v[w] = *reinterpret_cast<const float2 *>(ml + 2 * ((w * RB + rb) * 16 + n));
+      float m = v[0].x, l = 0.f;
 #pragma unroll
       for (int w = 1; w < MXA_WAVES; ++w) m = fmaxf(m, v[w].x);
-      l = 0.f;
 #pragma unroll
       for (int w = 0; w < MXA_WAVES; ++w) l += v[w].y * __builtin_amdgcn_exp2f(v[w].x - m);
-    };
-    const int64_t part = 2 * share + (k == seg ? 0 : 1);
+      scale[rb] = fresh ? 0.f : __builtin_amdgcn_exp2f(-minus[rb][0] - m);
+      minus[rb][0] = m, sum[rb] = l;
+    }
     constexpr int FW = G::NF / 4;  // fragments of a row block that a wavefront joins
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      const int32_t r = row0 + 16 * rb + n, head = r / a.q_len, tok = r - head * a.q_len;
-      const bool live = r < rows && tok < tokens;
-      float m, l;
-      joined(rb * 16 + n, m, l);
-      const float scale = __builtin_amdgcn_exp2f(ref[rb] - m);
       f32x4_t v[FW];
 #pragma unroll
       for (int h = 0; h < FW; ++h) {
-        lds_barrier();  // the last four fragments (the queries, at first) have been read
+        if (rb + h > 0) lds_barrier();  // the last four fragments have been read
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<f32x4_t *>(shared + ((q * MXA_WAVES + wave) * 64 + lane) * 16) = o[rb][q * FW + h] * scale;
+          *reinterpret_cast<f32x4_t *>(shared + ((q * MXA_WAVES + wave) * 64 + lane) * 16) = o[rb][q * FW + h] * scale[rb];
         lds_barrier();
         v[h] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -574,9 +732,12 @@ __global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttn
       }
       // Channels (4 g + i) NF + wave FW + h of row n.
       if (whole) {
-        if (live) {
-          const float inv = 1.f / l;
-          uint16_t *dst = a.o + (token0 + tok) * a.o_st + ((int64_t)cc.h * a.group + head) * a.o_sh + 4 * g * G::NF + wave * FW;
+        int32_t head;
+        const int64_t token = row_token(cc, rb, head);
+        if (token >= 0) {
+          const float inv = 1.f / sum[rb];
+          uint16_t *dst =
+              a.o + token * a.o_st + ((int64_t)cc.h * a.group + head) * a.o_sh + 4 * g * G::NF + wave * FW;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const uint32_t d = pack_bf16x2(v[0][i] * inv, v[FW - 1][i] * inv);
@@ -587,15 +748,14 @@ __global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttn
           }
         }
       } else {
-        const int64_t at = part * RB + rb;
+        const int64_t at = (int64_t)part * RB + rb;
 #pragma unroll
         for (int h = 0; h < FW; ++h)
           *reinterpret_cast<f32x4_t *>(a.part_o + ((at * G::NF + wave * FW + h) * 64 + lane) * 4) = v[h];
-        if (wave == 0 && g == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * (at * 16 + n)) = make_float2(m, l);
+        if (wave == 0 && g == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * (at * 16 + n)) = make_float2(minus[rb][0], sum[rb]);
       }
     }
-    cc.lt += seg - 1;
-    advance(a, line, cc);
+    cc = next;
   }
 }
 
@@ -604,50 +764,58 @@ __global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttn
 template <int D>
 __global__ __launch_bounds__(64 * MXA_WAVES) void attn_mx_join_kernel(const MxAttnArgs a, int rb_unit) {
   constexpr int NF = D / 16, FW = NF / 4;
-  __shared__ int32_t sums[2][MXA_WAVES];
+  __shared__ int32_t sums[4][MXA_WAVES];
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int n = lane & 15, g = lane >> 4;
   const int64_t ups = (int64_t)a.hkv * a.rgroups;
   const int b = (int)(blockIdx.x / ups), u = (int)(blockIdx.x - b * ups), h = u / a.rgroups, rg = u - h * a.rgroups;
   const int rb = blockIdx.y;
-  int32_t before = 0, all = 0;
-  if ((int)threadIdx.x < a.batch) all = steps_of(context_len(a, threadIdx.x));
-  before = (int)threadIdx.x < b ? all : 0;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o), all += __shfl_xor(all, o);
-  if (lane == 0) sums[0][wave] = before, sums[1][wave] = all;
-  __syncthreads();
-  before = all = 0;
-#pragma unroll
-  for (int w = 0; w < MXA_WAVES; ++w) before += sums[0][w], all += sums[1][w];
-  const int64_t total = ups * all, shares = total < a.shares ? total : a.shares;
   const int32_t steps = steps_of(context_len(a, b));
-  const int32_t tokens = tokens_of(a, b);
-  const int32_t r = (rg * rb_unit + rb) * 16 + n, head = r / a.q_len, tok = r - head * a.q_len;
+  int64_t token0 = a.token0 + (int64_t)b * a.q_len;
+  int32_t tokens = a.q_len;
+  if (a.cu_q != nullptr) token0 = a.cu_q[b], tokens = tokens_in(a, token0, a.cu_q[b + 1]);
+  const int32_t mine = (int)threadIdx.x < a.batch ? steps_of(context_len(a, threadIdx.x)) : 0;
+  int32_t v0 = mine, v1 = (int)threadIdx.x < b ? mine : 0;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v0 += __shfl_xor(v0, o), v1 += __shfl_xor(v1, o);
+  const int32_t v2 = __popcll(__ballot(mine > 0)), v3 = __popcll(__ballot(mine > 0 && (int)threadIdx.x < b));
+  if (lane == 0) sums[0][wave] = v0, sums[1][wave] = v1, sums[2][wave] = v2, sums[3][wave] = v3;
+  __syncthreads();
+  int32_t all[4] = {0, 0, 0, 0};  // steps, of them before b, sequences with steps, of them before b
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+#pragma unroll
+    for (int w = 0; w < MXA_WAVES; ++w) all[q] += sums[q][w];
+  const int32_t r = (rg * rb_unit + rb) * 16 + n, head = divided(r, a.q_mul, a.q_shift), tok = r - head * a.q_len;
   const bool live = r < a.group * a.q_len && tok < tokens;
   f32x4_t v[FW];
 #pragma unroll
   for (int f = 0; f < FW; ++f) v[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   float inv = 0.f;
   if (steps > 0) {
-    const int64_t s = ups * before + (int64_t)u * steps, e = s + steps;
-    const int64_t w0 = ((s + 1) * shares - 1) / total, w1 = (e * shares - 1) / total;
-    if (w0 == w1) return;
+    const MxPlan plan(a, all[0], all[2]);
+    const int64_t from = ups * (all[1] + (int64_t)plan.c * all[3]) + (int64_t)u * (steps + plan.c);
+    const int32_t w0 = plan.share_of(from + plan.c), w1 = plan.share_of(from + plan.c + steps - 1);
+    if (w0 == w1) return;  // whole in one share
+    // Share w0's part lies behind that of the unit it starts with, if that is another.
+    const int32_t p0 = 2 * w0 + (plan.share(w0) < from ? 1 : 0), parts = w1 - w0 + 1;
+    auto place = [&](int32_t i) { return (int64_t)(i == 0 ? p0 : 2 * (w0 + i)) * rb_unit + rb; };
     float m = -INFINITY, l = 0.f;
-    for (int64_t w = w0; w <= w1; ++w) {
-      const int64_t at = (2 * w + (share_at(w, total, shares) < s ? 1 : 0)) * rb_unit + rb;
+    for (int32_t i = 0; i < parts; ++i) m = fmaxf(m, a.part_ml[2 * (place(i) * 16 + n)]);
+#pragma unroll 4
+    for (int32_t i = 0; i < parts; ++i) {
+      const int64_t at = place(i);
       const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + 2 * (at * 16 + n));
-      const float top = fmaxf(m, ml.x), f0 = __builtin_amdgcn_exp2f(m - top), f1 = __builtin_amdgcn_exp2f(ml.x - top);
-      l = l * f0 + ml.y * f1;
+      const float f = __builtin_amdgcn_exp2f(ml.x - m);
+      l += ml.y * f;
 #pragma unroll
-      for (int f = 0; f < FW; ++f)
-        v[f] = v[f] * f0 + *reinterpret_cast<const f32x4_t *>(a.part_o + ((at * NF + wave * FW + f) * 64 + lane) * 4) * f1;
-      m = top;
+      for (int c = 0; c < FW; ++c)
+        v[c] += *reinterpret_cast<const f32x4_t *>(a.part_o + ((at * NF + wave * FW + c) * 64 + lane) * 4) * f;
     }
     inv = 1.f / l;
   }
   if (!live) return;
-  uint16_t *dst = a.o + (first_token(a, b) + tok) * a.o_st + ((int64_t)h * a.group + head) * a.o_sh + 4 * g * NF + wave * FW;
+  uint16_t *dst = a.o + (token0 + tok) * a.o_st + ((int64_t)h * a.group + head) * a.o_sh + 4 * g * NF + wave * FW;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t d = pack_bf16x2(v[0][i] * inv, v[FW - 1][i] * inv);
@@ -665,18 +833,20 @@ static int unit_blocks(int32_t rows, int32_t *rgroups) {
   return (blocks + *rgroups - 1) / *rgroups;
 }
 
-static int mx_attn_shares(int rb) {
+// Two workgroups a CU, rounded down to a power of two (see MxPlan).
+static int mx_attn_log_shares() {
   DeviceInfo info;
   const int cus = device_info(&info) == FM_OK ? info.cus : 256;
-  (void)rb;
-  return 2 * cus;
+  int log = 0;
+  while (2 << log <= 2 * cus) ++log;
+  return log;
 }
 
-static size_t mx_attn_part_floats(int rb, int d) { return (size_t)2 * mx_attn_shares(rb) * 16 * rb * (d + 2); }
+static size_t mx_attn_part_floats(int rb, int d) { return (size_t)2 * 16 * rb * (d + 2) << mx_attn_log_shares(); }
 
 template <int D, int RB>
 static int launch_attn_mx(const MxAttnArgs &a, hipStream_t stream) {
-  attn_mx_kernel<D, RB><<<dim3((unsigned)a.shares), dim3(64 * MXA_WAVES), MxGeo<D, RB>::SMEM, stream>>>(a);
+  attn_mx_kernel<D, RB><<<dim3(1u << a.log_shares), dim3(64 * MXA_WAVES), MxGeo<D, RB>::SMEM, stream>>>(a);
   FM_CHECK_HIP(hipGetLastError());
   const int64_t units = (int64_t)a.batch * a.hkv * a.rgroups;
   attn_mx_join_kernel<D><<<dim3((unsigned)units, RB), dim3(256), 0, stream>>>(a, RB);
@@ -732,13 +902,14 @@ extern "C" int fm_block_attn_paged_mx(
   FM_REQUIRE(row_stride % 16 == 0 && row_stride >= head_dim && scales_stride % 4 == 0 && scales_stride >= head_dim / 16,
              "cache rows hold %d code bytes at a stride of a multiple of 16 and %d scale bytes at one of 4", head_dim,
              head_dim / 16);
-  FM_REQUIRE(num_blocks > 0 && page_size > 0 && page_size < (1 << 30) &&
+  FM_REQUIRE(num_blocks > 0 && page_size > 0 && page_size < (1 << 24) &&
                  num_blocks <= ((int64_t)UINT32_MAX / num_kv_heads) / page_size,
              "a cache of 1 to 2^32 - 1 rows, got %lld blocks of %d heads and %d positions", (long long)num_blocks,
              num_kv_heads, page_size);
   FM_REQUIRE(block_table_width >= 0 && (batch == 1 || block_table_stride >= 0), "bad block table");
   FM_REQUIRE(softmax_scale >= 0.f && softmax_scale <= 3e38f, "softmax_scale must be finite and not negative");
-  FM_REQUIRE(q_norm_weight == nullptr || (rope_cos && rope_sin), "a query norm needs its rotary table");
+  FM_REQUIRE(q_norm_weight == nullptr || (rope_cos && rope_sin && rope_rows > 0 && rope_rows < (1ll << 31)),
+             "a query norm needs its rotary table of 1 to 2^31 - 1 rows");
   FM_REQUIRE(q_tokens >= 0 && (cu_seqlens_q || q_tokens >= (int64_t)batch * max_seqlen_q),
              "without cu_seqlens_q the query holds batch x max_seqlen_q = %lld rows, got %lld",
              (long long)batch * max_seqlen_q, (long long)q_tokens);
@@ -752,23 +923,31 @@ extern "C" int fm_block_attn_paged_mx(
   a.o = (uint16_t *)out, a.o_st = out_stride_token, a.o_sh = out_stride_head;
   a.q_len = max_seqlen_q, a.group = num_q_heads / num_kv_heads, a.hkv = num_kv_heads;
   a.codes = (const uint8_t *)codes, a.scales = (const uint8_t *)scales;
-  a.cs = row_stride, a.ss = scales_stride, a.num_blocks = num_blocks, a.page = page_size;
-  while ((1ll << a.page_shift) < page_size) ++a.page_shift;
-  a.page_mul = (uint32_t)(((1ull << (31 + a.page_shift)) + page_size - 1) / page_size);
+  const int64_t cache_rows = num_blocks * num_kv_heads * page_size, cs16 = row_stride / 16, ss4 = scales_stride / 4;
+  FM_REQUIRE(cs16 <= UINT32_MAX / cache_rows && ss4 <= UINT32_MAX / cache_rows,
+             "a cache of less than 2^36 bytes of code rows and 2^34 of scale rows");
+  a.cs16 = (uint32_t)cs16, a.ss4 = (uint32_t)ss4, a.num_blocks = (uint32_t)num_blocks, a.page = page_size;
+  a.head_rows = (uint32_t)num_kv_heads * page_size;
+  auto divisor = [](int64_t d, uint32_t &mul, uint32_t &shift) {
+    for (shift = 0; (1ll << shift) < d;) ++shift;
+    mul = (uint32_t)(((1ull << (31 + shift)) + d - 1) / d);
+  };
+  divisor(page_size, a.page_mul, a.page_shift);
+  divisor(max_seqlen_q, a.q_mul, a.q_shift);
   a.table_stride = block_table_stride;
   const int64_t held = block_table_width * page_size;
   const int64_t most = held < max_seqlen_k ? held : max_seqlen_k;
-  FM_REQUIRE(most <= (1 << 29), "contexts of at most 2^29 positions, got %lld", (long long)most);
+  FM_REQUIRE(most <= (1 << 24), "contexts of at most 2^24 positions, got %lld", (long long)most);
   a.max_len = (int32_t)most;
   a.scale_log2 = softmax_scale * 1.44269504088896341f;
   a.qn_w = q_norm_weight;
   a.rope = Rope{rope_cos, rope_sin, rope_row_stride, rope_pair_stride, rope_rows};
   a.q_pos = q_positions, a.eps = eps;
-  a.shares = mx_attn_shares(rb);
+  a.log_shares = mx_attn_log_shares();
   const size_t need = sizeof(float) * mx_attn_part_floats(rb, head_dim);
   if (workspace_bytes < need) return fail(FM_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
   a.part_o = (float *)workspace;
-  a.part_ml = a.part_o + (size_t)2 * a.shares * 16 * rb * head_dim;
+  a.part_ml = a.part_o + ((size_t)2 * 16 * rb * head_dim << a.log_shares);
   // Launches of up to MXA_BATCH sequences, one after another: they share the workspace.
   for (int32_t b0 = 0; b0 < batch; b0 += MXA_BATCH) {
     a.batch = batch - b0 < MXA_BATCH ? batch - b0 : MXA_BATCH;
