@@ -66,8 +66,11 @@ struct MxAttnArgs {
   float eps;
   float *part_o;   // (2 shares, 16 RB, D), relative to the row's reference
   float *part_ml;  // (2 shares, 16 RB, 2): the reference (log2) and the sum
-  int32_t log_shares;
+  int32_t shares;  // of a row group
+  double per_share;  // 1 / shares
 };
+
+constexpr int mx_resident(int rb) { return rb <= 2 ? 3 : 2; }  // workgroups a CU, as registers and LDS allow
 
 template <int D, int RB>
 struct MxGeo {
@@ -76,16 +79,18 @@ struct MxGeo {
   static constexpr int DMAS = CODES / 1024;               // 16-byte loads a lane of a tile's codes
   static constexpr int LOADS = DMAS + 2;                  // and its scales, and later page ids
   static constexpr int SLOT = CODES + SCALES + 4 * MXA_TILE;
-  static constexpr int NS = 3;                            // tiles in a wavefront's ring
+  static constexpr int RESIDENT = mx_resident(RB);
+  static constexpr int NS = RB <= 2 ? 2 : 3;              // tiles in a wavefront's ring
   static constexpr int RING = MXA_WAVES * NS * SLOT;
   static constexpr int QN = D == 128 ? 4 : 2;             // 16-byte operands a lane of a row block's queries
   static constexpr int QOP = QN * 1024 + 128;             // and the bytes of their two scales
-  static constexpr int MERGE = MXA_WAVES * 4 * 1024;      // four fragments of every wavefront
+  static constexpr int MF = RB <= 2 ? 2 : 4;              // fragments that are joined at a time
+  static constexpr int MERGE = MXA_WAVES * MF * 1024;
   static constexpr int SHARED = RB * QOP > MERGE ? RB * QOP : MERGE;  // one after the other
   static constexpr int ML = MXA_WAVES * RB * 16 * 8;
   static constexpr int LINE = 4 * (MXA_BATCH + 4) * 4;    // the sequences (MxLine)
   static constexpr int SMEM = RING + SHARED + ML + LINE + 4 * D;
-  static_assert(SMEM <= 80 * 1024, "two workgroups a CU");
+  static_assert(SMEM <= 160 * 1024 / RESIDENT, "LDS");
 };
 
 // ------------------------------------------------------------------------------ pieces
@@ -135,33 +140,40 @@ __device__ __forceinline__ int32_t quotient(int64_t a, int64_t b) {
   return q;
 }
 
-// The line of all units' steps, cut into n shares by cost: a unit counts its steps and, in front of
-// them, c more for its start and end (0 where shares are a few steps). Of 64 requests of 256 to 8192
-// positions the shares that hold the short ones would otherwise take twice the others' time. With fewer
-// steps than shares each is one; else n is 2^log_shares, and share s starts at s total >> log_shares.
+// The line of a row group's steps, all heads of all sequences, cut into n shares by cost: a unit counts
+// its steps and, in front of them, c more for its start and end (0 where shares are a few steps). Of
+// 64 requests of 256 to 8192 positions the shares that hold the short ones would otherwise take
+// twice the others' time. With fewer steps than shares each is one.
 struct MxPlan {
-  int64_t ups, total;
-  int32_t n, c, shift;
+  int64_t total, each;  // share s starts at s total / n = s each + s over / n
+  int32_t n, c, over;
+  bool few;
   __device__ __forceinline__ MxPlan(const MxAttnArgs &a, int32_t steps, int32_t sequences) {
-    ups = (int64_t)a.hkv * a.rgroups;
-    const int64_t all = ups * steps;
-    const bool few = all < 1ll << a.log_shares;
-    n = few ? (int32_t)all : 1 << a.log_shares;
-    shift = few ? 0 : a.log_shares;
-    const int64_t fair = few ? 0 : all >> (a.log_shares + 2);
+    const int64_t all = (int64_t)a.hkv * steps;
+    few = all < a.shares;
+    n = few ? (int32_t)all : a.shares;
+    const int64_t fair = few ? 0 : (int64_t)((double)all * a.per_share) >> 2;
     c = fair < MXA_UNIT_COST ? (int32_t)fair : MXA_UNIT_COST;
-    total = all + ups * c * sequences;
+    total = all + (int64_t)a.hkv * c * sequences;
+    each = (int64_t)((double)total * a.per_share);  // within 1: total is below 2^46
+    while (each * a.shares > total) --each;
+    while ((each + 1) * a.shares <= total) ++each;
+    over = (int32_t)(total - each * a.shares);
   }
-  __device__ __forceinline__ int64_t share(int64_t s) const { return shift ? s * total >> shift : s; }
+  __device__ __forceinline__ int64_t share(int32_t s) const { return few ? s : s * each + quotient(s * over, n); }
   // The share that `at` lies in: the last that starts there or before.
   __device__ __forceinline__ int32_t share_of(int64_t at) const {
-    return shift ? quotient(((at + 1) << shift) - 1, total) : (int32_t)at;
+    if (few) return (int32_t)at;
+    int32_t w = (int32_t)((float)at * (float)n * __builtin_amdgcn_rcpf((float)total));
+    while (share(w) > at) --w;
+    while (share(w + 1) <= at) ++w;
+    return w;
   }
 };
 
-// A place on the line: step lt of unit (b, h, rg).
+// A place on the line: step lt of unit (b, h).
 struct MxCursor {
-  int b, h, rg, lt, steps, len;
+  int b, h, lt, steps, len;
 };
 
 // In LDS, by sequence: the steps, and the sequences with steps, before it; its length; its first token.
@@ -176,8 +188,6 @@ struct MxLine {
 __device__ __forceinline__ void advance(const MxAttnArgs &a, const MxLine &line, MxCursor &c) {
   if (++c.lt < c.steps) return;
   c.lt = 0;
-  if (++c.rg < a.rgroups) return;
-  c.rg = 0;
   if (++c.h < a.hkv) return;
   c.h = 0;
   for (++c.b; c.b < a.batch; ++c.b) {  // sequences without context have no units
@@ -193,17 +203,16 @@ __device__ __forceinline__ int64_t locate(const MxAttnArgs &a, const MxPlan &pla
   int before = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     const int b = b0 + lane < a.batch ? b0 + lane : 0;
-    before += __popcll(__ballot(b0 + lane < a.batch && plan.ups * (line.pre[b] + (int64_t)plan.c * line.some[b]) <= at));
+    before += __popcll(__ballot(b0 + lane < a.batch && (int64_t)a.hkv * (line.pre[b] + plan.c * line.some[b]) <= at));
   }
   c.b = uniform(before - 1);  // the last that starts there or before: those without steps start where the next does
   line.load(c);
   const int32_t pre = uniform(line.pre[c.b]);
-  const int64_t off = at - plan.ups * (pre + (int64_t)plan.c * uniform(line.some[c.b]));
-  const int unit = uniform(quotient(off, c.steps + plan.c)), in = (int)(off - (int64_t)unit * (c.steps + plan.c)) - plan.c;
+  const int64_t off = at - (int64_t)a.hkv * (pre + plan.c * uniform(line.some[c.b]));
+  c.h = uniform(quotient(off, c.steps + plan.c));
+  const int in = (int)(off - (int64_t)c.h * (c.steps + plan.c)) - plan.c;
   c.lt = in > 0 ? in : 0;
-  c.h = a.rgroups == 1 ? unit : unit / a.rgroups;
-  c.rg = unit - c.h * a.rgroups;
-  return plan.ups * pre + (int64_t)unit * c.steps + c.lt;
+  return (int64_t)a.hkv * pre + (int64_t)c.h * c.steps + c.lt;
 }
 
 // LDS place of the 16-byte piece c of tile row r: rows of 128 bytes (D 128) or 64. Operand
@@ -224,6 +233,33 @@ __device__ __forceinline__ f32x4_t mfma_k_q(u32x4_t k, u32x4_t q0, u32x4_t q1, f
 }
 
 __device__ __forceinline__ uint32_t lo_byte(uint32_t byte) { return byte == 255u ? 255u : byte - 5; }
+
+// load_rope_ops for tables whose pairs lie side by side, or interleaved (the entry refuses others: their
+// addresses alone would take half the registers).
+template <int D>
+__device__ __forceinline__ void load_rope(PrologueOps<D> &ops, const Rope &rope, int64_t row, int g) {
+  const float *cs = rope.cos + row * rope.row_stride;
+  const bool apart = rope.pair_stride == 1;
+  const float *second = apart ? rope.sin + row * rope.row_stride : cs + 4;
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t) {
+    const int at = apart ? 16 * t + 4 * g : 32 * t + 8 * g;
+    const f32x4u_t v = *(g_f32x4u_t *)(cs + at), w = *(g_f32x4u_t *)(second + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ops.c[t][i] = v[i], ops.s[t][i] = w[i];
+  }
+}
+// As they were loaded: pairs apart, or two (cos, sin) in ops.c and two in ops.s.
+template <int D>
+__device__ __forceinline__ void sort_rope(PrologueOps<D> &ops, const Rope &rope) {
+  if (rope.pair_stride == 1) return;
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t) {
+    const float c1 = ops.c[t][2], s0 = ops.c[t][1], s1 = ops.c[t][3], c2 = ops.s[t][0], c3 = ops.s[t][2], s2 = ops.s[t][1];
+    ops.c[t][1] = c1, ops.c[t][2] = c2, ops.c[t][3] = c3;
+    ops.s[t][0] = s0, ops.s[t][1] = s1, ops.s[t][2] = s2;
+  }
+}
 
 // norm_rope_exact where the result is rounded to 8 bits: sums and root in float32 as they come.
 template <int D>
@@ -330,7 +366,7 @@ __device__ __forceinline__ void wait_tiles(int32_t behind) {
 // --------------------------------------------------------------------------- the kernel
 
 template <int D, int RB>
-__global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttnArgs a) {
+__global__ __launch_bounds__(64 * MXA_WAVES, (MxGeo<D, RB>::RESIDENT)) void attn_mx_kernel(const MxAttnArgs a) {
   using G = MxGeo<D, RB>;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int lane = threadIdx.x & 63, wave = wave_id();
@@ -362,14 +398,12 @@ __global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttn
   if (a.qn_w != nullptr && threadIdx.x < D) qn_w[threadIdx.x] = a.qn_w[threadIdx.x];
   wave_fence();
   const MxPlan plan(a, steps_all, some_all);
-  // Neighbouring shares on one XCD (workgroups go to the 8 XCDs in turn): the row groups of a head
-  // and the ends of units read the same cache rows.
-  const int64_t wg = blockIdx.x, per = gridDim.x >> 3;
-  const int64_t share = wg < 8 * per ? (wg & 7) * per + (wg >> 3) : wg;
+  // Neighbouring shares, and a share's row groups, on one XCD (workgroups go to the 8 XCDs in turn, and
+  // the grid's x is a multiple of 8): they read the same cache rows, the row groups at the same time.
+  const int32_t rg = blockIdx.y, share = (int32_t)((blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3));
   if (share >= plan.n) return;
   MxCursor cc, ci;
-  const int64_t end = share + 1 < plan.n ? locate(a, plan, line, plan.share(share + 1), ci)
-                                         : plan.ups * steps_all;
+  const int64_t end = share + 1 < plan.n ? locate(a, plan, line, plan.share(share + 1), ci) : (int64_t)a.hkv * steps_all;
   const int32_t count = uniform((int)(end - locate(a, plan, line, plan.share(share), cc)));
   if (count == 0) return;  // a part of a unit's start alone
 
@@ -382,7 +416,7 @@ __global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttn
       from = uniform(line.cu[c.b]);
       tokens = tokens_in(a, from, uniform(line.cu[c.b + 1]));
     }
-    const int32_t r = (c.rg * RB + rb) * 16 + n;
+    const int32_t r = (rg * RB + rb) * 16 + n;
     head = divided(r, a.q_mul, a.q_shift);
     const int32_t tok = r - head * a.q_len;
     return r < rows && tok < tokens ? from + tok : -1;
@@ -414,7 +448,7 @@ __global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttn
 #pragma unroll
     for (int t = 0; t < D / 32; ++t)
       if (live) qx[t] = load16(src + 32 * t);
-    if (a.qn_w != nullptr) load_rope_ops<D>(ops, a.rope, rope_row, g);
+    if (a.qn_w != nullptr) load_rope(ops, a.rope, rope_row, g);
   };
   // ---- the ring. A tile's page ids lie in its slot before its rows are asked for: those of tile
   // t + NS travel with the rows of tile t.
@@ -491,7 +525,7 @@ __global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttn
   int32_t read_at = 0;  // the slot of the tile to take
   for (int32_t k = 0; k < count;) {
     const int32_t seg = cc.steps - cc.lt < count - k ? cc.steps - cc.lt : count - k;
-    const int32_t part = 2 * (int32_t)share + (k > 0 ? 1 : 0);  // where the unit's sums go if it is not whole
+    const int32_t part = 2 * (rg * a.shares + share) + (k > 0 ? 1 : 0);  // where the unit's sums go if it is not whole
     const bool whole = seg == cc.steps, more = k + seg < count;
     MxCursor next = cc;
     next.lt += seg - 1;
@@ -500,6 +534,13 @@ __global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttn
     if (more) fetch_position(next);
     // The unit's queries as operands: a wavefront a row block.
     lds_barrier();  // nobody joins the last unit any more
+    // On every path the loads of the query end here, not where the tiles next write their registers.
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) {
+      asm volatile("" : "+v"(qx[t]));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(ops.c[t][i]), "+v"(ops.s[t][i]));
+    }
     if (wave < RB) {
       float y[D / 32][8];
       if (a.qn_w != nullptr) {
@@ -507,6 +548,7 @@ __global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttn
         for (int t = 0; t < D / 32; ++t)
 #pragma unroll
           for (int i = 0; i < 8; ++i) ops.w[t][i] = qn_w[32 * t + 8 * g + i];
+        sort_rope(ops, a.rope);
         norm_rope_query<D>(qx, ops, a.eps, y);
       } else {
 #pragma unroll
@@ -542,17 +584,17 @@ __global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttn
           (uint16_t)(D == 128 ? mine | low << 8 : g < 2 ? mine : low);
     }
     lds_barrier();
-    u32x4_t qr[RB <= 2 ? RB : 1][G::QN];
-    if constexpr (RB <= 2) {
+    constexpr bool QR = RB <= 2;  // the queries stay in registers, else in LDS
+    u32x4_t qr[QR ? RB : 1][G::QN];
+    int qrs[QR ? RB : 1];
+    if constexpr (QR) {
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
+      for (int rb = 0; rb < RB; ++rb) {
+        qrs[rb] = *reinterpret_cast<const uint16_t *>(qop + rb * G::QOP + G::QN * 1024 + 2 * lane);
 #pragma unroll
         for (int i = 0; i < G::QN; ++i) qr[rb][i] = load16(qop + rb * G::QOP + 1024 * i + 16 * lane);
+      }
     }
-
-    // The next unit's positions are there before the tiles: a load that the compiler waits for among
-    // them would wait for the whole ring every time.
-    asm volatile("" : "+v"(rope_row));
     f32x4_t o[RB][G::NF];
     f32x4_t minus[RB];  // less a row's reference, four times: what its scores' sums start from
     float sum[RB];      // of a row's probabilities in this lane
@@ -564,6 +606,9 @@ __global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttn
       for (int f = 0; f < G::NF; ++f) o[rb][f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
 
+    // The next unit's positions are there before the tiles: a load that the compiler waits for among
+    // them would wait for the whole ring every time.
+    asm volatile("" : "+v"(rope_row));
     for (int32_t i = 0; i < seg; ++i, ++k) {
       wait_tiles<G::LOADS, G::NS - 1>(count - k - 1);
       const bool again = k + G::NS < count;
@@ -583,14 +628,16 @@ __global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttn
         // repeat its last one.
         auto scores = [&](int rb, f32x4_t (&s)[2]) {
           u32x4_t q[G::QN];
+          int qs;
+          if constexpr (QR) {
 #pragma unroll
-          for (int x = 0; x < G::QN; ++x) {
-            if constexpr (RB <= 2)
-              q[x] = qr[rb][x];
-            else
-              q[x] = load16(qop + rb * G::QOP + 1024 * x + 16 * lane);
+            for (int x = 0; x < G::QN; ++x) q[x] = qr[rb][x];
+            qs = qrs[rb];
+          } else {
+#pragma unroll
+            for (int x = 0; x < G::QN; ++x) q[x] = load16(qop + rb * G::QOP + 1024 * x + 16 * lane);
+            qs = *reinterpret_cast<const uint16_t *>(qop + rb * G::QOP + G::QN * 1024 + 2 * lane);
           }
-          const int qs = *reinterpret_cast<const uint16_t *>(qop + rb * G::QOP + G::QN * 1024 + 2 * lane);
 #pragma unroll
           for (int tb = 0; tb < 2; ++tb) s[tb] = mfma_k_q(kf[tb], q[0], q[1], minus[rb], ks[tb], qs);
           if constexpr (D == 128) {
@@ -605,7 +652,7 @@ __global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttn
           for (int rb = 0; rb < RB; ++rb) {
             f32x4_t s[2];
             scores(rb, s);
-            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (!QR) __builtin_amdgcn_sched_barrier(0);
             float top = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 8; j += 2) top = fmaxf(fmaxf(top, s[j >> 2][j & 3]), s[j >> 2][(j & 3) + 1]);
@@ -639,7 +686,8 @@ __global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttn
               p[rb][c] = both_hi(__float_as_uint(e[2 * c]), __float_as_uint(e[2 * c + 1]));
               any |= p[rb][c];
             }
-            if (rb & 1) __builtin_amdgcn_sched_barrier(0);  // two row blocks' scores at a time: registers
+            if constexpr (!QR)  // two row blocks' scores at a time: registers
+              if (rb & 1) __builtin_amdgcn_sched_barrier(0);
           }
           // The highest exponent bit: a probability of 2 or more, 2^8 times what its row's reference meant.
           if (told == 2 || __ballot((any & 0x40004000u) != 0) == 0) break;
@@ -659,7 +707,7 @@ __global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttn
         for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
           for (int c = 0; c < 4; ++c) sum[rb] = add_both(p[rb][c], sum[rb]);
-        __builtin_amdgcn_sched_barrier(0);  // the values are read behind the scores: registers
+        if constexpr (!QR) __builtin_amdgcn_sched_barrier(0);  // the values are read behind the scores: registers
         typedef typename std::conditional<D == 128, uint32_t, uint16_t>::type vword_t;
         uint32_t vw[8];
         float vs[8];
@@ -693,7 +741,7 @@ __global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttn
     }
 
     fetch_query(more ? next : cc);  // on its way while this unit is joined
-    // The four wavefronts' parts of the unit together, four fragments of each at a time.
+    // The four wavefronts' parts of the unit together, MF fragments at a time.
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       sum[rb] = sum_over_groups(sum[rb]);
@@ -714,116 +762,190 @@ __global__ __launch_bounds__(64 * MXA_WAVES, 2) void attn_mx_kernel(const MxAttn
       scale[rb] = fresh ? 0.f : __builtin_amdgcn_exp2f(-minus[rb][0] - m);
       minus[rb][0] = m, sum[rb] = l;
     }
-    constexpr int FW = G::NF / 4;  // fragments of a row block that a wavefront joins
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      f32x4_t v[FW];
-#pragma unroll
-      for (int h = 0; h < FW; ++h) {
-        if (rb + h > 0) lds_barrier();  // the last four fragments have been read
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<f32x4_t *>(shared + ((q * MXA_WAVES + wave) * 64 + lane) * 16) = o[rb][q * FW + h] * scale[rb];
-        lds_barrier();
-        v[h] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < MXA_WAVES; ++w)
-          v[h] += *reinterpret_cast<const f32x4_t *>(shared + ((wave * MXA_WAVES + w) * 64 + lane) * 16);
-      }
-      // Channels (4 g + i) NF + wave FW + h of row n.
-      if (whole) {
+      const float inv = 1.f / sum[rb];
+      const int64_t at = (int64_t)part * RB + rb;
+      float *const part_o = a.part_o + at * 16 * D + 4 * lane;  // fragment 0's place
+      auto row_out = [&]() {  // row n's channels, or NULL
         int32_t head;
         const int64_t token = row_token(cc, rb, head);
-        if (token >= 0) {
-          const float inv = 1.f / sum[rb];
-          uint16_t *dst =
-              a.o + token * a.o_st + ((int64_t)cc.h * a.group + head) * a.o_sh + 4 * g * G::NF + wave * FW;
+        return token >= 0 ? a.o + token * a.o_st + ((int64_t)cc.h * a.group + head) * a.o_sh : nullptr;
+      };
+      if (!whole && wave == 0 && g == 0)
+        *reinterpret_cast<float2 *>(a.part_ml + 2 * (at * 16 + n)) = make_float2(minus[rb][0], sum[rb]);
+      if constexpr (G::MF == 2) {
+        // Fragments f and f + 1, of which each wavefront joins one of the lanes' four values.
+        uint16_t *const dst = whole ? row_out() : nullptr;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t d = pack_bf16x2(v[0][i] * inv, v[FW - 1][i] * inv);
-            if constexpr (FW == 2)
-              *reinterpret_cast<uint32_t *>(dst + i * G::NF) = d;
-            else
-              dst[i * G::NF] = (uint16_t)d;
-          }
+        for (int f = 0; f < G::NF; f += 2) {
+          if (rb + f > 0) lds_barrier();  // the last two have been read
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            *reinterpret_cast<f32x4_t *>(shared + ((q * MXA_WAVES + wave) * 64 + lane) * 16) = o[rb][f + q] * scale[rb];
+          lds_barrier();
+          float v[2] = {0.f, 0.f};
+#pragma unroll
+          for (int w = 0; w < MXA_WAVES; ++w)
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+              v[q] += *reinterpret_cast<const float *>(shared + ((q * MXA_WAVES + w) * 64 + lane) * 16 + 4 * wave);
+          if (!whole)
+            part_o[f * 256 + wave] = v[0], part_o[(f + 1) * 256 + wave] = v[1];
+          else if (dst != nullptr)
+            *reinterpret_cast<uint32_t *>(dst + (4 * g + wave) * G::NF + f) = pack_bf16x2(v[0] * inv, v[1] * inv);
         }
       } else {
-        const int64_t at = (int64_t)part * RB + rb;
+        // Every FWth fragment from h on, one for each wavefront: FW in all, whose channels lie side by side.
+        constexpr int FW = G::NF / 4;
+        f32x4_t v[FW];
 #pragma unroll
-        for (int h = 0; h < FW; ++h)
-          *reinterpret_cast<f32x4_t *>(a.part_o + ((at * G::NF + wave * FW + h) * 64 + lane) * 4) = v[h];
-        if (wave == 0 && g == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * (at * 16 + n)) = make_float2(minus[rb][0], sum[rb]);
+        for (int h = 0; h < FW; ++h) {
+          if (rb + h > 0) lds_barrier();  // the last four have been read
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<f32x4_t *>(shared + ((q * MXA_WAVES + wave) * 64 + lane) * 16) = o[rb][q * FW + h] * scale[rb];
+          lds_barrier();
+          v[h] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int w = 0; w < MXA_WAVES; ++w)
+            v[h] += *reinterpret_cast<const f32x4_t *>(shared + ((wave * MXA_WAVES + w) * 64 + lane) * 16);
+        }
+        if (!whole) {
+#pragma unroll
+          for (int h = 0; h < FW; ++h) *reinterpret_cast<f32x4_t *>(part_o + (wave * FW + h) * 256) = v[h];
+        } else if (uint16_t *const dst = row_out()) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint16_t *const to = dst + (4 * g + i) * G::NF + wave * FW;
+            const uint32_t d = pack_bf16x2(v[0][i] * inv, v[FW - 1][i] * inv);
+            if constexpr (FW == 2)
+              *reinterpret_cast<uint32_t *>(to) = d;
+            else
+              *to = (uint16_t)d;
+          }
+        }
       }
     }
+
     cc = next;
   }
 }
 
 // The units that shares cut, from their parts, and zeros for the sequences without context. A
-// workgroup a 16-row block of a unit, laid out as the parts are: a wavefront D / 64 fragments.
-template <int D>
+// workgroup a 16-row block of a unit, a wavefront a quarter of its fragments, as the parts hold them:
+// they are written and read whole lines at a time. SPLIT: the quarters lie with four workgroups, whose
+// wavefronts take every fourth part (calls of few units, which are cut into many).
+template <int D, bool SPLIT>
 __global__ __launch_bounds__(64 * MXA_WAVES) void attn_mx_join_kernel(const MxAttnArgs a, int rb_unit) {
   constexpr int NF = D / 16, FW = NF / 4;
+  constexpr int STEP = SPLIT ? MXA_WAVES : 1;
   __shared__ int32_t sums[4][MXA_WAVES];
+  __shared__ f32x4_t parts_sum[MXA_WAVES][64][FW + 1];
   const int lane = threadIdx.x & 63, wave = wave_id();
-  const int n = lane & 15, g = lane >> 4;
-  const int64_t ups = (int64_t)a.hkv * a.rgroups;
-  const int b = (int)(blockIdx.x / ups), u = (int)(blockIdx.x - b * ups), h = u / a.rgroups, rg = u - h * a.rgroups;
-  const int rb = blockIdx.y;
+  const int b = (int)blockIdx.x / a.hkv, h = (int)blockIdx.x - b * a.hkv;
+  const int block = blockIdx.y, rg = block / rb_unit, rb = block - rg * rb_unit;
   const int32_t steps = steps_of(context_len(a, b));
   int64_t token0 = a.token0 + (int64_t)b * a.q_len;
   int32_t tokens = a.q_len;
   if (a.cu_q != nullptr) token0 = a.cu_q[b], tokens = tokens_in(a, token0, a.cu_q[b + 1]);
   const int32_t mine = (int)threadIdx.x < a.batch ? steps_of(context_len(a, threadIdx.x)) : 0;
-  int32_t v0 = mine, v1 = (int)threadIdx.x < b ? mine : 0;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v0 += __shfl_xor(v0, o), v1 += __shfl_xor(v1, o);
-  const int32_t v2 = __popcll(__ballot(mine > 0)), v3 = __popcll(__ballot(mine > 0 && (int)threadIdx.x < b));
-  if (lane == 0) sums[0][wave] = v0, sums[1][wave] = v1, sums[2][wave] = v2, sums[3][wave] = v3;
+  const int32_t upto = wave_prefix(mine);
+  const uint64_t has = __ballot(mine > 0);
+  if (lane == 63) sums[0][wave] = upto, sums[1][wave] = __popcll(has);
+  if ((int)threadIdx.x == b) sums[2][0] = upto - mine, sums[3][0] = __popcll(has & ((1ull << lane) - 1));
   __syncthreads();
-  int32_t all[4] = {0, 0, 0, 0};  // steps, of them before b, sequences with steps, of them before b
+  int32_t all[4] = {0, sums[2][0], 0, sums[3][0]};  // steps, of them before b, sequences with steps, of them before b
 #pragma unroll
-  for (int q = 0; q < 4; ++q)
-#pragma unroll
-    for (int w = 0; w < MXA_WAVES; ++w) all[q] += sums[q][w];
-  const int32_t r = (rg * rb_unit + rb) * 16 + n, head = divided(r, a.q_mul, a.q_shift), tok = r - head * a.q_len;
-  const bool live = r < a.group * a.q_len && tok < tokens;
+  for (int w = 0; w < MXA_WAVES; ++w) {
+    all[0] += sums[0][w], all[2] += sums[1][w];
+    if (w < (b >> 6)) all[1] += sums[0][w], all[3] += sums[1][w];
+  }
+  // This thread: channels (4 g + i) NF + quarter FW + f of row n.
+  const int n = lane & 15, g = lane >> 4, quarter = SPLIT ? (int)blockIdx.z : wave;
+  const int32_t r = block * 16 + n, head = divided(r, a.q_mul, a.q_shift), tok = r - head * a.q_len;
+  const bool live = r < a.group * a.q_len && tok < tokens && (!SPLIT || wave == 0);
   f32x4_t v[FW];
 #pragma unroll
   for (int f = 0; f < FW; ++f) v[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  float inv = 0.f;
-  if (steps > 0) {
-    const MxPlan plan(a, all[0], all[2]);
-    const int64_t from = ups * (all[1] + (int64_t)plan.c * all[3]) + (int64_t)u * (steps + plan.c);
-    const int32_t w0 = plan.share_of(from + plan.c), w1 = plan.share_of(from + plan.c + steps - 1);
-    if (w0 == w1) return;  // whole in one share
-    // Share w0's part lies behind that of the unit it starts with, if that is another.
-    const int32_t p0 = 2 * w0 + (plan.share(w0) < from ? 1 : 0), parts = w1 - w0 + 1;
-    auto place = [&](int32_t i) { return (int64_t)(i == 0 ? p0 : 2 * (w0 + i)) * rb_unit + rb; };
-    float m = -INFINITY, l = 0.f;
-    for (int32_t i = 0; i < parts; ++i) m = fmaxf(m, a.part_ml[2 * (place(i) * 16 + n)]);
-#pragma unroll 4
-    for (int32_t i = 0; i < parts; ++i) {
-      const int64_t at = place(i);
-      const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + 2 * (at * 16 + n));
-      const float f = __builtin_amdgcn_exp2f(ml.x - m);
-      l += ml.y * f;
+  auto store = [&]() {
+    if (!live) return;
+    uint16_t *dst = a.o + (token0 + tok) * a.o_st + ((int64_t)h * a.group + head) * a.o_sh + 4 * g * NF + quarter * FW;
 #pragma unroll
-      for (int c = 0; c < FW; ++c)
-        v[c] += *reinterpret_cast<const f32x4_t *>(a.part_o + ((at * NF + wave * FW + c) * 64 + lane) * 4) * f;
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t d = pack_bf16x2(v[0][i], v[FW - 1][i]);
+      if constexpr (FW == 2)
+        *reinterpret_cast<uint32_t *>(dst + i * NF) = d;
+      else
+        dst[i * NF] = (uint16_t)d;
     }
-    inv = 1.f / l;
-  }
-  if (!live) return;
-  uint16_t *dst = a.o + (token0 + tok) * a.o_st + ((int64_t)h * a.group + head) * a.o_sh + 4 * g * NF + wave * FW;
+  };
+  if (steps == 0) return store();
+  const MxPlan plan(a, all[0], all[2]);
+  const int64_t from = (int64_t)a.hkv * (all[1] + plan.c * all[3]) + (int64_t)h * (steps + plan.c);
+  const int32_t w0 = plan.share_of(from + plan.c), w1 = plan.share_of(from + plan.c + steps - 1);
+  if (w0 == w1) return;  // whole in one share
+  // Share w0's part lies behind that of the unit it starts with, if that is another.
+  const int32_t p0 = 2 * (rg * a.shares + w0), behind = plan.share(w0) < from ? 1 : 0, parts = w1 - w0 + 1;
+  float m = -INFINITY, l = 0.f;
+  // Four parts at a time, their loads in flight together.
+  for (int32_t i0 = SPLIT ? wave : 0; i0 < parts; i0 += 4 * STEP) {
+    float2 ml[4];
+    f32x4_t pv[4][FW];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t d = pack_bf16x2(v[0][i] * inv, v[FW - 1][i] * inv);
-    if constexpr (FW == 2)
-      *reinterpret_cast<uint32_t *>(dst + i * NF) = d;
-    else
-      dst[i * NF] = (uint16_t)d;
+    for (int u = 0; u < 4; ++u) {
+      const int32_t i = i0 + u * STEP < parts ? i0 + u * STEP : i0;
+      const int64_t at = (int64_t)(p0 + 2 * i + (i == 0 ? behind : 0)) * rb_unit + rb;
+      ml[u] = *reinterpret_cast<const float2 *>(a.part_ml + 2 * (at * 16 + n));
+      if (i0 + u * STEP >= parts) ml[u] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int f = 0; f < FW; ++f)
+        pv[u][f] = *reinterpret_cast<const f32x4_t *>(a.part_o + ((at * NF + quarter * FW + f) * 64 + lane) * 4);
+    }
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) top = fmaxf(top, ml[u].x);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    l *= f;
+#pragma unroll
+    for (int c = 0; c < FW; ++c) v[c] *= f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (i0 + u * STEP >= parts) continue;
+      const float fu = __builtin_amdgcn_exp2f(ml[u].x - top);
+      l += ml[u].y * fu;
+#pragma unroll
+      for (int c = 0; c < FW; ++c) v[c] += pv[u][c] * fu;
+    }
+    m = top;
   }
+  if constexpr (SPLIT) {
+    f32x4_t *const to = parts_sum[wave][lane];
+    to[0] = f32x4_t{m, l, 0.f, 0.f};
+#pragma unroll
+    for (int f = 0; f < FW; ++f) to[1 + f] = v[f];
+    __syncthreads();
+    if (wave != 0) return;
+    float top = m;
+#pragma unroll
+    for (int w = 1; w < MXA_WAVES; ++w) top = fmaxf(top, parts_sum[w][lane][0][0]);
+    l = 0.f;
+#pragma unroll
+    for (int f = 0; f < FW; ++f) v[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < MXA_WAVES; ++w) {
+      const f32x4_t *src = parts_sum[w][lane];
+      if (src[0][0] == -INFINITY) continue;  // took no part
+      const float by = __builtin_amdgcn_exp2f(src[0][0] - top);
+      l += src[0][1] * by;
+#pragma unroll
+      for (int f = 0; f < FW; ++f) v[f] += src[1 + f] * by;
+    }
+  }
+  const float inv = 1.f / l;
+#pragma unroll
+  for (int f = 0; f < FW; ++f) v[f] *= inv;
+  store();
 }
 
 // Row blocks of a unit: up to 4, all units alike where the rows fill more than one.
@@ -833,23 +955,28 @@ static int unit_blocks(int32_t rows, int32_t *rgroups) {
   return (blocks + *rgroups - 1) / *rgroups;
 }
 
-// Two workgroups a CU, rounded down to a power of two (see MxPlan).
-static int mx_attn_log_shares() {
+// Shares of a row group: as many workgroups as the chip holds at once, by eights (a share an XCD).
+static int32_t mx_attn_shares(int rb, int32_t rgroups) {
   DeviceInfo info;
   const int cus = device_info(&info) == FM_OK ? info.cus : 256;
-  int log = 0;
-  while (2 << log <= 2 * cus) ++log;
-  return log;
+  const int32_t n = mx_resident(rb) * cus / rgroups / 8 * 8;
+  return n < 8 ? 8 : n;
 }
 
-static size_t mx_attn_part_floats(int rb, int d) { return (size_t)2 * 16 * rb * (d + 2) << mx_attn_log_shares(); }
+static size_t mx_attn_part_floats(int rb, int32_t rgroups, int d) {
+  return (size_t)2 * mx_attn_shares(rb, rgroups) * rgroups * 16 * rb * (d + 2);
+}
 
 template <int D, int RB>
 static int launch_attn_mx(const MxAttnArgs &a, hipStream_t stream) {
-  attn_mx_kernel<D, RB><<<dim3(1u << a.log_shares), dim3(64 * MXA_WAVES), MxGeo<D, RB>::SMEM, stream>>>(a);
+  attn_mx_kernel<D, RB><<<dim3(a.shares, a.rgroups), dim3(64 * MXA_WAVES), MxGeo<D, RB>::SMEM, stream>>>(a);
   FM_CHECK_HIP(hipGetLastError());
-  const int64_t units = (int64_t)a.batch * a.hkv * a.rgroups;
-  attn_mx_join_kernel<D><<<dim3((unsigned)units, RB), dim3(256), 0, stream>>>(a, RB);
+  const unsigned units = (unsigned)(a.batch * a.hkv), blocks = (unsigned)(a.rgroups * RB);
+  // With fewer row blocks than the chip takes workgroups at once they are cut into many parts.
+  if (units * blocks < 512)
+    attn_mx_join_kernel<D, true><<<dim3(units, blocks, 4), dim3(64 * MXA_WAVES), 0, stream>>>(a, RB);
+  else
+    attn_mx_join_kernel<D, false><<<dim3(units, blocks), dim3(64 * MXA_WAVES), 0, stream>>>(a, RB);
   FM_CHECK_HIP(hipGetLastError());
   return FM_OK;
 }
@@ -872,9 +999,10 @@ extern "C" size_t fm_block_attn_paged_mx_workspace_bytes(int32_t max_seqlen_q, i
                                                          int32_t num_kv_heads, int32_t head_dim) {
   if (max_seqlen_q <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads || head_dim <= 0) return 0;
   const int64_t rows = (int64_t)(num_q_heads / num_kv_heads) * max_seqlen_q;
-  if (rows > (1 << 24)) return 0;
+  if (rows > (1 << 20)) return 0;
   int32_t rgroups;
-  return sizeof(float) * mx_attn_part_floats(unit_blocks((int32_t)rows, &rgroups), head_dim);
+  const int rb = unit_blocks((int32_t)rows, &rgroups);
+  return sizeof(float) * mx_attn_part_floats(rb, rgroups, head_dim);
 }
 
 extern "C" int fm_block_attn_paged_mx(
@@ -910,14 +1038,16 @@ extern "C" int fm_block_attn_paged_mx(
   FM_REQUIRE(softmax_scale >= 0.f && softmax_scale <= 3e38f, "softmax_scale must be finite and not negative");
   FM_REQUIRE(q_norm_weight == nullptr || (rope_cos && rope_sin && rope_rows > 0 && rope_rows < (1ll << 31)),
              "a query norm needs its rotary table of 1 to 2^31 - 1 rows");
+  if (q_norm_weight != nullptr && rope_pair_stride != 1 && !(rope_pair_stride == 2 && rope_sin == rope_cos + 1))
+    return fail(FM_ERR_UNSUPPORTED, "rotary tables of pairs side by side, or (cos, sin) interleaved");
   FM_REQUIRE(q_tokens >= 0 && (cu_seqlens_q || q_tokens >= (int64_t)batch * max_seqlen_q),
              "without cu_seqlens_q the query holds batch x max_seqlen_q = %lld rows, got %lld",
              (long long)batch * max_seqlen_q, (long long)q_tokens);
   const int64_t rows = (int64_t)(num_q_heads / num_kv_heads) * max_seqlen_q;
-  FM_REQUIRE(rows <= (1 << 24), "at most 2^24 query rows for a KV head, got %lld", (long long)rows);
+  FM_REQUIRE(rows <= (1 << 20), "at most 2^20 query rows for a KV head, got %lld", (long long)rows);
   MxAttnArgs a{};
   const int rb = unit_blocks((int32_t)rows, &a.rgroups);
-  FM_REQUIRE((int64_t)MXA_BATCH * num_kv_heads * a.rgroups < (1ll << 31), "too many units");
+  FM_REQUIRE((int64_t)MXA_BATCH * num_kv_heads < (1ll << 31) && a.rgroups * rb < 65536, "too many units");
   a.q_tokens = q_tokens;
   a.q = (const uint16_t *)q, a.q_st = q_stride_token, a.q_sh = q_stride_head;
   a.o = (uint16_t *)out, a.o_st = out_stride_token, a.o_sh = out_stride_head;
@@ -943,11 +1073,12 @@ extern "C" int fm_block_attn_paged_mx(
   a.qn_w = q_norm_weight;
   a.rope = Rope{rope_cos, rope_sin, rope_row_stride, rope_pair_stride, rope_rows};
   a.q_pos = q_positions, a.eps = eps;
-  a.log_shares = mx_attn_log_shares();
-  const size_t need = sizeof(float) * mx_attn_part_floats(rb, head_dim);
+  a.shares = mx_attn_shares(rb, a.rgroups);
+  a.per_share = 1.0 / a.shares;
+  const size_t need = sizeof(float) * mx_attn_part_floats(rb, a.rgroups, head_dim);
   if (workspace_bytes < need) return fail(FM_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
   a.part_o = (float *)workspace;
-  a.part_ml = a.part_o + ((size_t)2 * 16 * rb * head_dim << a.log_shares);
+  a.part_ml = a.part_o + (size_t)2 * a.shares * a.rgroups * 16 * rb * head_dim;
   // Launches of up to MXA_BATCH sequences, one after another: they share the workspace.
   for (int32_t b0 = 0; b0 < batch; b0 += MXA_BATCH) {
     a.batch = batch - b0 < MXA_BATCH ? batch - b0 : MXA_BATCH;

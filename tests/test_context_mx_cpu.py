@@ -239,8 +239,8 @@ def test_entries_refuse():
     assert attend(scale=-1.0) == n.FM_ERR_INVALID and attend(scale=float("nan")) == n.FM_ERR_INVALID
     assert attend(norm=x) == n.FM_ERR_INVALID and "rotary" in _err()
     assert attend(q_tokens=7) == n.FM_ERR_INVALID and "batch x max_seqlen_q" in _err()
-    assert attend(q_len=1 << 24, q_tokens=1 << 40) == n.FM_ERR_INVALID and "2^24" in _err()
-    assert attend(width=1 << 30, max_k=2 ** 31 - 1) == n.FM_ERR_INVALID and "2^29" in _err()
+    assert attend(q_len=1 << 20, q_tokens=1 << 40) == n.FM_ERR_INVALID and "2^20" in _err()
+    assert attend(width=1 << 30, max_k=2 ** 31 - 1) == n.FM_ERR_INVALID and "2^24" in _err()
     assert attend(ws_bytes=64) == n.FM_ERR_WORKSPACE
 
     def judge(dtype=0, rows=2, vocab=100, stride=100, top=4, logits=x, out=x, ws=x, ws_bytes=1 << 30, tokens=x):
