@@ -111,11 +111,6 @@ __device__ __forceinline__ void ring_wait() {
 }
 // Every LDS read issued so far has its data: what lies there may be loaded over.
 __device__ __forceinline__ void ring_read_done() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
-__device__ __forceinline__ void wave_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
-
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 __device__ __forceinline__ int32_t context_len(const MxAttnArgs &a, int b) {

@@ -111,6 +111,12 @@ __device__ __forceinline__ float max_over_groups(float v) {
 // so that everything derived from it stays in SGPRs and uniform branches.
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
 
+// What a wavefront's lanes wrote to LDS before it, its lanes read behind it.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 __device__ __forceinline__ u32x4_t load16(const void *p) {
   return *reinterpret_cast<const u32x4_t *>(p);
 }

@@ -5,9 +5,18 @@
 //   rank(t) = 1 + #{j : x_j > x_t},  and the largest logits with their lp, the lower index first
 //   among equals, a NaN before any number.
 //
-// A workgroup takes a tile of a row: its maximum, then its S, D, count and largest logits, as one
-// record; wavefronts then put 64 records together at a time until a row has one. A logit and its
-// index are one 64-bit key, whose order is the order of the list.
+// A row is cut into parts, one where there are rows for the whole chip, and a part is a workgroup's:
+// its lanes keep a maximum, S and D of their own, put in line with each new maximum, so that nothing is
+// joined before the part's end; the next 16 KB of logits travel meanwhile. Parts leave records, which a
+// workgroup a row puts together the same way; a row of one part is done at once.
+//
+// The list: a logit and its index are one 64-bit key, whose order is the order of the list. A
+// wavefront meets its columns in rising order and keeps the keys that may be among its largest in LDS. A
+// tile whose maximum does not pass the last of them is left at once. Where many lanes pass (the first
+// tile), the k-th largest of the lanes' own largest keys, found a bit at a time by ballots, bounds the k-th
+// largest of all: about k keys of 2048 remain. They are put in order by counting: a key's place is the
+// number of keys above it. A list of any length up to 32 costs so little that it stays hidden behind
+// the loads; what costs is rising logits, whose tiles all pass.
 #include <math.h>
 
 #include "fm_host.h"
@@ -16,10 +25,11 @@
 namespace fm {
 
 constexpr int LP_THREADS = 256, LP_WAVES = LP_THREADS / 64;
-constexpr int LP_IT = 4;                          // chunks of 8 logits a thread
-constexpr int LP_TILE = 8 * LP_IT * LP_THREADS;   // logits of a workgroup
-constexpr int LP_TOP = 32;                        // the longest list
-constexpr int LP_JOIN = 64;                       // records that a wavefront puts together
+constexpr int LP_TOP = 32;        // the longest list
+constexpr int LP_KEPT = 64;       // keys that a wavefront keeps before it puts them in order
+constexpr int LP_ROOM = LP_KEPT + 8 * 64;  // and those that one step may add
+constexpr int LP_GROUPS = 1024;   // workgroups that few rows are cut into: 4 a CU
+constexpr int LP_SMALL = 8 * LP_THREADS;   // logits of the smallest part
 
 struct LogProbsArgs {
   const char *logits;
@@ -31,10 +41,10 @@ struct LogProbsArgs {
   // outputs
   float *token, *entropy, *top_lp;
   int64_t *rank, *top_ids;
-  // records of this step and of the next: (rows, parts) of float4 and (rows, parts, top) of keys
-  float4 *stats, *stats_out;
-  uint64_t *keys, *keys_out;
-  int32_t parts, parts_out;
+  // records of the parts, (rows, parts) of (m, S, D, count) and (rows, parts, top) of keys
+  float4 *stats;
+  uint64_t *keys;
+  int32_t parts, tiles;  // tiles: of a part
 };
 
 __device__ __forceinline__ uint32_t logit_order(float x) {
@@ -48,14 +58,6 @@ __device__ __forceinline__ float logit_of(uint32_t o) {
 // 0: no logit.
 __device__ __forceinline__ uint64_t logit_key(float x, uint32_t col) { return (uint64_t)logit_order(x) << 32 | (uint32_t)~col; }
 
-__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const uint64_t w = __shfl_xor((unsigned long long)v, o);
-    v = w > v ? w : v;
-  }
-  return v;
-}
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
@@ -79,164 +81,311 @@ __device__ __forceinline__ float token_logit(const LogProbsArgs &a, int64_t row)
   return reinterpret_cast<const float *>(src)[t];
 }
 
-// Part blockIdx.x of row blockIdx.y.
-template <int TY>
-__global__ __launch_bounds__(LP_THREADS) void log_probs_tile_kernel(const LogProbsArgs a) {
-  __shared__ float red[3][LP_WAVES];
-  __shared__ int32_t counts[LP_WAVES];
-  __shared__ uint64_t best[2][LP_WAVES];
+// The largest t that at least k lanes' v reach.
+__device__ __forceinline__ uint32_t kth_largest(uint32_t v, int k) {
+  uint32_t t = 0;
+#pragma nounroll
+  for (uint32_t bit = 1u << 31; bit != 0; bit >>= 1)
+    if (__popcll(__ballot(v >= (t | bit))) >= k) t |= bit;
+  return t;
+}
+
+// A wavefront's largest keys. Keys of no logit are 0 and never kept.
+struct LpList {
+  uint64_t *kept;      // LP_ROOM and then LP_TOP places in LDS
+  int top, n;          // n: kept so far, uniform
+  uint64_t least;      // keys up to this are not among the largest (0: nothing is known)
+  float least_logit;   // its logit, NaN where that says nothing
+
+  __device__ __forceinline__ void start(uint64_t *lds, int k) { kept = lds, top = k, n = 0, least = 0, least_logit = NAN; }
+  __device__ __forceinline__ void raise(uint64_t to) {
+    if (to <= least) return;
+    least = to;
+    least_logit = logit_of((uint32_t)(to >> 32));
+  }
+  // `mine`: a lane's largest key of those that are about to come.
+  __device__ __forceinline__ void bound(uint64_t mine) {
+    const uint32_t v = (uint32_t)(mine >> 32), t = kth_largest(v, top);
+    if (t == 0) return;
+    uint64_t to = (uint64_t)t << 32;
+    if (__popcll(__ballot(v >= t)) > top)  // equals: by their columns
+      to |= kth_largest(v == t ? (uint32_t)mine : 0, top - __popcll(__ballot(v > t)));
+    raise(to - 1);
+  }
+  __device__ __forceinline__ void add(uint64_t key) {
+    const bool pass = key > least;
+    const uint64_t mask = __ballot(pass);
+    if (pass) kept[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0))] = key;
+    n += __popcll(mask);
+  }
+  // The largest in order at the front, the others gone.
+  __device__ __forceinline__ void order(int lane) {
+    wave_fence();
+    uint64_t *const sorted = kept + LP_ROOM;
+#pragma nounroll
+    for (int from = 0; from < n; from += 64) {
+      const uint64_t key = from + lane < n ? kept[from + lane] : 0;
+      int place = 0;
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) place += kept[i] > key;
+      if (key != 0 && place < top) sorted[place] = key;
+    }
+    n = n < top ? n : top;
+    wave_fence();
+    const uint64_t key = lane < n ? sorted[lane] : 0;
+    if (lane < LP_TOP) kept[lane] = key;  // and none behind them
+    wave_fence();
+    if (n == top) raise(kept[top - 1]);
+  }
+};
+
+// A lane's share of m, S, D and the count, and another one in.
+struct LpSums {
+  float m, s, d;
+  int32_t above;
+  // Everything in line with the maximum `to`; c: log2(e) / T.
+  __device__ __forceinline__ void line(float to, float c) {
+    const float from = to == -INFINITY ? 0.f : to;  // of -inf alone every exponential is 0, none is of inf - inf
+    const float off = fmaxf(m - from, -3e38f), f = __builtin_amdgcn_exp2f((m - from) * c);
+    s *= f;
+    d = __builtin_fmaf(off, s, d * f);  // off is as low as -3e38 where f is 0
+    m = to;
+  }
+  __device__ __forceinline__ void add(float m2, float s2, float d2, int32_t above2, float c) {
+    LpSums other{m2, s2, d2, above2};
+    const float to = fmaxf(m, m2);
+    line(to, c), other.line(to, c);
+    s += other.s, d += other.d, above += above2;
+  }
+};
+
+struct LpShared {
+  uint64_t keys[LP_WAVES][LP_ROOM + LP_TOP];
+  float sums[LP_WAVES][4];
+};
+
+// The lanes' sums and the wavefronts' lists to one record, or to the row's results.
+template <int TY, bool RESULTS>
+__device__ __forceinline__ void finish(const LogProbsArgs &a, LpShared &lds, LpSums sums, LpList &list, int64_t row,
+                                       int64_t record) {
+  const int lane = threadIdx.x & 63, wave = wave_id();
+  const float temp = a.temps == nullptr ? 1.f : a.temps[row], c = 1.f / temp * 1.44269504f;
+  sums.line(wave_max(sums.m), c);
+  const float s = wave_sum(sums.s), d = wave_sum(sums.d);
+  const int32_t above = wave_sum(sums.above);
+  if (lane == 0) *reinterpret_cast<float4 *>(lds.sums[wave]) = make_float4(sums.m, s, d, __int_as_float(above));
+  if (a.top > 0) list.order(lane);
+  __syncthreads();
+  LpSums all{-INFINITY, 0.f, 0.f, 0};
+#pragma unroll
+  for (int w = 0; w < LP_WAVES; ++w) {
+    const float4 v = *reinterpret_cast<const float4 *>(lds.sums[w]);
+    all.add(v.x, v.y, v.z, __float_as_int(v.w), c);
+  }
+  const float log_s = logf(all.s);
+  if (threadIdx.x == 0) {
+    if constexpr (!RESULTS) {
+      a.stats[record] = make_float4(all.m, all.s, all.d, __int_as_float(all.above));
+    } else {
+      a.entropy[row] = log_s - all.d / (temp * all.s);
+      if (a.tokens != nullptr) {
+        const int64_t t = a.tokens[row];
+        a.token[row] = (token_logit<TY>(a, row) - all.m) / temp - log_s;
+        a.rank[row] = t < 0 || t >= a.vocab ? 0 : (int64_t)all.above + 1;
+      }
+    }
+  }
+  if (lane >= a.top) return;
+  // A key's place among all wavefronts' lists; those of no logit last, in any order of their own.
+  const uint64_t key = lds.keys[wave][lane];
+  int place = 0;
+  for (int i = 0; i < a.top; ++i)
+#pragma unroll
+    for (int w = 0; w < LP_WAVES; ++w) {
+      const uint64_t other = lds.keys[w][i];
+      place += other > key || (other == key && (w < wave || (w == wave && i < lane)));
+    }
+  if (place >= a.top) return;
+  if constexpr (!RESULTS) {
+    a.keys[record * a.top + place] = key;
+  } else {
+    a.top_ids[row * a.top + place] = (int64_t)(uint32_t)~(uint32_t)key;
+    a.top_lp[row * a.top + place] = (logit_of((uint32_t)(key >> 32)) - all.m) / temp - log_s;
+  }
+}
+
+// Part blockIdx.x of row blockIdx.y, tiles of IT chunks of 8 logits a thread.
+template <int TY, int IT, bool RESULTS>
+__global__ __launch_bounds__(LP_THREADS) void log_probs_part_kernel(const LogProbsArgs a) {
+  __shared__ LpShared lds;
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int64_t row = a.first_row + blockIdx.y;
   const RowView<TY> view(a.logits + row * a.row_bytes, a.vocab);
-  const uint32_t g0 = blockIdx.x * (LP_IT * LP_THREADS);
-  Chunk<TY> x[LP_IT];
+  const uint32_t first = blockIdx.x * (uint32_t)a.tiles * (IT * LP_THREADS);
+  Chunk<TY> next[IT];
 #pragma unroll
-  for (int it = 0; it < LP_IT; ++it) x[it] = view.chunk(g0 + it * LP_THREADS + threadIdx.x);
+  for (int it = 0; it < IT; ++it) next[it] = view.chunk(first + it * LP_THREADS + threadIdx.x);
   const float mine = token_logit<TY>(a, row);
-  const float inv_t = a.temps == nullptr ? 1.f : 1.f / a.temps[row];
-  const float c = inv_t * 1.44269504f;
-  if (view.edge(g0, LP_IT * LP_THREADS)) {
+  const float c = a.temps == nullptr ? 1.44269504f : 1.f / a.temps[row] * 1.44269504f;
+  LpSums sums{-INFINITY, 0.f, 0.f, 0};
+  LpList list;
+  list.start(lds.keys[wave], a.top);
+  int32_t above = 0;  // of the wavefront
+#pragma nounroll
+  for (int32_t t = 0; t < a.tiles; ++t) {
+    const uint32_t g0 = first + t * (IT * LP_THREADS);
+    if ((uint64_t)g0 * 8 >= (uint64_t)view.skip + view.vocab) break;  // behind the row
+    Chunk<TY> x[IT];
 #pragma unroll
-    for (int it = 0; it < LP_IT; ++it) view.trim(x[it], g0 + it * LP_THREADS + threadIdx.x);
-  }
-  float m = -INFINITY;
+    for (int it = 0; it < IT; ++it) x[it] = next[it];
+    if (t + 1 < a.tiles) {
 #pragma unroll
-  for (int it = 0; it < LP_IT; ++it)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = fmaxf(m, x[it].at(j));
-  m = wave_max(m);
-  if (lane == 0) red[0][wave] = m;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < LP_WAVES; ++w) m = fmaxf(m, red[0][w]);
-  // A tile of -inf alone: every exponential is 0, none is of inf - inf.
-  const float from = m == -INFINITY ? 0.f : m;
-  float s = 0.f, d = 0.f;
-  int32_t above = 0;
-#pragma unroll
-  for (int it = 0; it < LP_IT; ++it)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float v = x[it].at(j), t = v - from;
-      const float e = __builtin_amdgcn_exp2f(t * c);
-      s += e;
-      d = __builtin_fmaf(fmaxf(t, -3e38f), e, d);  // -inf stands for 0 here
-      above += v > mine;
+      for (int it = 0; it < IT; ++it) next[it] = view.chunk(g0 + (IT + it) * LP_THREADS + threadIdx.x);
     }
-  s = wave_sum(s), d = wave_sum(d), above = wave_sum(above);
-  if (lane == 0) red[1][wave] = s, red[2][wave] = d, counts[wave] = above;
-  __syncthreads();
-  const int64_t record = (int64_t)blockIdx.y * a.parts + blockIdx.x;
-  if (threadIdx.x == 0) {
-    s = d = 0.f, above = 0;
-    for (int w = 0; w < LP_WAVES; ++w) s += red[1][w], d += red[2][w], above += counts[w];
-    a.stats[record] = make_float4(m, s, d, __int_as_float(above));
-  }
-  uint64_t last = ~0ull;
-  for (int k = 0; k < a.top; ++k) {
-    uint64_t top = 0;
+    if (view.edge(g0, IT * LP_THREADS)) {
 #pragma unroll
-    for (int it = 0; it < LP_IT; ++it)
+      for (int it = 0; it < IT; ++it) view.trim(x[it], g0 + it * LP_THREADS + threadIdx.x);
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int it = 0; it < IT; ++it)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = fmaxf(m, x[it].at(j));
+    if (__ballot(m > sums.m) != 0) sums.line(fmaxf(m, sums.m), c);
+    const float from = sums.m == -INFINITY ? 0.f : sums.m;
+    float s[2] = {sums.s, 0.f}, d[2] = {sums.d, 0.f};
+#pragma unroll
+    for (int it = 0; it < IT; ++it)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint32_t col = 8 * (g0 + it * LP_THREADS + threadIdx.x) - view.skip + j;
-        const uint64_t key = col < view.vocab ? logit_key(x[it].at(j), col) : 0;
-        if (key < last && key > top) top = key;
+        const float v = x[it].at(j), off = v - from;
+        const float e = __builtin_amdgcn_exp2f(off * c);
+        s[j & 1] += e;
+        d[j & 1] = __builtin_fmaf(fmaxf(off, -3e38f), e, d[j & 1]);  // -inf stands for 0 here
       }
-    top = wave_max(top);
-    if (lane == 0) best[k & 1][wave] = top;
-    __syncthreads();
+    sums.s = s[0] + s[1], sums.d = d[0] + d[1];
+    if (a.tokens != nullptr) {
 #pragma unroll
-    for (int w = 0; w < LP_WAVES; ++w) top = best[k & 1][w] > top ? best[k & 1][w] : top;
-    last = top;
-    if (threadIdx.x == 0) a.keys[record * a.top + k] = top;
-    if (top == 0) last = 1;  // none left: zeros to the list's end
-  }
-}
-
-// Records blockIdx.x * 64 to that + 63 of row blockIdx.y; where they are all, the row's results.
-template <int TY>
-__global__ __launch_bounds__(64) void log_probs_join_kernel(const LogProbsArgs a) {
-  __shared__ uint64_t lists[LP_JOIN * LP_TOP];
-  const int lane = threadIdx.x;
-  const int64_t row = a.first_row + blockIdx.y;
-  const int first = blockIdx.x * LP_JOIN, n = a.parts - first < LP_JOIN ? a.parts - first : LP_JOIN;
-  const int64_t record = (int64_t)blockIdx.y * a.parts + first;
-  for (int i = lane; i < n * a.top; i += 64) lists[i] = a.keys[record * a.top + i];
-  const bool results = a.parts_out == 1;
-  const float mine = results ? token_logit<TY>(a, row) : 0.f;
-  const float temp = a.temps == nullptr ? 1.f : a.temps[row];
-  float4 st = lane < n ? a.stats[record + lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
-  const float m = wave_max(st.x);
-  const float off = fmaxf(st.x - m, -3e38f), f = __builtin_amdgcn_exp2f(off * (1.44269504f / temp));
-  // A record of -inf alone has S 0 (and f NaN where all are).
-  float s = st.y == 0.f ? 0.f : st.y * f;
-  float d = st.y == 0.f ? 0.f : __builtin_fmaf(off, s, st.z * f);
-  s = wave_sum(s), d = wave_sum(d);
-  const int32_t above = wave_sum(lane < n ? __float_as_int(st.w) : 0);
-  const int64_t to = (int64_t)blockIdx.y * a.parts_out + blockIdx.x;
-  const float log_s = logf(s);
-  if (lane == 0) {
-    if (!results) {
-      a.stats_out[to] = make_float4(m, s, d, __int_as_float(above));
-    } else {
-      a.entropy[row] = log_s - d / (temp * s);
-      if (a.tokens != nullptr) {
-        const int64_t t = a.tokens[row];
-        a.token[row] = (mine - m) / temp - log_s;
-        a.rank[row] = t < 0 || t >= a.vocab ? 0 : (int64_t)above + 1;
+      for (int it = 0; it < IT; ++it) {
+        x[it].forget();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) above += __popcll(__ballot(x[it].at(j) > mine));
       }
     }
-  }
-  __syncthreads();
-  int at = 0;
-  for (int k = 0; k < a.top; ++k) {
-    const uint64_t head = lane < n && at < a.top ? lists[lane * a.top + at] : 0;
-    const uint64_t top = wave_max(head);
-    if (head == top) ++at;
-    if (lane != 0) continue;
-    if (!results) {
-      a.keys_out[to * a.top + k] = top;
-    } else {
-      a.top_ids[row * a.top + k] = (int64_t)(uint32_t)~(uint32_t)top;
-      a.top_lp[row * a.top + k] = (logit_of((uint32_t)(top >> 32)) - m) / temp - log_s;
+    // All columns kept lie before this tile's: an equal logit comes behind them.
+    const uint64_t passed = a.top == 0 ? 0 : __ballot(!(m <= list.least_logit) || sums.s != sums.s);
+    if (passed == 0) continue;
+    auto column = [&](int it, int j) { return 8 * (g0 + it * LP_THREADS + threadIdx.x) - view.skip + j; };
+    auto key_at = [&](int it, int j) {
+      const uint32_t col = column(it, j);
+      return col < view.vocab ? logit_key(x[it].at(j), col) : 0;
+    };
+    if (__popcll(passed) > 16) {  // each lane that passes adds a key or more: worth a bound
+      uint64_t largest = 0;
+#pragma unroll
+      for (int it = 0; it < IT; ++it) {
+        x[it].forget();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint64_t key = key_at(it, j);
+          largest = key > largest ? key : largest;
+        }
+      }
+      list.bound(largest);
     }
+#pragma unroll
+    for (int it = 0; it < IT; ++it) {
+      x[it].forget();
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (__ballot(!(x[it].at(j) < list.least_logit)) != 0) list.add(key_at(it, j));
+      if (list.n > LP_KEPT) list.order(lane);
+    }
+    if (list.least == 0 || list.n > 2 * a.top) list.order(lane);
   }
+  sums.above = lane == 0 ? above : 0;
+  finish<TY, RESULTS>(a, lds, sums, list, row, (int64_t)blockIdx.y * a.parts + blockIdx.x);
 }
 
-static int64_t lp_parts(int64_t vocab) { return (vocab + 7 + LP_TILE - 1) / LP_TILE; }  // rows may start inside a granule
+// The records of row blockIdx.x.
+template <int TY>
+__global__ __launch_bounds__(LP_THREADS) void log_probs_join_kernel(const LogProbsArgs a) {
+  __shared__ LpShared lds;
+  const int lane = threadIdx.x & 63, wave = wave_id();
+  const int64_t row = a.first_row + blockIdx.x, record = (int64_t)blockIdx.x * a.parts;
+  const float c = a.temps == nullptr ? 1.44269504f : 1.f / a.temps[row] * 1.44269504f;
+  LpSums sums{-INFINITY, 0.f, 0.f, 0};
+  LpList list;
+  list.start(lds.keys[wave], a.top);
+  for (int32_t r = threadIdx.x; r < a.parts; r += LP_THREADS) {
+    const float4 v = a.stats[record + r];
+    sums.add(v.x, v.y, v.z, __float_as_int(v.w), c);
+  }
+  const int32_t total = a.parts * a.top;
+#pragma nounroll
+  for (int32_t at = 0; at < total; at += 8 * LP_THREADS) {
+    uint64_t key[8], largest = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int32_t i = at + j * LP_THREADS + (int32_t)threadIdx.x;
+      key[j] = i < total ? a.keys[record * a.top + i] : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) largest = key[j] > largest ? key[j] : largest;
+    list.bound(largest);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) list.add(key[j]);
+    if (list.n > LP_KEPT) list.order(lane);
+  }
+  finish<TY, true>(a, lds, sums, list, row, 0);
+}
 
-// Rows of one pass: what a launch's grid and the workspace are made for.
-static int64_t lp_rows(int64_t rows) { return rows < 32768 ? rows : 32768; }
+// How a call is cut: rows for 4 workgroups a CU are a part each, fewer are cut into parts for as
+// many, of whole tiles; where those would be less than one of 16 KB, tiles are 8 logits a thread (one row
+// of 151936 bf16 logits: ? us in 75 parts, ? in 19).
+struct LpCut {
+  int64_t parts;
+  int32_t tiles;
+  bool small;
+  LpCut(int64_t rows, int64_t vocab, int es) {
+    const int64_t wide = LP_SMALL * 8 / es, n = vocab + 7;  // rows may start inside a granule
+    const int64_t most = rows >= LP_GROUPS ? 1 : (LP_GROUPS + rows - 1) / rows;
+    small = (n + wide - 1) / wide < most;
+    const int64_t tile = small ? LP_SMALL : wide, all = (n + tile - 1) / tile;
+    tiles = (int32_t)((all + most - 1) / most);
+    parts = (all + tiles - 1) / tiles;
+  }
+};
+
+// Rows of one launch.
+constexpr int64_t LP_ROWS = 32768;
 
 static size_t lp_bytes(int64_t records, int64_t top) { return (size_t)records * (16 + 8 * (size_t)top); }
 
 template <int TY>
 static int run_log_probs(LogProbsArgs a, int64_t rows, char *ws, hipStream_t stream) {
-  const int64_t parts = lp_parts(a.vocab), joined = (parts + LP_JOIN - 1) / LP_JOIN, most = lp_rows(rows);
-  for (int64_t first = 0; first < rows; first += most) {
-    const unsigned n = (unsigned)(rows - first < most ? rows - first : most);
+  constexpr int IT = TY == LOGITS_F32 ? 2 : 4;
+  const LpCut cut(rows, a.vocab, TY == LOGITS_F32 ? 4 : 2);
+  a.parts = (int32_t)cut.parts, a.tiles = cut.tiles;
+  a.stats = (float4 *)ws;
+  a.keys = (uint64_t *)(a.stats + rows * cut.parts);
+  for (int64_t first = 0; first < rows; first += LP_ROWS) {
     a.first_row = first;
-    a.parts = (int32_t)parts;
-    auto set = [&](float4 *&stats, uint64_t *&keys, int64_t at, int64_t records) {
-      stats = (float4 *)(ws + at);
-      keys = (uint64_t *)(stats + records);
-    };
-    // Two areas that take turns: the tiles' records, and a 64th of them.
-    const int64_t area[2] = {0, (int64_t)lp_bytes(most * parts, a.top)}, room[2] = {most * parts, most * joined};
-    int from = 0;
-    set(a.stats, a.keys, area[0], room[0]);
-    log_probs_tile_kernel<TY><<<dim3((unsigned)parts, n), dim3(LP_THREADS), 0, stream>>>(a);
-    FM_CHECK_HIP(hipGetLastError());
-    do {
-      a.parts_out = (a.parts + LP_JOIN - 1) / LP_JOIN;
-      set(a.stats, a.keys, area[from], room[from]);
-      set(a.stats_out, a.keys_out, area[1 - from], room[1 - from]);
-      log_probs_join_kernel<TY><<<dim3((unsigned)a.parts_out, n), dim3(64), 0, stream>>>(a);
+    const dim3 grid((unsigned)cut.parts, (unsigned)(rows - first < LP_ROWS ? rows - first : LP_ROWS));
+    if (cut.parts == 1) {
+      if (cut.small)
+        log_probs_part_kernel<TY, 1, true><<<grid, LP_THREADS, 0, stream>>>(a);
+      else
+        log_probs_part_kernel<TY, IT, true><<<grid, LP_THREADS, 0, stream>>>(a);
+    } else {
+      if (cut.small)
+        log_probs_part_kernel<TY, 1, false><<<grid, LP_THREADS, 0, stream>>>(a);
+      else
+        log_probs_part_kernel<TY, IT, false><<<grid, LP_THREADS, 0, stream>>>(a);
       FM_CHECK_HIP(hipGetLastError());
-      a.parts = a.parts_out;
-      from = 1 - from;
-    } while (a.parts > 1);
+      log_probs_join_kernel<TY><<<dim3(grid.y), LP_THREADS, 0, stream>>>(a);
+    }
+    FM_CHECK_HIP(hipGetLastError());
   }
   return FM_OK;
 }
@@ -247,8 +396,13 @@ using namespace fm;
 
 extern "C" size_t fm_log_probs_workspace_bytes(int64_t rows, int64_t vocab, int32_t top) {
   if (rows <= 0 || vocab <= 0 || vocab > INT32_MAX || top < 0 || top > LP_TOP) return 0;
-  const int64_t parts = lp_parts(vocab);
-  return lp_bytes(lp_rows(rows) * (parts + (parts + LP_JOIN - 1) / LP_JOIN), top);
+  size_t bytes = 16;  // either type's cut
+  for (int es = 2; es <= 4; es += 2) {
+    const LpCut cut(rows, vocab, es);
+    const size_t need = cut.parts == 1 ? 0 : lp_bytes(rows * cut.parts, top);
+    bytes = need > bytes ? need : bytes;
+  }
+  return bytes;
 }
 
 extern "C" int fm_log_probs_rows(const void *logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t row_stride,
