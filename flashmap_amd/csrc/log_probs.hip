@@ -7,16 +7,17 @@
 //
 // A row is cut into parts, one where there are rows for the whole chip, and a part is a workgroup's:
 // its lanes keep a maximum, S and D of their own, put in line with each new maximum, so that nothing is
-// joined before the part's end; the next 16 KB of logits travel meanwhile. Parts leave records, which a
+// joined before the part's end; the next tile's logits travel meanwhile. Parts leave records, which a
 // workgroup a row puts together the same way; a row of one part is done at once.
-//
+// 1024 rows of 151936 bf16 logits with a list of 8: 84 us (3.7 TB/s); without a list 67, with loads
+// alone 61: the exponentials and the list's tests (10 to 14 operations a logit) are nearly as long
+// as the loads, and only partly hidden by them.
 // The list: a logit and its index are one 64-bit key, whose order is the order of the list. A
 // wavefront meets its columns in rising order and keeps the keys that may be among its largest in LDS. A
 // tile whose maximum does not pass the last of them is left at once. Where many lanes pass (the first
 // tile), the k-th largest of the lanes' own largest keys, found a bit at a time by ballots, bounds the k-th
 // largest of all: about k keys of 2048 remain. They are put in order by counting: a key's place is the
-// number of keys above it. A list of any length up to 32 costs so little that it stays hidden behind
-// the loads; what costs is rising logits, whose tiles all pass.
+// number of keys above it. What costs most is rising logits, whose tiles all pass.
 #include <math.h>
 
 #include "fm_host.h"
@@ -29,7 +30,7 @@ constexpr int LP_TOP = 32;        // the longest list
 constexpr int LP_KEPT = 64;       // keys that a wavefront keeps before it puts them in order
 constexpr int LP_ROOM = LP_KEPT + 8 * 64;  // and those that one step may add
 constexpr int LP_GROUPS = 1024;   // workgroups that few rows are cut into: 4 a CU
-constexpr int LP_SMALL = 8 * LP_THREADS;   // logits of the smallest part
+constexpr int LP_SMALL = 8 * LP_THREADS, LP_WIDE = 2 * LP_SMALL;  // logits of a tile
 
 struct LogProbsArgs {
   const char *logits;
@@ -81,17 +82,25 @@ __device__ __forceinline__ float token_logit(const LogProbsArgs &a, int64_t row)
   return reinterpret_cast<const float *>(src)[t];
 }
 
-// The largest t that at least k lanes' v reach.
-__device__ __forceinline__ uint32_t kth_largest(uint32_t v, int k) {
+// The largest t below 2^bits that at least k lanes' v reach, two bits at a time.
+__device__ __forceinline__ uint32_t kth_largest(uint32_t v, int k, int bits) {
   uint32_t t = 0;
 #pragma nounroll
-  for (uint32_t bit = 1u << 31; bit != 0; bit >>= 1)
-    if (__popcll(__ballot(v >= (t | bit))) >= k) t |= bit;
+  for (int at = bits - 2; at >= 0; at -= 2) {
+    int more = 0;
+#pragma unroll
+    for (uint32_t q = 1; q < 4; ++q) more += __popcll(__ballot(v >= (t | q << at))) >= k;
+    t |= (uint32_t)more << at;
+  }
   return t;
 }
 
 // A wavefront's largest keys. Keys of no logit are 0 and never kept.
+template <int TY>
 struct LpList {
+  // Bits of logit_order() in which logits of the type differ, from the highest: below them negative
+  // ones have ones, the others zeros.
+  static constexpr int BITS = TY == LOGITS_F32 ? 32 : TY == LOGITS_BF16 ? 16 : 20;
   uint64_t *kept;      // LP_ROOM and then LP_TOP places in LDS
   int top, n;          // n: kept so far, uniform
   uint64_t least;      // keys up to this are not among the largest (0: nothing is known)
@@ -103,13 +112,16 @@ struct LpList {
     least = to;
     least_logit = logit_of((uint32_t)(to >> 32));
   }
-  // `mine`: a lane's largest key of those that are about to come.
-  __device__ __forceinline__ void bound(uint64_t mine) {
-    const uint32_t v = (uint32_t)(mine >> 32), t = kth_largest(v, top);
+  // `order`: of a lane's largest logit of those that are about to come; low(order): the low word of its
+  // largest key with that logit.
+  template <typename F>
+  __device__ __forceinline__ void bound(uint32_t order, const F &low) {
+    const uint32_t v = order >> (32 - BITS), t = kth_largest(v, top, BITS);
     if (t == 0) return;
-    uint64_t to = (uint64_t)t << 32;
+    uint64_t to = (uint64_t)t << (64 - BITS);
+    if (t >> (BITS - 1) == 0) to |= (uint64_t)((1ull << (32 - BITS)) - 1) << 32;
     if (__popcll(__ballot(v >= t)) > top)  // equals: by their columns
-      to |= kth_largest(v == t ? (uint32_t)mine : 0, top - __popcll(__ballot(v > t)));
+      to |= kth_largest(v == t ? low(order) : 0, top - __popcll(__ballot(v > t)), 32);
     raise(to - 1);
   }
   __device__ __forceinline__ void add(uint64_t key) {
@@ -166,7 +178,7 @@ struct LpShared {
 
 // The lanes' sums and the wavefronts' lists to one record, or to the row's results.
 template <int TY, bool RESULTS>
-__device__ __forceinline__ void finish(const LogProbsArgs &a, LpShared &lds, LpSums sums, LpList &list, int64_t row,
+__device__ __forceinline__ void finish(const LogProbsArgs &a, LpShared &lds, LpSums sums, LpList<TY> &list, float mine, int64_t row,
                                        int64_t record) {
   const int lane = threadIdx.x & 63, wave = wave_id();
   const float temp = a.temps == nullptr ? 1.f : a.temps[row], c = 1.f / temp * 1.44269504f;
@@ -190,7 +202,7 @@ __device__ __forceinline__ void finish(const LogProbsArgs &a, LpShared &lds, LpS
       a.entropy[row] = log_s - all.d / (temp * all.s);
       if (a.tokens != nullptr) {
         const int64_t t = a.tokens[row];
-        a.token[row] = (token_logit<TY>(a, row) - all.m) / temp - log_s;
+        a.token[row] = (mine - all.m) / temp - log_s;
         a.rank[row] = t < 0 || t >= a.vocab ? 0 : (int64_t)all.above + 1;
       }
     }
@@ -199,6 +211,7 @@ __device__ __forceinline__ void finish(const LogProbsArgs &a, LpShared &lds, LpS
   // A key's place among all wavefronts' lists; those of no logit last, in any order of their own.
   const uint64_t key = lds.keys[wave][lane];
   int place = 0;
+#pragma unroll 4
   for (int i = 0; i < a.top; ++i)
 #pragma unroll
     for (int w = 0; w < LP_WAVES; ++w) {
@@ -216,7 +229,7 @@ __device__ __forceinline__ void finish(const LogProbsArgs &a, LpShared &lds, LpS
 
 // Part blockIdx.x of row blockIdx.y, tiles of IT chunks of 8 logits a thread.
 template <int TY, int IT, bool RESULTS>
-__global__ __launch_bounds__(LP_THREADS) void log_probs_part_kernel(const LogProbsArgs a) {
+__global__ __launch_bounds__(LP_THREADS, 4) void log_probs_part_kernel(const LogProbsArgs a) {
   __shared__ LpShared lds;
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int64_t row = a.first_row + blockIdx.y;
@@ -228,7 +241,7 @@ __global__ __launch_bounds__(LP_THREADS) void log_probs_part_kernel(const LogPro
   const float mine = token_logit<TY>(a, row);
   const float c = a.temps == nullptr ? 1.44269504f : 1.f / a.temps[row] * 1.44269504f;
   LpSums sums{-INFINITY, 0.f, 0.f, 0};
-  LpList list;
+  LpList<TY> list;
   list.start(lds.keys[wave], a.top);
   int32_t above = 0;  // of the wavefront
 #pragma nounroll
@@ -246,16 +259,19 @@ __global__ __launch_bounds__(LP_THREADS) void log_probs_part_kernel(const LogPro
 #pragma unroll
       for (int it = 0; it < IT; ++it) view.trim(x[it], g0 + it * LP_THREADS + threadIdx.x);
     }
-    float m = -INFINITY;
+    float m = -INFINITY, chunk[IT];
 #pragma unroll
-    for (int it = 0; it < IT; ++it)
+    for (int it = 0; it < IT; ++it) {
+      chunk[it] = x[it].at(0);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = fmaxf(m, x[it].at(j));
+      for (int j = 1; j < 8; ++j) chunk[it] = fmaxf(chunk[it], x[it].at(j));
+      m = fmaxf(m, chunk[it]);
+    }
     if (__ballot(m > sums.m) != 0) sums.line(fmaxf(m, sums.m), c);
     const float from = sums.m == -INFINITY ? 0.f : sums.m;
     float s[2] = {sums.s, 0.f}, d[2] = {sums.d, 0.f};
 #pragma unroll
-    for (int it = 0; it < IT; ++it)
+    for (int it = 0; it < IT; ++it) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float v = x[it].at(j), off = v - from;
@@ -263,8 +279,9 @@ __global__ __launch_bounds__(LP_THREADS) void log_probs_part_kernel(const LogPro
         s[j & 1] += e;
         d[j & 1] = __builtin_fmaf(fmaxf(off, -3e38f), e, d[j & 1]);  // -inf stands for 0 here
       }
+    }
     sums.s = s[0] + s[1], sums.d = d[0] + d[1];
-    if (a.tokens != nullptr) {
+    if (__ballot(m > mine) != 0) {  // without a token it is NaN
 #pragma unroll
       for (int it = 0; it < IT; ++it) {
         x[it].forget();
@@ -273,38 +290,46 @@ __global__ __launch_bounds__(LP_THREADS) void log_probs_part_kernel(const LogPro
       }
     }
     // All columns kept lie before this tile's: an equal logit comes behind them.
-    const uint64_t passed = a.top == 0 ? 0 : __ballot(!(m <= list.least_logit) || sums.s != sums.s);
+    const bool none = sums.s != sums.s;  // there may be NaNs, which no maximum shows
+    const uint64_t passed = a.top == 0 ? 0 : __ballot(!(m <= list.least_logit) || none);
     if (passed == 0) continue;
-    auto column = [&](int it, int j) { return 8 * (g0 + it * LP_THREADS + threadIdx.x) - view.skip + j; };
-    auto key_at = [&](int it, int j) {
-      const uint32_t col = column(it, j);
-      return col < view.vocab ? logit_key(x[it].at(j), col) : 0;
+    // Columns are worked out anew where they are asked for: kept, they would take 32 registers.
+    auto column = [&](int it) {
+      uint32_t col = 8 * (g0 + it * LP_THREADS + threadIdx.x) - view.skip;
+      asm volatile("" : "+v"(col));
+      return col;
+    };
+    auto key_at = [&](int it, int j, uint32_t col) {
+      return col + j < view.vocab ? logit_key(x[it].at(j), col + j) : 0;
     };
     if (__popcll(passed) > 16) {  // each lane that passes adds a key or more: worth a bound
-      uint64_t largest = 0;
+      list.bound(logit_order(m), [&](uint32_t order) {  // rare: from memory again, or it takes 60 registers
+        uint32_t low = 0;
+#pragma nounroll
+        for (int it = 0; it < IT; ++it) {
+          const Chunk<TY> again = view.chunk(g0 + it * LP_THREADS + threadIdx.x);
+          const uint32_t col = column(it);
 #pragma unroll
-      for (int it = 0; it < IT; ++it) {
-        x[it].forget();
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint64_t key = key_at(it, j);
-          largest = key > largest ? key : largest;
+          for (int j = 0; j < 8; ++j)
+            if (col + j < view.vocab && logit_order(again.at(j)) == order && ~(col + j) > low) low = ~(col + j);
         }
-      }
-      list.bound(largest);
+        return low;
+      });
     }
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
+      if (__ballot(!(chunk[it] < list.least_logit) || none) == 0) continue;
       x[it].forget();
+      const uint32_t col = column(it);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (__ballot(!(x[it].at(j) < list.least_logit)) != 0) list.add(key_at(it, j));
+        if (__ballot(!(x[it].at(j) < list.least_logit)) != 0) list.add(key_at(it, j, col));
       if (list.n > LP_KEPT) list.order(lane);
     }
     if (list.least == 0 || list.n > 2 * a.top) list.order(lane);
   }
   sums.above = lane == 0 ? above : 0;
-  finish<TY, RESULTS>(a, lds, sums, list, row, (int64_t)blockIdx.y * a.parts + blockIdx.x);
+  finish<TY, RESULTS>(a, lds, sums, list, mine, row, (int64_t)blockIdx.y * a.parts + blockIdx.x);
 }
 
 // The records of row blockIdx.x.
@@ -313,9 +338,10 @@ __global__ __launch_bounds__(LP_THREADS) void log_probs_join_kernel(const LogPro
   __shared__ LpShared lds;
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int64_t row = a.first_row + blockIdx.x, record = (int64_t)blockIdx.x * a.parts;
+  const float mine = threadIdx.x == 0 ? token_logit<TY>(a, row) : 0.f;
   const float c = a.temps == nullptr ? 1.44269504f : 1.f / a.temps[row] * 1.44269504f;
   LpSums sums{-INFINITY, 0.f, 0.f, 0};
-  LpList list;
+  LpList<TY> list;
   list.start(lds.keys[wave], a.top);
   for (int32_t r = threadIdx.x; r < a.parts; r += LP_THREADS) {
     const float4 v = a.stats[record + r];
@@ -332,26 +358,27 @@ __global__ __launch_bounds__(LP_THREADS) void log_probs_join_kernel(const LogPro
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) largest = key[j] > largest ? key[j] : largest;
-    list.bound(largest);
+    list.bound((uint32_t)(largest >> 32), [&](uint32_t) { return (uint32_t)largest; });
 #pragma unroll
     for (int j = 0; j < 8; ++j) list.add(key[j]);
     if (list.n > LP_KEPT) list.order(lane);
   }
-  finish<TY, true>(a, lds, sums, list, row, 0);
+  finish<TY, true>(a, lds, sums, list, mine, row, 0);
 }
 
-// How a call is cut: rows for 4 workgroups a CU are a part each, fewer are cut into parts for as
-// many, of whole tiles; where those would be less than one of 16 KB, tiles are 8 logits a thread (one row
-// of 151936 bf16 logits: ? us in 75 parts, ? in 19).
+// How a call is cut: rows for 4 workgroups a CU are a part each, fewer are cut into parts for as many,
+// of whole tiles: with parts for 6 or 8 a CU, 1024 rows of 151936 bf16 logits take 100 or 156 us instead of
+// 84, with tiles twice as long 84. Where there are fewer tiles than that, they are halved (one such row: 75
+// parts of 2048 logits).
 struct LpCut {
   int64_t parts;
   int32_t tiles;
   bool small;
-  LpCut(int64_t rows, int64_t vocab, int es) {
-    const int64_t wide = LP_SMALL * 8 / es, n = vocab + 7;  // rows may start inside a granule
+  LpCut(int64_t rows, int64_t vocab) {
+    const int64_t n = vocab + 7;  // rows may start inside a granule
     const int64_t most = rows >= LP_GROUPS ? 1 : (LP_GROUPS + rows - 1) / rows;
-    small = (n + wide - 1) / wide < most;
-    const int64_t tile = small ? LP_SMALL : wide, all = (n + tile - 1) / tile;
+    small = (n + LP_WIDE - 1) / LP_WIDE < most;
+    const int64_t tile = small ? LP_SMALL : LP_WIDE, all = (n + tile - 1) / tile;
     tiles = (int32_t)((all + most - 1) / most);
     parts = (all + tiles - 1) / tiles;
   }
@@ -364,8 +391,8 @@ static size_t lp_bytes(int64_t records, int64_t top) { return (size_t)records * 
 
 template <int TY>
 static int run_log_probs(LogProbsArgs a, int64_t rows, char *ws, hipStream_t stream) {
-  constexpr int IT = TY == LOGITS_F32 ? 2 : 4;
-  const LpCut cut(rows, a.vocab, TY == LOGITS_F32 ? 4 : 2);
+  constexpr int IT = LP_WIDE / LP_SMALL;
+  const LpCut cut(rows, a.vocab);
   a.parts = (int32_t)cut.parts, a.tiles = cut.tiles;
   a.stats = (float4 *)ws;
   a.keys = (uint64_t *)(a.stats + rows * cut.parts);
@@ -396,13 +423,8 @@ using namespace fm;
 
 extern "C" size_t fm_log_probs_workspace_bytes(int64_t rows, int64_t vocab, int32_t top) {
   if (rows <= 0 || vocab <= 0 || vocab > INT32_MAX || top < 0 || top > LP_TOP) return 0;
-  size_t bytes = 16;  // either type's cut
-  for (int es = 2; es <= 4; es += 2) {
-    const LpCut cut(rows, vocab, es);
-    const size_t need = cut.parts == 1 ? 0 : lp_bytes(rows * cut.parts, top);
-    bytes = need > bytes ? need : bytes;
-  }
-  return bytes;
+  const LpCut cut(rows, vocab);
+  return cut.parts == 1 ? 16 : lp_bytes(rows * cut.parts, top);
 }
 
 extern "C" int fm_log_probs_rows(const void *logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t row_stride,
