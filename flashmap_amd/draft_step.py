@@ -187,11 +187,16 @@ class DraftStep:
     # -- the context -----------------------------------------------------------------
 
     @staticmethod
-    def cache_layout(caches: list[torch.Tensor]):
-        """``(base addresses (layers,) int64 on the device, (block, head, token, value)
+    def cache_layout(caches: "list[torch.Tensor] | list[ops.MX]"):
+        """What the writer takes for ``caches``: per-layer caches in microscaled 4 bits (``ops.mx_cache``)
+        themselves, else ``(base addresses (layers,) int64 on the device, (block, head, token, value)
         strides, page size)`` of per-layer vLLM caches ``(blocks, heads, page, 2D)``
         (flashmap/vllm/model.py:707-733)."""
         c0 = caches[0]
+        if isinstance(c0, ops.MX):
+            if not all(isinstance(c, ops.MX) for c in caches):
+                raise TypeError("the layers' caches must all be microscaled, or none")
+            return list(caches)
         if any(c.shape != c0.shape or c.stride() != c0.stride() or c.dtype != torch.bfloat16 for c in caches):
             raise ValueError("the layers' caches must be bf16 and share one shape and strides")
         bases = torch.tensor([c.data_ptr() for c in caches], dtype=torch.int64, device=c0.device)
@@ -203,9 +208,12 @@ class DraftStep:
         weights are) for every layer: one GEMM over the layers' K/V weights and one writer launch
         (flashmap/vllm/model.py:735-777)."""
         kv = F.linear(rows, self.context_kv_weight) if self.mx_layers is None else product(rows, self.context_kv_weight)
+        kv = kv.view(rows.shape[0], len(self.model.layers), 2, self.heads, self.head_dim)
+        if isinstance(layout, list):
+            ops.write_context_kv_mx(kv, positions, slots, self.context_k_norm, self.rope, layout, self.k_eps)
+            return
         bases, strides, page = layout
-        ops.write_context_kv(kv.view(rows.shape[0], len(self.model.layers), 2, self.heads, self.head_dim),
-                             positions, slots, self.context_k_norm, self.rope, bases, strides, page, self.k_eps)
+        ops.write_context_kv(kv, positions, slots, self.context_k_norm, self.rope, bases, strides, page, self.k_eps)
 
     @torch.no_grad()
     def write_context(self, states: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, layout) -> None:
@@ -222,14 +230,15 @@ class DraftStep:
 
     @torch.no_grad()
     def __call__(self, anchors: torch.Tensor, anchor_positions: torch.Tensor, anchor_slots: torch.Tensor,
-                 z: torch.Tensor, caches: list[torch.Tensor], block_table: torch.Tensor, layout=None,
+                 z: torch.Tensor, caches: "list[torch.Tensor] | list[ops.MX]", block_table: torch.Tensor, layout=None,
                  plan: torch.Tensor | None = None) -> torch.Tensor:
         """One draft for ``B`` requests: writes each anchor's context row at its position /
         slot, then returns the final AdaLN output ``(B * block_size, dim)`` of the last
         jump for the block rows at positions ``anchor + 1 ..`` attending to positions ``0 ..
         anchor``. ``z (B * block_size, noise_columns)`` float32 is the starting noise: in
         the folded space for one jump, the vocabulary-sized state for several
-        (flashmap/vllm/model.py:1016-1038)."""
+        (flashmap/vllm/model.py:1016-1038). ``caches``, one per layer: bf16, or in microscaled 4 bits
+        (``ops.mx_cache``), whose attention takes no ``plan``."""
         model = self.model
         batch, k = anchors.shape[0], self.block
         if z.shape != (batch * k, self.noise_columns) or z.dtype != torch.float32:
@@ -244,7 +253,7 @@ class DraftStep:
             anchor_rows = ops.rms_norm_mx(anchor_rows, model.anchor_norm.weight, model.anchor_norm.eps)[1]
         self.write_rows(anchor_rows, anchor_positions, anchor_slots, layout)
         seqused_k = (anchor_positions + 1).to(torch.int32)
-        if plan is None:
+        if plan is None and not isinstance(layout, list):
             plan = ops.attention_plan(seqused_k)
         attend = (caches, block_table, seqused_k, plan,
                   (anchor_positions[:, None] + 1 + torch.arange(k, device=anchors.device)).reshape(-1),
@@ -319,8 +328,12 @@ class DraftStep:
             hidden, h = self._norm(i)(hidden, y, g_self, (c_scale, c_shift), layer.cross_attn_adaln.eps, x_out=hidden)
             query = product(h, held.cross_q if held else layer.cross_attn.q_proj.weight).view(tokens, heads, hd)
             prologue = ops.Prologue(cross_qn, self.rope, slot_positions, layer.cross_attn.q_norm.eps)
-            ctx = ops.block_attention_paged(query, caches[i], cu, seqused_k, block_table, k, self.max_model_len,
-                                            self.scale, prologue=prologue, plan=plan)
+            if isinstance(caches[i], ops.MX):
+                ctx = ops.block_attention_paged_mx(query, caches[i], cu, seqused_k, block_table, k, self.max_model_len,
+                                                   self.scale, prologue=prologue)
+            else:
+                ctx = ops.block_attention_paged(query, caches[i], cu, seqused_k, block_table, k, self.max_model_len,
+                                                self.scale, prologue=prologue, plan=plan)
             y = product(ctx.view(tokens, self.dim), held.cross_o if held else layer.cross_attn.o_proj.weight)
             hidden, h = self._norm(i)(hidden, y, g_cross, (m_scale, m_shift), layer.mlp_adaln.eps, x_out=hidden)
             y = held.mlp(h) if held else layer.mlp(h)

@@ -1798,8 +1798,8 @@ def _mx_cache_args(cache: MX, dims: int, name: str) -> tuple[int, int, int, int]
                          f"head_dim 64 or 128; got {tuple(shape)}")
     d, rows = shape[-1] // 2, math.prod(shape[:-1])
     if codes.shape != (rows, d) or scales.shape != (rows, d // 16):
-        raise ValueError(f"{name} of shape {tuple(shape)} holds codes ({rows}, {d}) and scales ({rows}, {d // 16}); got "
-                         f"{tuple(codes.shape)} and {tuple(scales.shape)}")
+        raise ValueError(f"{name} of shape {tuple(shape)} holds codes ({rows}, {d}) and scales ({rows}, {d // 16}); "
+                         f"got {tuple(codes.shape)} and {tuple(scales.shape)}")
     cs, ss = codes.stride(0) if rows > 1 else d, scales.stride(0) if rows > 1 else d // 16
     if (codes.stride(1) != 1 or scales.stride(1) != 1 or cs < d or ss < d // 16 or cs % 16 or ss % 4
             or codes.data_ptr() % 16 or scales.data_ptr() % 4):

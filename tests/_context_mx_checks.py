@@ -2,8 +2,10 @@
 
 A row's bound, with ``A = sum p |v| / sum p`` of the float64 result ``o``:
 
-- the output's rounding to bf16, 2^-8 of ``o``;
-- the probabilities' rounding to bf16, 2^-8 of ``A``;
+- the output's rounding to bf16, 2^-8 of ``|o|``;
+- the probabilities cut to bf16: ``p (1 - 2^-8 + x)`` with ``|x| <= 2^-8``, and the sum of what was cut in
+  the quotient: the common factor leaves it, ``x`` moves it by 2^-8 of ``sum p |v - o| / sum p <= A + |o|``;
+- the query, scaled, as the sum of two e4m3 operands of 4 bits each: 2^-8 of each of its channels at most;
 - a score off by ``e`` moves its probability by ``exp(e) - 1`` and the sum by as much: ``2 (exp(e) - 1)`` of
   ``A``. The matrix instruction cuts the products of a group of 8 below 2^-13 of the power of two of the
   group's largest: 7 2^-13 < 2^-10 of the group's absolute sum, and its float32 sums 2^-15 of it; the
@@ -50,9 +52,10 @@ def make(lens, hkv, d, page, seed, device, spread=1.0, shuffle=True):
     return cache, table.to(device), rows
 
 
-def check(out: torch.Tensor, query: torch.Tensor, rows, lens_q, scale: float, bits: float = 0.0) -> None:
+def check(out: torch.Tensor, query: torch.Tensor, rows, lens_q, scale: float, bits: float = 2.0 ** -8) -> None:
     """``out`` and ``query (tokens, hq, d)`` (what attends: normed and rotated) against float64.
-    ``bits``: what the query's channels may be off by, relative to them."""
+    ``bits``: what the query's channels may be off by, relative to them: the kernel's rounding, and more
+    where they were rounded on their way here."""
     hq, d = query.shape[1:]
     out, query, at = out.cpu().double(), query.cpu().double(), 0
     for b, n in enumerate(lens_q):
@@ -69,7 +72,7 @@ def check(out: torch.Tensor, query: torch.Tensor, rows, lens_q, scale: float, bi
         p = torch.softmax(s, -1)
         want = torch.einsum("qhk,khd->qhd", p, v)
         total = torch.einsum("qhk,khd->qhd", p, v.abs())
-        tol = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2 * torch.expm1(off)[..., None] + 2.0 ** -12) * total
+        tol = 2.0 ** -7 * want.abs() + (2.0 ** -8 + 2 * torch.expm1(off)[..., None] + 2.0 ** -12) * total
         bad = ~((got - want).abs() <= tol)
         worst = ((got - want).abs() / total).max()
         assert not bad.any(), (f"request {b} ({kv.shape[0]} positions): {int(bad.sum())} of {bad.numel()} off, by up "

@@ -219,8 +219,8 @@ def test_entries_refuse():
 
     def attend(q=x, q_tokens=8, qst=256, qsh=64, rs=64, ss=4, blocks=4, page=8, width=4, batch=2, q_len=4, max_k=32,
                hq=4, hkv=2, d=64, scale=0.1, norm=None, table=None, ws=x, ws_bytes=1 << 40, cu=None):
-        return lib.fm_block_attn_paged_mx(q, q_tokens, qst, qsh, x, 256, 64, cu, x, rs, x, ss, blocks, page, x, 4, width,
-                                          x, batch, q_len, max_k, hq, hkv, d, f(scale), norm, table, table, 64, 1, 8,
+        return lib.fm_block_attn_paged_mx(q, q_tokens, qst, qsh, x, 256, 64, cu, x, rs, x, ss, blocks, page, x, 4,
+                                          width, x, batch, q_len, max_k, hq, hkv, d, f(scale), norm, table, table, 64, 1, 8,
                                           None, f(1e-6), ws, ws_bytes, None)
 
     assert attend(batch=0) == n.FM_OK and attend(q_len=0) == n.FM_OK
@@ -256,15 +256,16 @@ def test_entries_refuse():
     assert judge(logits=ctypes.c_void_p(257)) == n.FM_ERR_INVALID and "aligned" in _err()
     assert judge(ws=ctypes.c_void_p(8)) == n.FM_ERR_INVALID and "16 bytes" in _err()
     assert judge(out=None) == n.FM_ERR_INVALID and judge(ws=None) == n.FM_ERR_INVALID
-    assert judge(ws_bytes=16) == n.FM_ERR_WORKSPACE
+    assert judge(vocab=10_000, stride=10_000, ws_bytes=16) == n.FM_ERR_WORKSPACE
 
 
 def test_workspace_sizes():
     lib = _native.lib()
     assert lib.fm_log_probs_workspace_bytes(0, 100, 4) == 0 and lib.fm_log_probs_workspace_bytes(3, 100, 33) == 0
     small, large = (lib.fm_log_probs_workspace_bytes(r, 151936, 20) for r in (1, 32))
-    assert 0 < small and large == 32 * small
-    # rows are taken in parts: the workspace stops growing with them
-    assert lib.fm_log_probs_workspace_bytes(1 << 20, 1000, 1) == lib.fm_log_probs_workspace_bytes(1 << 21, 1000, 1)
+    assert 75 * (16 + 8 * 20) == small < large
+    # rows that fill the chip are a part each and leave no records
+    for rows, vocab in ((1 << 20, 1000), (1024, 151936)):
+        assert lib.fm_log_probs_workspace_bytes(rows, vocab, 32) == 16
     assert lib.fm_block_attn_paged_mx_workspace_bytes(0, 4, 2, 64) == 0
     assert lib.fm_block_attn_paged_mx_workspace_bytes(1 << 30, 4, 2, 64) == 0

@@ -268,7 +268,8 @@ def _written(kv, positions, weight, table, eps):
 
 
 @pytest.mark.parametrize("tokens,layers,heads,d,page", [(1, 1, 1, 128, 1), (1, 6, 16, 128, 16), (33, 2, 5, 64, 8),
-                                                        (200, 3, 4, 128, 24), (7, 40, 1, 64, 16), (513, 1, 20, 128, 16)])
+                                                        (200, 3, 4, 128, 24), (7, 40, 1, 64, 16),
+                                                        (513, 1, 20, 128, 16)])
 def test_append(dev, tokens, layers, heads, d, page):
     g = torch.Generator().manual_seed(30)
     kv = (torch.randn(tokens, layers, 2, heads, d, generator=g) * torch.exp(torch.randn(d, generator=g))).to(BF)

@@ -3,8 +3,10 @@
 Bounds, in nats of float32 half steps u = 2^-24. A log probability is (x - m) / T - log S: the difference
 and the quotient 2 u of |x - m| / T, the subtraction u of the result. S: each exponential's argument is off by
 3 u of |x - m| / T (the difference, 1 / T, the product), where it matters at most by 3 u 20 (below exp(-20) of
-the maximum the terms of 2^18 logits are under 2^-10 of it together, times 3 u 100), the exponential and the
-sums 2 u + 40 u (32 in a thread, 8 and 6 to join), so that log S is off by about 110 u; its own rounding u of it.
+the maximum the terms of 2^18 logits are under 2^-10 of it together, times 3 u 100), the exponential 2 u, the
+joining of lanes, wavefronts and parts 40 u, so that log S is off by about 110 u; a lane's sums in between by u for
+each of up to vocab / 512 additions in a row and by 3 u for each of up to vocab / 4096 tiles with a new maximum (the
+exponential and the product); its own rounding u of it.
 """
 
 import pytest
@@ -23,7 +25,8 @@ def _check(logits, tokens, top, temps, got: ops.LogProbs) -> None:
     m = x.amax(-1, keepdim=True)
     lp = torch.log_softmax(x / t[:, None], -1)
     d = ((x - m) / t[:, None]).abs()
-    tol = 3 * U * d + 110 * U + 2 * U * lp.abs()
+    sums = 110 + vocab / 512 + 3 * vocab / 4096
+    tol = 3 * U * d + sums * U + 2 * U * lp.abs()
 
     def near(a, want, tol):
         a = a.cpu().double()
@@ -41,8 +44,8 @@ def _check(logits, tokens, top, temps, got: ops.LogProbs) -> None:
     else:
         assert got.token is None and got.rank is None
     entropy = torch.where(m[:, 0].isfinite() & ~x.isnan().any(-1), torch.special.entr(lp.exp()).sum(-1), float("nan"))
-    # log S, and D / S: its terms (x - m) / T off by 3 u of them, as S by 110 u
-    near(got.entropy, entropy, 230 * U * (1 + (lp.exp() * d.nan_to_num(0, 0, 0)).sum(-1)))
+    # log S, and D / S: its terms (x - m) / T off by 3 u of them, as S
+    near(got.entropy, entropy, (10 + 2 * sums) * U * (1 + (lp.exp() * d.nan_to_num(0, 0, 0)).sum(-1)))
     assert got.top_ids.shape == got.top.shape == (rows, top)
     if top:
         order = torch.sort(torch.where(x.isnan(), float("inf"), x), dim=-1, descending=True, stable=True)
@@ -109,7 +112,8 @@ def test_masked(dev, dtype, left):
         _check(y, k, 20, None, ops.log_probs_rows(y, k, 20))
 
 
-@pytest.mark.parametrize("value", [0.0, -3.5, float("-inf"), torch.finfo(torch.bfloat16).min, torch.finfo(torch.bfloat16).max])
+@pytest.mark.parametrize("value", [0.0, -3.5, float("-inf"), torch.finfo(torch.bfloat16).min,
+                                   torch.finfo(torch.bfloat16).max])
 def test_equal(dev, value):
     """Rows of one value: the lowest indexes; of -inf: NaN."""
     x = torch.full((3, 20_000), value, dtype=torch.bfloat16, device=dev)
@@ -177,3 +181,24 @@ def test_sampled_tokens(dev):
     _check(x, tokens, 4, temps, got)
     assert (got.rank[greedy] == 1).all() and torch.equal(got.top_ids[greedy, 0], tokens[greedy])
     assert torch.equal(got.top_ids[:, 0], ops.argmax_rows(x))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,vocab", [(1, 20_000), (9, 70_001), (1100, 9_000)])
+@pytest.mark.parametrize("kind", ["rising", "falling", "two", "late", "lowest", "nan"])
+def test_orders(dev, dtype, rows, vocab, kind):
+    """Rows whose lists change with every tile, or in the last one alone; many equals; whole tiles of -inf or
+    of the type's lowest value; NaN in one tile."""
+    x, tokens = _logits(rows, vocab, dtype, 12)
+    if kind in ("rising", "falling"):
+        x = x.sort(-1, descending=kind == "falling").values
+    elif kind == "two":
+        x = torch.where(x > 0, 1.0, -1.0).to(dtype)
+    elif kind == "nan":
+        x[::3, vocab // 2] = float("nan")
+    else:
+        x[:, :vocab - 37] = torch.finfo(dtype).min if kind == "lowest" else float("-inf")
+        tokens = vocab - 1 - tokens % 37
+    x, tokens = x.to(dev), tokens.to(dev)
+    for top in (1, 8, 32):
+        _check(x, tokens, top, None, ops.log_probs_rows(x, tokens, top))
