@@ -15,16 +15,29 @@
 //
 // Scores: K on the block-scaled matrix instruction as it is stored, against the query as a sum of
 // two e4m3 operands, hi = e4m3(q / 2^e) and lo = e4m3((q - hi 2^e) / 2^(e - 5)): 4 + 4 significant
-// bits, all 8 of a bf16 (2^e puts a block's largest magnitude to [128, 256); a value below 2^-13 of
-// that loses at most 2^-22 of it). The query's norm and rotation, where they go with the call, are
-// float32 and rounded only there, by at most 2^-8. K needs no conversion and no register but the 16 bytes a
+// bits (2^e puts a block's largest magnitude to [128, 256); a value below 2^-13 of that loses at most 2^-22
+// of it). The query is scaled by log2(e) softmax_scale in float32, behind its norm and rotation where
+// they go with the call, and rounded only there, by at most 2^-8: as many bits as bf16 has. K needs no
+// conversion and no register but the 16 bytes a
 // lane that it comes in. S^T = K Q^T leaves a query row's scores in the lanes that take that row's
 // probabilities in O^T = V^T P^T: nothing crosses lanes.
 // Values: each lane widens 8 tokens' dwords (8 channels each) with their block's scale, exactly, to
-// bf16 pairs, and pairs of tokens by byte permutes. Probabilities are rounded to bf16 (2^-9 of each, as
-// the bf16 attention does); maxima, sums and outputs are float32.
+// bf16 pairs, and pairs of tokens by byte permutes. Probabilities are rounded to bf16 (2^-8 of each at
+// most, as the bf16 attention does) and summed as they were rounded; maxima, sums and outputs are float32.
 // A row's maximum is a reference that moves only when a score passes it by 2^8: the sums stay far
-// inside float32 and bf16 keeps its 8 bits wherever its exponent is.
+// inside float32 and bf16 keeps its 8 bits wherever its exponent is. A tile's scores start from less
+// their rows' references, so that a probability is one exponential, and one test of the tile's
+// exponents finds those that passed.
+//
+// What bounds it: with 16 rows a head the cache's bytes (8 contexts of 131072 positions, 16 query rows on
+// each of 8 heads: 222 us, 5.1 TB/s, what a copy reaches); with 64 rows a head matrix and vector instructions
+// and the loads take equal times that overlap only in part (the same contexts 332 us: 239 for the loads
+// alone, 265 for the instructions alone). Row blocks of a unit share its loads and the widening of its
+// values, so a unit takes up to four: as two units of two, the second reads everything again (420 us).
+// One or two leave registers for three workgroups a CU (5 ragged requests 26 -> 22 us with the third), three or
+// four for two, with a tile more in each ring and the queries' operands in LDS.
+// Nothing among the tiles may be loaded through registers: a wait for it would wait for the whole
+// ring (8 contexts of 32768 positions: 100 us, 108 with one such wait).
 #include <math.h>
 
 #include <type_traits>
@@ -678,7 +691,7 @@ __global__ __launch_bounds__(64 * MXA_WAVES, (MxGeo<D, RB>::RESIDENT)) void attn
             for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f(s[j >> 2][j & 3]);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              p[rb][c] = both_hi(__float_as_uint(e[2 * c]), __float_as_uint(e[2 * c + 1]));
+              p[rb][c] = pack_bf16x2(e[2 * c], e[2 * c + 1]);
               any |= p[rb][c];
             }
             if constexpr (!QR)  // two row blocks' scores at a time: registers

@@ -1883,9 +1883,9 @@ def block_attention_paged_mx(
     """:func:`block_attention_paged` onto a cache in microscaled 4 bits (:func:`mx_cache`,
     ``(num_blocks, Hkv, page, 2D)``; pages of one position make ``block_table`` a table of positions):
     ``query (tokens, Hq, D)`` bf16, each request reading its first ``seqused_k[b]`` positions (at most
-    ``max_seqlen_k``), zeros for a request of none. The cache's values enter exactly, the query with its
-    8 bits (a prologue's norm and rotation are float32 in front of that one rounding), scores and sums
-    are float32, probabilities are rounded to bf16. ``out`` (bf16, may be ``query``) receives the
+    ``max_seqlen_k``), zeros for a request of none. The cache's values enter exactly, the query, behind a
+    float32 prologue and times the scale, rounded once by at most 2^-8; scores and sums are float32,
+    probabilities are rounded to bf16. ``out`` (bf16, may be ``query``) receives the
     result; its rows behind the last request are left alone. The context is cut over the chip by
     lengths read on the device: a row's result may differ in its last place between calls of other
     batches."""
