@@ -1029,7 +1029,10 @@ extern "C" int fm_block_attn_paged_mx(
     return fail(FM_ERR_UNSUPPORTED, "head_dim %d not supported (64 or 128)", head_dim);
   FM_REQUIRE(num_kv_heads > 0 && num_q_heads > 0 && num_q_heads % num_kv_heads == 0,
              "%d query heads do not divide into %d KV heads", num_q_heads, num_kv_heads);
-  FM_REQUIRE(q && out && codes && scales && block_table && seqused_k && workspace, "NULL pointer");
+  // Where no context has a position the table is not read, and an empty one may have no address.
+  FM_REQUIRE(q && out && codes && scales && seqused_k && workspace &&
+                 (block_table || block_table_width == 0 || max_seqlen_k == 0),
+             "NULL pointer");
   FM_REQUIRE(((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 15) == 0 && ((uintptr_t)codes & 15) == 0 &&
                  ((uintptr_t)scales & 3) == 0 && ((uintptr_t)workspace & 15) == 0,
              "q, out, codes and workspace must be 16-byte aligned, scales 4-byte aligned");
@@ -1092,7 +1095,7 @@ extern "C" int fm_block_attn_paged_mx(
     a.batch = batch - b0 < MXA_BATCH ? batch - b0 : MXA_BATCH;
     a.cu_q = cu_seqlens_q == nullptr ? nullptr : cu_seqlens_q + b0;
     a.token0 = (int64_t)b0 * max_seqlen_q;
-    a.table = block_table + b0 * block_table_stride;
+    a.table = block_table == nullptr ? nullptr : block_table + b0 * block_table_stride;
     a.lens = seqused_k + b0;
     const int rc = head_dim == 128 ? run_attn_mx<128>(a, rb, (hipStream_t)stream) : run_attn_mx<64>(a, rb, (hipStream_t)stream);
     if (rc != FM_OK) return rc;

@@ -1,0 +1,28 @@
+"""The ends of what 4-bit contexts and log probabilities take, without a GPU: calls that the C entries and the
+wrappers let through to the launch, and those that they refuse."""
+
+import ctypes
+
+import pytest
+import torch
+
+from flashmap_amd import _native, ops
+
+BF = torch.bfloat16
+X = ctypes.c_void_p(256)
+
+
+def _attend(table=X, width=4, max_k=32, q_len=4, batch=2, q_tokens=1 << 40, hq=4, hkv=2, d=64, blocks=4, page=8,
+            ws_bytes=64):
+    """The entry on addresses that nothing reads: a workspace of 64 bytes is the last thing that it refuses."""
+    return _native.lib().fm_block_attn_paged_mx(
+        X, q_tokens, hq * d, d, X, hq * d, d, None, X, d, X, d // 16, blocks, page, table, width, width, X, batch, q_len,
+        max_k, hq, hkv, d, ctypes.c_float(0.1), None, None, None, 0, 0, 0, None, ctypes.c_float(1e-6), X, ws_bytes, None)
+
+
+def test_table_without_columns():
+    """A batch of empty contexts may come with a table of no columns, whose tensor has no address."""
+    assert _attend() == _native.FM_ERR_WORKSPACE
+    assert _attend(table=None) == _native.FM_ERR_INVALID and "NULL" in _native.last_error()
+    assert _attend(table=None, width=0) == _native.FM_ERR_WORKSPACE
+    assert _attend(table=None, max_k=0) == _native.FM_ERR_WORKSPACE
