@@ -51,6 +51,7 @@ constexpr int MXA_WAVES = 4;
 constexpr int MXA_TILE = 32;                     // positions of a wavefront's tile
 constexpr int MXA_STEP = MXA_WAVES * MXA_TILE;   // of a workgroup's step
 constexpr int MXA_BATCH = 256;                   // sequences of one launch: their steps lie in LDS
+constexpr int MXA_GROUPS = 256;                  // row groups of one launch: their parts lie in the workspace
 constexpr int MXA_UNIT_COST = 6;                 // steps that a unit's start and end cost
 constexpr float MXA_SLACK = 8.f;                 // log2 that scores may pass their row's reference by
 
@@ -61,7 +62,8 @@ struct MxAttnArgs {
   int64_t o_st, o_sh;
   const int32_t *cu_q;  // NULL: sequence b's tokens start at token0 + b q_len
   int64_t token0, q_tokens;  // q_tokens: rows of q and out; what cu_q says past them is left alone
-  int32_t q_len, group, hkv, rgroups;
+  int32_t q_len, group, hkv;
+  int32_t rgroup0, rgroups;  // row groups of this launch: the first and how many
   uint32_t q_mul, q_shift;  // n / q_len, as n / page below
   const uint8_t *codes, *scales;
   uint32_t cs16, ss4;  // row strides in 16 and in 4 bytes (the last row's offsets in them below 2^32)
@@ -424,7 +426,7 @@ __global__ __launch_bounds__(64 * MXA_WAVES, (MxGeo<D, RB>::RESIDENT)) void attn
       from = uniform(line.cu[c.b]);
       tokens = tokens_in(a, from, uniform(line.cu[c.b + 1]));
     }
-    const int32_t r = (rg * RB + rb) * 16 + n;
+    const int32_t r = ((a.rgroup0 + rg) * RB + rb) * 16 + n;
     head = divided(r, a.q_mul, a.q_shift);
     const int32_t tok = r - head * a.q_len;
     return r < rows && tok < tokens ? from + tok : -1;
@@ -871,7 +873,7 @@ __global__ __launch_bounds__(64 * MXA_WAVES) void attn_mx_join_kernel(const MxAt
   }
   // This thread: channels (4 g + i) NF + quarter FW + f of row n.
   const int n = lane & 15, g = lane >> 4, quarter = SPLIT ? (int)blockIdx.z : wave;
-  const int32_t r = block * 16 + n, head = divided(r, a.q_mul, a.q_shift), tok = r - head * a.q_len;
+  const int32_t r = (a.rgroup0 * rb_unit + block) * 16 + n, head = divided(r, a.q_mul, a.q_shift), tok = r - head * a.q_len;
   const bool live = r < a.group * a.q_len && tok < tokens && (!SPLIT || wave == 0);
   f32x4_t v[FW];
 #pragma unroll
@@ -956,12 +958,20 @@ __global__ __launch_bounds__(64 * MXA_WAVES) void attn_mx_join_kernel(const MxAt
   store();
 }
 
-// Row blocks of a unit: up to 4, all units alike where the rows fill more than one.
-static int unit_blocks(int32_t rows, int32_t *rgroups) {
-  const int32_t blocks = (rows + 15) / 16;
-  *rgroups = (blocks + 3) / 4;
-  return (blocks + *rgroups - 1) / *rgroups;
-}
+constexpr int64_t MXA_ROWS = 1 << 20;  // query rows of a KV head
+
+// How a KV head's query rows are cut: row blocks of a unit (up to 4, all units alike where the rows fill more
+// than one), the row groups that they make, and those of one launch (even slices of at most MXA_GROUPS).
+struct MxRows {
+  int32_t rb, rgroups, slice;
+  explicit MxRows(int64_t rows) {
+    const int32_t blocks = (int32_t)((rows + 15) / 16);
+    rgroups = (blocks + 3) / 4;
+    rb = (blocks + rgroups - 1) / rgroups;
+    const int32_t launches = (rgroups + MXA_GROUPS - 1) / MXA_GROUPS;
+    slice = (rgroups + launches - 1) / launches;
+  }
+};
 
 // Shares of a row group: as many workgroups as the chip holds at once, by eights (a share an XCD).
 static int32_t mx_attn_shares(int rb, int32_t rgroups) {
@@ -1007,10 +1017,9 @@ extern "C" size_t fm_block_attn_paged_mx_workspace_bytes(int32_t max_seqlen_q, i
                                                          int32_t num_kv_heads, int32_t head_dim) {
   if (max_seqlen_q <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads || head_dim <= 0) return 0;
   const int64_t rows = (int64_t)(num_q_heads / num_kv_heads) * max_seqlen_q;
-  if (rows > (1 << 20)) return 0;
-  int32_t rgroups;
-  const int rb = unit_blocks((int32_t)rows, &rgroups);
-  return sizeof(float) * mx_attn_part_floats(rb, rgroups, head_dim);
+  if (rows > MXA_ROWS) return 0;
+  const MxRows cut(rows);
+  return sizeof(float) * mx_attn_part_floats(cut.rb, cut.slice, head_dim);
 }
 
 extern "C" int fm_block_attn_paged_mx(
@@ -1055,10 +1064,11 @@ extern "C" int fm_block_attn_paged_mx(
              "without cu_seqlens_q the query holds batch x max_seqlen_q = %lld rows, got %lld",
              (long long)batch * max_seqlen_q, (long long)q_tokens);
   const int64_t rows = (int64_t)(num_q_heads / num_kv_heads) * max_seqlen_q;
-  FM_REQUIRE(rows <= (1 << 20), "at most 2^20 query rows for a KV head, got %lld", (long long)rows);
+  FM_REQUIRE(rows <= MXA_ROWS, "at most 2^20 query rows for a KV head, got %lld", (long long)rows);
   MxAttnArgs a{};
-  const int rb = unit_blocks((int32_t)rows, &a.rgroups);
-  FM_REQUIRE((int64_t)MXA_BATCH * num_kv_heads < (1ll << 31) && a.rgroups * rb < 65536, "too many units");
+  const MxRows cut(rows);
+  const int64_t units = (int64_t)(batch < MXA_BATCH ? batch : MXA_BATCH) * num_kv_heads;  // of a launch and row group
+  FM_REQUIRE(units < (1 << 24), "%lld KV heads of a launch's sequences, at most 2^24 - 1", (long long)units);
   a.q_tokens = q_tokens;
   a.q = (const uint16_t *)q, a.q_st = q_stride_token, a.q_sh = q_stride_head;
   a.o = (uint16_t *)out, a.o_st = out_stride_token, a.o_sh = out_stride_head;
@@ -1084,21 +1094,27 @@ extern "C" int fm_block_attn_paged_mx(
   a.qn_w = q_norm_weight;
   a.rope = Rope{rope_cos, rope_sin, rope_row_stride, rope_pair_stride, rope_rows};
   a.q_pos = q_positions, a.eps = eps;
-  a.shares = mx_attn_shares(rb, a.rgroups);
+  a.shares = mx_attn_shares(cut.rb, cut.slice);
+  // A share's steps are counted in 32 bits.
+  FM_REQUIRE(units * ((most + MXA_STEP - 1) / MXA_STEP) / a.shares < INT32_MAX, "too many positions for one launch");
   a.per_share = 1.0 / a.shares;
-  const size_t need = sizeof(float) * mx_attn_part_floats(rb, a.rgroups, head_dim);
+  const size_t need = sizeof(float) * mx_attn_part_floats(cut.rb, cut.slice, head_dim);
   if (workspace_bytes < need) return fail(FM_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
   a.part_o = (float *)workspace;
-  a.part_ml = a.part_o + (size_t)2 * a.shares * a.rgroups * 16 * rb * head_dim;
-  // Launches of up to MXA_BATCH sequences, one after another: they share the workspace.
+  a.part_ml = a.part_o + (size_t)2 * a.shares * cut.slice * 16 * cut.rb * head_dim;
+  // Launches of up to MXA_BATCH sequences and MXA_GROUPS row groups, one after another: they share the workspace.
   for (int32_t b0 = 0; b0 < batch; b0 += MXA_BATCH) {
     a.batch = batch - b0 < MXA_BATCH ? batch - b0 : MXA_BATCH;
     a.cu_q = cu_seqlens_q == nullptr ? nullptr : cu_seqlens_q + b0;
     a.token0 = (int64_t)b0 * max_seqlen_q;
     a.table = block_table == nullptr ? nullptr : block_table + b0 * block_table_stride;
     a.lens = seqused_k + b0;
-    const int rc = head_dim == 128 ? run_attn_mx<128>(a, rb, (hipStream_t)stream) : run_attn_mx<64>(a, rb, (hipStream_t)stream);
-    if (rc != FM_OK) return rc;
+    for (a.rgroup0 = 0; a.rgroup0 < cut.rgroups; a.rgroup0 += cut.slice) {
+      a.rgroups = cut.rgroups - a.rgroup0 < cut.slice ? cut.rgroups - a.rgroup0 : cut.slice;
+      const int rc = head_dim == 128 ? run_attn_mx<128>(a, cut.rb, (hipStream_t)stream)
+                                     : run_attn_mx<64>(a, cut.rb, (hipStream_t)stream);
+      if (rc != FM_OK) return rc;
+    }
   }
   return FM_OK;
 }

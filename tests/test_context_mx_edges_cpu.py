@@ -26,3 +26,24 @@ def test_table_without_columns():
     assert _attend(table=None) == _native.FM_ERR_INVALID and "NULL" in _native.last_error()
     assert _attend(table=None, width=0) == _native.FM_ERR_WORKSPACE
     assert _attend(table=None, max_k=0) == _native.FM_ERR_WORKSPACE
+
+
+def test_query_rows():
+    """2^20 query rows a KV head are taken, for a workspace that does not grow with them; more are refused."""
+    size = _native.lib().fm_block_attn_paged_mx_workspace_bytes
+    for rows in (1 << 20, (1 << 20) - 1, (1 << 20) - 63, 1_048_513, 1_048_512):
+        assert _attend(q_len=rows, hq=2, hkv=2) == _native.FM_ERR_WORKSPACE
+        assert 0 < size(rows, 2, 2, 128) < 150_000_000
+    assert _attend(q_len=1 << 19, hq=4, hkv=2) == _native.FM_ERR_WORKSPACE
+    assert _attend(q_len=(1 << 20) + 1, hq=2, hkv=2) == _native.FM_ERR_INVALID and "2^20" in _native.last_error()
+    assert size((1 << 20) + 1, 2, 2, 128) == 0
+
+
+def test_units():
+    """What one launch counts in 32 bits: KV heads of its sequences, and a share's steps."""
+    many = dict(batch=256, blocks=1, page=1, width=1)
+    assert _attend(hq=65535, hkv=65535, **many) == _native.FM_ERR_WORKSPACE
+    assert _attend(hq=65536, hkv=65536, **many) == _native.FM_ERR_INVALID and "2^24" in _native.last_error()
+    long = dict(batch=256, blocks=1, page=256, width=1 << 16, max_k=1 << 24, q_len=1 << 14)
+    assert _attend(hq=500, hkv=500, **long) == _native.FM_ERR_WORKSPACE
+    assert _attend(hq=5000, hkv=5000, **long) == _native.FM_ERR_INVALID and "positions" in _native.last_error()
