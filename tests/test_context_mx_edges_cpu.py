@@ -33,7 +33,7 @@ def test_query_rows():
     size = _native.lib().fm_block_attn_paged_mx_workspace_bytes
     for rows in (1 << 20, (1 << 20) - 1, (1 << 20) - 63, 1_048_513, 1_048_512):
         assert _attend(q_len=rows, hq=2, hkv=2) == _native.FM_ERR_WORKSPACE
-        assert 0 < size(rows, 2, 2, 128) < 150_000_000
+        assert 0 < size(rows, 2, 2, 128) < 600_000_000
     assert _attend(q_len=1 << 19, hq=4, hkv=2) == _native.FM_ERR_WORKSPACE
     assert _attend(q_len=(1 << 20) + 1, hq=2, hkv=2) == _native.FM_ERR_INVALID and "2^20" in _native.last_error()
     assert size((1 << 20) + 1, 2, 2, 128) == 0

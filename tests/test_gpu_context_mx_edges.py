@@ -38,14 +38,14 @@ def test_most_query_rows(dev, rows):
 
 def test_sliced_requests(dev):
     """Several heads a KV head and ragged requests, their rows more than one launch takes; the query as out."""
-    lens, lens_q = [300, 0, 41], [20000, 7, 12345]
+    lens, lens_q = [300, 0, 41], [40000, 7, 12345]
     cache, table, held = make(lens, 2, 128, 16, 4, dev)
     query = torch.randn(sum(lens_q), 4, 128, generator=torch.Generator(dev).manual_seed(5), device=dev).to(BF)
-    cu = torch.tensor([0, 20000, 20007, 32352], dtype=torch.int32, device=dev)
+    cu = torch.tensor([0, 40000, 40007, 52352], dtype=torch.int32, device=dev)
     seq = torch.tensor(lens, dtype=torch.int32, device=dev)
-    want = ops.block_attention_paged_mx(query, cache, cu, seq, table, 20000, 300, 0.1)
-    some = [0, 1, 8191, 8192, 16383, 16384, 19999]
-    at = torch.tensor(some + [20000, 20006] + [20007 + t for t in (0, 4096, 12344)], device=dev)
+    want = ops.block_attention_paged_mx(query, cache, cu, seq, table, 40000, 300, 0.1)
+    some = [0, 1, 16383, 16384, 25535, 25536, 39999]
+    at = torch.tensor(some + [40000, 40006] + [40007 + t for t in (0, 4096, 12344)], device=dev)
     check(want[at], query[at], held, [7, 2, 3], 0.1)
     same = query.clone()
-    assert torch.equal(ops.block_attention_paged_mx(same, cache, cu, seq, table, 20000, 300, 0.1, out=same), want)
+    assert torch.equal(ops.block_attention_paged_mx(same, cache, cu, seq, table, 40000, 300, 0.1, out=same), want)
