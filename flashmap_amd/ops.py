@@ -1419,6 +1419,12 @@ class MX:
         at = slice(index % self.shape[0] * rows, (index % self.shape[0] + 1) * rows)
         return MX(self.codes[at], self.scales[at], self.bits, tuple(self.shape[1:]))
 
+    def __iter__(self):
+        """The parts of the leading dimension; rows of two dimensions have none."""
+        if len(self.shape) < 3:
+            raise TypeError(f"microscaled rows of shape {self.shape} have no parts to iterate over")
+        return (self[i] for i in range(self.shape[0]))
+
     def to(self, *args, **kwargs) -> "MX":
         """On another device (``Tensor.to`` of the codes and the scales)."""
         codes, scales = self.codes.to(*args, **kwargs), self.scales.to(*args, **kwargs)

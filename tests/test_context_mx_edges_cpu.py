@@ -47,3 +47,15 @@ def test_units():
     long = dict(batch=256, blocks=1, page=256, width=1 << 16, max_k=1 << 24, q_len=1 << 14)
     assert _attend(hq=500, hkv=500, **long) == _native.FM_ERR_WORKSPACE
     assert _attend(hq=5000, hkv=5000, **long) == _native.FM_ERR_INVALID and "positions" in _native.last_error()
+
+
+def test_parts():
+    """Microscaled rows of two dimensions have no parts; those of more have their leading dimension's."""
+    cache = ops.mx_cache(3, 2, 4, 64, "cpu", layers=2)
+    parts = list(cache)
+    assert [p.shape for p in parts] == [(3, 2, 4, 128)] * 2
+    assert [p.codes.data_ptr() for p in parts] == [cache[0].codes.data_ptr(), cache[1].codes.data_ptr()]
+    rows = ops.MX(cache.codes, cache.scales, 4, (48, 128))
+    for use in (list, iter, lambda q: print(*q), lambda q: 1 in q):
+        with pytest.raises(TypeError):
+            use(rows)
