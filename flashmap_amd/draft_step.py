@@ -192,9 +192,9 @@ class DraftStep:
         themselves, else ``(base addresses (layers,) int64 on the device, (block, head, token, value)
         strides, page size)`` of per-layer vLLM caches ``(blocks, heads, page, 2D)``
         (flashmap/vllm/model.py:707-733)."""
-        c0 = caches[0]
-        if isinstance(c0, ops.MX):
-            if not all(isinstance(c, ops.MX) for c in caches):
+        c0, held = caches[0], [isinstance(c, ops.MX) for c in caches]
+        if any(held):
+            if not all(held):
                 raise TypeError("the layers' caches must all be microscaled, or none")
             return list(caches)
         if any(c.shape != c0.shape or c.stride() != c0.stride() or c.dtype != torch.bfloat16 for c in caches):

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from flashmap_amd import _native, ops
+from flashmap_amd.draft_step import DraftStep
 
 BF = torch.bfloat16
 X = ctypes.c_void_p(256)
@@ -59,3 +60,14 @@ def test_parts():
     for use in (list, iter, lambda q: print(*q), lambda q: 1 in q):
         with pytest.raises(TypeError):
             use(rows)
+
+
+def test_mixed_caches():
+    """A draft step's caches are all in 4 bits or none, whichever comes first."""
+    cache, plain = ops.mx_cache(2, 2, 16, 128, "cpu"), torch.zeros(2, 2, 16, 256, dtype=BF)
+    for caches in ([cache, plain], [plain, cache], [plain, plain, cache]):
+        with pytest.raises(TypeError, match="all be microscaled"):
+            DraftStep.cache_layout(caches)
+    assert DraftStep.cache_layout([cache, cache]) == [cache, cache]
+    joined = ops.mx_cache(2, 2, 16, 128, "cpu", layers=3)
+    assert [c.shape for c in DraftStep.cache_layout(joined)] == [(2, 2, 16, 256)] * 3
