@@ -71,6 +71,10 @@ __device__ __forceinline__ T wave_sum(T v) {
   return v;
 }
 
+// log2(e) / T, inside float32 where T is so small (below 5e-39) that it is not: the largest logit's
+// exponent is 0 then too, and of any other one the exponential is 0 either way.
+__device__ __forceinline__ float exponent_factor(float temp) { return fminf(1.f / temp * 1.44269504f, 3e38f); }
+
 // The logit of the row's token (NaN: the token is none).
 template <int TY>
 __device__ __forceinline__ float token_logit(const LogProbsArgs &a, int64_t row) {
@@ -181,7 +185,7 @@ template <int TY, bool RESULTS>
 __device__ __forceinline__ void finish(const LogProbsArgs &a, LpShared &lds, LpSums sums, LpList<TY> &list, float mine, int64_t row,
                                        int64_t record) {
   const int lane = threadIdx.x & 63, wave = wave_id();
-  const float temp = a.temps == nullptr ? 1.f : a.temps[row], c = 1.f / temp * 1.44269504f;
+  const float temp = a.temps == nullptr ? 1.f : a.temps[row], c = exponent_factor(temp);
   sums.line(wave_max(sums.m), c);
   const float s = wave_sum(sums.s), d = wave_sum(sums.d);
   const int32_t above = wave_sum(sums.above);
@@ -239,7 +243,7 @@ __global__ __launch_bounds__(LP_THREADS, 4) void log_probs_part_kernel(const Log
 #pragma unroll
   for (int it = 0; it < IT; ++it) next[it] = view.chunk(first + it * LP_THREADS + threadIdx.x);
   const float mine = token_logit<TY>(a, row);
-  const float c = a.temps == nullptr ? 1.44269504f : 1.f / a.temps[row] * 1.44269504f;
+  const float c = a.temps == nullptr ? 1.44269504f : exponent_factor(a.temps[row]);
   LpSums sums{-INFINITY, 0.f, 0.f, 0};
   LpList<TY> list;
   list.start(lds.keys[wave], a.top);
@@ -339,7 +343,7 @@ __global__ __launch_bounds__(LP_THREADS) void log_probs_join_kernel(const LogPro
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int64_t row = a.first_row + blockIdx.x, record = (int64_t)blockIdx.x * a.parts;
   const float mine = threadIdx.x == 0 ? token_logit<TY>(a, row) : 0.f;
-  const float c = a.temps == nullptr ? 1.44269504f : 1.f / a.temps[row] * 1.44269504f;
+  const float c = a.temps == nullptr ? 1.44269504f : exponent_factor(a.temps[row]);
   LpSums sums{-INFINITY, 0.f, 0.f, 0};
   LpList<TY> list;
   list.start(lds.keys[wave], a.top);
