@@ -1138,8 +1138,9 @@ def log_probs_rows(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
     larger logits), the entropy ``-sum p log p`` in nats, and the ``top`` (at most 32) likeliest tokens
     with their log probabilities, in falling order, the lower index first among equals, a NaN before
     any number. ``temperatures (rows,)`` must be positive (None: 1). A token outside the
-    vocabulary (padding) has NaN and rank 0; a row with a NaN or an infinite logit, or of -inf alone,
-    has NaN for every probability. No gradient."""
+    vocabulary (padding) has NaN and rank 0; a logit of -inf (a masked one) has the log probability -inf;
+    a row with a NaN or +inf, or of -inf alone, has NaN for every probability, and a token whose own
+    logit is NaN rank 1. No gradient."""
     _check_cuda(logits, tokens, temperatures)
     _no_gradient("log_probs_rows", logits, temperatures)
     logits = _logits(logits)

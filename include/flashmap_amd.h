@@ -586,9 +586,9 @@ int fm_block_attn_paged_mx(const void *q, int64_t q_tokens, int64_t q_stride_tok
  *   entropy[r] = -sum p log p,
  *   top_ids, top_log_probs (rows, top): the `top` largest logits in falling order, the lower
  *   index first among equals, a NaN before any number (top at most 32 and the vocabulary).
- * A row with a NaN or +infinity, or of -infinity alone, has NaN for every probability. No
- * reference counterpart (its servers take log probabilities from the engine). Workspace (16-byte
- * aligned): fm_log_probs_workspace_bytes(rows, vocab, top) bytes.
+ * A row with a NaN or +infinity, or of -infinity alone, has NaN for every probability, and a token
+ * whose own logit is NaN rank 1. No reference counterpart (its servers take log probabilities from the
+ * engine). Workspace (16-byte aligned): fm_log_probs_workspace_bytes(rows, vocab, top) bytes.
  */
 size_t fm_log_probs_workspace_bytes(int64_t rows, int64_t vocab, int32_t top);
 int fm_log_probs_rows(const void *logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t row_stride,

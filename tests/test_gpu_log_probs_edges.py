@@ -41,3 +41,21 @@ def test_hot(dev, rows, vocab, temp):
     x[:, 1::2] = float("-inf")
     x, k, temps = x.to(dev), k.to(dev), torch.full((rows,), temp, device=dev)
     _check(x, k, 3, temps, ops.log_probs_rows(x, k, 3, temps))
+
+
+@pytest.mark.parametrize("rows,vocab", [(4, 9000), (1100, 500)])
+def test_infinite_and_nan_tokens(dev, rows, vocab):
+    """-inf is a probability of 0 and leaves the row's others alone; a NaN is the first of its row."""
+    x, _ = _logits(rows, vocab, torch.bfloat16, 22)
+    x[0, 7] = float("-inf")
+    x[1, 7] = float("nan")
+    x[2, 7] = float("inf")
+    k = torch.full((rows,), 7, device=dev)
+    x = x.to(dev)
+    got = ops.log_probs_rows(x, k, 4)
+    _check(x, k, 4, None, got)
+    assert got.token[0] == float("-inf") and got.rank[0] == vocab and got.top[0].isfinite().all()
+    assert got.entropy[0].isfinite()
+    assert got.token[1].isnan() and got.token[2].isnan() and got.rank[1:3].tolist() == [1, 1]
+    assert got.top[1:3].isnan().all() and got.top_ids[1, 0] == 7 and got.top_ids[2, 0] == 7
+    assert got.top[3:].isfinite().all()
