@@ -1855,6 +1855,8 @@ def write_context_kv_mx(
                          f"{tuple(slots.shape)}")
     if tokens == 0:
         return
+    if len({(a[0], a[2]) for a in args}) < len(args):
+        raise ValueError("the layers' caches must be different ones")
     if joined:
         rows = blocks * heads * page
         at = [(args[0][0] + i * rows * cs, args[0][2] + i * rows * ss) for i in range(layers)]

@@ -71,3 +71,25 @@ def test_mixed_caches():
     assert DraftStep.cache_layout([cache, cache]) == [cache, cache]
     joined = ops.mx_cache(2, 2, 16, 128, "cpu", layers=3)
     assert [c.shape for c in DraftStep.cache_layout(joined)] == [(2, 2, 16, 256)] * 3
+
+
+@pytest.fixture
+def launched(monkeypatch):
+    """The wrappers' own checks on CPU tensors: the names of the entries that a call would have launched."""
+    names = []
+    monkeypatch.setattr(ops, "_check_cuda", lambda *t: torch.device("cpu"))
+    monkeypatch.setattr(ops, "_mx_call", lambda name, *a: names.append(name))
+    monkeypatch.setattr(ops, "_attn_mx_workspace_bytes", lambda *a: 64)
+    return names
+
+
+def test_one_cache_for_two_layers(launched):
+    kv, idx = torch.zeros(2, 2, 2, 2, 64, dtype=BF), torch.zeros(2, dtype=torch.int64)
+    caches = [ops.mx_cache(4, 2, 8, 64, "cpu") for _ in range(2)]
+    rope = ops.rope_from_table(torch.zeros(8, 32, 2))
+    with pytest.raises(ValueError, match="different"):
+        ops.write_context_kv_mx(kv, idx, idx, torch.ones(2, 64), rope, [caches[0], caches[0]], 1e-6)
+    assert launched == []
+    ops.write_context_kv_mx(kv, idx, idx, torch.ones(2, 64), rope, caches, 1e-6)
+    ops.write_context_kv_mx(kv, idx, idx, torch.ones(2, 64), rope, ops.mx_cache(4, 2, 8, 64, "cpu", 2), 1e-6)
+    assert launched == ["fm_write_context_kv_mx"] * 2
