@@ -1894,8 +1894,8 @@ def block_attention_paged_mx(
     ``query (tokens, Hq, D)`` bf16, each request reading its first ``seqused_k[b]`` positions (at most
     ``max_seqlen_k``), zeros for a request of none. The cache's values enter exactly, the query, behind a
     float32 prologue and times the scale, rounded once by at most 2^-8; scores and sums are float32,
-    probabilities are rounded to bf16. ``out`` (bf16, may be ``query``) receives the
-    result; its rows behind the last request are left alone. The context is cut over the chip by
+    probabilities are rounded to bf16. ``out`` (bf16; it may be ``query``, and may not overlap it or anything
+    else that the call reads) receives the result; its rows behind the last request are left alone. The context is cut over the chip by
     lengths read on the device: a row's result may differ in its last place between calls of other
     batches."""
     index = _mx_device(query, cache.codes, cache.scales, cu_seqlens_q, seqused_k, block_table, out)
@@ -1929,11 +1929,18 @@ def block_attention_paged_mx(
         if (out.stride(2) != 1 or out.data_ptr() % 16 or out.stride(0) % 8 or out.stride(1) % 8 or out.stride(1) < d
                 or (tokens > 1 and out.stride(0) < (hq - 1) * out.stride(1) + d)):
             raise ValueError("out must hold 16-byte aligned heads of unit channel stride that do not overlap")
-        same = out.data_ptr() == query.data_ptr() and out.stride() == query.stride()
-        if not same and tokens and _meet(out, query):
-            raise ValueError("out overlaps the query (it may be the query itself)")
-        if tokens and (_meet(out, cache.codes) or _meet(out, cache.scales)):
-            raise ValueError("out overlaps the cache")
+        if tokens:
+            span = _span(out)
+            same = out.data_ptr() == query.data_ptr() and out.stride() == query.stride()
+            if not same and _meet(span, query) and _heads_meet(out, query):
+                raise ValueError("out overlaps the query (it may be the query itself)")
+            if _meet(span, cache.codes) or _meet(span, cache.scales):
+                raise ValueError("out overlaps the cache")
+            read = [cu_seqlens_q, seqused_k, block_table]
+            if prologue is not None:
+                read += [prologue.weight, *prologue.rope.keep, prologue.positions]
+            if any(t is not None and t.numel() and _meet(span, t) for t in read):
+                raise ValueError("out overlaps what the call reads")
     if batch == 0 or tokens == 0 or max_seqlen_q == 0:
         return out
     pro = _prologue_args(prologue, tokens, d)
@@ -1949,13 +1956,33 @@ def block_attention_paged_mx(
     return out
 
 
-def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the address ranges of two tensors (not empty) meet."""
-    def span(t):
-        first = t.data_ptr()
-        return first, first + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """The addresses from a tensor's (not empty) first byte to behind its last."""
+    first, size = t.data_ptr(), t.element_size()
+    if t.is_contiguous():
+        return first, first + t.numel() * size
+    return first, first + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * size
+
+
+def _meet(span: tuple[int, int], t: torch.Tensor) -> bool:
+    """Whether the addresses of ``t`` (not empty) meet a span."""
+    first, end = _span(t)
+    return span[0] < end and first < span[1]
+
+
+def _heads_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors ``(tokens, heads, D)`` of one shape whose addresses meet share an element; those of
+    different strides are taken to."""
+    tokens, heads, d = a.shape
+    by, step = a.stride()[:2]
+    if b.stride() != a.stride() or by == 0 or a.dtype != b.dtype:
+        return True
+    apart = (b.data_ptr() - a.data_ptr()) / a.element_size()
+    for h in range(1 - heads, heads):  # a head of a and one of b, h heads on, the nearest tokens
+        t = min(max(round((apart + h * step) / by), 1 - tokens), tokens - 1)
+        if abs(apart + h * step - t * by) < d:
+            return True
+    return False
 
 
 def noise_rows(z: torch.Tensor, eigvals: torch.Tensor, eps: float, gain: float,

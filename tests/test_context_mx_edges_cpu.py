@@ -93,3 +93,47 @@ def test_one_cache_for_two_layers(launched):
     ops.write_context_kv_mx(kv, idx, idx, torch.ones(2, 64), rope, caches, 1e-6)
     ops.write_context_kv_mx(kv, idx, idx, torch.ones(2, 64), rope, ops.mx_cache(4, 2, 8, 64, "cpu", 2), 1e-6)
     assert launched == ["fm_write_context_kv_mx"] * 2
+
+
+def test_out_beside_and_over_operands(launched):
+    """An output between the query's own values is taken; one over anything that the call reads is refused."""
+    cache, wide = ops.mx_cache(4, 2, 8, 64, "cpu"), torch.zeros(6, 4, 160, dtype=BF)
+    lens, table = torch.tensor([8, 8], dtype=torch.int32), torch.zeros(2, 4, dtype=torch.int32)
+    cu, query = torch.tensor([0, 3, 6], dtype=torch.int32), torch.zeros(6, 4, 64, dtype=BF)
+    rope, weight = ops.rope_from_table(torch.zeros(8, 32, 2)), torch.ones(64)
+
+    def attend(query=query, cache=cache, cu=cu, lens=lens, table=table, pro=None, **more):
+        return ops.block_attention_paged_mx(query, cache, cu, lens, table, 3, 32, 0.1, prologue=pro, **more)
+
+    for q, out in ((wide[:, :, :64], wide[:, :, 64:128]), (wide[:, :, 64:128], wide[:, :, :64]),
+                   (wide[:, :2, :64], wide[:, 2:, :64]), (wide[:3, :, 64:128], wide[3:, :, 64:128]),
+                   (wide[1:, :, 64:128], wide[:5, :, :64])):
+        n = q.shape[0]
+        own = torch.tensor([0, n // 2, n], dtype=torch.int32)
+        assert attend(query=q, cu=own, out=out) is out
+    assert launched == ["fm_block_attn_paged_mx"] * 5
+    for q, out in ((wide[:, :, :64], wide[:, :, 32:96]), (wide[:, :, 32:96], wide[:, :, :64]),
+                   (wide[:5, :, :64], wide[1:, :, :64]), (wide[:, :2, :64], wide[:, 1:3, :64]),
+                   (wide[:3, :2, :64], wide[1:4, 1:3, 32:96])):
+        with pytest.raises(ValueError, match="overlaps the query"):
+            attend(query=q, cu=None, lens=lens[:1], table=table[:1], out=out)
+
+    # `size` values of out's memory as an operand
+    memory = torch.zeros(6 * 4 * 64, dtype=BF)
+    out = memory.view(6, 4, 64)
+
+    def held(dtype, *shape):
+        size = torch.Size(shape).numel() * dtype.itemsize // 2
+        return memory[64:64 + size].view(dtype).view(shape)
+
+    for more in (dict(cu=held(torch.int32, 3)), dict(lens=held(torch.int32, 2)), dict(lens=held(torch.int64, 2)),
+                 dict(table=held(torch.int32, 2, 4)), dict(pro=ops.Prologue(held(torch.float32, 64), rope, None, 1e-6)),
+                 dict(pro=ops.Prologue(weight, ops.rope_from_table(held(torch.float32, 8, 32, 2)), None, 1e-6)),
+                 dict(pro=ops.Prologue(weight, ops.rope_from_split(torch.zeros(8, 32), held(torch.float32, 8, 32)), None,
+                                       1e-6)),
+                 dict(pro=ops.Prologue(weight, rope, held(torch.int64, 6), 1e-6))):
+        with pytest.raises(ValueError, match="overlaps what the call reads"):
+            attend(out=out, **more)
+    with pytest.raises(ValueError, match="overlaps the cache"):
+        attend(cache=ops.MX(cache.codes, held(torch.uint8, 64, 4), 4, cache.shape), out=out)
+    assert attend(query=out, out=out) is out and attend(out=out) is out
