@@ -160,6 +160,8 @@ def rope_from_split(cos: torch.Tensor, sin: torch.Tensor) -> Rope:
     if cos.shape != sin.shape or cos.dim() == 0:
         raise ValueError(f"cos and sin tables must share one shape (..., head_dim/2), got "
                          f"{tuple(cos.shape)} and {tuple(sin.shape)}")
+    if cos.device != sin.device:
+        raise ValueError(f"cos and sin tables on different devices: {cos.device} and {sin.device}")
     cos, sin = _f32(cos), _f32(sin)
     half = cos.shape[-1]
     return Rope(cos, sin.data_ptr(), half, 1, cos.numel() // half if half else 0, half, (cos, sin))

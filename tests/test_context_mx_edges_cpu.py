@@ -137,3 +137,8 @@ def test_out_beside_and_over_operands(launched):
     with pytest.raises(ValueError, match="overlaps the cache"):
         attend(cache=ops.MX(cache.codes, held(torch.uint8, 64, 4), 4, cache.shape), out=out)
     assert attend(query=out, out=out) is out and attend(out=out) is out
+
+
+def test_rotary_halves_on_one_device():
+    with pytest.raises(ValueError, match="device"):
+        ops.rope_from_split(torch.zeros(8, 32), torch.zeros(8, 32, device="meta"))
