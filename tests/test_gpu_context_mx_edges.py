@@ -49,3 +49,14 @@ def test_sliced_requests(dev):
     check(want[at], query[at], held, [7, 2, 3], 0.1)
     same = query.clone()
     assert torch.equal(ops.block_attention_paged_mx(same, cache, cu, seq, table, 40000, 300, 0.1, out=same), want)
+
+
+def test_out_between_the_querys_values(dev):
+    lens = [200, 90]
+    cache, table, _ = make(lens, 2, 128, 16, 22, dev)
+    wide = torch.randn(10, 4, 264, device=dev).to(BF)
+    query, out, seq = wide[:, :, :128], wide[:, :, 136:], torch.tensor(lens, device=dev)
+    before = wide[:, :, :136].clone()
+    want = ops.block_attention_paged_mx(query.contiguous(), cache, None, seq, table, 5, 200, 0.1)
+    ops.block_attention_paged_mx(query, cache, None, seq, table, 5, 200, 0.1, out=out)
+    assert torch.equal(out, want) and torch.equal(wide[:, :, :136], before)
