@@ -59,3 +59,59 @@ def test_infinite_and_nan_tokens(dev, rows, vocab):
     assert got.token[1].isnan() and got.token[2].isnan() and got.rank[1:3].tolist() == [1, 1]
     assert got.top[1:3].isnan().all() and got.top_ids[1, 0] == 7 and got.top_ids[2, 0] == 7
     assert got.top[3:].isfinite().all()
+
+
+# Rows cut into parts of several tiles: wide tiles of 4096 logits (the first four), small ones of 2048. Where rows are
+# fewer than 1024, 1024 / rows parts a row at most; wide where a row has at least as many wide tiles.
+CUTS = [(61, 128_257), (200, 50_257), (700, 9_000), (600, 40_000), (64, 60_000), (128, 28_000), (33, 120_001)]
+
+
+def _tiles(rows, vocab):
+    """(logits of a tile, tiles of a part) as the documents of the cut have it."""
+    most = -(-1024 // rows)
+    tile = 2048 if -(-(vocab + 7) // 4096) < most else 4096
+    return tile, -(-(-(-(vocab + 7) // tile)) // most)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,vocab", CUTS)
+def test_parts_of_tiles(dev, dtype, rows, vocab):
+    tile, tiles = _tiles(rows, vocab)
+    assert tiles > 1 and tile == (2048 if (rows, vocab) in CUTS[4:] else 4096)
+    # 11 columns aside, at every alignment of a row's start
+    x, k = _logits(rows, vocab + 11, dtype, 23)
+    x, k = x.to(dev), (k % vocab).to(dev)
+    temps = torch.linspace(0.4, 1.7, rows, device=dev)
+    for at, top, t in ((0, 20, None), (3, 32, temps), (11, 0, temps), (8, 1, None)):
+        y = x[:, at:at + vocab]
+        _check(y, k, top, t, ops.log_probs_rows(y, k, top, t))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,vocab", [(61, 128_257), (700, 9_000), (64, 60_000)])
+@pytest.mark.parametrize("kind", ["rising", "falling", "equal", "ties", "ends", "late", "lowest", "nan", "first part"])
+def test_parts_in_order(dev, dtype, rows, vocab, kind):
+    """What the lists and sums carry from tile to tile, and what parts that hold nothing leave."""
+    tile, tiles = _tiles(rows, vocab)
+    x, k = _logits(rows, vocab, dtype, 24)
+    edges = [c + o for c in range(tile, vocab, tile) for o in (-1, 0)]  # the ends of tiles (aligned rows) and parts
+    if kind in ("rising", "falling"):
+        x = x.sort(-1, descending=kind == "falling").values
+    elif kind == "equal":
+        x = torch.full_like(x, -2.5)
+    elif kind == "ties":
+        x = x.round().clamp(-3, 3)
+    elif kind == "ends":
+        x[:, edges] = 15.0
+        k[::2] = edges[-1]
+    elif kind == "nan":
+        x[::3, edges[len(edges) // 2]] = float("nan")
+        x[1::3, [edges[0], vocab - 1]] = float("nan")
+    elif kind == "first part":
+        x[:, tile * tiles:] = float("-inf")
+    else:
+        x[:, :vocab - 37] = torch.finfo(dtype).min if kind == "lowest" else float("-inf")
+        k = vocab - 1 - k % 37
+    x, k = x.to(dev), k.to(dev)
+    for top in (1, 9, 32):
+        _check(x, k, top, None, ops.log_probs_rows(x, k, top))
