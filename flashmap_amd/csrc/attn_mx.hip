@@ -34,8 +34,8 @@
 // and the loads take equal times that overlap only in part (the same contexts 332 us: 239 for the loads
 // alone, 265 for the instructions alone). Row blocks of a unit share its loads and the widening of its
 // values, so a unit takes up to four: as two units of two, the second reads everything again (420 us).
-// One or two leave registers for three workgroups a CU (5 ragged requests 26 -> 22 us with the third), three or
-// four for two, with a tile more in each ring and the queries' operands in LDS.
+// One or two keep the queries' operands in registers and leave LDS for three workgroups a CU (mx_resident), three
+// or four keep them in LDS, with a tile more in each ring.
 // Nothing among the tiles may be loaded through registers: a wait for it would wait for the whole
 // ring (8 contexts of 32768 positions: 100 us, 108 with one such wait).
 #include <math.h>
@@ -85,7 +85,11 @@ struct MxAttnArgs {
   double per_share;  // 1 / shares
 };
 
-constexpr int mx_resident(int rb) { return rb <= 2 ? 3 : 2; }  // workgroups a CU, as registers and LDS allow
+// Workgroups a CU, as registers and LDS allow. Two row blocks of 128 channels need more registers than three
+// workgroups leave (43 would be spilled): 64 requests of 256 to 8192 positions, 32 query rows on each of 8 heads, 90 us
+// with two, 116 with three. One row block (256 requests of 16 to 512 positions, 16 rows: 61 with two, 56 with
+// three) and 64 channels (32 rows of the 64 requests: 62 and 59) gain from the third.
+constexpr int mx_resident(int d, int rb) { return rb == 1 || (rb == 2 && d == 64) ? 3 : 2; }
 
 template <int D, int RB>
 struct MxGeo {
@@ -94,7 +98,7 @@ struct MxGeo {
   static constexpr int DMAS = CODES / 1024;               // 16-byte loads a lane of a tile's codes
   static constexpr int LOADS = DMAS + 2;                  // and its scales, and later page ids
   static constexpr int SLOT = CODES + SCALES + 4 * MXA_TILE;
-  static constexpr int RESIDENT = mx_resident(RB);
+  static constexpr int RESIDENT = mx_resident(D, RB);
   static constexpr int NS = RB <= 2 ? 2 : 3;              // tiles in a wavefront's ring
   static constexpr int RING = MXA_WAVES * NS * SLOT;
   static constexpr int QN = D == 128 ? 4 : 2;             // 16-byte operands a lane of a row block's queries
@@ -976,15 +980,15 @@ struct MxRows {
 };
 
 // Shares of a row group: as many workgroups as the chip holds at once, by eights (a share an XCD).
-static int32_t mx_attn_shares(int rb, int32_t rgroups) {
+static int32_t mx_attn_shares(int d, int rb, int32_t rgroups) {
   DeviceInfo info;
   const int cus = device_info(&info) == FM_OK ? info.cus : 256;
-  const int32_t n = mx_resident(rb) * cus / rgroups / 8 * 8;
+  const int32_t n = mx_resident(d, rb) * cus / rgroups / 8 * 8;
   return n < 8 ? 8 : n;
 }
 
-static size_t mx_attn_part_floats(int rb, int32_t rgroups, int d) {
-  return (size_t)2 * mx_attn_shares(rb, rgroups) * rgroups * 16 * rb * (d + 2);
+static size_t mx_attn_part_floats(int d, int rb, int32_t rgroups) {
+  return (size_t)2 * mx_attn_shares(d, rb, rgroups) * rgroups * 16 * rb * (d + 2);
 }
 
 template <int D, int RB>
@@ -1021,7 +1025,7 @@ extern "C" size_t fm_block_attn_paged_mx_workspace_bytes(int32_t max_seqlen_q, i
   const int64_t rows = (int64_t)(num_q_heads / num_kv_heads) * max_seqlen_q;
   if (rows > MXA_ROWS) return 0;
   const MxRows cut(rows);
-  return sizeof(float) * mx_attn_part_floats(cut.rb, cut.slice, head_dim);
+  return sizeof(float) * mx_attn_part_floats(head_dim, cut.rb, cut.slice);
 }
 
 extern "C" int fm_block_attn_paged_mx(
@@ -1096,11 +1100,11 @@ extern "C" int fm_block_attn_paged_mx(
   a.qn_w = q_norm_weight;
   a.rope = Rope{rope_cos, rope_sin, rope_row_stride, rope_pair_stride, rope_rows};
   a.q_pos = q_positions, a.eps = eps;
-  a.shares = mx_attn_shares(cut.rb, cut.slice);
+  a.shares = mx_attn_shares(head_dim, cut.rb, cut.slice);
   // A share's steps are counted in 32 bits.
   FM_REQUIRE(units * ((most + MXA_STEP - 1) / MXA_STEP) / a.shares < INT32_MAX, "too many positions for one launch");
   a.per_share = 1.0 / a.shares;
-  const size_t need = sizeof(float) * mx_attn_part_floats(cut.rb, cut.slice, head_dim);
+  const size_t need = sizeof(float) * mx_attn_part_floats(head_dim, cut.rb, cut.slice);
   if (workspace_bytes < need) return fail(FM_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
   a.part_o = (float *)workspace;
   a.part_ml = a.part_o + (size_t)2 * a.shares * cut.slice * 16 * cut.rb * head_dim;

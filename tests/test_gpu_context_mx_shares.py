@@ -1,7 +1,7 @@
 """The attention over a 4-bit context where there is more to do than workgroups: shares of several steps and units,
 units cut by them and joined, references that move, rings that are used again.
 
-A share is one workgroup's, ``resident`` a CU (3 for up to 32 query rows a KV head, 2 for more) over the row groups of
+A share is one workgroup's, at most 3 a CU for up to 32 query rows a KV head and 2 for more, over the row groups of
 64 rows; below that many steps of 128 positions every share is one step. Results are held to float64 by
 _context_mx_norms."""
 
@@ -16,7 +16,7 @@ pytestmark = pytest.mark.gpu
 
 
 def _shares(dev, rows: int) -> int:
-    """Workgroups of a row group for so many query rows a KV head."""
+    """Workgroups of a row group for so many query rows a KV head, at most."""
     blocks = -(-rows // 16)
     groups = -(-blocks // 4)
     per_cu = 3 if -(-blocks // groups) <= 2 else 2
