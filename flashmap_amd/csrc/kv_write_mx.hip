@@ -127,8 +127,8 @@ extern "C" int fm_write_context_kv_mx(const void *kv, int64_t tokens, int32_t la
   FM_REQUIRE(row_stride % 16 == 0 && row_stride >= head_dim && scales_stride % 4 == 0 && scales_stride >= head_dim / 16,
              "cache rows hold %d code bytes at a stride of a multiple of 16 and %d scale bytes at one of 4", head_dim,
              head_dim / 16);
-  FM_REQUIRE(tokens <= INT64_MAX / 4 / layers / heads && (tokens * layers * heads + 63) / 64 < (1ll << 31),
-             "too many rows");
+  FM_REQUIRE(tokens <= INT64_MAX / 4 / layers / heads && (tokens * layers * heads + 63) / 64 < (1ll << 24),
+             "too many rows: at most 2^30 - 64 of tokens, layers and heads");
   for (int i = 0; i < layers; ++i)
     FM_REQUIRE(codes[i] && scales[i] && ((uintptr_t)codes[i] & 15) == 0 && ((uintptr_t)scales[i] & 3) == 0,
                "the codes of layer %d must be 16-byte aligned, its scales 4-byte aligned", i);

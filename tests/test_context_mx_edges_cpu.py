@@ -142,3 +142,15 @@ def test_out_beside_and_over_operands(launched):
 def test_rotary_halves_on_one_device():
     with pytest.raises(ValueError, match="device"):
         ops.rope_from_split(torch.zeros(8, 32), torch.zeros(8, 32, device="meta"))
+
+
+def test_rows_of_a_write():
+    """What a launch can count threads for: a call of more rows is refused before any is written."""
+    pointers = (ctypes.c_void_p * 2)(256, 256)
+
+    def write(tokens):
+        return _native.lib().fm_write_context_kv_mx(X, tokens, 2, 16, 64, X, X, X, X, X, 64, 1, 8,
+                                                    pointers, pointers, 64, 4, 4, 8, ctypes.c_float(1e-6), None)
+
+    assert write(1 << 25) == _native.FM_ERR_INVALID and "too many" in _native.last_error()
+    assert write((1 << 25) - 1) == _native.FM_ERR_INVALID and "too many" in _native.last_error()
