@@ -30,14 +30,16 @@
 // exponents finds those that passed.
 //
 // What bounds it: with 16 rows a head the cache's bytes (8 contexts of 131072 positions, 16 query rows on
-// each of 8 heads: 222 us, 5.1 TB/s, what a copy reaches); with 64 rows a head matrix and vector instructions
-// and the loads take equal times that overlap only in part (the same contexts 332 us: 239 for the loads
-// alone, 265 for the instructions alone). Row blocks of a unit share its loads and the widening of its
-// values, so a unit takes up to four: as two units of two, the second reads everything again (420 us).
+// each of 8 heads: 221 us, 5.2 TB/s, what a copy reaches); with 64 rows a head matrix and vector instructions
+// and the loads take nearly equal times that overlap only in part (the same contexts 320 us: 238 for the loads
+// alone, 267 for the instructions alone), and a unit's end, four wavefronts' sums of 64 rows, some microseconds
+// a share (8 contexts of 32768 positions: 98 us). Row blocks of a unit share its loads and the widening of its
+// values, so a unit takes up to four: as two units of two, the second reads everything again (419 us).
 // One or two keep the queries' operands in registers and leave LDS for three workgroups a CU (mx_resident), three
-// or four keep them in LDS, with a tile more in each ring.
+// or four keep them in LDS, with a tile more in each ring. Four of 128 channels take all 256 registers: 29 that
+// are not used among the tiles are spilled and come back between units.
 // Nothing among the tiles may be loaded through registers: a wait for it would wait for the whole
-// ring (8 contexts of 32768 positions: 100 us, 108 with one such wait).
+// ring (8 contexts of 32768 positions: 8 % more with one such wait).
 #include <math.h>
 
 #include <type_traits>
@@ -87,8 +89,8 @@ struct MxAttnArgs {
 
 // Workgroups a CU, as registers and LDS allow. Two row blocks of 128 channels need more registers than three
 // workgroups leave (43 would be spilled): 64 requests of 256 to 8192 positions, 32 query rows on each of 8 heads, 90 us
-// with two, 116 with three. One row block (256 requests of 16 to 512 positions, 16 rows: 61 with two, 56 with
-// three) and 64 channels (32 rows of the 64 requests: 62 and 59) gain from the third.
+// with two, 114 with three. One row block (256 requests of 16 to 512 positions, 16 rows: 60 with two, 55 with
+// three) and 64 channels (32 rows of the 64 requests: 60 and 55) gain from the third.
 constexpr int mx_resident(int d, int rb) { return rb == 1 || (rb == 2 && d == 64) ? 3 : 2; }
 
 template <int D, int RB>
@@ -275,7 +277,8 @@ __device__ __forceinline__ void sort_rope(PrologueOps<D> &ops, const Rope &rope)
   }
 }
 
-// norm_rope_exact where the result is rounded to 8 bits: sums and root in float32 as they come.
+// norm_rope_exact where the result is rounded to 8 bits, not 2: sums in float32 as they come, the root's reciprocal
+// by its instruction (1 ulp), products fused.
 template <int D>
 __device__ __forceinline__ void norm_rope_query(const u32x4_t (&x)[D / 32], const PrologueOps<D> &ops, float eps,
                                                 float (&y)[D / 32][8]) {

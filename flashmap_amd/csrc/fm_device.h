@@ -318,7 +318,7 @@ __device__ __forceinline__ void norm_rope_f32(const u32x4_t (&x)[D / 32], const 
 }
 
 // RMSNorm + RoPE in fp32 from one end to the other: y = (x r) w, rotated, nothing rounded to bf16 (the
-// microscaled cache's writer and the queries that attend to it round once, to their codes).
+// microscaled cache's writer rounds once, to its codes), every step rounded as written.
 template <int D>
 __device__ __forceinline__ void norm_rope_exact(const u32x4_t (&x)[D / 32], const PrologueOps<D> &ops, float eps,
                                                 float (&y)[D / 32][8]) {

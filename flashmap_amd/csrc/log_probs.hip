@@ -336,7 +336,8 @@ __global__ __launch_bounds__(LP_THREADS, 4) void log_probs_part_kernel(const Log
   finish<TY, RESULTS>(a, lds, sums, list, mine, row, (int64_t)blockIdx.y * a.parts + blockIdx.x);
 }
 
-// The records of row blockIdx.x.
+// The records of row blockIdx.x. Of one row of 75 parts with lists of 20: 9.8 us (the parts take 12), loads that follow
+// one another (token, its logit, records, then keys) and every key's way through the bound and the order.
 template <int TY>
 __global__ __launch_bounds__(LP_THREADS) void log_probs_join_kernel(const LogProbsArgs a) {
   __shared__ LpShared lds;

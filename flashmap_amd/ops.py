@@ -1896,10 +1896,10 @@ def block_attention_paged_mx(
     ``query (tokens, Hq, D)`` bf16, each request reading its first ``seqused_k[b]`` positions (at most
     ``max_seqlen_k``), zeros for a request of none. The cache's values enter exactly, the query, behind a
     float32 prologue and times the scale, rounded once by at most 2^-8; scores and sums are float32,
-    probabilities are rounded to bf16. ``out`` (bf16; it may be ``query``, and may not overlap it or anything
-    else that the call reads) receives the result; its rows behind the last request are left alone. The context is cut over the chip by
-    lengths read on the device: a row's result may differ in its last place between calls of other
-    batches."""
+    probabilities are rounded to bf16; a score past float32's range may make its row NaN. ``out`` (bf16; it
+    may be ``query``, and may not overlap it or anything else that the call reads) receives the result;
+    its rows behind the last request are left alone. The context is cut over the chip by lengths read on the
+    device: a row's result may differ in its last place between calls of other batches."""
     index = _mx_device(query, cache.codes, cache.scales, cu_seqlens_q, seqused_k, block_table, out)
     _no_gradient("block_attention_paged_mx", query)
     if query.dim() != 3:

@@ -560,8 +560,8 @@ int fm_write_context_kv_mx(const void *kv, int64_t tokens, int32_t layers, int32
  * sequence's positions below min(seqused_k[b], max_seqlen_k, block_table_width * page_size)
  * through its row of block_table (which may be NULL where its width or max_seqlen_k is 0); a page
  * outside the cache is read as page 0. Sequences of length 0 get zeros. The query's norm and rotation
- * are applied on the way when q_norm_weight is given, in fp32 as the writer's, and the scaled query is
- * rounded once, by at most 2^-8. softmax_scale >= 0; num_blocks * num_kv_heads * page_size < 2^32. The
+ * are applied on the way when q_norm_weight is given, in fp32 (the writer's formula; the root to 1 ulp), and
+ * the scaled query is rounded once, by at most 2^-8, with or without them. softmax_scale >= 0; num_blocks * num_kv_heads * page_size < 2^32. The
  * workspace (16-byte aligned) holds fm_block_attn_paged_mx_workspace_bytes(...) bytes for the current
  * device; calls that may overlap in time must not share it. */
 size_t fm_block_attn_paged_mx_workspace_bytes(int32_t max_seqlen_q, int32_t num_q_heads, int32_t num_kv_heads,
