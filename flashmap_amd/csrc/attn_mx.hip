@@ -46,6 +46,7 @@
 
 #include "fm_host.h"
 #include "mx_device.h"
+#include "wave_device.h"
 
 namespace fm {
 
@@ -277,7 +278,7 @@ __device__ __forceinline__ void sort_rope(PrologueOps<D> &ops, const Rope &rope)
   }
 }
 
-// norm_rope_exact where the result is rounded to 8 bits, not 2: sums in float32 as they come, the root's reciprocal
+// The writer's norm and rotation (kv_write_mx.hip) where the result is rounded to 8 bits, not 2: sums in float32 as they come, the root's reciprocal
 // by its instruction (1 ulp), products fused.
 template <int D>
 __device__ __forceinline__ void norm_rope_query(const u32x4_t (&x)[D / 32], const PrologueOps<D> &ops, float eps,

@@ -111,12 +111,6 @@ __device__ __forceinline__ float max_over_groups(float v) {
 // so that everything derived from it stays in SGPRs and uniform branches.
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
 
-// What a wavefront's lanes wrote to LDS before it, its lanes read behind it.
-__device__ __forceinline__ void wave_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
-
 __device__ __forceinline__ u32x4_t load16(const void *p) {
   return *reinterpret_cast<const u32x4_t *>(p);
 }
@@ -315,38 +309,6 @@ __device__ __forceinline__ void norm_rope_f32(const u32x4_t (&x)[D / 32], const 
       y[t][2 * q + 1] = add_rn(mul_rn(o, c), mul_rn(e, s));
     }
   }
-}
-
-// RMSNorm + RoPE in fp32 from one end to the other: y = (x r) w, rotated, nothing rounded to bf16 (the
-// microscaled cache's writer rounds once, to its codes), every step rounded as written.
-template <int D>
-__device__ __forceinline__ void norm_rope_exact(const u32x4_t (&x)[D / 32], const PrologueOps<D> &ops, float eps,
-                                                float (&y)[D / 32][8]) {
-  constexpr int KT = D / 32;
-  // The row's sum of squares in float64 (products of bf16 are exact in float32): its rounding to
-  // float32 is then the same whatever the order, and with it the codes next to a midpoint.
-  double ss = 0;
-#pragma unroll
-  for (int t = 0; t < KT; ++t)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float e = bf16_lo(x[t][q]), o = bf16_hi(x[t][q]);
-      ss += (double)(e * e);
-      ss += (double)(o * o);
-    }
-  ss += __shfl_xor(ss, 16);
-  ss += __shfl_xor(ss, 32);
-  const float r = __fdiv_rn(1.0f, __fsqrt_rn(add_rn(__fdiv_rn((float)ss, (float)D), eps)));
-#pragma unroll
-  for (int t = 0; t < KT; ++t)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float e = mul_rn(mul_rn(bf16_lo(x[t][q]), r), ops.w[t][2 * q]);
-      const float o = mul_rn(mul_rn(bf16_hi(x[t][q]), r), ops.w[t][2 * q + 1]);
-      const float c = ops.c[t][q], s = ops.s[t][q];
-      y[t][2 * q] = sub_rn(mul_rn(e, c), mul_rn(o, s));
-      y[t][2 * q + 1] = add_rn(mul_rn(o, c), mul_rn(e, s));
-    }
 }
 
 // OCP e4m3 (the fp8 KV caches): round to nearest even, saturated to the largest finite

@@ -37,6 +37,38 @@ struct KvWriteMxArgs {
   uint8_t *codes[MX_KV_LAYERS], *scales[MX_KV_LAYERS];
 };
 
+// RMSNorm + RoPE in fp32 from one end to the other: y = (x r) w, rotated, every step rounded as
+// written and nothing to bf16: the codes are the one rounding to fewer bits.
+template <int D>
+__device__ __forceinline__ void norm_rope_exact(const u32x4_t (&x)[D / 32], const PrologueOps<D> &ops, float eps,
+                                                float (&y)[D / 32][8]) {
+  constexpr int KT = D / 32;
+  // The row's sum of squares in float64 (products of bf16 are exact in float32): its rounding to
+  // float32 is then the same whatever the order, and with it the codes next to a midpoint.
+  double ss = 0;
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float e = bf16_lo(x[t][q]), o = bf16_hi(x[t][q]);
+      ss += (double)(e * e);
+      ss += (double)(o * o);
+    }
+  ss += __shfl_xor(ss, 16);
+  ss += __shfl_xor(ss, 32);
+  const float r = __fdiv_rn(1.0f, __fsqrt_rn(add_rn(__fdiv_rn((float)ss, (float)D), eps)));
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float e = mul_rn(mul_rn(bf16_lo(x[t][q]), r), ops.w[t][2 * q]);
+      const float o = mul_rn(mul_rn(bf16_hi(x[t][q]), r), ops.w[t][2 * q + 1]);
+      const float c = ops.c[t][q], s = ops.s[t][q];
+      y[t][2 * q] = sub_rn(mul_rn(e, c), mul_rn(o, s));
+      y[t][2 * q + 1] = add_rn(mul_rn(o, c), mul_rn(e, s));
+    }
+}
+
 // Lane g of a row holds dword g of blocks 0 .. 3 in w[0 .. 3]; afterwards block g's dwords 0 .. 3.
 __device__ __forceinline__ u32x4_t transpose_quad(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
   const auto a = __builtin_amdgcn_permlane32_swap(w0, w2, false, false);

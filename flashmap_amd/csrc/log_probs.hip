@@ -22,6 +22,7 @@
 
 #include "fm_host.h"
 #include "logits_device.h"
+#include "wave_device.h"
 
 namespace fm {
 
