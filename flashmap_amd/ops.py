@@ -1857,7 +1857,7 @@ def write_context_kv_mx(
                          f"{tuple(slots.shape)}")
     if tokens == 0:
         return
-    if len({(a[0], a[2]) for a in args}) < len(args):
+    if len({a[0] for a in args}) < len(args) or len({a[2] for a in args}) < len(args):
         raise ValueError("the layers' caches must be different ones")
     if joined:
         rows = blocks * heads * page

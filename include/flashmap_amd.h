@@ -547,7 +547,7 @@ int fm_adaln_residual_mx(const void *x, int64_t x_stride, const void *y, int64_t
  * (tokens, layers, 2, heads, head_dim) bf16 (contiguous, 16-byte aligned) into row slots[t] %
  * page_size of block slots[t] / page_size of every layer's cache. A slot outside the cache (negative:
  * padding) is skipped; slots of one call that are kept must differ. codes, scales: HOST arrays of
- * `layers` device addresses, read during the call. */
+ * `layers` device addresses, of caches that do not overlap, read during the call. */
 int fm_write_context_kv_mx(const void *kv, int64_t tokens, int32_t layers, int32_t heads, int32_t head_dim,
                            const int64_t *positions, const int64_t *slots, const float *k_norm_weight,
                            const float *rope_cos, const float *rope_sin, int64_t rope_row_stride,

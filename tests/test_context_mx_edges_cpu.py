@@ -89,6 +89,9 @@ def test_one_cache_for_two_layers(launched):
     rope = ops.rope_from_table(torch.zeros(8, 32, 2))
     with pytest.raises(ValueError, match="different"):
         ops.write_context_kv_mx(kv, idx, idx, torch.ones(2, 64), rope, [caches[0], caches[0]], 1e-6)
+    halves = ops.MX(caches[0].codes, caches[1].scales, 4, caches[0].shape)
+    with pytest.raises(ValueError, match="different"):
+        ops.write_context_kv_mx(kv, idx, idx, torch.ones(2, 64), rope, [caches[0], halves], 1e-6)
     assert launched == []
     ops.write_context_kv_mx(kv, idx, idx, torch.ones(2, 64), rope, caches, 1e-6)
     ops.write_context_kv_mx(kv, idx, idx, torch.ones(2, 64), rope, ops.mx_cache(4, 2, 8, 64, "cpu", 2), 1e-6)
