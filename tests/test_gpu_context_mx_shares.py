@@ -180,3 +180,65 @@ def test_captured_lengths(dev):
         torch.cuda.synchronize()
         assert torch.equal(out, want)
         check_norm(out, query, [_context(cache, table[b], n) for b, n in enumerate(now)], [q_len] * 5, d ** -0.5)
+
+
+def _rotated(query, weight, angles, at):
+    """Norm and rotation in float64: what attends."""
+    x = query.double()
+    x = x / torch.sqrt((x * x).mean(-1, keepdim=True) + 1e-6) * weight.double()
+    e, o, (c, s) = x[..., 0::2], x[..., 1::2], angles.double()[at][:, None].unbind(-1)
+    return torch.stack([e * c - o * s, o * c + e * s], -1).flatten(-2)
+
+
+@pytest.mark.parametrize("d", [128, 64])
+@pytest.mark.parametrize("q_len,group", ROWS)
+@pytest.mark.parametrize("table_of", ["interleaved", "apart"])
+def test_prologue_and_query_as_out(dev, d, q_len, group, table_of):
+    """The next unit's positions, rotary rows and queries fetched while one ends, and written over as results."""
+    hkv, most = 16, 9
+    lens = _cost(dev, q_len, group, hkv, most)
+    assert hkv * _steps(lens) > (most - 1) * _shares(dev, q_len * group)
+    cache, table, rows = _cache(lens, hkv, d, 8, 11, dev)
+    g = torch.Generator(dev).manual_seed(12)
+    q_lens = [max(1, q_len - 5 * b % q_len) for b in range(len(lens))]
+    q_lens[-1] = q_len
+    tokens = sum(q_lens)
+    query = (3 * torch.randn(tokens, hkv * group, d, generator=g, device=dev)).to(BF)
+    weight = 0.5 + torch.rand(d, generator=g, device=dev)
+    angle = torch.arange(900, device=dev).double()[:, None] * 1e4 ** -(torch.arange(0, d, 2, device=dev).double() / d)
+    angles = torch.stack([angle.cos(), angle.sin()], -1).float()
+    at = torch.randint(0, 900, (tokens,), generator=g, device=dev)
+    rope = ops.rope_from_table(angles) if table_of == "interleaved" else ops.rope_from_split(*angles.unbind(-1))
+    cu = torch.tensor([0, *torch.tensor(q_lens).cumsum(0).tolist()], dtype=torch.int32, device=dev)
+    seq = torch.tensor(lens, dtype=torch.int32, device=dev)
+    args = cache, cu, seq, table, q_len, max(lens), d ** -0.5, ops.Prologue(weight, rope, at, 1e-6)
+    out = ops.block_attention_paged_mx(query, *args)
+    check_norm(out, _rotated(query, weight, angles, at), rows, q_lens, d ** -0.5)
+    same = query.clone()
+    assert torch.equal(ops.block_attention_paged_mx(same, *args, out=same), out)
+
+
+@pytest.mark.parametrize("q_len,group", [(3, 1), (16, 4)])
+def test_many_requests(dev, q_len, group):
+    """More requests than a launch takes, each launch with more steps than shares."""
+    hkv, d = 32, 64
+    g = torch.Generator().manual_seed(13)
+    lens = torch.randint(0, 700, (600,), generator=g).tolist()
+    lens[255], lens[256], lens[511], lens[512], lens[599] = 600, 0, 0, 650, 1
+    for first in (0, 256):
+        assert hkv * _steps(lens[first:first + 256]) > 4 * _shares(dev, q_len * group)
+    cache, table, rows = _cache(lens, hkv, d, 16, 14, dev)
+    q_lens = [1 + b % q_len for b in range(600)]
+    query, out = _run(cache, table, lens, q_lens, hkv * group, d, 15, dev)
+    some = [0, 1, 2, 100, 254, 255, 256, 257, 300, 511, 512, 513, 598, 599]
+    starts = [0, *torch.tensor(q_lens).cumsum(0).tolist()]
+    for b in some:
+        part = slice(starts[b], starts[b + 1])
+        check_norm(out[part], query[part], [rows[b]], [q_lens[b]], d ** -0.5)
+    # the others as calls of their own: the same terms, in another order of sums
+    for first in range(0, 600, 100):
+        part = slice(starts[first], starts[first + 100])
+        cu = torch.tensor(starts[first:first + 101], dtype=torch.int32, device=dev) - starts[first]
+        few = ops.block_attention_paged_mx(query[part], cache, cu, torch.tensor(lens[first:first + 100], device=dev),
+                                           table[first:first + 100], q_len, 700, d ** -0.5)
+        assert (few.float() - out[part].float()).abs().max() <= 2.0 ** -7 * out.float().abs().max()

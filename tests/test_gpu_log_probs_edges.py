@@ -67,7 +67,7 @@ CUTS = [(61, 128_257), (200, 50_257), (700, 9_000), (600, 40_000), (64, 60_000),
 
 
 def _tiles(rows, vocab):
-    """(logits of a tile, tiles of a part) as the documents of the cut have it."""
+    """(logits of a tile, tiles of a part), as rows are cut."""
     most = -(-1024 // rows)
     tile = 2048 if -(-(vocab + 7) // 4096) < most else 4096
     return tile, -(-(-(-(vocab + 7) // tile)) // most)
