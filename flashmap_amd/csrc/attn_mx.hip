@@ -278,8 +278,8 @@ __device__ __forceinline__ void sort_rope(PrologueOps<D> &ops, const Rope &rope)
   }
 }
 
-// The writer's norm and rotation (kv_write_mx.hip) where the result is rounded to 8 bits, not 2: sums in float32 as they come, the root's reciprocal
-// by its instruction (1 ulp), products fused.
+// The writer's norm and rotation (kv_write_mx.hip) where the result is rounded to 8 bits, not 2: sums in float32 as
+// they come, the root's reciprocal by its instruction (1 ulp), products fused.
 template <int D>
 __device__ __forceinline__ void norm_rope_query(const u32x4_t (&x)[D / 32], const PrologueOps<D> &ops, float eps,
                                                 float (&y)[D / 32][8]) {
@@ -881,7 +881,8 @@ __global__ __launch_bounds__(64 * MXA_WAVES) void attn_mx_join_kernel(const MxAt
   }
   // This thread: channels (4 g + i) NF + quarter FW + f of row n.
   const int n = lane & 15, g = lane >> 4, quarter = SPLIT ? (int)blockIdx.z : wave;
-  const int32_t r = (a.rgroup0 * rb_unit + block) * 16 + n, head = divided(r, a.q_mul, a.q_shift), tok = r - head * a.q_len;
+  const int32_t r = (a.rgroup0 * rb_unit + block) * 16 + n;
+  const int32_t head = divided(r, a.q_mul, a.q_shift), tok = r - head * a.q_len;
   const bool live = r < a.group * a.q_len && tok < tokens && (!SPLIT || wave == 0);
   f32x4_t v[FW];
 #pragma unroll

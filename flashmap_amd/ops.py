@@ -1828,8 +1828,8 @@ def write_context_kv_mx(
     """k-norm + RoPE + store of ``kv (tokens, layers, 2, heads, D)`` bf16 into caches in microscaled
     4 bits (:func:`mx_cache`) at ``slots`` (page ``slots[t] // page``, place ``slots[t] % page``; a slot
     outside the cache, such as a negative one, is skipped, and kept slots must differ): ``caches``
-    one of ``shape (layers, blocks, heads, page, 2D)`` or a ``(blocks, heads, page, 2D)`` per layer, all
-    laid out alike. Keys are normed and rotated in float32, ``(k / sqrt(mean(k^2) + eps)) * k_norm``,
+    one of ``shape (layers, blocks, heads, page, 2D)`` or a ``(blocks, heads, page, 2D)`` per layer,
+    different ones that are laid out alike. Keys are normed and rotated in float32, ``(k / sqrt(mean(k^2) + eps)) * k_norm``,
     and rounded once, to their code. See fm_write_context_kv_mx."""
     if kv.dim() != 5 or kv.shape[2] != 2:
         raise ValueError(f"kv must be (tokens, layers, 2, heads, head_dim), got {tuple(kv.shape)}")
